@@ -2,7 +2,7 @@
 // hipStreamEndCapture?  (CUDA allows cudaEventDestroy at any time; torch.cuda.Event objects created inside a captured
 // region and dropped before the region ends do exactly this.)
 //
-//   hipcc --offload-arch=gfx950 -O2 bench/dev/hip_capture_event_destroy.cpp -o bench/micro/bin/hip_capture_event_destroy
+//   hipcc --offload-arch=gfx950 -O2 -Xclang -target-feature -Xclang -packed-fp32-ops bench/dev/hip_capture_event_destroy.cpp -o bench/micro/bin/hip_capture_event_destroy
 //   ./hip_capture_event_destroy keep      # control: events destroyed after hipStreamEndCapture
 //   ./hip_capture_event_destroy destroy   # events destroyed while the capture is still open
 //

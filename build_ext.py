@@ -86,7 +86,10 @@ def build(jobs: int = 8, verbose: bool = False, force: bool = False, kernel_defi
     inc, tlib, abi = _torch_paths()
     hip, cpp, hdr = _sources()
     hipcc = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
-    dev_flags = [f"--offload-arch={ARCH}", "-O3", "-std=c++17", "-fPIC", "-ffp-contract=fast", "-Wno-unused-result"]
+    # (no packed fp32 instructions: hipcc -O3 forms v_pk_add / mul / fma_f32 from ordinary float code, and some of their
+    # forms have given wrong results on this hardware now and then; the host pass warns that it does not know the feature)
+    dev_flags = [f"--offload-arch={ARCH}", "-O3", "-std=c++17", "-fPIC", "-ffp-contract=fast", "-Wno-unused-result",
+                 "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
     dev_flags += [f"-D{d}" for d in kernel_defines]
     host_flags = ["-O2", "-std=c++17", "-fPIC", "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1",
                   "-DTORCH_EXTENSION_NAME=_C", "-DTORCH_API_INCLUDE_EXTENSION_H",

@@ -185,8 +185,7 @@ __device__ __forceinline__ uint32_t drop_keep8(const DropKey& k, uint64_t g, uin
 // below 16-bit output rounding): one v_exp_f32 + one v_rcp_f32 + a 5-term Horner chain.  With x = u/sqrt(2) the
 // exponential exp(-x^2) = exp(-u^2/2) is also the Gaussian of the derivative, so gelu and gelu' share it.
 // The GEMM epilogues call this once per output element; the libm erff costs ~3x more VALU work there.
-// Two elements at a time on <2 x float>: the multiply/add chain becomes packed fp32 instructions
-// (v_pk_mul_f32 / v_pk_fma_f32, two lanes' worth of math per issue); exp and rcp stay scalar.
+// Two elements at a time on <2 x float> (the build switches packed fp32 instructions off: each half is a scalar chain).
 __device__ __forceinline__ void gelu_parts2(float2v u, float2v& cdf, float2v& pdf) {
   const float2v x = float2v{fabsf(u.x), fabsf(u.y)} * 0.70710678118654752f;
   const float2v nx2 = -(x * x) * 1.4426950408889634f;

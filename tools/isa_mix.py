@@ -2,7 +2,7 @@
 """Instruction mix of every kernel in a `hipcc -S` listing: total, MFMA, packed-fp32, transcendental, conversions, selects,
 24-bit multiplies, LDS and memory instructions, scratch use.
 
-    hipcc --offload-arch=gfx950 -O3 -std=c++17 -ffp-contract=fast --cuda-device-only -S csrc/kernels/attention.hip -o /tmp/attn.s
+    hipcc --offload-arch=gfx950 -O3 -std=c++17 -ffp-contract=fast -Xclang -target-feature -Xclang -packed-fp32-ops --cuda-device-only -S csrc/kernels/attention.hip -o /tmp/attn.s
     python tools/isa_mix.py /tmp/attn.s [substring of the kernel name]
 """
 import collections
