@@ -46,10 +46,10 @@ def _sources():
     return hip, cpp, hdr
 
 
-# attention.hip writes its packed fp32 math as explicit vector operations; the SLP vectoriser on top of that pairs up the
+# the attention kernels write their fp32 math as explicit vector operations; the SLP vectoriser on top of that pairs up the
 # scalar adds of the DPP row reductions (v_mov_b32_dpp + v_pk_add_f32, 6 instructions per 4 values and step) where the
 # un-paired adds fold into v_add_f32_dpp (4 instructions)
-PER_SOURCE_FLAGS = {"attention.hip": ["-fno-slp-vectorize"]}
+PER_SOURCE_FLAGS = {"attention.hip": ["-fno-slp-vectorize"], "rel_attention.hip": ["-fno-slp-vectorize"]}
 
 
 def _stamp(paths, flags):

@@ -169,6 +169,62 @@ int pdt_attn_bwd(int dtype, const void* qkv, const int32_t* mask, const int32_t*
                  const void* ctx, const void* dctx, const float* lse, float* delta, void* dqkv, float* dbias, int B, int S,
                  int A, float drop_scale, uint32_t drop_thr, PdtRng rng, void* stream);
 
+// ---- Attention with a relative position bias ----------------------------------------------------------
+// s = scale q.k + table[bucket(key - query)][h] over the attended keys; any S, head dim D <= 128 (multiple of 8).
+// bucket(d), per side (half = buckets / 2, exact = half / 2): |d| below exact, then exact + the number of steps[j] <= |d|
+// over 1 <= j < half - exact; + half for d > 0.  steps[j] is the first distance of logarithmic bucket j, steps[0] = exact,
+// and no step exceeds max_distance (<= 512).
+typedef struct PdtRelView {  // element (b, i, h, c) at p[b * batch + i * row + h * head + c]; packed rows: batch unused
+  void* p;
+  int64_t batch, row, head;
+} PdtRelView;
+typedef struct PdtRelAttn {
+  PdtRelView q, k, v, o;        // 16-byte aligned, strides multiples of 8 elements
+  PdtRelView dout, dq, dk, dv;  // backward
+  float* lse;                   // fp32 [B, A, S], log2 domain (forward: null = not wanted)
+  float* delta;                 // fp32 [B, A, S] scratch of the backward
+  const void* table;            // [buckets, A], 16-bit or (table_f32) fp32; null: no bias (buckets = max_distance = 0)
+  float* dtable_part;           // null, or fp32 [pdt_rel_attn_dtable_rows()][buckets][A]: partial sums of the table gradient
+                                // (finish with pdt_colsum_finish(part, rows, buckets * A, 1, ...))
+  int table_f32, buckets, max_distance;
+  int steps[33];
+  const uint64_t* mask_bits;    // null, or one bit per key [B][mask_words], mask_words = ceil(S / 64) (pdt_rel_attn_mask)
+  int mask_words;
+  const int32_t* cu;            // null, or first rows of the samples in packed [T, ...] tensors, int32 [B + 1]; rows from
+                                // cu[B] on become zero.  S is then the longest sample.
+  int B, S, A, D, T;
+  float scale, drop_scale;
+  uint32_t drop_thr;
+  PdtRng rng;
+} PdtRelAttn;
+// key mask [B, S] (`bytes` = 1 or 4 per key, `stride` keys from sample to sample; non-zero = attended) -> bits
+int pdt_rel_attn_mask(const void* mask, int bytes, int64_t stride, int B, int S, uint64_t* bits, void* stream);
+int pdt_rel_attn_fwd(int dtype, const PdtRelAttn* a, void* stream);
+int pdt_rel_attn_dtable_rows(const PdtRelAttn* a);
+int pdt_rel_attn_bwd(int dtype, const PdtRelAttn* a, void* stream);
+
+// ---- Per-head RMS norm of queries and keys with the position rotation -----------------------------------
+// y = R(position) (x * rsqrt(mean(x^2) + eps) * w) for every head of q (side 0) and k (side 1) of T tokens.  w null: no norm;
+// R = 0: no rotation.  The first R elements of a head are turned in pairs: (i, i + R/2), or neighbours (2i, 2i + 1) when
+// `interleaved`, by the angle whose cosine / sine are row `position` of cos / sin, fp32 [P, R/2].  Position of token t: pos[t]
+// clamped into the table, or t % seq when pos is null.  Element (t, h, c) of a view is p[(t / seq) * batch + (t % seq) * row +
+// h * head + c].  D <= 256, D and R multiples of 8 (R of 16 unless interleaved).
+typedef struct PdtQkRope {
+  PdtRelView x[2], y[2];        // forward: x -> y.  Backward: x, dy (in y) -> dx
+  PdtRelView dx[2];
+  const void* w[2];             // [D], 16-bit or (w_f32) fp32
+  const float *cos, *sin;
+  const int64_t* pos;
+  int heads[2];
+  int T, seq, D, R, P, w_f32, interleaved;
+  float eps;
+} PdtQkRope;
+int pdt_qk_rope_fwd(int dtype, const PdtQkRope* a, void* stream);
+// partial: fp32 [pdt_qk_rope_bwd_blocks(a)][2][D] column partial sums of the two weight gradients, or null (finish with
+// pdt_colsum_finish(partial, blocks, D, 2, dwq, dwk, ...))
+int pdt_qk_rope_bwd_blocks(const PdtQkRope* a);
+int pdt_qk_rope_bwd(int dtype, const PdtQkRope* a, float* partial, void* stream);
+
 // ---- Classification head ------------------------------------------------------------------------------
 // logits[b][c] = dot(dropout(pooled[b]), W[c]) + bias[c]; loss[0] = mean CE.  pooled 16-bit [B,H];
 // W, bias, logits, loss fp32; C <= 8; labels may be null (no loss)

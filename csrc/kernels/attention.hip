@@ -14,14 +14,13 @@
 #include <type_traits>
 #include <unordered_set>
 
-#include "common.hpp"
+#include "attn_common.hpp"
 
 namespace pdt {
 
 constexpr int HD = 64;       // head dim (the MFMA tiling of every kernel here is built on it; the model checks it)
 constexpr float ATT_SCALE = 0.125f;  // 1 / sqrt(HD)
 static_assert(ATT_SCALE * ATT_SCALE * HD == 1.0f, "softmax scale must be 1 / sqrt(head dim)");
-constexpr float LOG2E = 1.4426950408889634f;
 constexpr int ATT_WAVES = 8;  // waves per workgroup: 8 x 16 = 128 query rows (or keys) share one K/V (or Q/dO) image
 constexpr int ATT_THREADS = ATT_WAVES * 64;
 constexpr int ATT_ROWS = ATT_WAVES * 16;
@@ -46,26 +45,6 @@ struct AttnArgs {
   uint32_t drop_thr;  // round(p * 65536), 0 = off
   RngArgs rng;
 };
-
-// Dropout decision for probability (bh, q, key): a function of (seed, offset, site, micro, b*A+h, q, key) only,
-// so every kernel agrees whatever its lane mapping is.  It is split in two so that the per-element cost is one
-// 32-bit multiply: a strongly mixed 32-bit seed per query row (computed once per row - in the dK/dV sweeps it
-// is staged in LDS), and per element  x = low24(row_seed ^ key * GOLD) * MIX24,  keep <=> x[31:16] >= thr.
-// key * GOLD is a Weyl sequence over the keys; an unrolled sweep forms it with one add per element.
-__device__ __forceinline__ uint32_t lowbias32(uint32_t x) {
-  x ^= x >> 16; x *= 0x7feb352du; x ^= x >> 15; x *= 0x846ca68bu; x ^= x >> 16;
-  return x;
-}
-constexpr uint32_t ATT_GOLD = 0x9E3779B9u, ATT_MIX = 0xEBCA6Bu;
-__device__ __forceinline__ uint32_t attn_row_seed(const DropKey& dk, uint32_t bh, uint32_t q) {
-  uint32_t x = lowbias32(q ^ dk.key.x);
-  return lowbias32(x ^ (bh * 0x9E3779B9u) ^ dk.key.y ^ (dk.stream * 0x85EBCA6Bu) ^ (dk.micro * 0xC2B2AE35u));
-}
-// thr_hi = drop threshold << 16 (see attn_thr_hi); kmul = key * ATT_GOLD
-__device__ __forceinline__ bool attn_keep(uint32_t row_seed, uint32_t kmul, uint32_t thr_hi) {
-  return __umul24(row_seed ^ kmul, ATT_MIX) >= thr_hi;  // 24 x 24 -> low 32 bits: a full-rate multiply
-}
-__device__ __forceinline__ uint32_t attn_thr_hi(uint32_t thr) { return (thr > 65535u ? 65535u : thr) << 16; }
 
 // LDS-DMA fill of one 128-row image of 64 16-bit values per row (2 x 1 KiB pieces per wave) from rows
 // [0, 128) of `src` (row stride `stride` elements): the swizzle (16-B chunk ^= row & 6) is applied on the per-lane
@@ -101,53 +80,11 @@ __device__ __forceinline__ short8 tr_frag(const char* img, int r0, int db, int l
   r[4] = hi[0]; r[5] = hi[1]; r[6] = hi[2]; r[7] = hi[3];
   return r;
 }
-// The per-score arithmetic of these kernels is written on whole float4v accumulator tiles (scale + mask, subtract the
-// maximum, dropout factor, dS = P * (dP - delta)).  The build switches packed fp32 instructions off (build_ext.py), so an
-// operation on 4-vectors is four scalar ones; with them on, the same kernels took the same time (forward 251 / 251 us,
-// fused backward 584 / 584 us at batch 1024, both builds in turn).  Pairs of results are converted with one
-// v_cvt_pk_f16_f32 / v_cvt_pk_bf16_f32.  Only exp2 and the dropout hash stay per element.  (This file is built without
-// the SLP vectoriser, see build_ext.py: it would also pair up the adds of the DPP row reductions, which then cost a
-// v_mov_b32_dpp each instead of folding into v_add_f32_dpp.)
-typedef float float2v __attribute__((ext_vector_type(2)));
-template <typename T> struct Pk2;
-template <> struct Pk2<_Float16> { typedef _Float16 type __attribute__((ext_vector_type(2))); };
-template <> struct Pk2<__bf16> { typedef __bf16 type __attribute__((ext_vector_type(2))); };
-template <typename T>
-__device__ __forceinline__ int cvt_pk(float lo, float hi) {  // two fp32 -> one dword of two 16-bit values (round to nearest even)
-  return __builtin_bit_cast(int, __builtin_convertvector(float2v{lo, hi}, typename Pk2<T>::type));
-}
-__device__ __forceinline__ float4v splat4(float v) { return float4v{v, v, v, v}; }
-// A 4-vector whose elements are consumed one by one (exp2 of each) would be taken apart by the optimiser BEFORE the
-// operation that produced it ("extract of a vector op = scalar op of the extracts"), i.e. four v_sub_f32 instead of two
-// v_pk_add_f32.  Passing the two halves through an empty asm statement as 64-bit operands keeps the producing operation
-// packed; it emits nothing.
-__device__ __forceinline__ float4v packed4(float4v v) {
-  float2v lo = {v[0], v[1]}, hi = {v[2], v[3]};
-  asm("" : "+v"(lo));
-  asm("" : "+v"(hi));
-  return float4v{lo[0], lo[1], hi[0], hi[1]};
-}
-template <typename T>
-__device__ __forceinline__ short8 pack_pair(const float4v& a, const float4v& b) {
-  const int4v r = {cvt_pk<T>(a[0], a[1]), cvt_pk<T>(a[2], a[3]), cvt_pk<T>(b[0], b[1]), cvt_pk<T>(b[2], b[3])};
-  return __builtin_bit_cast(short8, r);
-}
 // lane's 8 k-values of row (lane&15) of a row-major global matrix, k-step ks: B-operand style fragment
 template <typename T>
 __device__ __forceinline__ short8 gfrag(const T* base, int row, int stride, int ks, int lane) {
   return *reinterpret_cast<const short8*>(base + (size_t)row * stride + ks * 32 + (lane >> 4) * 8);
 }
-__device__ __forceinline__ float quad_sum(float v) {  // sum over the 4 lane groups (lanes l, l^16, l^32, l^48)
-  v += __shfl_xor(v, 16, 64);
-  v += __shfl_xor(v, 32, 64);
-  return v;
-}
-__device__ __forceinline__ float quad_max(float v) {
-  v = fmaxf(v, __shfl_xor(v, 16, 64));
-  v = fmaxf(v, __shfl_xor(v, 32, 64));
-  return v;
-}
-
 // Store a wave's 16 x 64 tile as 16-bit values: lane (lm, g) holds the fp32 values t[db][r] of row lm, columns
 // 16 db + 4 g + r (the accumulator layout), `row` points at the 64 elements of its row.  Lanes g and g ^ 1 of a row swap
 // half of their blocks first, so that each lane writes two 16-byte chunks and every store instruction covers 64
@@ -333,18 +270,6 @@ __global__ __launch_bounds__(ATT_THREADS) PDT_ATT_FWD_OCC void attn_fwd_kernel(A
   store_tile16x64<T>((T*)a.ctx + ((size_t)row0 + qc) * a.H + h * HD, o, inv, g, q < S);
 }
 
-template <int CTRL>
-__device__ __forceinline__ float dpp_f(float v) {
-  return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), CTRL, 0xF, 0xF, false));
-}
-// sum over the 16 lanes of a DPP row (lanes sharing lane>>4); every lane of the row receives the total
-__device__ __forceinline__ float row16_sum(float v) {
-  v += dpp_f<0x128>(v);  // row_ror:8
-  v += dpp_f<0x124>(v);  // row_ror:4
-  v += dpp_f<0x122>(v);  // row_ror:2
-  v += dpp_f<0x121>(v);  // row_ror:1
-  return v;
-}
 // ------------------------------------------------------------------------------------------------ dQ (S > 128)
 // One wave = 16 query rows, sweeps the keys chunk by chunk; also produces delta = rowsum(dO * O) for the
 // dK/dV kernel.  Log2-domain recomputation with the softmax scale folded into the exponent.

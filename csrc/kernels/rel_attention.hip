@@ -1,0 +1,805 @@
+// Softmax attention with a learned relative position bias for gfx950: any length, any head dim up to 128 that is a
+// multiple of 8, strided or packed rows, key mask with holes, dropout on the probabilities, gradients of q, k, v and of
+// the bias table.
+//
+//   s_ij = scale q_i . k_j + table[bucket(j - i)][h],   p = softmax over the attended keys,   o_i = sum_j p_ij v_j
+//   backward: dp = do . v,  ds = p (dp - delta),  delta_i = do_i . o_i,  dq = scale ds k,  dk = scale ds^T q,
+//             dv = p^T do,  dtable[t][h] = sum of ds_ij over the batch and all (i, j) with bucket(j - i) = t
+//
+// The bias depends on (head, j - i) only, and is constant once |j - i| reaches max_distance: every workgroup expands its
+// head's column of the table into an LDS array over the near distances, and score tiles that lie completely beyond them
+// use one constant.  The array exists in four copies shifted by one element, so that the four consecutive distances of a
+// lane's accumulator registers are one aligned 16-byte read whatever the lane's query row is.
+//
+// The table gradient is the sum of ds along its diagonals.  A 16x16 tile of ds (keys in registers, queries in lanes) is
+// reduced to its 31 diagonals with DPP row shifts (register r shifted by r lanes lines the diagonals up) and added to an
+// LDS array that belongs to the wave; far tiles only add up their elements.  No two waves share an array and nothing is
+// accumulated through global atomics, so the gradient does not depend on the order in which workgroups run.
+//
+// Products put the key (forward, dQ) or the query (dK / dV) on the register axis, so that an accumulator tile is directly
+// the B operand of the next product; rows come through LDS in chunks of 64, double-buffered, filled by LDS-DMA.  A row
+// that no query may attend to is read as zeros: whatever its memory holds, NaN included, never meets a product.
+#include <mutex>
+#include <unordered_set>
+
+#include "attn_common.hpp"
+
+namespace pdt {
+
+constexpr int RA_WAVES = 4, RA_THREADS = RA_WAVES * 64;
+constexpr int RA_CHUNK = 64;                    // rows per LDS image
+constexpr int RA_IMG = RA_CHUNK * 128;          // bytes of a 64-row x 64-column image
+constexpr int RA_MAX_FAR = 512;                 // largest max_distance
+constexpr int RA_MAX_STEPS = 32;                // logarithmic buckets per side
+
+
+// rows [0, 64) of a [rows][D] matrix (row stride `stride` elements) into NH 64-column images: 16-byte chunk c of row r is
+// stored at chunk c ^ (r & 6).  Rows whose bit in `rows` is clear, and columns from D on, arrive as zeros.
+template <typename T, int NH>
+__device__ __forceinline__ void ra_stage(char* img, const T* src, uint32_t stride, uint64_t rows, int D, int lane, int wave) {
+  const int4v rsrc = pdt_make_rsrc(src, rows ? (uint32_t)((RA_CHUNK - 1) * stride + D) * 2u : 0u);
+#pragma unroll
+  for (int h = 0; h < NH; ++h) {
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      const int piece = u * RA_WAVES + wave, row = piece * 8 + (lane >> 3);
+      const int col = h * 64 + (((lane & 7) ^ (row & 6)) << 3);
+      const bool ok = ((rows >> row) & 1) && col < D;
+      pdt_lds_dma16(rsrc, img + h * RA_IMG + piece * 1024, ok ? (row * stride + col) * 2u : 0x80000000u);
+    }
+  }
+}
+// rows x0..x0+15 as an A operand: lane -> row x0 + (lane & 15), k = 8 (lane >> 4) + j of the 32-column step ks
+__device__ __forceinline__ short8 ra_row_frag(const char* img, int x0, int ks, int lane) {
+  const int row = x0 + (lane & 15), c = (ks & 1) * 4 + (lane >> 4);
+  return *reinterpret_cast<const short8*>(img + (ks >> 1) * RA_IMG + row * 128 + ((c ^ (row & 6)) << 4));
+}
+// transposed operand over 32 rows from r0: lane -> column 16 db + (lane & 15); k-value j < 4: row r0 + 4 g + j, j >= 4:
+// row r0 + 16 + 4 g + (j - 4) - the order in which pack_pair() lays out two accumulator tiles
+__device__ __forceinline__ short8 ra_tr_frag(const char* img, int r0, int db, int lane) {
+  const int g = lane >> 4, q = (lane & 15) >> 2, p = lane & 3;
+  const int row = r0 + 4 * g + q, c = 2 * (db & 3) + (p >> 1);
+  const char* a = img + (db >> 2) * RA_IMG + row * 128 + ((c ^ (row & 6)) << 4) + (p & 1) * 8;
+  const short4r lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((short4r __attribute__((address_space(3)))*)PDT_LDS_PTR(a));
+  const short4r hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((short4r __attribute__((address_space(3)))*)PDT_LDS_PTR(a + 16 * 128));
+  return short8{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+}
+// the lane's 8 values of a row in global memory (zeros from column D on, or when the row is not there)
+template <typename T>
+__device__ __forceinline__ short8 ra_gfrag(const T* row, int ks, int D, int lane, bool ok) {
+  const int col = ks * 32 + (lane >> 4) * 8;
+  short8 r = {0, 0, 0, 0, 0, 0, 0, 0};
+  if (ok && col < D) r = *reinterpret_cast<const short8*>(row + col);
+  return r;
+}
+// A wave's 16-row tile t[2 KS] (lane (lm, g) holds row lm, columns 16 db + 4 g + r) as 16-bit rows: lanes g and g ^ 1
+// swap a block of every pair, so that each stores 16 contiguous bytes.  Call with the whole wave.
+template <typename T, int KS>
+__device__ __forceinline__ void ra_store(T* row, const float4v (&t)[2 * KS], float mul, int g, int D, bool valid) {
+  const bool odd = g & 1;
+#pragma unroll
+  for (int ks = 0; ks < KS; ++ks) {
+    int2v pk[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const float4v v = t[2 * ks + i] * mul;
+      pk[i] = int2v{cvt_pk<T>(v[0], v[1]), cvt_pk<T>(v[2], v[3])};
+    }
+    const int2v own = odd ? pk[1] : pk[0], snd = odd ? pk[0] : pk[1];
+    int2v rcv;
+    rcv[0] = __shfl_xor(snd[0], 16, 64); rcv[1] = __shfl_xor(snd[1], 16, 64);
+    const int col = ks * 32 + (odd ? 16 : 0) + 4 * (g & ~1);
+    if (valid && col < D)
+      *reinterpret_cast<int4v*>(row + col) = odd ? int4v{rcv[0], rcv[1], own[0], own[1]} : int4v{own[0], own[1], rcv[0], rcv[1]};
+  }
+}
+
+// ---- one (batch, head) of a launch
+struct RaSpan {
+  int b, h, n;      // sample, head, length
+  int64_t row0;     // first packed row (packed) or 0
+};
+__device__ __forceinline__ RaSpan ra_span(const PdtRelAttn& p, int bh) {
+  RaSpan s;
+  s.b = bh / p.A;
+  s.h = bh - s.b * p.A;
+  if (p.cu) {  // (lengths that do not fit the tensors are cut to them)
+    const int lo = min(max(uniform_load_i32(p.cu, s.b), 0), p.T), hi = min(max(uniform_load_i32(p.cu, s.b + 1), lo), p.T);
+    s.row0 = lo;
+    s.n = min(hi - lo, p.S);
+  } else {
+    s.row0 = 0;
+    s.n = p.S;
+  }
+  return s;
+}
+template <typename T>
+__device__ __forceinline__ T* ra_base(const PdtRelView& v, const RaSpan& s, bool packed) {
+  return (T*)v.p + (packed ? s.row0 * v.row : (int64_t)s.b * v.batch) + (int64_t)s.h * v.head;
+}
+// attended keys of chunk c, one bit each
+__device__ __forceinline__ uint64_t ra_word(const PdtRelAttn& p, const RaSpan& s, int c) {
+  const int left = s.n - c * RA_CHUNK;
+  if (left <= 0) return 0;
+  uint64_t w = left >= RA_CHUNK ? ~0ull : (1ull << left) - 1;
+  if (p.mask_bits) w &= ((const __attribute__((address_space(4))) uint64_t*)p.mask_bits)[(int64_t)s.b * p.mask_words + c];
+  return w;
+}
+// next chunk at or after c with an attended key
+__device__ __forceinline__ int ra_next(const PdtRelAttn& p, const RaSpan& s, int c, int nc, uint64_t& w) {
+  w = 0;
+  for (; c < nc; ++c)
+    if ((w = ra_word(p, s, c)) != 0) break;
+  return c;
+}
+
+// ---- the bias array: entry i of copy j is the bias (times log2 e) of distance sign * (i + j - off); `off` and the
+// clamp leave room so that a tile beyond the near distances reads the constant part.
+struct RaBias {
+  float* t;
+  int len, off, far;  // far: max_distance rounded up to the tile size
+};
+__device__ __forceinline__ int ra_far(int max_distance) { return (max_distance + 15) & ~15; }
+__host__ __device__ inline int ra_bias_len(int max_distance) {
+  const int n = 2 * ((max_distance + 15) & ~15) + 64 + 16;
+  return ((n + 63) & ~63) + 16;  // the copies start 64 bytes apart modulo the 256 bytes of one access
+}
+__device__ __forceinline__ int ra_bucket(const PdtRelAttn& p, int d) {
+  const int n = d < 0 ? -d : d, half = p.buckets >> 1, exact = half >> 1;
+  int b = n;
+  if (n >= exact) {
+    b = exact;
+    for (int j = 1; j < half - exact; ++j) b += n >= p.steps[j] ? 1 : 0;
+  }
+  return b + (d > 0 ? half : 0);
+}
+template <typename T>
+__device__ __forceinline__ float ra_table(const PdtRelAttn& p, int bucket, int h) {
+  const int64_t i = (int64_t)bucket * p.A + h;
+  return p.table_f32 ? ((const float*)p.table)[i] : Half16<T>::to_f(((const short*)p.table)[i]);
+}
+template <typename T>
+__device__ __forceinline__ RaBias ra_bias_fill(const PdtRelAttn& p, float* mem, int h, int sign, int tid) {
+  RaBias t{mem, ra_bias_len(p.max_distance), ra_far(p.max_distance) + 32, ra_far(p.max_distance)};
+  if (p.table) {
+    for (int i = tid; i < t.len + 4; i += RA_THREADS) {
+      const float v = ra_table<T>(p, ra_bucket(p, sign * (i - t.off)), h) * LOG2E;
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (i - j >= 0 && i - j < t.len) mem[j * t.len + i - j] = v;
+    }
+  }
+  return t;
+}
+// the lane's offset into the array: distances u + 4 g + r - lm (r = 0..3) of a tile u apart start at t[lane_off + u]
+__device__ __forceinline__ int ra_bias_lane(const RaBias& t, int lm, int g) {
+  const int j = -lm & 3;
+  return j * t.len + t.off + 4 * g - lm - j;
+}
+__device__ __forceinline__ float4v ra_bias4(const RaBias& t, int lane_off, int u) {
+  const int uc = min(max(u, -(t.far + 16)), t.far + 16);
+  return *reinterpret_cast<const float4v*>(t.t + lane_off + uc);
+}
+
+// ------------------------------------------------------------------------------------------------ forward
+// One wave = 16 QB query rows; online softmax in the log2 domain.
+template <typename T, int KS, int QB, bool DROP>
+__global__ __launch_bounds__(RA_THREADS) void rel_attn_fwd_kernel(PdtRelAttn p) {
+  constexpr int NH = (KS + 1) / 2, BUF = 2 * NH * RA_IMG;
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+  const int tid = threadIdx.x, lane = tid & 63, lm = lane & 15, g = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const RaSpan s = ra_span(p, blockIdx.x);
+  const int w0 = blockIdx.y * (RA_WAVES * 16 * QB), q0 = w0 + wave * 16 * QB;
+  if (w0 >= s.n) return;
+  const bool packed = p.cu != nullptr;
+  const T* qb_ = ra_base<const T>(p.q, s, packed);
+  const T* kb_ = ra_base<const T>(p.k, s, packed);
+  const T* vb_ = ra_base<const T>(p.v, s, packed);
+  const int nc = (s.n + RA_CHUNK - 1) / RA_CHUNK;
+  auto stage = [&](int c, int buf, uint64_t w) {
+    char* m = smem + buf * BUF;
+    ra_stage<T, NH>(m, kb_ + (int64_t)c * RA_CHUNK * p.k.row, (uint32_t)p.k.row, w, p.D, lane, wave);
+    ra_stage<T, NH>(m + NH * RA_IMG, vb_ + (int64_t)c * RA_CHUNK * p.v.row, (uint32_t)p.v.row, w, p.D, lane, wave);
+  };
+  uint64_t w;
+  int c = ra_next(p, s, 0, nc, w);
+  if (c < nc) stage(c, 0, w);
+  const RaBias bias = ra_bias_fill<T>(p, reinterpret_cast<float*>(smem + 2 * BUF), s.h, 1, tid);
+  const int boff = ra_bias_lane(bias, lm, g);
+  const bool has_bias = p.table != nullptr, active = q0 < s.n;
+  short8 qf[QB][KS];
+  uint32_t seed[QB];
+#pragma unroll
+  for (int i = 0; i < QB; ++i) {
+    const int q = q0 + 16 * i + lm;
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) qf[i][ks] = ra_gfrag<T>(qb_ + (int64_t)q * p.q.row, ks, p.D, lane, q < s.n);
+    seed[i] = DROP ? attn_row_seed(drop_key(p.rng), drop_sample(p.rng, s.b) * p.A + s.h, q) : 0u;
+  }
+  const float k2 = p.scale * LOG2E;
+  const uint32_t thr_hi = attn_thr_hi(p.drop_thr), kmul0 = (uint32_t)(4 * g) * ATT_GOLD;
+  float m[QB];
+  float4v l4[QB], o[QB][2 * KS];
+#pragma unroll
+  for (int i = 0; i < QB; ++i) {
+    m[i] = -INFINITY;
+    l4[i] = splat4(0.f);
+#pragma unroll
+    for (int db = 0; db < 2 * KS; ++db) o[i][db] = splat4(0.f);
+  }
+  for (int buf = 0; c < nc; buf ^= 1) {
+    uint64_t wn;
+    const int cn = ra_next(p, s, c + 1, nc, wn);
+    __syncthreads();  // every wave is done with the other buffer (first time: the bias array is complete)
+    if (cn < nc) {
+      stage(cn, buf ^ 1, wn);
+      if (NH == 1) asm volatile("s_waitcnt vmcnt(4)" ::: "memory");
+      else asm volatile("s_waitcnt vmcnt(8)" ::: "memory");
+    } else {
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    }
+    __syncthreads();
+    if (active) {
+      const char* kimg = smem + buf * BUF;
+      const char* vimg = kimg + NH * RA_IMG;
+      float4v sc[QB][4];
+#pragma unroll
+      for (int kb = 0; kb < 4; ++kb) {
+#pragma unroll
+        for (int i = 0; i < QB; ++i) sc[i][kb] = splat4(0.f);
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) {
+          const short8 kf = ra_row_frag(kimg, kb * 16, ks, lane);
+#pragma unroll
+          for (int i = 0; i < QB; ++i) sc[i][kb] = Half16<T>::mfma(kf, qf[i][ks], sc[i][kb]);
+        }
+      }
+      const bool whole = w == ~0ull;
+#pragma unroll
+      for (int i = 0; i < QB; ++i) {
+        float cmax = -INFINITY;
+#pragma unroll
+        for (int kb = 0; kb < 4; ++kb) {
+          float4v t = sc[i][kb] * k2;
+          if (has_bias) t += ra_bias4(bias, boff, c * RA_CHUNK + kb * 16 - (q0 + 16 * i));
+          if (!whole) {
+            const uint32_t bits = (uint32_t)(w >> (kb * 16 + 4 * g));
+#pragma unroll
+            for (int r = 0; r < 4; ++r) t[r] = (bits >> r) & 1 ? t[r] : -INFINITY;
+          }
+          cmax = fmaxf(fmaxf(cmax, t[0]), fmaxf(fmaxf(t[1], t[2]), t[3]));
+          sc[i][kb] = t;
+        }
+        cmax = quad_max(cmax);
+        const float m_new = fmaxf(m[i], cmax);
+        const float m_use = m_new == -INFINITY ? 0.f : m_new;  // no attended key so far: exp2(-inf - 0) = 0
+        const float alpha = __builtin_amdgcn_exp2f(m[i] - m_use);
+        m[i] = m_new;
+        l4[i] *= alpha;
+#pragma unroll
+        for (int db = 0; db < 2 * KS; ++db) o[i][db] *= alpha;
+#pragma unroll
+        for (int kb = 0; kb < 4; ++kb) {
+          float4v t = sc[i][kb] - m_use;
+#pragma unroll
+          for (int r = 0; r < 4; ++r) t[r] = __builtin_amdgcn_exp2f(t[r]);
+          l4[i] += t;
+          if (DROP) {
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+              t[r] *= attn_keep(seed[i], kmul0 + (uint32_t)(c * RA_CHUNK + kb * 16 + r) * ATT_GOLD, thr_hi) ? p.drop_scale : 0.f;
+          }
+          sc[i][kb] = t;
+        }
+      }
+#pragma unroll
+      for (int pb = 0; pb < 2; ++pb) {
+        short8 pf[QB];
+#pragma unroll
+        for (int i = 0; i < QB; ++i) pf[i] = pack_pair<T>(sc[i][2 * pb], sc[i][2 * pb + 1]);
+#pragma unroll
+        for (int db = 0; db < 2 * KS; ++db) {
+          const short8 vf = ra_tr_frag(vimg, pb * 32, db, lane);
+#pragma unroll
+          for (int i = 0; i < QB; ++i) o[i][db] = Half16<T>::mfma(vf, pf[i], o[i][db]);
+        }
+      }
+    }
+    c = cn;
+    w = wn;
+  }
+  if (!active) return;
+  T* ob = ra_base<T>(p.o, s, packed);
+#pragma unroll
+  for (int i = 0; i < QB; ++i) {
+    const int q = q0 + 16 * i + lm;
+    const float l = quad_sum((l4[i][0] + l4[i][1]) + (l4[i][2] + l4[i][3]));
+    // a row without an attended key has no probability mass: a zero output, and lse = +inf makes every p of backward 0
+    // (l is NaN, not 0, when a score was: the output is then NaN as well)
+    if (p.lse && g == 0 && q < s.n) p.lse[((int64_t)s.b * p.A + s.h) * p.S + q] = l == 0.f ? INFINITY : m[i] + __log2f(l);
+    ra_store<T, KS>(ob + (int64_t)q * p.o.row, o[i], l == 0.f ? 0.f : 1.0f / l, g, p.D, q < s.n);
+  }
+}
+
+// Sum of ds over the distances: tile t (lane (lm, g): keys 4 g + r, query lm) of blocks u apart, into diag[u + off + ...].
+// N: lane l holds the sum over r of the elements at (4 g + r, l + r), distance u + 4 g - l; W: those with l + r >= 16,
+// i.e. query l + r - 16, distance u + 4 g - l + 16 (lanes 13..15 only).  Lanes l in [4 i, 4 i + 4) of the four groups
+// write different distances, so the array needs one add per i for N and one for W, each to distinct addresses; adds of
+// one wave to its own array execute in order.
+__device__ __forceinline__ void ra_diag_add(float* diag, int at, const float4v& t, int lm, int g) {
+  float n = t[0];
+  n += dpp_f<0x101>(t[1]);  // row_shl:1
+  n += dpp_f<0x102>(t[2]);
+  n += dpp_f<0x103>(t[3]);
+  float w = dpp_f<0x11F>(t[1]);  // row_shr:15
+  w += dpp_f<0x11E>(t[2]);
+  w += dpp_f<0x11D>(t[3]);
+  float* d = diag + at + 4 * g - lm;
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    if ((lm >> 2) == i) atomicAdd(d, n);
+  if (lm >= 13) atomicAdd(d + 16, w);
+}
+
+// ------------------------------------------------------------------------------------------------ dQ and the table gradient
+// One wave = 16 QB query rows, sweeps the keys; also stores delta = rowsum(dO * O) for the dK / dV kernel.
+template <typename T, int KS, int QB, bool DROP>
+__global__ __launch_bounds__(RA_THREADS) void rel_attn_dq_kernel(PdtRelAttn p) {
+  constexpr int NH = (KS + 1) / 2, BUF = 2 * NH * RA_IMG;
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+  const int tid = threadIdx.x, lane = tid & 63, lm = lane & 15, g = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const RaSpan s = ra_span(p, blockIdx.x);
+  const int w0 = blockIdx.y * (RA_WAVES * 16 * QB), q0 = w0 + wave * 16 * QB;
+  float* part = p.dtable_part ? p.dtable_part + ((int64_t)s.b * gridDim.y + blockIdx.y) * p.buckets * p.A + s.h : nullptr;
+  if (w0 >= s.n) {
+    if (part)
+      for (int i = tid; i < p.buckets; i += RA_THREADS) part[(int64_t)i * p.A] = 0.f;
+    return;
+  }
+  const bool packed = p.cu != nullptr;
+  const T* qb_ = ra_base<const T>(p.q, s, packed);
+  const T* kb_ = ra_base<const T>(p.k, s, packed);
+  const T* vb_ = ra_base<const T>(p.v, s, packed);
+  const T* ob_ = ra_base<const T>(p.o, s, packed);
+  const T* gb_ = ra_base<const T>(p.dout, s, packed);
+  const int nc = (s.n + RA_CHUNK - 1) / RA_CHUNK;
+  auto stage = [&](int c, int buf, uint64_t w) {
+    char* m = smem + buf * BUF;
+    ra_stage<T, NH>(m, kb_ + (int64_t)c * RA_CHUNK * p.k.row, (uint32_t)p.k.row, w, p.D, lane, wave);
+    ra_stage<T, NH>(m + NH * RA_IMG, vb_ + (int64_t)c * RA_CHUNK * p.v.row, (uint32_t)p.v.row, w, p.D, lane, wave);
+  };
+  uint64_t w;
+  int c = ra_next(p, s, 0, nc, w);
+  if (c < nc) stage(c, 0, w);
+  const RaBias bias = ra_bias_fill<T>(p, reinterpret_cast<float*>(smem + 2 * BUF), s.h, 1, tid);
+  const int boff = ra_bias_lane(bias, lm, g);
+  const bool has_bias = p.table != nullptr, active = q0 < s.n;
+  // diagonal sums of this wave: index 0 is distance -(far + 31)
+  const int dlen = 2 * bias.far + 80;
+  float* diag = bias.t + 4 * bias.len + wave * dlen;
+  for (int i = lane; i < dlen; i += 64) diag[i] = 0.f;
+  short8 qf[QB][KS], df[QB][KS];
+  uint32_t seed[QB];
+  float nlse[QB], nd[QB];
+  const int64_t bh = (int64_t)s.b * p.A + s.h;
+#pragma unroll
+  for (int i = 0; i < QB; ++i) {
+    const int q = q0 + 16 * i + lm;
+    float d = 0.f;
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) {
+      qf[i][ks] = ra_gfrag<T>(qb_ + (int64_t)q * p.q.row, ks, p.D, lane, q < s.n);
+      df[i][ks] = ra_gfrag<T>(gb_ + (int64_t)q * p.dout.row, ks, p.D, lane, q < s.n);
+      const short8 of = ra_gfrag<T>(ob_ + (int64_t)q * p.o.row, ks, p.D, lane, q < s.n);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) d += Half16<T>::to_f(df[i][ks][j]) * Half16<T>::to_f(of[j]);
+    }
+    d = quad_sum(d);
+    if (g == 0 && q < s.n) p.delta[bh * p.S + q] = d;
+    nd[i] = -d;
+    nlse[i] = q < s.n ? -p.lse[bh * p.S + q] : -INFINITY;  // rows that are not there: p = 0
+    seed[i] = DROP ? attn_row_seed(drop_key(p.rng), drop_sample(p.rng, s.b) * p.A + s.h, q) : 0u;
+  }
+  const float k2 = p.scale * LOG2E;
+  const uint32_t thr_hi = attn_thr_hi(p.drop_thr), kmul0 = (uint32_t)(4 * g) * ATT_GOLD;
+  float4v dq[QB][2 * KS];
+#pragma unroll
+  for (int i = 0; i < QB; ++i)
+#pragma unroll
+    for (int db = 0; db < 2 * KS; ++db) dq[i][db] = splat4(0.f);
+  for (int buf = 0; c < nc; buf ^= 1) {
+    uint64_t wn;
+    const int cn = ra_next(p, s, c + 1, nc, wn);
+    __syncthreads();
+    if (cn < nc) {
+      stage(cn, buf ^ 1, wn);
+      if (NH == 1) asm volatile("s_waitcnt vmcnt(4)" ::: "memory");
+      else asm volatile("s_waitcnt vmcnt(8)" ::: "memory");
+    } else {
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    }
+    __syncthreads();
+    if (active) {
+      const char* kimg = smem + buf * BUF;
+      const char* vimg = kimg + NH * RA_IMG;
+      const bool whole = w == ~0ull;
+#pragma unroll
+      for (int pb = 0; pb < 2; ++pb) {
+        float4v ds[QB][2];
+#pragma unroll
+        for (int hb = 0; hb < 2; ++hb) {
+          const int kb = 2 * pb + hb;
+          float4v sc[QB], dp[QB];
+#pragma unroll
+          for (int i = 0; i < QB; ++i) { sc[i] = splat4(0.f); dp[i] = splat4(0.f); }
+#pragma unroll
+          for (int ks = 0; ks < KS; ++ks) {
+            const short8 kf = ra_row_frag(kimg, kb * 16, ks, lane), vf = ra_row_frag(vimg, kb * 16, ks, lane);
+#pragma unroll
+            for (int i = 0; i < QB; ++i) {
+              sc[i] = Half16<T>::mfma(kf, qf[i][ks], sc[i]);
+              dp[i] = Half16<T>::mfma(vf, df[i][ks], dp[i]);
+            }
+          }
+          const uint32_t bits = (uint32_t)(w >> (kb * 16 + 4 * g));
+#pragma unroll
+          for (int i = 0; i < QB; ++i) {
+            const int u = c * RA_CHUNK + kb * 16 - (q0 + 16 * i);
+            float4v t = sc[i] * k2 + nlse[i];
+            if (has_bias) t += ra_bias4(bias, boff, u);
+#pragma unroll
+            for (int r = 0; r < 4; ++r) t[r] = __builtin_amdgcn_exp2f(t[r]);
+            if (!whole) {
+#pragma unroll
+              for (int r = 0; r < 4; ++r) t[r] = (bits >> r) & 1 ? t[r] : 0.f;
+            }
+            float4v e = dp[i];
+            if (DROP) {
+#pragma unroll
+              for (int r = 0; r < 4; ++r)
+                e[r] *= attn_keep(seed[i], kmul0 + (uint32_t)(c * RA_CHUNK + kb * 16 + r) * ATT_GOLD, thr_hi) ? p.drop_scale : 0.f;
+            }
+            e = t * (e + nd[i]);
+            if (part) {
+              const int uc = min(max(u, -(bias.far + 16)), bias.far + 16);
+              ra_diag_add(diag, uc + bias.far + 31, e, lm, g);
+            }
+            ds[i][hb] = e;
+          }
+        }
+        short8 df_[QB];
+#pragma unroll
+        for (int i = 0; i < QB; ++i) df_[i] = pack_pair<T>(ds[i][0], ds[i][1]);
+#pragma unroll
+        for (int db = 0; db < 2 * KS; ++db) {
+          const short8 kf = ra_tr_frag(kimg, pb * 32, db, lane);
+#pragma unroll
+          for (int i = 0; i < QB; ++i) dq[i][db] = Half16<T>::mfma(kf, df_[i], dq[i][db]);
+        }
+      }
+    }
+    c = cn;
+    w = wn;
+  }
+  if (active) {
+    T* dqb = ra_base<T>(p.dq, s, packed);
+#pragma unroll
+    for (int i = 0; i < QB; ++i) {
+      const int q = q0 + 16 * i + lm;
+      ra_store<T, KS>(dqb + (int64_t)q * p.dq.row, dq[i], p.scale, g, p.D, q < s.n);
+    }
+  }
+  if (part) {  // distances -> buckets: eight lanes per bucket walk its range of distances over the four waves' arrays
+    __syncthreads();
+    const float* all = bias.t + 4 * bias.len;
+    const int half = p.buckets >> 1, exact = half >> 1, top = bias.far + 31;
+    for (int b0 = 0; b0 < p.buckets; b0 += RA_THREADS / 8) {
+      const int b = b0 + (tid >> 3), j = b >= half ? b - half : b;
+      float sum = 0.f;
+      if (b < p.buckets) {
+        int lo = j < exact ? j : p.steps[j - exact], hi = j < exact ? j : (j == half - 1 ? top : p.steps[j + 1 - exact] - 1);
+        if (j < exact && j == half - 1) hi = top;
+        if (b >= half) lo = max(lo, 1);
+        for (int n = lo + (tid & 7); n <= hi; n += 8) {
+          const int at = (b >= half ? n : -n) + top;
+          sum += (all[at] + all[dlen + at]) + (all[2 * dlen + at] + all[3 * dlen + at]);
+        }
+      }
+      sum += __shfl_xor(sum, 1, 64);
+      sum += __shfl_xor(sum, 2, 64);
+      sum += __shfl_xor(sum, 4, 64);
+      if (b < p.buckets && (tid & 7) == 0) part[(int64_t)b * p.A] = sum;
+    }
+  }
+}
+
+// ------------------------------------------------------------------------------------------------ dK, dV
+// One wave = 16 KB keys, sweeps the queries (Q and dO images); lse, delta and dropout seeds of a chunk's queries in LDS.
+template <typename T, int KS, int KB, bool DROP>
+__global__ __launch_bounds__(RA_THREADS) void rel_attn_dkv_kernel(PdtRelAttn p) {
+  constexpr int NH = (KS + 1) / 2, BUF = 2 * NH * RA_IMG + 1024;  // Q | dO | lse, delta, seeds (64 each), 256 spare bytes
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+  const int tid = threadIdx.x, lane = tid & 63, lm = lane & 15, g = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const RaSpan s = ra_span(p, blockIdx.x);
+  const int w0 = blockIdx.y * (RA_WAVES * 16 * KB), k0 = w0 + wave * 16 * KB;
+  if (w0 >= s.n) return;
+  const bool packed = p.cu != nullptr;
+  const T* qb_ = ra_base<const T>(p.q, s, packed);
+  const T* kb_ = ra_base<const T>(p.k, s, packed);
+  const T* vb_ = ra_base<const T>(p.v, s, packed);
+  const T* gb_ = ra_base<const T>(p.dout, s, packed);
+  const int64_t bh = (int64_t)s.b * p.A + s.h;
+  const int nc = (s.n + RA_CHUNK - 1) / RA_CHUNK;
+  const DropKey dkey = drop_key(p.rng);
+  const uint32_t sbh = drop_sample(p.rng, s.b) * p.A + s.h;
+  auto stage = [&](int c, int buf) {
+    char* m = smem + buf * BUF;
+    const int left = s.n - c * RA_CHUNK;
+    const uint64_t rows = left >= RA_CHUNK ? ~0ull : (1ull << left) - 1;
+    ra_stage<T, NH>(m, qb_ + (int64_t)c * RA_CHUNK * p.q.row, (uint32_t)p.q.row, rows, p.D, lane, wave);
+    ra_stage<T, NH>(m + NH * RA_IMG, gb_ + (int64_t)c * RA_CHUNK * p.dout.row, (uint32_t)p.dout.row, rows, p.D, lane, wave);
+    // lse (wave 0) and delta (wave 1) of the chunk; waves 2 and 3 read delta again into the spare bytes, so that every
+    // wave has the same number of transfers in flight.
+    const float* src = (wave == 0 ? p.lse : p.delta) + bh * p.S + (int64_t)c * RA_CHUNK;
+    const int slot = wave == 0 ? 0 : (wave == 1 ? 1 : 3);
+    pdt_lds_dma4(pdt_make_rsrc(src, 256u), m + 2 * NH * RA_IMG + slot * 256, lane < left ? lane * 4u : 0x80000000u);
+    if (DROP && tid < 64)
+      reinterpret_cast<uint32_t*>(m + 2 * NH * RA_IMG + 512)[tid] = attn_row_seed(dkey, sbh, c * RA_CHUNK + tid);
+  };
+  stage(0, 0);
+  const RaBias bias = ra_bias_fill<T>(p, reinterpret_cast<float*>(smem + 2 * BUF), s.h, -1, tid);
+  const int boff = ra_bias_lane(bias, lm, g);
+  const bool has_bias = p.table != nullptr;
+  short8 kf[KB][KS], vf[KB][KS];
+  bool kok[KB];
+  uint32_t kmul[KB];
+  const uint64_t kw = k0 < s.n ? ra_word(p, s, k0 / RA_CHUNK) >> (k0 % RA_CHUNK) : 0;
+  const bool active = (kw & (KB == 2 ? 0xFFFFFFFFull : 0xFFFFull)) != 0;  // (a wave's keys lie in one chunk)
+#pragma unroll
+  for (int i = 0; i < KB; ++i) {
+    const int key = k0 + 16 * i + lm;
+    kok[i] = (kw >> (16 * i + lm)) & 1;
+    kmul[i] = (uint32_t)key * ATT_GOLD;
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) {
+      kf[i][ks] = ra_gfrag<T>(kb_ + (int64_t)key * p.k.row, ks, p.D, lane, kok[i]);
+      vf[i][ks] = ra_gfrag<T>(vb_ + (int64_t)key * p.v.row, ks, p.D, lane, kok[i]);
+    }
+  }
+  const float k2 = p.scale * LOG2E;
+  const uint32_t thr_hi = attn_thr_hi(p.drop_thr);
+  float4v dk_[KB][2 * KS], dv_[KB][2 * KS];
+#pragma unroll
+  for (int i = 0; i < KB; ++i)
+#pragma unroll
+    for (int db = 0; db < 2 * KS; ++db) { dk_[i][db] = splat4(0.f); dv_[i][db] = splat4(0.f); }
+  for (int c = 0, buf = 0; c < nc; ++c, buf ^= 1) {
+    __syncthreads();
+    if (c + 1 < nc) {
+      stage(c + 1, buf ^ 1);
+      if (NH == 1) asm volatile("s_waitcnt vmcnt(5)" ::: "memory");
+      else asm volatile("s_waitcnt vmcnt(9)" ::: "memory");
+    } else {
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    }
+    __syncthreads();
+    if (!active) continue;
+    const char* qimg = smem + buf * BUF;
+    const char* gimg = qimg + NH * RA_IMG;
+    const float* sc_ = reinterpret_cast<const float*>(gimg + NH * RA_IMG);
+    const int left = s.n - c * RA_CHUNK;
+#pragma unroll
+    for (int pb = 0; pb < 2; ++pb) {
+      float4v pp[KB][2], ds[KB][2];
+#pragma unroll
+      for (int hb = 0; hb < 2; ++hb) {
+        const int qb = 2 * pb + hb;
+        float4v sc[KB], dp[KB];
+#pragma unroll
+        for (int i = 0; i < KB; ++i) { sc[i] = splat4(0.f); dp[i] = splat4(0.f); }
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) {
+          const short8 qf = ra_row_frag(qimg, qb * 16, ks, lane), gf = ra_row_frag(gimg, qb * 16, ks, lane);
+#pragma unroll
+          for (int i = 0; i < KB; ++i) {
+            sc[i] = Half16<T>::mfma(qf, kf[i][ks], sc[i]);
+            dp[i] = Half16<T>::mfma(gf, vf[i][ks], dp[i]);
+          }
+        }
+        const float4v lse = *reinterpret_cast<const float4v*>(sc_ + qb * 16 + 4 * g);
+        const float4v del = *reinterpret_cast<const float4v*>(sc_ + 64 + qb * 16 + 4 * g);
+        const uint4v sd = *reinterpret_cast<const uint4v*>(sc_ + 128 + qb * 16 + 4 * g);
+#pragma unroll
+        for (int i = 0; i < KB; ++i) {
+          float4v t = sc[i] * k2 - lse;
+          if (has_bias) t += ra_bias4(bias, boff, c * RA_CHUNK + qb * 16 - (k0 + 16 * i));
+          if (left < RA_CHUNK) {  // queries that are not there
+#pragma unroll
+            for (int r = 0; r < 4; ++r) t[r] = qb * 16 + 4 * g + r < left ? t[r] : -INFINITY;
+          }
+          float4v e = dp[i], pd;
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            t[r] = kok[i] ? __builtin_amdgcn_exp2f(t[r]) : 0.f;
+            const float keep = !DROP ? 1.f : (attn_keep(sd[r], kmul[i], thr_hi) ? p.drop_scale : 0.f);
+            pd[r] = DROP ? t[r] * keep : t[r];
+            if (DROP) e[r] *= keep;
+          }
+          pp[i][hb] = pd;
+          ds[i][hb] = t * (e - del);
+        }
+      }
+      short8 pf[KB], sf[KB];
+#pragma unroll
+      for (int i = 0; i < KB; ++i) { pf[i] = pack_pair<T>(pp[i][0], pp[i][1]); sf[i] = pack_pair<T>(ds[i][0], ds[i][1]); }
+#pragma unroll
+      for (int db = 0; db < 2 * KS; ++db) {
+        const short8 gf = ra_tr_frag(gimg, pb * 32, db, lane), qf = ra_tr_frag(qimg, pb * 32, db, lane);
+#pragma unroll
+        for (int i = 0; i < KB; ++i) {
+          dv_[i][db] = Half16<T>::mfma(gf, pf[i], dv_[i][db]);
+          dk_[i][db] = Half16<T>::mfma(qf, sf[i], dk_[i][db]);
+        }
+      }
+    }
+  }
+  T* dkb = ra_base<T>(p.dk, s, packed);
+  T* dvb = ra_base<T>(p.dv, s, packed);
+#pragma unroll
+  for (int i = 0; i < KB; ++i) {
+    const int key = k0 + 16 * i + lm;
+    ra_store<T, KS>(dkb + (int64_t)key * p.dk.row, dk_[i], p.scale, g, p.D, key < s.n);
+    ra_store<T, KS>(dvb + (int64_t)key * p.dv.row, dv_[i], 1.0f, g, p.D, key < s.n);
+  }
+}
+
+// ------------------------------------------------------------------------------------------------ helpers
+// key mask [B][S] (1 or 4 bytes per key, non-zero = attended) -> one bit per key; one wave per 64 keys
+__global__ __launch_bounds__(256) void rel_attn_mask_kernel(const void* mask, int bytes, int64_t stride, int S, int words,
+                                                            int total, uint64_t* bits) {
+  const int i = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
+  if (i >= total) return;
+  const int b = i / words, c = i - b * words, k = c * 64 + lane;
+  bool on = false;
+  if (k < S) {
+    const int64_t at = (int64_t)b * stride + k;
+    on = bytes == 1 ? ((const uint8_t*)mask)[at] != 0 : ((const int32_t*)mask)[at] != 0;
+  }
+  const uint64_t w = __ballot(on);
+  if (lane == 0) bits[i] = w;
+}
+
+// rows [cu[B], T) of a packed output: no sample owns them, they are zero
+template <typename T>
+__global__ __launch_bounds__(256) void rel_attn_tail_kernel(PdtRelView v, const int32_t* cu, int B, int T_, int A, int D) {
+  const int first = min(max(cu[B], 0), T_), per = A * (D >> 3);
+  const int64_t n = (int64_t)(T_ - first) * per;
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
+    const int r = (int)(i / per), rest = (int)(i - (int64_t)r * per), h = rest / (D >> 3), c = rest - h * (D >> 3);
+    *reinterpret_cast<int4v*>((T*)v.p + (int64_t)(first + r) * v.row + (int64_t)h * v.head + c * 8) = int4v{0, 0, 0, 0};
+  }
+}
+
+// more dynamic LDS than 64 KiB needs the attribute; set once per kernel and device (not a stream operation: done at the
+// first launch, i.e. in the warm-up of a step that is captured later)
+static int ra_allow_lds(const void* kern, size_t bytes) {
+  static std::mutex mu;
+  static std::unordered_set<const void*> done[64];
+  int dev = 0;
+  if (hipError_t e = hipGetDevice(&dev); e != hipSuccess) return (int)e;
+  std::lock_guard<std::mutex> lock(mu);
+  if (bytes > 160 * 1024 || dev < 0 || dev >= 64) return -3;
+  if (done[dev].count(kern)) return 0;
+  const hipError_t e = hipFuncSetAttribute(kern, hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024);
+  if (e != hipSuccess) return (int)e;
+  done[dev].insert(kern);
+  return 0;
+}
+
+constexpr int RA_QB = 1;  // 16-row blocks per wave
+
+static size_t ra_bias_bytes(const PdtRelAttn& p) { return (size_t)4 * ra_bias_len(p.max_distance) * sizeof(float); }
+
+template <typename KernT>
+static int ra_launch(KernT kern, const PdtRelAttn& p, int rows_per_block, size_t lds, hipStream_t stream) {
+  if (int e = ra_allow_lds((const void*)kern, lds)) return e;
+  hipLaunchKernelGGL(kern, dim3(p.B * p.A, (p.S + rows_per_block - 1) / rows_per_block), dim3(RA_THREADS), lds, stream, p);
+  return (int)hipGetLastError();
+}
+
+// which: 0 forward, 1 dQ + table gradient, 2 dK / dV
+template <typename T, int KS, bool DROP>
+static int ra_dispatch(int which, const PdtRelAttn& p, hipStream_t st) {
+  constexpr int NH = (KS + 1) / 2;
+  const int rows = RA_WAVES * 16 * RA_QB;
+  const size_t imgs = (size_t)4 * NH * RA_IMG, tab = ra_bias_bytes(p);
+  if (which == 0) return ra_launch(rel_attn_fwd_kernel<T, KS, RA_QB, DROP>, p, rows, imgs + tab, st);
+  if (which == 1) {
+    const size_t diag = (size_t)RA_WAVES * (2 * ((p.max_distance + 15) & ~15) + 80) * sizeof(float);
+    return ra_launch(rel_attn_dq_kernel<T, KS, RA_QB, DROP>, p, rows, imgs + tab + diag, st);
+  }
+  return ra_launch(rel_attn_dkv_kernel<T, KS, RA_QB, DROP>, p, rows, imgs + 2048 + tab, st);
+}
+template <typename T>
+static int ra_dispatch_ks(int which, const PdtRelAttn& p, hipStream_t st) {
+  const bool drop = p.drop_thr != 0;
+  switch ((p.D + 31) / 32) {
+    case 1: return drop ? ra_dispatch<T, 1, true>(which, p, st) : ra_dispatch<T, 1, false>(which, p, st);
+    case 2: return drop ? ra_dispatch<T, 2, true>(which, p, st) : ra_dispatch<T, 2, false>(which, p, st);
+    case 3: return drop ? ra_dispatch<T, 3, true>(which, p, st) : ra_dispatch<T, 3, false>(which, p, st);
+    case 4: return drop ? ra_dispatch<T, 4, true>(which, p, st) : ra_dispatch<T, 4, false>(which, p, st);
+  }
+  return -3;
+}
+static int ra_run(int dtype, int which, const PdtRelAttn& p, hipStream_t st) {
+  return dtype == PDT_F16 ? ra_dispatch_ks<_Float16>(which, p, st) : ra_dispatch_ks<__bf16>(which, p, st);
+}
+
+static int ra_check(int dtype, const PdtRelAttn& p) {
+  if (dtype != PDT_F16 && dtype != PDT_BF16) return -1;
+  if (p.B < 0 || p.S < 0 || p.A <= 0 || p.D <= 0 || p.D > 128 || p.D % 8) return -3;
+  if ((int64_t)p.B * p.A > 0x7FFFFFFF || (p.S + RA_CHUNK - 1) / RA_CHUNK > 65535) return -3;
+  const PdtRelView* views[9] = {&p.q, &p.k, &p.v, &p.o, &p.dout, &p.dq, &p.dk, &p.dv, nullptr};
+  for (int i = 0; views[i]; ++i)  // 16-byte rows, and 64 rows within the 31-bit window of a transfer
+    if (views[i]->p && (views[i]->row % 8 || views[i]->head % 8 || views[i]->batch % 8 || views[i]->row < 0 ||
+                        views[i]->row > (1 << 23) || (uintptr_t)views[i]->p % 16))
+      return -4;
+  if (!p.q.p || !p.k.p || !p.v.p || !p.o.p) return -2;
+  if (p.table && (p.buckets < 4 || p.buckets % 2 || p.buckets > 4 * RA_MAX_STEPS || p.max_distance <= p.buckets / 4 ||
+                  p.max_distance > RA_MAX_FAR))
+    return -5;
+  if (!p.table && p.max_distance != 0) return -5;
+  return 0;
+}
+
+static int ra_tail(int dtype, const PdtRelView& v, const PdtRelAttn& p, hipStream_t st) {
+  if (!p.cu) return 0;
+  if (dtype == PDT_F16) hipLaunchKernelGGL(rel_attn_tail_kernel<_Float16>, dim3(64), dim3(256), 0, st, v, p.cu, p.B, p.T, p.A, p.D);
+  else hipLaunchKernelGGL(rel_attn_tail_kernel<__bf16>, dim3(64), dim3(256), 0, st, v, p.cu, p.B, p.T, p.A, p.D);
+  return (int)hipGetLastError();
+}
+
+}  // namespace pdt
+
+using namespace pdt;
+
+extern "C" int pdt_rel_attn_mask(const void* mask, int bytes, int64_t stride, int B, int S, uint64_t* bits, void* stream) {
+  if (!mask || !bits || (bytes != 1 && bytes != 4) || B < 0 || S < 0) return -1;
+  const int words = (S + 63) / 64;
+  const int64_t total = (int64_t)B * words;
+  if (total == 0) return 0;
+  if (total > 0x7FFFFFFF) return -3;
+  hipLaunchKernelGGL(rel_attn_mask_kernel, dim3((unsigned)((total + 3) / 4)), dim3(256), 0, (hipStream_t)stream, mask, bytes,
+                     stride, S, words, (int)total, bits);
+  return (int)hipGetLastError();
+}
+
+extern "C" int pdt_rel_attn_fwd(int dtype, const PdtRelAttn* a, void* stream) {
+  if (int e = ra_check(dtype, *a)) return e;
+  hipStream_t st = (hipStream_t)stream;
+  if (int e = ra_tail(dtype, a->o, *a, st)) return e;
+  if (a->B == 0 || a->S == 0) return 0;
+  return ra_run(dtype, 0, *a, st);
+}
+
+extern "C" int pdt_rel_attn_dtable_rows(const PdtRelAttn* a) {
+  const int rows = RA_WAVES * 16 * RA_QB;
+  return a->B * ((a->S + rows - 1) / rows);
+}
+
+extern "C" int pdt_rel_attn_bwd(int dtype, const PdtRelAttn* a, void* stream) {
+  if (int e = ra_check(dtype, *a)) return e;
+  if (!a->dout.p || !a->dq.p || !a->dk.p || !a->dv.p) return -2;
+  if (a->B > 0 && a->S > 0 && (!a->lse || !a->delta)) return -2;
+  if (a->dtable_part && !a->table) return -2;
+  hipStream_t st = (hipStream_t)stream;
+  const PdtRelView* outs[3] = {&a->dq, &a->dk, &a->dv};
+  for (const PdtRelView* v : outs)
+    if (int e = ra_tail(dtype, *v, *a, st)) return e;
+  if (a->B == 0 || a->S == 0) return 0;
+  if (int e = ra_run(dtype, 1, *a, st)) return e;
+  return ra_run(dtype, 2, *a, st);
+}

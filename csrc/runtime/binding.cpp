@@ -378,6 +378,287 @@ Tensor ln_fwd(const Tensor& x, const Tensor& gamma, const Tensor& beta, Tensor& 
 }
 
 // ---------------------------------------------------------------------------------------------------
+// Attention with a relative position bias, and the per-head norm + rotation of queries and keys
+// ---------------------------------------------------------------------------------------------------
+// [B, S, A, D] (or packed [T, A, D]) as the kernels address it; a tensor whose rows they cannot (inner stride other than 1,
+// rows off the 16-byte grid, rows too far apart) is copied.
+Tensor head_rows(const Tensor& t, const char* name) {
+  TORCH_CHECK(t.is_cuda(), name, " must be on the GPU");
+  TORCH_CHECK(t.scalar_type() == at::kHalf || t.scalar_type() == at::kBFloat16, name, " must be 16-bit float");
+  bool ok = (reinterpret_cast<uintptr_t>(t.data_ptr()) & 15) == 0 && (t.size(-1) == 1 || t.stride(-1) == 1);
+  for (int64_t i = 0; i + 1 < t.dim(); ++i)
+    ok = ok && (t.size(i) <= 1 || (t.stride(i) % 8 == 0 && t.stride(i) >= 0 && (i != t.dim() - 3 || t.stride(i) <= (1 << 23))));
+  return ok ? t : t.clone(at::MemoryFormat::Contiguous);
+}
+PdtRelView rel_view(const Tensor& t) {
+  const int64_t d = t.dim();
+  auto st = [&](int64_t i) { return t.size(i) <= 1 ? (int64_t)0 : t.stride(i); };
+  return PdtRelView{t.data_ptr(), d == 4 ? st(0) : 0, st(d - 3), st(d - 2)};
+}
+void same_gpu(const Tensor& t, const Tensor& as, const char* name) {
+  TORCH_CHECK(t.device() == as.device(), name, " must be on the device of q");
+}
+
+// What the three kernels of one call share.  q, k, v come from head_rows().
+struct RelCall {
+  const OptTensor &table, &bits, &cu;
+  const std::vector<int64_t>& steps;
+  int64_t max_distance, S;
+  double scale, p;
+};
+PdtRelAttn rel_args(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& o, const RelCall& c, const PdtRng& rng) {
+  const bool packed = c.cu.has_value();
+  TORCH_CHECK(q.dim() == (packed ? 3 : 4), "q must be ", packed ? "[T, heads, dim] with cu_seqlens" : "[B, S, heads, dim]");
+  TORCH_CHECK(k.sizes() == q.sizes() && v.sizes() == q.sizes(), "q, k and v must have one shape (as many key and value heads as query heads)");
+  TORCH_CHECK(k.scalar_type() == q.scalar_type() && v.scalar_type() == q.scalar_type(), "q, k and v must have one dtype");
+  same_gpu(k, q, "k"); same_gpu(v, q, "v");
+  const int64_t D = q.size(-1), A = q.size(-2);
+  TORCH_CHECK(D >= 8 && D <= 128 && D % 8 == 0, "the head dim must be a multiple of 8, at most 128 (got ", D, ")");
+  TORCH_CHECK(A >= 1, "at least one head");
+  PdtRelAttn a{};
+  if (packed) {
+    TORCH_CHECK(c.cu->scalar_type() == at::kInt && c.cu->is_contiguous() && c.cu->dim() == 1 && c.cu->numel() >= 1,
+                "cu_seqlens must be a contiguous int32 [B + 1] tensor");
+    same_gpu(*c.cu, q, "cu_seqlens");
+    TORCH_CHECK(!c.bits.has_value(), "packed rows take no key mask");
+    TORCH_CHECK(q.size(0) <= 0x7FFFFFFF && c.S >= 0 && c.S <= 0x7FFFFFFF, "too many rows");
+    TORCH_CHECK(c.S >= 1 || q.size(0) == 0 || c.cu->numel() == 1, "max_seqlen must be at least the longest sequence");
+    a.cu = c.cu->data_ptr<int32_t>();
+    a.B = (int)c.cu->numel() - 1;
+    a.S = (int)std::min<int64_t>(c.S, q.size(0));
+    a.T = (int)q.size(0);
+  } else {
+    a.B = (int)q.size(0); a.S = (int)q.size(1);
+    if (c.bits.has_value()) {
+      TORCH_CHECK(c.bits->scalar_type() == at::kLong && c.bits->is_contiguous() && c.bits->dim() == 2 &&
+                  c.bits->size(0) == a.B && c.bits->size(1) == (a.S + 63) / 64, "mask bits must be int64 [B, ceil(S / 64)]");
+      same_gpu(*c.bits, q, "mask bits");
+      a.mask_bits = reinterpret_cast<const uint64_t*>(c.bits->data_ptr<int64_t>());
+      a.mask_words = (int)c.bits->size(1);
+    }
+  }
+  a.A = (int)A; a.D = (int)D;
+  a.q = rel_view(q); a.k = rel_view(k); a.v = rel_view(v); a.o = rel_view(o);
+  if (c.table.has_value()) {
+    const Tensor& t = *c.table;
+    same_gpu(t, q, "the bias table");
+    TORCH_CHECK(t.dim() == 2 && t.size(1) == A && t.is_contiguous(), "the bias table must be a contiguous [buckets, heads] tensor");
+    TORCH_CHECK(t.scalar_type() == at::kFloat || t.scalar_type() == q.scalar_type(), "the bias table must be fp32 or of q's dtype");
+    const int64_t half = t.size(0) / 2;
+    TORCH_CHECK((int64_t)c.steps.size() == half - half / 2 && c.steps.size() <= 32, "one step per logarithmic bucket");
+    a.table = t.data_ptr();
+    a.table_f32 = t.scalar_type() == at::kFloat;
+    a.buckets = (int)t.size(0);
+    a.max_distance = (int)c.max_distance;
+    for (size_t i = 0; i < c.steps.size(); ++i) {
+      TORCH_CHECK(c.steps[i] >= (i ? c.steps[i - 1] : half / 2) && c.steps[i] <= c.max_distance, "steps must ascend up to max_distance");
+      a.steps[i] = (int)c.steps[i];
+    }
+  }
+  a.scale = (float)c.scale;
+  a.drop_thr = thr16(c.p);
+  a.drop_scale = keep_scale(c.p);
+  a.rng = rng;
+  return a;
+}
+// key mask [B, S] (bool, uint8 or int32; non-zero = attended) -> one bit per key, int64 [B, ceil(S / 64)]
+Tensor rel_mask_bits(const Tensor& mask) {
+  TORCH_CHECK(mask.is_cuda() && mask.dim() == 2, "the key mask must be a [B, S] GPU tensor");
+  DeviceGuard guard(mask.device());
+  const auto st = mask.scalar_type();
+  TORCH_CHECK(st == at::kBool || st == at::kByte || st == at::kInt, "the key mask must be bool, uint8 or int32 (non-zero = attended), got ", st);
+  const int64_t B = mask.size(0), S = mask.size(1);
+  TORCH_CHECK(B <= 0x7FFFFFFF && S <= 0x7FFFFFFF, "the key mask is too large");
+  const Tensor m = S <= 1 || mask.stride(1) == 1 ? mask : mask.contiguous();
+  Tensor bits = at::empty({B, (S + 63) / 64}, mask.options().dtype(at::kLong));
+  if (bits.numel())
+    check(pdt_rel_attn_mask(m.data_ptr(), st == at::kInt ? 4 : 1, B <= 1 ? 0 : m.stride(0), (int)B, (int)S,
+                            reinterpret_cast<uint64_t*>(bits.data_ptr<int64_t>()), cur_stream()), "rel_attn_mask");
+  return bits;
+}
+PdtRng rel_rng(const OptTensor& state, double p, int64_t micro, int64_t site, const OptTensor& sids, int64_t B) {
+  if (p <= 0.0 || !state.has_value()) {
+    TORCH_CHECK(p <= 0.0, "dropout needs a generator state");
+    return PdtRng{nullptr, 0, 0, nullptr, 1u, 0u, nullptr};
+  }
+  TORCH_CHECK(p < 1.0, "the dropout probability must be below 1");
+  // (the masks derive from (sample, head, query, key): the sequence length plays no part)
+  return make_rng(*state, micro, site, sids, 1, B);
+}
+// -> o, lse (lse only when wanted)
+std::vector<Tensor> rel_attn_forward(const Tensor& q_in, const Tensor& k_in, const Tensor& v_in, const OptTensor& table,
+                                     int64_t max_distance, const std::vector<int64_t>& steps, const OptTensor& bits,
+                                     const OptTensor& cu, int64_t max_seqlen, double scale, const OptTensor& rng_state,
+                                     double p, int64_t micro, int64_t site, const OptTensor& sids, bool want_lse) {
+  TORCH_CHECK(q_in.is_cuda(), "q must be on the GPU");
+  DeviceGuard guard(q_in.device());
+  const Tensor q = head_rows(q_in, "q"), k = head_rows(k_in, "k"), v = head_rows(v_in, "v");
+  Tensor o = at::empty(q.sizes(), q.options());
+  const RelCall c{table, bits, cu, steps, max_distance, max_seqlen, scale, p};
+  PdtRelAttn a = rel_args(q, k, v, o, c, PdtRng{});
+  a.rng = rel_rng(rng_state, p, micro, site, sids, a.B);
+  if (q.numel() == 0) return {o, want_lse ? at::empty({a.B, a.A, a.S}, q.options().dtype(at::kFloat)) : Tensor()};
+  Tensor lse;
+  if (want_lse) {
+    lse = at::empty({a.B, a.A, a.S}, q.options().dtype(at::kFloat));
+    a.lse = lse.data_ptr<float>();
+  }
+  check(pdt_rel_attn_fwd(dt_code(q), &a, cur_stream()), "rel_attn_fwd");
+  return {o, lse};
+}
+// dq, dk, dv into the given tensors; the table gradient (fp32 [buckets, A]) into `dtable` (+= when accumulate)
+void rel_attn_backward_into(const Tensor& dout_in, const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& o,
+                            const Tensor& lse, const RelCall& c, const PdtRng& rng, Tensor dq, Tensor dk, Tensor dv,
+                            float* dtable, bool accumulate) {
+  PdtRelAttn a = rel_args(q, k, v, o, c, rng);
+  const Tensor dout = head_rows(dout_in, "dout");
+  TORCH_CHECK(dout.sizes() == q.sizes() && dout.scalar_type() == q.scalar_type(), "dout must have q's shape and dtype");
+  chkf32(lse, "lse");
+  TORCH_CHECK(lse.dim() == 3 && lse.size(0) == a.B && lse.size(1) == a.A && lse.size(2) == a.S, "lse must be [B, heads, S]");
+  Tensor delta = at::empty_like(lse), part;
+  a.dout = rel_view(dout); a.dq = rel_view(dq); a.dk = rel_view(dk); a.dv = rel_view(dv);
+  a.lse = lse.data_ptr<float>(); a.delta = delta.data_ptr<float>();
+  const int rows = pdt_rel_attn_dtable_rows(&a);
+  if (dtable) {
+    part = at::empty({rows, (int64_t)a.buckets * a.A}, lse.options());
+    a.dtable_part = part.data_ptr<float>();
+  }
+  check(pdt_rel_attn_bwd(dt_code(q), &a, cur_stream()), "rel_attn_bwd");
+  if (dtable)
+    check(pdt_colsum_finish(a.dtable_part, rows, a.buckets * a.A, 1, dtable, nullptr, nullptr, nullptr, accumulate ? 1 : 0,
+                            cur_stream()), "colsum_finish");
+}
+std::vector<Tensor> rel_attn_backward(const Tensor& dout, const Tensor& q_in, const Tensor& k_in, const Tensor& v_in, const Tensor& o,
+                                      const Tensor& lse, const OptTensor& table, int64_t max_distance,
+                                      const std::vector<int64_t>& steps, const OptTensor& bits, const OptTensor& cu,
+                                      int64_t max_seqlen, double scale, const OptTensor& rng_state, double p, int64_t micro,
+                                      int64_t site, const OptTensor& sids, bool want_dtable) {
+  TORCH_CHECK(q_in.is_cuda(), "q must be on the GPU");
+  DeviceGuard guard(q_in.device());
+  const Tensor q = head_rows(q_in, "q"), k = head_rows(k_in, "k"), v = head_rows(v_in, "v");
+  Tensor dq = at::empty(q.sizes(), q.options()), dk = at::empty(q.sizes(), q.options()), dv = at::empty(q.sizes(), q.options());
+  Tensor dtable;
+  want_dtable = want_dtable && table.has_value();
+  if (q.numel() == 0) {
+    if (want_dtable) dtable = at::zeros(table->sizes(), q.options().dtype(at::kFloat));
+    return {dq, dk, dv, dtable};
+  }
+  if (want_dtable) dtable = at::empty(table->sizes(), q.options().dtype(at::kFloat));
+  const RelCall c{table, bits, cu, steps, max_distance, max_seqlen, scale, p};
+  rel_attn_backward_into(dout, q, k, v, o, lse, c, rel_rng(rng_state, p, micro, site, sids, lse.size(0)), dq, dk, dv,
+                         want_dtable ? dtable.data_ptr<float>() : nullptr, false);
+  return {dq, dk, dv, dtable};
+}
+
+// ---- per-head norm + rotation
+struct RopeCall {
+  const OptTensor &wq, &wk, &cos, &sin, &pos;
+  bool interleaved;
+  double eps;
+};
+PdtQkRope rope_args(const Tensor& q, const Tensor& k, const RopeCall& c) {
+  TORCH_CHECK(q.dim() == 3 || q.dim() == 4, "q must be [T, heads, dim] or [B, S, heads, dim]");
+  TORCH_CHECK(k.dim() == q.dim() && k.size(0) == q.size(0) && k.size(-1) == q.size(-1) && (q.dim() == 3 || k.size(1) == q.size(1)),
+              "q and k must agree in everything but the number of heads");
+  TORCH_CHECK(k.scalar_type() == q.scalar_type(), "q and k must have one dtype");
+  same_gpu(k, q, "k");
+  const int64_t D = q.size(-1);
+  TORCH_CHECK(D >= 8 && D <= 256 && D % 8 == 0, "the head dim must be a multiple of 8, at most 256 (got ", D, ")");
+  PdtQkRope a{};
+  const int64_t T = q.dim() == 4 ? q.size(0) * q.size(1) : q.size(0);
+  TORCH_CHECK(T <= (1 << 30), "too many tokens");
+  a.T = (int)T;
+  a.seq = (int)std::max<int64_t>(1, q.dim() == 4 ? q.size(1) : q.size(0));
+  a.D = (int)D;
+  a.heads[0] = (int)q.size(-2); a.heads[1] = (int)k.size(-2);
+  a.x[0] = rel_view(q); a.x[1] = rel_view(k);
+  a.interleaved = c.interleaved;
+  a.eps = (float)c.eps;
+  const OptTensor* ws[2] = {&c.wq, &c.wk};
+  TORCH_CHECK(c.wq.has_value() == c.wk.has_value(), "give both norm weights or neither");
+  for (int i = 0; i < 2; ++i) {
+    if (!ws[i]->has_value()) continue;
+    const Tensor& w = **ws[i];
+    same_gpu(w, q, "the norm weights");
+    TORCH_CHECK(w.dim() == 1 && w.size(0) == D && w.is_contiguous(), "a norm weight must be a contiguous [dim] tensor");
+    TORCH_CHECK(w.scalar_type() == at::kFloat || w.scalar_type() == q.scalar_type(), "norm weights must be fp32 or of q's dtype");
+    TORCH_CHECK(w.scalar_type() == c.wq->scalar_type(), "the norm weights must have one dtype");
+    TORCH_CHECK((reinterpret_cast<uintptr_t>(w.data_ptr()) & 15) == 0, "norm weights must be 16-byte aligned");
+    a.w[i] = w.data_ptr();
+    a.w_f32 = w.scalar_type() == at::kFloat;
+  }
+  TORCH_CHECK(!c.wq.has_value() || c.eps > 0.0, "eps must be positive");
+  TORCH_CHECK(c.cos.has_value() == c.sin.has_value(), "give cosines and sines");
+  if (c.cos.has_value()) {
+    chkf32(*c.cos, "cos"); chkf32(*c.sin, "sin");
+    same_gpu(*c.cos, q, "cos"); same_gpu(*c.sin, q, "sin");
+    TORCH_CHECK(c.cos->dim() == 2 && c.cos->sizes() == c.sin->sizes() && c.cos->size(0) >= 1, "cos and sin must be [positions, rotated / 2]");
+    const int64_t R = 2 * c.cos->size(1);
+    TORCH_CHECK(R >= 8 && R <= D && R % (c.interleaved ? 8 : 16) == 0, "the rotated part must be a multiple of ", c.interleaved ? 8 : 16,
+                " elements, at most the head dim (got ", R, " of ", D, ")");
+    TORCH_CHECK((reinterpret_cast<uintptr_t>(c.cos->data_ptr()) & 15) == 0 && (reinterpret_cast<uintptr_t>(c.sin->data_ptr()) & 15) == 0,
+                "cos and sin must be 16-byte aligned");
+    a.cos = c.cos->data_ptr<float>(); a.sin = c.sin->data_ptr<float>();
+    a.R = (int)R;
+    a.P = (int)std::min<int64_t>(c.cos->size(0), 0x7FFFFFFF);
+    if (c.pos.has_value()) {
+      same_gpu(*c.pos, q, "positions");
+      TORCH_CHECK(c.pos->scalar_type() == at::kLong && c.pos->is_contiguous() && c.pos->numel() == T, "positions must be a contiguous int64 tensor, one per token");
+      a.pos = c.pos->data_ptr<int64_t>();
+    } else {
+      TORCH_CHECK(a.seq <= c.cos->size(0) || T == 0, "cos and sin have ", c.cos->size(0), " positions, the sequence ", a.seq);
+    }
+  }
+  return a;
+}
+void rope_forward_into(const Tensor& q, const Tensor& k, const RopeCall& c, Tensor yq, Tensor yk) {
+  PdtQkRope a = rope_args(q, k, c);
+  a.y[0] = rel_view(yq); a.y[1] = rel_view(yk);
+  check(pdt_qk_rope_fwd(dt_code(q), &a, cur_stream()), "qk_rope_fwd");
+}
+// dxq, dxk into the given tensors; weight gradients (fp32 [D]) into dwq / dwk (+= when accumulate) unless null
+void rope_backward_into(const Tensor& dyq_in, const Tensor& dyk_in, const Tensor& q, const Tensor& k, const RopeCall& c, Tensor dxq,
+                        Tensor dxk, float* dwq, float* dwk, bool accumulate) {
+  PdtQkRope a = rope_args(q, k, c);
+  const Tensor dyq = head_rows(dyq_in, "dq"), dyk = head_rows(dyk_in, "dk");
+  TORCH_CHECK(dyq.sizes() == q.sizes() && dyk.sizes() == k.sizes() && dyq.scalar_type() == q.scalar_type() &&
+              dyk.scalar_type() == q.scalar_type(), "gradients must have the shape and dtype of q and k");
+  a.y[0] = rel_view(dyq); a.y[1] = rel_view(dyk);
+  a.dx[0] = rel_view(dxq); a.dx[1] = rel_view(dxk);
+  Tensor part;
+  const int blocks = pdt_qk_rope_bwd_blocks(&a);
+  if (dwq || dwk) part = at::empty({blocks, 2 * (int64_t)a.D}, q.options().dtype(at::kFloat));
+  check(pdt_qk_rope_bwd(dt_code(q), &a, part.defined() ? part.data_ptr<float>() : nullptr, cur_stream()), "qk_rope_bwd");
+  if (part.defined())
+    check(pdt_colsum_finish(part.data_ptr<float>(), blocks, a.D, 2, dwq, dwk, nullptr, nullptr, accumulate ? 1 : 0, cur_stream()),
+          "colsum_finish");
+}
+std::vector<Tensor> qk_rope_forward(const Tensor& q_in, const Tensor& k_in, const OptTensor& wq, const OptTensor& wk,
+                                    const OptTensor& cos, const OptTensor& sin, const OptTensor& pos, bool interleaved, double eps) {
+  TORCH_CHECK(q_in.is_cuda(), "q must be on the GPU");
+  DeviceGuard guard(q_in.device());
+  const Tensor q = head_rows(q_in, "q"), k = head_rows(k_in, "k");
+  Tensor yq = at::empty(q.sizes(), q.options()), yk = at::empty(k.sizes(), k.options());
+  rope_forward_into(q, k, RopeCall{wq, wk, cos, sin, pos, interleaved, eps}, yq, yk);
+  return {yq, yk};
+}
+std::vector<Tensor> qk_rope_backward(const Tensor& dyq, const Tensor& dyk, const Tensor& q_in, const Tensor& k_in, const OptTensor& wq,
+                                     const OptTensor& wk, const OptTensor& cos, const OptTensor& sin, const OptTensor& pos,
+                                     bool interleaved, double eps, bool want_dw) {
+  TORCH_CHECK(q_in.is_cuda(), "q must be on the GPU");
+  DeviceGuard guard(q_in.device());
+  const Tensor q = head_rows(q_in, "q"), k = head_rows(k_in, "k");
+  Tensor dxq = at::empty(q.sizes(), q.options()), dxk = at::empty(k.sizes(), k.options()), dwq, dwk;
+  if (want_dw && wq.has_value()) {
+    dwq = at::empty({q.size(-1)}, q.options().dtype(at::kFloat));
+    dwk = at::empty({q.size(-1)}, q.options().dtype(at::kFloat));
+  }
+  rope_backward_into(dyq, dyk, q, k, RopeCall{wq, wk, cos, sin, pos, interleaved, eps}, dxq, dxk,
+                     dwq.defined() ? dwq.data_ptr<float>() : nullptr, dwk.defined() ? dwk.data_ptr<float>() : nullptr, false);
+  return {dxq, dxk, dwq, dwk};
+}
+
+// ---------------------------------------------------------------------------------------------------
 // Encoder layer.  Weight list order (16-bit compute copies):
 //   0 wqkv[3H,H] 1 bqkv[3H] 2 wo[H,H] 3 bo[H] 4 ln1_g 5 ln1_b 6 w1[F,H] 7 b1[F] 8 w2[H,F] 9 b2[H] 10 ln2_g 11 ln2_b
 // Gradient list: the same order, fp32 views of the gradient arena.
@@ -846,6 +1127,11 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("head_forward", &head_forward, nogil());
   m.def("head_backward", &head_backward, nogil());
   m.def("dropout16", &dropout16);
+  m.def("rel_mask_bits", &rel_mask_bits);
+  m.def("rel_attn_forward", &rel_attn_forward, nogil());
+  m.def("rel_attn_backward", &rel_attn_backward, nogil());
+  m.def("qk_rope_forward", &qk_rope_forward, nogil());
+  m.def("qk_rope_backward", &qk_rope_backward, nogil());
   m.def("adamw_step", &adamw_step);
   m.def("grad_check", &grad_check);
   m.def("scaler_update", &scaler_update);

@@ -48,3 +48,7 @@ def native():
             "Build it with `python build_ext.py` (hipcc --offload-arch=gfx950)."
         )
     return _C
+
+
+from .attention import bucket_steps, relative_attention, relative_bucket  # noqa: E402,F401
+from .rotary import qk_norm_rope, rotary_table  # noqa: E402,F401
