@@ -48,7 +48,7 @@ def direct():
         h = x
         t0 = time.perf_counter()
         for i, l in enumerate(layers):
-            outs = C.layer_forward(h, mask, kvl, l._native.w, state, B, S, A, 0.1, 0.1, 1e-12, 1, i, None, None, None)
+            outs = C.layer_forward(h, mask, kvl, l._native.w, state, B, S, A, 0.1, 0.1, 1e-12, 1, i, None, None, None, None, None, None)
             saved.append((h, outs[1:]))
             h = outs[0]
         t1 = time.perf_counter()
@@ -57,7 +57,7 @@ def direct():
             l = layers[i]
             hin, sv = saved[i]
             dy = C.layer_backward(dy, hin, list(sv), mask, kvl, l._native.w, l._native.g, state, B, S, A, 0.1, 0.1, 1, i,
-                                  True, None, None, None)
+                                  True, None, None, None, None, None, None)
         t2 = time.perf_counter()
         tf += t1 - t0
         tb += t2 - t1

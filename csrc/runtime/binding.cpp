@@ -662,14 +662,76 @@ std::vector<Tensor> qk_rope_backward(const Tensor& dyq, const Tensor& dyk, const
 // Encoder layer.  Weight list order (16-bit compute copies):
 //   0 wqkv[3H,H] 1 bqkv[3H] 2 wo[H,H] 3 bo[H] 4 ln1_g 5 ln1_b 6 w1[F,H] 7 b1[F] 8 w2[H,F] 9 b2[H] 10 ln2_g 11 ln2_b
 // Gradient list: the same order, fp32 views of the gradient arena.
-// Saved list: 0 qkv 1 ctx 2 lse 3 z1 4 stats1 5 x1 6 u 7 gact 8 z2 9 stats2
+// Saved list: 0 qkv 1 ctx 2 lse 3 z1 4 stats1 5 x1 6 u 7 gact 8 z2 9 stats2 (10 normalised / rotated queries and keys
+// [T, 2, A, 64] of a layer with such a position option)
 // ---------------------------------------------------------------------------------------------------
+// What a layer's attention does with positions: a bias table and / or a norm and rotation of its queries and keys.  The
+// gradients of `table`, `wq`, `wk` (those that are there) follow the twelve of the gradient list, in this order.
+struct LayerPosition {
+  OptTensor table, wq, wk, cos, sin;
+  int64_t max_distance = 0;
+  std::vector<int64_t> steps;
+  double eps = 1e-6;
+  bool turns() const { return wq.has_value() || cos.has_value(); }
+};
+using LayerPositionPtr = std::shared_ptr<LayerPosition>;
+
+// thirds of a fused projection [T, 3H] as [B, S, A, 64] (padded) or [T, A, 64] (packed)
+Tensor head_third(const Tensor& qkv, int i, int64_t B, int64_t S, int64_t A, bool packed) {
+  const Tensor t = qkv.view({qkv.size(0), qkv.size(1) / (A * 64), A, 64}).select(1, i);
+  return packed ? t : t.view({B, S, A, 64});
+}
+Tensor head_view(const Tensor& x, int64_t B, int64_t S, int64_t A, bool packed) {
+  return packed ? x.view({x.size(0), A, 64}) : x.view({B, S, A, 64});
+}
+// attention of a layer with position options: ctx and lse are filled; returns the normalised / rotated queries and keys
+Tensor position_attention_forward(const LayerPosition& pos, const Tensor& qkv, Tensor ctx, Tensor lse, const OptTensor& positions,
+                                  const OptTensor& bits, const OptTensor& cu, int64_t B, int64_t S, int64_t A, double p, const PdtRng& rng) {
+  const bool packed = cu.has_value();
+  TORCH_CHECK(!packed || !pos.cos.has_value() || positions.has_value(), "packed rows need their positions for the rotation");
+  Tensor q = head_third(qkv, 0, B, S, A, packed), k = head_third(qkv, 1, B, S, A, packed), qk;
+  const Tensor v = head_third(qkv, 2, B, S, A, packed);
+  if (pos.turns()) {
+    qk = at::empty({qkv.size(0), 2 * A * 64}, qkv.options());
+    const Tensor yq = head_third(qk, 0, B, S, A, packed), yk = head_third(qk, 1, B, S, A, packed);
+    rope_forward_into(q, k, RopeCall{pos.wq, pos.wk, pos.cos, pos.sin, positions, false, pos.eps}, yq, yk);
+    q = yq; k = yk;
+  }
+  const Tensor o = head_view(ctx, B, S, A, packed);
+  const RelCall c{pos.table, bits, cu, pos.steps, pos.max_distance, S, 0.125, p};
+  PdtRelAttn a = rel_args(q, k, v, o, c, rng);
+  TORCH_CHECK(lse.numel() >= (int64_t)a.B * a.A * a.S, "lse is too small");
+  a.lse = lse.data_ptr<float>();
+  if (qkv.size(0)) check(pdt_rel_attn_fwd(dt_code(qkv), &a, cur_stream()), "rel_attn_fwd");
+  return qk;
+}
+void position_attention_backward(const LayerPosition& pos, const Tensor& qkv, const Tensor& qk, const Tensor& ctx, const Tensor& dctx,
+                                 const Tensor& lse, Tensor dqkv, const std::vector<Tensor>& gr, const OptTensor& positions,
+                                 const OptTensor& bits, const OptTensor& cu, int64_t B, int64_t S, int64_t A, double p,
+                                 const PdtRng& rng, bool accumulate) {
+  const bool packed = cu.has_value();
+  auto third = [&](const Tensor& t, int i) { return head_third(t, i, B, S, A, packed); };
+  const bool turns = pos.turns();
+  TORCH_CHECK((int)gr.size() == 12 + (pos.table.has_value() ? 1 : 0) + (pos.wq.has_value() ? 2 : 0), "layer_backward: gradients of the position parameters missing");
+  size_t at = 12;
+  float* dtable = pos.table.has_value() ? gr[at++].data_ptr<float>() : nullptr;
+  const RelCall c{pos.table, bits, cu, pos.steps, pos.max_distance, S, 0.125, p};
+  const Tensor dqk = turns ? at::empty_like(qk) : dqkv;
+  rel_attn_backward_into(head_view(dctx, B, S, A, packed), third(turns ? qk : qkv, 0), third(turns ? qk : qkv, 1), third(qkv, 2),
+                         head_view(ctx, B, S, A, packed), lse, c, rng, third(dqk, 0), third(dqk, 1), third(dqkv, 2), dtable, accumulate);
+  if (turns)
+    rope_backward_into(third(dqk, 0), third(dqk, 1), third(qkv, 0), third(qkv, 1),
+                       RopeCall{pos.wq, pos.wk, pos.cos, pos.sin, positions, false, pos.eps}, third(dqkv, 0), third(dqkv, 1),
+                       pos.wq.has_value() ? gr[at].data_ptr<float>() : nullptr, pos.wq.has_value() ? gr[at + 1].data_ptr<float>() : nullptr,
+                       accumulate);
+}
 struct LayerDims { int B, S, A; double p_attn, p_hidden, eps; int64_t micro, layer; };
 
 std::vector<Tensor> layer_forward(const Tensor& x, const Tensor& mask, const Tensor& kv_len,
                                   const std::vector<Tensor>& w, const Tensor& rng_state, int64_t B, int64_t S, int64_t A,
                                   double p_attn, double p_hidden, double eps, int64_t micro, int64_t layer,
-                                  const OptTensor& sids, const OptTensor& cu, const OptTensor& rowmap) {
+                                  const OptTensor& sids, const OptTensor& cu, const OptTensor& rowmap,
+                                  const LayerPositionPtr& pos, const OptTensor& positions, const OptTensor& bits) {
   DeviceGuard guard(x.device());
   chk16(x, "x");
   TORCH_CHECK(w.size() == 12, "layer_forward: 12 weight tensors expected");
@@ -692,10 +754,16 @@ std::vector<Tensor> layer_forward(const Tensor& x, const Tensor& mask, const Ten
   Tensor qkv = gemm_nt(x, w[0], e_bias);
 
   Tensor ctx = at::empty({T, H}, x.options());
-  Tensor lse = at::empty({B, A, S}, f32);
-  check(pdt_attn_fwd(dt_code(x), qkv.data_ptr(), mask.data_ptr<int32_t>(), kv_len.data_ptr<int32_t>(), cup, ctx.data_ptr(),
-                     lse.data_ptr<float>(), (int)B, (int)S, (int)A, keep_scale(p_attn), thr16(p_attn),
-                     make_rng(rng_state, micro, site + 0, sids, S, B), cur_stream()), "attn_fwd");
+  Tensor qk;
+  // (the position kernels count packed rows by the longest sample there can be: no more than the rows there are)
+  Tensor lse = at::empty({B, A, pos && cup ? std::min<int64_t>(S, T) : S}, f32);
+  if (pos)
+    qk = position_attention_forward(*pos, qkv, ctx, lse, positions, bits, cu, B, S, A, p_attn,
+                                    make_rng(rng_state, micro, site + 0, sids, S, B));
+  else
+    check(pdt_attn_fwd(dt_code(x), qkv.data_ptr(), mask.data_ptr<int32_t>(), kv_len.data_ptr<int32_t>(), cup, ctx.data_ptr(),
+                       lse.data_ptr<float>(), (int)B, (int)S, (int)A, keep_scale(p_attn), thr16(p_attn),
+                       make_rng(rng_state, micro, site + 0, sids, S, B), cur_stream()), "attn_fwd");
 
   Epi e_ao; e_ao.kind = PDT_EPI_BIAS_DROP_RES; e_ao.bias = &w[3]; e_ao.res = &x; e_ao.drop_p = p_hidden;
   e_ao.rng = make_rng(rng_state, micro, site + 1, sids, S, B, rowmap);
@@ -712,17 +780,19 @@ std::vector<Tensor> layer_forward(const Tensor& x, const Tensor& mask, const Ten
   Tensor z2 = gemm_nt(gact, w[8], e_f2);
   Tensor stats2 = at::empty({T, 2}, f32);
   Tensor x2 = ln_fwd(z2, w[10], w[11], stats2, eps);
-  return {x2, qkv, ctx, lse, z1, stats1, x1, u, gact, z2, stats2};
+  std::vector<Tensor> out = {x2, qkv, ctx, lse, z1, stats1, x1, u, gact, z2, stats2};
+  if (qk.defined()) out.push_back(qk);
+  return out;
 }
 
 Tensor layer_backward(const Tensor& dy_in, const Tensor& x, const std::vector<Tensor>& sv, const Tensor& mask,
                       const Tensor& kv_len, const std::vector<Tensor>& w, std::vector<Tensor> gr,
                       const Tensor& rng_state, int64_t B, int64_t S, int64_t A, double p_attn, double p_hidden,
                       int64_t micro, int64_t layer, bool accumulate, const OptTensor& sids, const OptTensor& cu,
-                      const OptTensor& rowmap) {
+                      const OptTensor& rowmap, const LayerPositionPtr& pos, const OptTensor& positions, const OptTensor& bits) {
   DeviceGuard guard(x.device());
   const int32_t* cup = cu.has_value() ? cu->data_ptr<int32_t>() : nullptr;
-  TORCH_CHECK(sv.size() == 10 && w.size() == 12 && gr.size() == 12, "layer_backward: bad list sizes");
+  TORCH_CHECK(sv.size() == (pos && pos->turns() ? 11u : 10u) && w.size() == 12 && (pos || gr.size() == 12), "layer_backward: bad list sizes");
   const Tensor dy = dy_in.contiguous();
   chk16(dy, "dy");
   const Tensor &qkv = sv[0], &ctx = sv[1], &lse = sv[2], &z1 = sv[3], &stats1 = sv[4], &x1 = sv[5], &u = sv[6],
@@ -754,10 +824,14 @@ Tensor layer_backward(const Tensor& dy_in, const Tensor& x, const std::vector<Te
   Tensor dqkv = at::empty_like(qkv);
   Tensor delta = at::empty_like(lse);
   // the short-sequence backward kernel also emits per-sample column sums of dqkv (the QKV bias gradient)
-  const bool fused_db = pdt_attn_bwd_fuses_dbias((int)S) != 0;
+  const bool fused_db = !pos && pdt_attn_bwd_fuses_dbias((int)S) != 0;
   const int db_rows = pdt_attn_bwd_dbias_rows((int)B, (int)S);
   Tensor db_part = fused_db ? at::empty({(int64_t)db_rows, 3 * (int64_t)H}, lse.options()) : Tensor();
-  check(pdt_attn_bwd(dt_code(x), qkv.data_ptr(), mask.data_ptr<int32_t>(), kv_len.data_ptr<int32_t>(), cup, ctx.data_ptr(),
+  if (pos)
+    position_attention_backward(*pos, qkv, pos->turns() ? sv[10] : Tensor(), ctx, dctx, lse, dqkv, gr, positions, bits, cu, B, S, A,
+                                p_attn, make_rng(rng_state, micro, site + 0, sids, S, B), accumulate);
+  else
+    check(pdt_attn_bwd(dt_code(x), qkv.data_ptr(), mask.data_ptr<int32_t>(), kv_len.data_ptr<int32_t>(), cup, ctx.data_ptr(),
                      dctx.data_ptr(), lse.data_ptr<float>(), delta.data_ptr<float>(), dqkv.data_ptr(),
                      fused_db ? db_part.data_ptr<float>() : nullptr, (int)B, (int)S, (int)A, keep_scale(p_attn),
                      thr16(p_attn), make_rng(rng_state, micro, site + 0, sids, S, B), cur_stream()),
@@ -788,21 +862,22 @@ std::vector<Tensor> stack_forward(const Tensor& x, const Tensor& mask, const Ten
                                   const std::vector<std::vector<Tensor>>& w, const Tensor& rng_state, int64_t B, int64_t S,
                                   int64_t A, double p_attn, double p_hidden, double eps, int64_t micro,
                                   const std::vector<int64_t>& layer_ids, const OptTensor& sids, const OptTensor& cu,
-                                  const OptTensor& rowmap) {
-  TORCH_CHECK(!w.empty() && w.size() == layer_ids.size(), "stack_forward: one weight list and one id per layer");
+                                  const OptTensor& rowmap, const std::vector<LayerPositionPtr>& pos, const OptTensor& positions,
+                                  const OptTensor& bits) {
+  TORCH_CHECK(!w.empty() && w.size() == layer_ids.size() && pos.size() == w.size(), "stack_forward: one weight list and one id per layer");
   std::vector<Tensor> all;
-  all.reserve(w.size() * 11);
+  all.reserve(w.size() * 12);
   Tensor h = x;
   for (size_t l = 0; l < w.size(); ++l) {
     std::vector<Tensor> o = layer_forward(h, mask, kv_len, w[l], rng_state, B, S, A, p_attn, p_hidden, eps, micro,
-                                          layer_ids[l], sids, cu, rowmap);
+                                          layer_ids[l], sids, cu, rowmap, pos[l], positions, bits);
     h = o[0];
     for (auto& t : o) all.push_back(std::move(t));
   }
   return all;
 }
 
-// Backward of the run, last layer first.  `saved[l]` = the 11 tensors stack_forward returned for layer l;
+// Backward of the run, last layer first.  `saved[l]` = the 11 (12) tensors stack_forward returned for layer l;
 // `accumulate[l]`: add to layer l's gradients instead of overwriting them.  After every layer its saved tensors
 // are dropped and `layer_done(l)` is called with the GIL held (the Python side drops ITS references there and
 // reports the layer's gradient segment as complete: bucket all-reduce, gradient-lane merge).
@@ -811,17 +886,18 @@ Tensor stack_backward(const Tensor& dy_in, const Tensor& x0, std::vector<std::ve
                       const std::vector<std::vector<Tensor>>& gr, const Tensor& rng_state, int64_t B, int64_t S, int64_t A,
                       double p_attn, double p_hidden, int64_t micro, const std::vector<int64_t>& layer_ids,
                       const std::vector<int64_t>& accumulate, const OptTensor& sids, const OptTensor& cu,
-                      const OptTensor& rowmap, py::handle layer_done) {
+                      const OptTensor& rowmap, py::handle layer_done, const std::vector<LayerPositionPtr>& pos,
+                      const OptTensor& positions, const OptTensor& bits) {
   const size_t L = w.size();
-  TORCH_CHECK(L > 0 && saved.size() == L && gr.size() == L && layer_ids.size() == L && accumulate.size() == L,
+  TORCH_CHECK(L > 0 && saved.size() == L && gr.size() == L && layer_ids.size() == L && accumulate.size() == L && pos.size() == L,
               "stack_backward: per-layer lists of different lengths");
   Tensor dy = dy_in;
   for (size_t i = L; i-- > 0;) {
-    TORCH_CHECK(saved[i].size() == 11, "stack_backward: 11 saved tensors per layer expected");
+    TORCH_CHECK(saved[i].size() >= 11, "stack_backward: 11 saved tensors per layer expected");
     const Tensor& xin = i == 0 ? x0 : saved[i - 1][0];
     std::vector<Tensor> sv(saved[i].begin() + 1, saved[i].end());
     dy = layer_backward(dy, xin, sv, mask, kv_len, w[i], gr[i], rng_state, B, S, A, p_attn, p_hidden, micro, layer_ids[i],
-                        accumulate[i] != 0, sids, cu, rowmap);
+                        accumulate[i] != 0, sids, cu, rowmap, pos[i], positions, bits);
     sv.clear();
     saved[i].clear();
     if (!layer_done.is_none()) {
@@ -1116,6 +1192,16 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   // thread can enqueue the next micro-batch's forward on its own stream meanwhile (Engine.accumulate) - short
   // micro-batches are bound by the rate at which ONE host thread can launch kernels.
   using nogil = py::call_guard<py::gil_scoped_release>;
+  py::class_<LayerPosition, LayerPositionPtr>(m, "LayerPosition", "position options of an encoder layer's attention")
+      .def(py::init<>())
+      .def_readwrite("table", &LayerPosition::table)
+      .def_readwrite("wq", &LayerPosition::wq)
+      .def_readwrite("wk", &LayerPosition::wk)
+      .def_readwrite("cos", &LayerPosition::cos)
+      .def_readwrite("sin", &LayerPosition::sin)
+      .def_readwrite("max_distance", &LayerPosition::max_distance)
+      .def_readwrite("steps", &LayerPosition::steps)
+      .def_readwrite("eps", &LayerPosition::eps);
   m.def("layer_forward", &layer_forward, nogil());
   m.def("layer_backward", &layer_backward, nogil());
   m.def("stack_forward", &stack_forward, nogil());

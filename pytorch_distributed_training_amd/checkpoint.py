@@ -54,6 +54,7 @@ def save_pretrained(model: nn.Module, directory: str, suffix: str = "", write_co
     return path
 
 
+POSITION_PARAMS = (".relative_attention_bias.weight", ".query_norm.weight", ".key_norm.weight")
 _LEGACY = ((".LayerNorm.gamma", ".LayerNorm.weight"), (".LayerNorm.beta", ".LayerNorm.bias"))
 
 
@@ -86,7 +87,8 @@ def load_state_dict_into(model: nn.Module, sd: Dict[str, torch.Tensor], strict: 
     own = dict(m.named_parameters())
     missing = [k for k in own if k not in sd]
     unexpected = [k for k in sd if k not in own]
-    head_only = all(k.startswith("classifier") or ".pooler." in k for k in missing)
+    # (the tables and norm weights of the position options start neutral: a checkpoint from before they were switched on may lack them)
+    head_only = all(k.startswith("classifier") or ".pooler." in k or k.endswith(POSITION_PARAMS) for k in missing)
     if strict and (unexpected or (missing and not head_only)):
         raise KeyError(f"state_dict mismatch: missing {missing[:4]}, unexpected {unexpected[:4]}")
     with torch.no_grad():

@@ -39,6 +39,11 @@ class TrainConfig:
     # reference literals
     model: str = "bert-large-cased"
     num_warmup_steps: int = 100
+    # position options of the encoder's attention on top of `model` (see EncoderConfig)
+    relative_buckets: int = 0   # > 0: learned relative position bias with this many buckets
+    relative_max_distance: int = 128
+    qk_norm: bool = False       # per-head RMS norm of queries and keys
+    rotary_dim: int = 0         # > 0: rotation of the first so many elements of every query and key head
     # precision / device flags
     fp16: bool = False
     bf16: bool = False
@@ -73,6 +78,18 @@ class TrainConfig:
     resume: Optional[str] = None
     save_every: int = 0
     init_from: Optional[str] = None  # directory with HF-layout weights (config.json + safetensors / bin)
+
+    def position_overrides(self) -> dict:
+        """The EncoderConfig fields that the position flags set (flags left at their defaults set none)."""
+        out = {}
+        if self.relative_buckets:
+            out.update(relative_attention_num_buckets=self.relative_buckets,
+                       relative_attention_max_distance=self.relative_max_distance)
+        if self.qk_norm:
+            out["qk_norm"] = True
+        if self.rotary_dim:
+            out["rotary_dim"] = self.rotary_dim
+        return out
 
     def micro_batch_cap(self, device=None, model_cfg=None, free_bytes: Optional[int] = None) -> int:
         """Largest micro-batch one GPU runs.  An explicit ``--max-gpu-batch-size N`` wins.  0 (default) sizes it for the

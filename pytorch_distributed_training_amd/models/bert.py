@@ -61,12 +61,15 @@ class MaskInfo:
     so it can skip key blocks that are entirely padding.
     """
 
-    def __init__(self, mask: Optional[torch.Tensor], batch: int, seq: int, device, cu_seqlens=None, rowmap=None):
-        """`cu_seqlens` / `rowmap`: an UNPADDED batch (native path only) - the hidden states are the packed [T, H] rows
-        of the real tokens, sample b owns rows cu_seqlens[b] .. cu_seqlens[b+1], `seq` is the longest sample and
-        `rowmap[t]` the dropout row (sample id * 512 + position) of packed row t."""
+    def __init__(self, mask: Optional[torch.Tensor], batch: int, seq: int, device, cu_seqlens=None, rowmap=None,
+                 positions=None):
+        """`cu_seqlens` / `rowmap` / `positions`: an UNPADDED batch (native path only) - the hidden states are the packed
+        [T, H] rows of the real tokens, sample b owns rows cu_seqlens[b] .. cu_seqlens[b+1], `seq` is the longest sample,
+        `rowmap[t]` the dropout row (sample id * 512 + position) of packed row t and `positions[t]` (int64) its position."""
         self.batch, self.seq = batch, seq
-        self.cu, self.rowmap = cu_seqlens, rowmap
+        self.cu, self.rowmap, self.positions = cu_seqlens, rowmap, positions
+        self._all_attended = mask is None
+        self._bits = None
         if mask is None and cu_seqlens is None:
             mask = torch.ones(batch, seq, dtype=torch.int32, device=device)
         self.mask = mask
@@ -77,6 +80,15 @@ class MaskInfo:
         if dtype not in self._ext:
             self._ext[dtype] = get_extended_attention_mask(self.mask, dtype)
         return self._ext[dtype]
+
+    def bits(self) -> Optional[torch.Tensor]:
+        """The mask as the position-aware attention reads it: one bit per key (None: every key is attended)."""
+        if self._bits is None and not self._all_attended:
+            from ..ops.attention import mask_bits
+
+            m = self.mask
+            self._bits = mask_bits(m if m.dtype in (torch.bool, torch.uint8, torch.int32) else m.ne(0))
+        return self._bits
 
     def native(self):
         if self._native is None and self.cu is not None:
@@ -142,6 +154,23 @@ class BertEmbeddings(nn.Module):
         return F.dropout(x, self.dropout_p, self.training)
 
 
+class HeadNorm(nn.Module):
+    """Weight of the RMS norm over one query or key head."""
+
+    def __init__(self, dim: int):
+        super().__init__()
+        self.weight = nn.Parameter(torch.ones(dim))
+
+
+class RelativeBias(nn.Module):
+    """Bias of the attention scores by bucket of the relative position, one column per head.  It starts at zero: a model
+    that takes its other weights from a checkpoint without the table computes what that checkpoint computes."""
+
+    def __init__(self, buckets: int, heads: int):
+        super().__init__()
+        self.weight = nn.Parameter(torch.zeros(buckets, heads))
+
+
 class BertSelfAttention(nn.Module):
     def __init__(self, cfg: EncoderConfig):
         super().__init__()
@@ -149,6 +178,11 @@ class BertSelfAttention(nn.Module):
         self.query = nn.Linear(h, h)
         self.key = nn.Linear(h, h)
         self.value = nn.Linear(h, h)
+        if cfg.relative_attention_num_buckets:
+            self.relative_attention_bias = RelativeBias(cfg.relative_attention_num_buckets, cfg.num_attention_heads)
+        if cfg.qk_norm:
+            self.query_norm = HeadNorm(cfg.head_dim)
+            self.key_norm = HeadNorm(cfg.head_dim)
 
 
 class BertSelfOutput(nn.Module):
@@ -197,6 +231,12 @@ class BertLayer(nn.Module):
         the weight of the fused QKV GEMM, and its gradient is written by a single wgrad.
         """
         a, s, o = self.attention, self.attention.self, self.attention.output
+        extra: List[Tuple[str, nn.Parameter]] = []
+        if self.cfg.relative_attention_num_buckets:
+            extra.append(("attention.self.relative_attention_bias.weight", s.relative_attention_bias.weight))
+        if self.cfg.qk_norm:
+            extra += [("attention.self.query_norm.weight", s.query_norm.weight),
+                      ("attention.self.key_norm.weight", s.key_norm.weight)]
         return [
             ("attention.self.query.weight", s.query.weight),
             ("attention.self.key.weight", s.key.weight),
@@ -214,7 +254,7 @@ class BertLayer(nn.Module):
             ("output.dense.bias", self.output.dense.bias),
             ("output.LayerNorm.weight", self.output.LayerNorm.weight),
             ("output.LayerNorm.bias", self.output.LayerNorm.bias),
-        ]
+        ] + extra
 
     def forward(self, hidden: torch.Tensor, mask: MaskInfo, rng=None) -> torch.Tensor:
         if self._native is not None and hidden.is_cuda:
@@ -232,15 +272,34 @@ class BertLayer(nn.Module):
         def heads(t):
             return t.view(b, s, a, d).transpose(1, 2)
 
-        q, k, v = heads(sa.query(x)), heads(sa.key(x)), heads(sa.value(x))
-        scores = torch.matmul(q, k.transpose(-1, -2)) / math.sqrt(d)
-        scores = scores + mask.extended(scores.dtype)
-        probs = F.dropout(torch.softmax(scores, dim=-1), cfg.attention_probs_dropout_prob, self.training)
-        ctx = torch.matmul(probs, v).transpose(1, 2).reshape(b, s, h)
+        if cfg.position_ops:
+            ctx = self._position_attention_torch(sa.query(x).view(b, s, a, d), sa.key(x).view(b, s, a, d),
+                                                 sa.value(x).view(b, s, a, d), mask).reshape(b, s, h)
+        else:
+            q, k, v = heads(sa.query(x)), heads(sa.key(x)), heads(sa.value(x))
+            scores = torch.matmul(q, k.transpose(-1, -2)) / math.sqrt(d)
+            scores = scores + mask.extended(scores.dtype)
+            probs = F.dropout(torch.softmax(scores, dim=-1), cfg.attention_probs_dropout_prob, self.training)
+            ctx = torch.matmul(probs, v).transpose(1, 2).reshape(b, s, h)
         x = so.LayerNorm(F.dropout(so.dense(ctx), cfg.hidden_dropout_prob, self.training) + x)
         inter = F.gelu(self.intermediate.dense(x))
         y = F.dropout(self.output.dense(inter), cfg.hidden_dropout_prob, self.training)
         return self.output.LayerNorm(y + x)
+
+
+    def _position_attention_torch(self, q, k, v, mask: MaskInfo) -> torch.Tensor:
+        from ..ops.attention import relative_attention_reference
+        from ..ops.rotary import qk_norm_rope_reference, rotary_table
+
+        cfg, sa = self.cfg, self.attention.self
+        rope = rotary_table(q.shape[1], cfg.rotary_dim, cfg.rotary_base, q.device) if cfg.rotary_dim else None
+        if cfg.qk_norm or rope is not None:
+            q = qk_norm_rope_reference(q, sa.query_norm.weight if cfg.qk_norm else None, rope=rope, eps=cfg.qk_norm_eps)
+            k = qk_norm_rope_reference(k, sa.key_norm.weight if cfg.qk_norm else None, rope=rope, eps=cfg.qk_norm_eps)
+        bias = sa.relative_attention_bias.weight if cfg.relative_attention_num_buckets else None
+        return relative_attention_reference(q, k, v, bias, max_distance=cfg.relative_attention_max_distance,
+                                            key_mask=mask.mask, dropout_p=cfg.attention_probs_dropout_prob,
+                                            training=self.training)
 
 
 class BertEncoder(nn.Module):
@@ -407,7 +466,8 @@ class _ClassifierBase(nn.Module):
         sid = sample_ids.reshape(-1).to(torch.int64)[b_of] if sample_ids is not None else b_of
         rowmap = (sid * 512 + (tok - b_of * S)).to(torch.int32)
         cu = cu_seqlens.to(torch.int32)
-        mask = MaskInfo(None, B, S, tok.device, cu_seqlens=cu, rowmap=rowmap)
+        mask = MaskInfo(None, B, S, tok.device, cu_seqlens=cu, rowmap=rowmap,
+                        positions=tok - b_of * S if self.config.rotary_dim else None)
         if emb is not None:
             ids = input_ids.reshape(-1)[tok] if lookup else None
             types = (token_type_ids.reshape(-1)[tok] if token_type_ids is not None else torch.zeros_like(tok))
@@ -454,6 +514,10 @@ class _ClassifierBase(nn.Module):
                 elif isinstance(m, nn.LayerNorm):
                     m.weight.fill_(1.0)
                     m.bias.zero_()
+                elif isinstance(m, HeadNorm):
+                    m.weight.fill_(1.0)
+                elif isinstance(m, RelativeBias):
+                    m.weight.zero_()
 
     def num_parameters(self) -> int:
         return sum(p.numel() for p in self.parameters())

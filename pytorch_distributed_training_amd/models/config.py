@@ -34,6 +34,21 @@ class EncoderConfig:
     pad_token_id: int = 0
     num_labels: int = 2
     hidden_act: str = "gelu"
+    # What attention knows of positions besides the absolute table of the embeddings (all off by default):
+    # a learned bias of the scores by the bucket of (key - query), one table [buckets, heads] per layer (0 = none);
+    relative_attention_num_buckets: int = 0
+    relative_attention_max_distance: int = 128
+    # an RMS norm of every query and key head, weights [head_dim] per layer;
+    qk_norm: bool = False
+    qk_norm_eps: float = 1e-6
+    # and the rotation of the first rotary_dim elements of every query and key head by their position (0 = none)
+    rotary_dim: int = 0
+    rotary_base: float = 10000.0
+
+    @property
+    def position_ops(self) -> bool:
+        """Whether the encoder layers use any of the position options (relative bias, query / key norm, rotation)."""
+        return bool(self.relative_attention_num_buckets or self.qk_norm or self.rotary_dim)
 
     @property
     def head_dim(self) -> int:
@@ -51,6 +66,12 @@ class EncoderConfig:
             raise ValueError("only the exact-erf GELU of BERT/RoBERTa is implemented")
         if self.model_type not in ("bert", "roberta"):
             raise ValueError(f"unknown model_type {self.model_type!r}")
+        if self.relative_attention_num_buckets:
+            from ..ops.attention import bucket_steps
+
+            bucket_steps(self.relative_attention_num_buckets, self.relative_attention_max_distance)
+        if self.rotary_dim and (self.rotary_dim % 16 or not 0 < self.rotary_dim <= self.head_dim):
+            raise ValueError(f"rotary_dim must be a multiple of 16, at most the head dim {self.head_dim} (got {self.rotary_dim})")
 
     # -- HF config.json round trip -------------------------------------------------
     def to_hf_dict(self) -> Dict:

@@ -22,6 +22,7 @@ from __future__ import annotations
 
 import os
 import time
+from dataclasses import replace
 from typing import List, Optional
 
 import torch
@@ -298,7 +299,8 @@ def run_tower_training(rank: int, world_size: int, cfg) -> dict:
     engine = Engine(fp16=cfg.fp16, bf16=cfg.bf16, cpu=cfg.cpu, seed=cfg.seed, process_group=mesh.dp_group,
                     min_bucket_mb=cfg.min_bucket_mb, init_scale=cfg.init_scale,
                     comm_backend=cfg.comm_backend, update_in_backward=False)
-    model_cfg = preset(cfg.model)
+    model_cfg = replace(preset(cfg.model), **cfg.position_overrides())
+    model_cfg.validate()
     train_ds, val_ds = build_datasets(cfg, model_cfg)
     accum, micro_bs = cfg.accumulation(engine.device, model_cfg)
     collate = _collator(cfg, model_cfg)

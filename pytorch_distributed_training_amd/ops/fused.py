@@ -65,6 +65,16 @@ class NativeRuntime:
         # i.e. before the data-parallel reducer sees it.
         self.lane = 0
         self.merge_on_done = False
+        self._rotary = {}
+
+    def rotary_table(self, cfg):
+        """The angles' cosines and sines of a configuration's positions, shared by its layers."""
+        from .rotary import rotary_table
+
+        key = (cfg.max_position_embeddings, cfg.rotary_dim, cfg.rotary_base)
+        if key not in self._rotary:
+            self._rotary[key] = rotary_table(*key, device=self.arena.device)
+        return self._rotary[key]
 
     def reseed(self, seed: int) -> None:
         self.rng_state[0] = seed
@@ -123,7 +133,33 @@ class LayerNative:
         ]
         self.w: List[torch.Tensor] = [arena.view16(n, s) for n, s in spec]
         self.g: List[torch.Tensor] = [arena.gview(n, s) for n, s in spec]
-        self._spec, self._g_alt = spec, None
+        self._g_alt = None
+        # what attention does with positions besides the plain softmax: the layer's table and norm weights (fp32 masters)
+        # and their gradients, which follow the twelve above in the gradient list
+        self.position = None
+        self.saved = 11  # tensors the layer's forward returns
+        if cfg.position_ops:
+            from .attention import bucket_steps
+
+            pos = native().LayerPosition()
+            D, extra = cfg.head_dim, []
+            if cfg.relative_attention_num_buckets:
+                extra.append((a + "self.relative_attention_bias.weight", (cfg.relative_attention_num_buckets, cfg.num_attention_heads)))
+                pos.table = arena.mview(*extra[-1])
+                pos.max_distance = cfg.relative_attention_max_distance
+                pos.steps = bucket_steps(cfg.relative_attention_num_buckets, cfg.relative_attention_max_distance)
+            if cfg.qk_norm:
+                extra += [(a + "self.query_norm.weight", (D,)), (a + "self.key_norm.weight", (D,))]
+                pos.wq, pos.wk = arena.mview(*extra[-2]), arena.mview(*extra[-1])
+                pos.eps = cfg.qk_norm_eps
+            if cfg.rotary_dim:
+                pos.cos, pos.sin = runtime.rotary_table(cfg)
+            if cfg.qk_norm or cfg.rotary_dim:
+                self.saved = 12
+            spec = spec + extra
+            self.g += [arena.gview(n, s) for n, s in extra]
+            self.position = pos
+        self._spec = spec
         self.segment = segment
         self.rt = runtime
         self.arena = arena
@@ -151,8 +187,10 @@ class _LayerFn(torch.autograd.Function):
         outs = native().layer_forward(
             x2, m, kvl, nat.w, key.state, B, S, cfg.num_attention_heads,
             cfg.attention_probs_dropout_prob if train else 0.0, cfg.hidden_dropout_prob if train else 0.0,
-            cfg.layer_norm_eps, key.counter, layer.index + nat.site_offset, key.sample_ids, mask.cu, mask.rowmap)
+            cfg.layer_norm_eps, key.counter, layer.index + nat.site_offset, key.sample_ids, mask.cu, mask.rowmap,
+            nat.position, *_position_inputs(nat, mask))
         ctx.layer, ctx.mask, ctx.x2, ctx.saved = layer, (m, kvl, mask.cu, mask.rowmap), x2, outs[1:]
+        ctx.position_inputs = _position_inputs(nat, mask)
         ctx.meta = (B, S, H, train, key, packed)
         ctx.lane = nat.rt.lane
         return outs[0] if packed else outs[0].view(B, S, H)
@@ -168,10 +206,16 @@ class _LayerFn(torch.autograd.Function):
             dy.reshape(-1, H), ctx.x2, list(ctx.saved), ctx.mask[0], ctx.mask[1], nat.w, nat.grads(ctx.lane), key.state,
             B, S, cfg.num_attention_heads,
             cfg.attention_probs_dropout_prob if train else 0.0, cfg.hidden_dropout_prob if train else 0.0,
-            key.counter, layer.index + nat.site_offset, acc, key.sample_ids, ctx.mask[2], ctx.mask[3])
+            key.counter, layer.index + nat.site_offset, acc, key.sample_ids, ctx.mask[2], ctx.mask[3],
+            nat.position, *ctx.position_inputs)
         ctx.saved = ctx.x2 = None
         nat.rt.done(nat.segment)
         return (dx if packed else dx.view(B, S, H)), None, None
+
+
+def _position_inputs(nat: LayerNative, mask):
+    """(positions of packed rows, key mask bits) of a batch, for layers that use them."""
+    return (mask.positions, mask.bits()) if nat.position is not None else (None, None)
 
 
 def encoder_layer_forward(layer, hidden, mask, rng=None):
@@ -207,12 +251,15 @@ class _StackFn(torch.autograd.Function):
         outs = native().stack_forward(
             x2, m, kvl, [l._native.w for l in layers], key.state, B, S, cfg.num_attention_heads,
             cfg.attention_probs_dropout_prob if train else 0.0, cfg.hidden_dropout_prob if train else 0.0,
-            cfg.layer_norm_eps, key.counter, ids, key.sample_ids, mask.cu, mask.rowmap)
+            cfg.layer_norm_eps, key.counter, ids, key.sample_ids, mask.cu, mask.rowmap,
+            [l._native.position for l in layers], *_position_inputs(first._native, mask))
         ctx.layers, ctx.mask, ctx.x2, ctx.ids = layers, (m, kvl, mask.cu, mask.rowmap), x2, ids
-        ctx.saved = [outs[i * 11:(i + 1) * 11] for i in range(len(layers))]
+        ctx.position_inputs = _position_inputs(first._native, mask)
+        n = first._native.saved
+        ctx.saved = [outs[i * n:(i + 1) * n] for i in range(len(layers))]
         ctx.meta = (B, S, H, train, key, packed)
         ctx.lane = first._native.rt.lane
-        y = outs[-11]
+        y = outs[-n]
         return y if packed else y.view(B, S, H)
 
     @staticmethod
@@ -233,7 +280,8 @@ class _StackFn(torch.autograd.Function):
             dy.reshape(-1, H), ctx.x2, saved, ctx.mask[0], ctx.mask[1], [l._native.w for l in layers],
             [l._native.grads(lane) for l in layers], key.state, B, S, cfg.num_attention_heads,
             cfg.attention_probs_dropout_prob if train else 0.0, cfg.hidden_dropout_prob if train else 0.0,
-            key.counter, ctx.ids, acc, key.sample_ids, ctx.mask[2], ctx.mask[3], layer_done)
+            key.counter, ctx.ids, acc, key.sample_ids, ctx.mask[2], ctx.mask[3], layer_done,
+            [l._native.position for l in layers], *ctx.position_inputs)
         ctx.x2 = None
         return (dx if packed else dx.view(B, S, H)), None, None
 

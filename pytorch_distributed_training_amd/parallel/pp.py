@@ -45,6 +45,7 @@ def build_stage(model_cfg, stage: int, stages: int, full_state: Optional[Dict[st
     """Module of one pipeline stage.  Its initial weights are the corresponding slice of the FULL model
     built from `seed` (or of `full_state`), so a pipelined run starts from the same point as a
     single-process run - a precondition for matching loss curves."""
+    from ..checkpoint import POSITION_PARAMS
     from ..models.bert import build_model
 
     lo, hi = split_layers(model_cfg.num_hidden_layers, stages)[stage]
@@ -54,10 +55,12 @@ def build_stage(model_cfg, stage: int, stages: int, full_state: Optional[Dict[st
         full_state = build_model(model_cfg).state_dict()
     part = build_model(model_cfg, layer_range=(lo, hi), with_embeddings=stage == 0, with_head=stage == stages - 1)
     own = part.state_dict()
-    missing = [k for k in own if k not in full_state]
+    # (tables and norm weights of position options that the full state was saved without keep their neutral start)
+    fresh = {k for k in own if k not in full_state and k.endswith(POSITION_PARAMS)}
+    missing = [k for k in own if k not in full_state and k not in fresh]
     if missing:
         raise KeyError(f"stage {stage}: parameters missing from the full state dict: {missing[:4]}")
-    part.load_state_dict({k: full_state[k] for k in own})
+    part.load_state_dict({k: own[k] if k in fresh else full_state[k] for k in own})
     return part
 
 
@@ -269,9 +272,8 @@ def run_pipeline_training(rank: int, world_size: int, cfg) -> dict:
     from .. import checkpoint as ckpt
     from ..engine import Engine
     from ..metrics import load_metric
-    from ..models.config import preset
     from ..optim import AdamW, get_linear_schedule_with_warmup
-    from ..recipes import _collator, build_datasets, model_parallel_loaders
+    from ..recipes import _collator, build_datasets, model_config, model_parallel_loaders
     from ..utils.logging import StepLogger
     from ..utils.seed import seed_step, set_seed
     from ..utils.watchdog import StepWatchdog, inject_fault
@@ -291,7 +293,7 @@ def run_pipeline_training(rank: int, world_size: int, cfg) -> dict:
     engine = Engine(fp16=cfg.fp16, bf16=cfg.bf16, cpu=cfg.cpu, seed=cfg.seed, process_group=mesh.dp_group,
                     min_bucket_mb=cfg.min_bucket_mb, init_scale=cfg.init_scale,
                     comm_backend=cfg.comm_backend, update_in_backward=False)
-    model_cfg = preset(cfg.model) if not cfg.init_from else ckpt.EncoderConfig.load(cfg.init_from)
+    model_cfg = model_config(cfg)
     train_ds, val_ds = build_datasets(cfg, model_cfg)
     accum, micro_bs = cfg.accumulation(engine.device, model_cfg)
     collate = _collator(cfg, model_cfg)

@@ -25,6 +25,7 @@ from __future__ import annotations
 
 import os
 import time
+from dataclasses import replace
 from typing import Optional
 
 import torch
@@ -64,10 +65,18 @@ def build_datasets(cfg: TrainConfig, model_cfg):
     return train, val
 
 
+def model_config(cfg: TrainConfig):
+    """Architecture of a run: the preset (or the checkpoint's configuration) with the position options of the flags."""
+    base = preset(cfg.model) if not cfg.init_from else ckpt.EncoderConfig.load(cfg.init_from)
+    out = replace(base, **cfg.position_overrides())
+    out.validate()
+    return out
+
+
 def make_model(cfg: TrainConfig):
     if cfg.init_from:
-        return ckpt.load_pretrained(cfg.init_from)
-    return build_model(cfg.model)
+        return ckpt.load_pretrained(cfg.init_from, **cfg.position_overrides())
+    return build_model(model_config(cfg))
 
 
 def _collator(cfg: TrainConfig, model_cfg) -> PadCollator:
@@ -126,7 +135,7 @@ def run_data_parallel(cfg: TrainConfig, engine: Optional[Engine] = None) -> dict
     print("DEVICE: ", engine.device)
     print("process_index: ", engine.process_index)
 
-    model_cfg = preset(cfg.model) if not cfg.init_from else ckpt.EncoderConfig.load(cfg.init_from)
+    model_cfg = model_config(cfg)
     train_ds, val_ds = build_datasets(cfg, model_cfg)
     metric = load_metric("glue", "mrpc")
     accum, micro_bs = cfg.accumulation(engine.device, model_cfg)

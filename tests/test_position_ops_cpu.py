@@ -1,0 +1,199 @@
+"""Position options without a GPU: the bucket rule, refusals, the fp32 model path, configuration and checkpoints."""
+import copy
+import math
+
+import pytest
+import torch
+
+from pytorch_distributed_training_amd.config import TrainConfig, parse_config
+from pytorch_distributed_training_amd.models.bert import build_model
+from pytorch_distributed_training_amd.models.config import EncoderConfig, preset
+from pytorch_distributed_training_amd.ops import bucket_steps, qk_norm_rope, relative_attention, relative_bucket, rotary_table
+from pytorch_distributed_training_amd.ops.attention import relative_attention_reference
+from pytorch_distributed_training_amd.ops.rotary import qk_norm_rope_reference
+
+POSITION = dict(relative_attention_num_buckets=16, relative_attention_max_distance=40, qk_norm=True, rotary_dim=32)
+
+
+@pytest.mark.parametrize("buckets,max_distance", [(4, 2), (6, 9), (32, 128), (30, 77), (64, 100), (128, 512)])
+def test_bucket_rule(buckets, max_distance):
+    half = buckets // 2
+    exact, m = half // 2, half - half // 2
+    d = torch.arange(-700, 701)
+    b = relative_bucket(d, buckets, max_distance)
+    for n, got in zip(d.tolist(), b.tolist()):
+        a = abs(n)
+        want = a if a < exact else exact + max(j for j in range(m) if a ** m * exact ** j >= max_distance ** j * exact ** m)
+        assert got == want + (half if n > 0 else 0)
+    assert b.max() < buckets and relative_bucket(torch.tensor([max_distance]), buckets, max_distance).item() == buckets - 1
+    assert list(bucket_steps(buckets, max_distance)) == sorted(bucket_steps(buckets, max_distance))
+
+
+def test_bucket_borders_lie_in_the_upper_bucket():
+    # 32 buckets, 128: 8 exact per side, and the eight logarithmic ones start at 8 * 16^(j / 8)
+    assert bucket_steps(32, 128) == (8, 12, 16, 23, 32, 46, 64, 91)
+    assert relative_bucket(torch.tensor([-15, -16, 0, 1, 16]), 32, 128).tolist() == [9, 10, 0, 17, 26]
+
+
+@pytest.mark.parametrize("buckets,max_distance", [(2, 128), (31, 128), (130, 400), (32, 8), (32, 513), (0, 128)])
+def test_bucket_refusals(buckets, max_distance):
+    with pytest.raises(ValueError):
+        bucket_steps(buckets, max_distance)
+
+
+def _qkv(*shape, dtype=torch.float16):
+    return [torch.zeros(*shape, dtype=dtype) for _ in range(3)]
+
+
+@pytest.mark.parametrize("kwargs,shape,what", [
+    (dict(), (4, 2, 64), "B, S, heads"),
+    (dict(cu_seqlens=torch.zeros(2, dtype=torch.int32), max_seqlen=4), (1, 4, 2, 64), "B, S, heads"),
+    (dict(cu_seqlens=torch.zeros(2, dtype=torch.int32)), (4, 2, 64), "max_seqlen"),
+    (dict(cu_seqlens=torch.zeros(2, dtype=torch.int32), max_seqlen=4, key_mask=torch.ones(1, 4)), (4, 2, 64), "no key mask"),
+    (dict(key_mask=torch.ones(1, 5, dtype=torch.bool)), (1, 4, 2, 64), "key_mask must be"),
+    (dict(key_mask=torch.zeros(1, 4)), (1, 4, 2, 64), "truth values"),
+    (dict(bias=torch.zeros(31, 2)), (1, 4, 2, 64), "num_buckets"),
+    (dict(bias=torch.zeros(32)), (1, 4, 2, 64), "buckets, heads"),
+    (dict(bias=torch.zeros(32, 2), max_distance=600), (1, 4, 2, 64), "max_distance"),
+    (dict(dropout_p=0.1), (1, 4, 2, 64), "rng"),
+])
+def test_relative_attention_refusals(kwargs, shape, what):
+    with pytest.raises(ValueError, match=what):
+        relative_attention(*_qkv(*shape), **kwargs)
+
+
+def test_host_tensors_are_refused():
+    from pytorch_distributed_training_amd.ops import available
+
+    if not available():
+        pytest.skip("the native extension is not built")
+    with pytest.raises(RuntimeError, match="on the GPU"):
+        relative_attention(*_qkv(1, 4, 2, 64))
+    with pytest.raises(RuntimeError, match="on the GPU"):
+        qk_norm_rope(*_qkv(1, 4, 2, 64)[:2])
+    with pytest.raises(ValueError, match="positions"):
+        qk_norm_rope(*_qkv(1, 4, 2, 64)[:2], positions=torch.zeros(4))
+    with pytest.raises(ValueError, match="constants"):
+        qk_norm_rope(*_qkv(1, 4, 2, 64)[:2], rope=(torch.zeros(4, 32, requires_grad=True), torch.zeros(4, 32)))
+
+
+def test_rotary_table():
+    cos, sin = rotary_table(100_000, 64, device="cpu")
+    want = 99_999 * 10000.0 ** (-2 * 3 / 64)
+    assert abs(cos[99_999, 3].item() - math.cos(want)) < 1e-6 and abs(sin[99_999, 3].item() - math.sin(want)) < 1e-6
+    for bad in ((0, 64), (4, 7), (4, 0)):
+        with pytest.raises(ValueError):
+            rotary_table(*bad, device="cpu")
+
+
+def test_rotation_keeps_scores_of_relative_positions():
+    torch.manual_seed(0)
+    q, k = (torch.randn(1, 20, 2, 32, dtype=torch.float64) for _ in range(2))
+    cos, sin = rotary_table(500, 16, device="cpu")
+    scores = []
+    for shift in (0, 300):
+        pos = torch.arange(20)[None] + shift
+        a, b = (qk_norm_rope_reference(t, torch.ones(32, dtype=torch.float64), rope=(cos, sin), positions=pos) for t in (q, k))
+        scores.append(torch.einsum("bihd,bjhd->bhij", a, b))
+    torch.testing.assert_close(scores[0], scores[1], rtol=0, atol=1e-5)  # (fp32 tables)
+
+
+def test_reference_attention_rows_without_keys():
+    torch.manual_seed(0)
+    q, k, v = (torch.randn(2, 6, 1, 8) for _ in range(3))
+    mask = torch.tensor([[1] * 6, [0] * 6])
+    out = relative_attention_reference(q, k, v, torch.randn(8, 1), max_distance=4, key_mask=mask)
+    assert out[1].abs().max() == 0 and torch.isfinite(out).all()
+
+
+def test_config_round_trip_and_refusals(tmp_path):
+    cfg = preset("bert-tiny", **POSITION)
+    assert cfg.position_ops and not preset("bert-tiny").position_ops
+    cfg.save(str(tmp_path))
+    assert EncoderConfig.load(str(tmp_path)) == cfg
+    old = {k: v for k, v in preset("bert-tiny").to_hf_dict().items() if k not in ("qk_norm", "rotary_dim", "relative_attention_num_buckets")}
+    assert not EncoderConfig.from_hf_dict(old).position_ops  # a config from before the options existed
+    for bad in (dict(relative_attention_num_buckets=7), dict(relative_attention_num_buckets=32, relative_attention_max_distance=4),
+                dict(rotary_dim=24), dict(rotary_dim=128)):
+        with pytest.raises(ValueError):
+            preset("bert-tiny", **bad)
+
+
+def test_model_parameters_and_gradients():
+    torch.manual_seed(0)
+    model = build_model("bert-tiny-nodrop", **POSITION)
+    names = [n for n, _ in model.named_parameters()]
+    assert sum("relative_attention_bias" in n for n in names) == 2 and sum("_norm.weight" in n for n in names) == 4
+    with torch.no_grad():
+        for n, p in model.named_parameters():
+            if "relative_attention_bias" in n:
+                p.normal_()
+    ids = torch.randint(5, 500, (3, 50))
+    mask = (torch.arange(50)[None] < torch.tensor([50, 20, 1])[:, None]).long()
+    out = model(input_ids=ids, attention_mask=mask, labels=torch.tensor([0, 1, 0]))
+    out.loss.backward()
+    for n, p in model.named_parameters():
+        if "relative_attention_bias" in n or "query_norm" in n or "key_norm" in n:
+            assert p.grad.abs().sum() > 0, n
+    # padding does not matter: the first sample alone, cut to its length
+    alone = model(input_ids=ids[1:2, :20], attention_mask=mask[1:2, :20])
+    torch.testing.assert_close(alone.logits, out.logits[1:2], rtol=1e-4, atol=1e-5)
+
+
+def test_zero_table_is_the_plain_model_and_checkpoints_convert(tmp_path):
+    from pytorch_distributed_training_amd.checkpoint import load_pretrained, save_pretrained
+
+    torch.manual_seed(0)
+    plain = build_model("bert-tiny-nodrop").eval()
+    save_pretrained(plain, str(tmp_path / "plain"))
+    rel = load_pretrained(str(tmp_path / "plain"), relative_attention_num_buckets=16).eval()
+    ids = torch.randint(5, 500, (2, 30))
+    torch.testing.assert_close(rel(input_ids=ids).logits, plain(input_ids=ids).logits, rtol=1e-5, atol=1e-6)
+    with torch.no_grad():
+        rel.bert.encoder.layers()[0].attention.self.relative_attention_bias.weight.normal_()
+    save_pretrained(rel, str(tmp_path / "rel"))
+    again = load_pretrained(str(tmp_path / "rel")).eval()
+    assert torch.equal(again(input_ids=ids).logits, rel(input_ids=ids).logits)
+    with pytest.raises(KeyError):  # the other way round the table would be dropped
+        load_pretrained(str(tmp_path / "rel"), relative_attention_num_buckets=0)
+
+
+def test_arena_holds_the_position_parameters():
+    from pytorch_distributed_training_amd.ops.arena import ParamArena
+
+    model = build_model("bert-tiny-nodrop", **POSITION)
+    want = copy.deepcopy(model.state_dict())
+    arena = ParamArena(model, torch.device("cpu"))
+    for k, v in model.state_dict().items():
+        assert torch.equal(v, want[k])
+    assert any(n.endswith("relative_attention_bias.weight") for n in arena.offsets)
+
+
+def test_pipeline_stage_slices_and_fresh_tables():
+    from pytorch_distributed_training_amd.parallel.pp import build_stage
+
+    cfg = preset("bert-tiny-nodrop", **POSITION)
+    full = build_model(cfg).state_dict()
+    for stage in range(2):
+        part = build_stage(cfg, stage, 2, full)
+        assert all(torch.equal(v, full[k]) for k, v in part.state_dict().items())
+    plain = build_model("bert-tiny-nodrop").state_dict()
+    part = build_stage(cfg, 0, 2, plain)
+    assert part.state_dict()["bert.encoder.layer.0.attention.self.relative_attention_bias.weight"].abs().max() == 0
+
+
+def test_flags_and_recipe_train_the_tables(tmp_path):
+    from pytorch_distributed_training_amd import recipes
+
+    cfg = parse_config(["--model", "bert-tiny", "--cpu", "--relative-buckets", "16", "--relative-max-distance", "40", "--qk-norm",
+                        "--rotary-dim", "32", "--train-examples", "24", "--eval-examples", "8", "--batch-size", "8", "--num-epochs", "1",
+                        "--max-steps", "2", "--num-warmup-steps", "0", "--lr", "1e-3", "--output-dir", str(tmp_path)])
+    arch = recipes.model_config(cfg)
+    assert (arch.relative_attention_num_buckets, arch.relative_attention_max_distance, arch.qk_norm, arch.rotary_dim) == (16, 40, True, 32)
+    assert TrainConfig().position_overrides() == {}
+    recipes.run_data_parallel(cfg)
+    from pytorch_distributed_training_amd.checkpoint import load_pretrained
+
+    model = load_pretrained(str(tmp_path))
+    assert model.config.rotary_dim == 32
+    assert model.bert.encoder.layers()[1].attention.self.relative_attention_bias.weight.abs().max() > 0
