@@ -49,7 +49,10 @@ def _sources():
 # the attention kernels write their fp32 math as explicit vector operations; the SLP vectoriser on top of that pairs up the
 # scalar adds of the DPP row reductions (v_mov_b32_dpp + v_pk_add_f32, 6 instructions per 4 values and step) where the
 # un-paired adds fold into v_add_f32_dpp (4 instructions)
-PER_SOURCE_FLAGS = {"attention.hip": ["-fno-slp-vectorize"], "rel_attention.hip": ["-fno-slp-vectorize"]}
+# rel_attention.hip: matrix products accumulate in ordinary registers (the other form moves every accumulator that is not a
+# pure sum through v_accvgpr_read / write: 416 of 2726 instructions of the forward kernel)
+PER_SOURCE_FLAGS = {"attention.hip": ["-fno-slp-vectorize"],
+                    "rel_attention.hip": ["-fno-slp-vectorize", "-mllvm", "-amdgpu-mfma-vgpr-form=1"]}
 
 
 def _stamp(paths, flags):

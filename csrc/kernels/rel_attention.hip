@@ -20,6 +20,7 @@
 // the B operand of the next product; rows come through LDS in chunks of 64, double-buffered, filled by LDS-DMA.  A row
 // that no query may attend to is read as zeros: whatever its memory holds, NaN included, never meets a product.
 #include <mutex>
+#include <type_traits>
 #include <unordered_set>
 
 #include "attn_common.hpp"
@@ -31,7 +32,13 @@ constexpr int RA_CHUNK = 64;                    // rows per LDS image
 constexpr int RA_IMG = RA_CHUNK * 128;          // bytes of a 64-row x 64-column image
 constexpr int RA_MAX_FAR = 512;                 // largest max_distance
 constexpr int RA_MAX_STEPS = 32;                // logarithmic buckets per side
-
+constexpr float RA_SLACK = 8.0f;
+#ifndef RA_WF
+#define RA_WF 3
+#endif
+// Waves per SIMD that the register allocation of a kernel with QB blocks of KS 32-column steps must allow
+#define RA_OCC_FWD __attribute__((amdgpu_waves_per_eu(KS * QB <= 4 ? RA_WF : 2, 8)))
+#define RA_OCC_BWD __attribute__((amdgpu_waves_per_eu(KS * QB <= 2 ? 3 : 2, 8)))
 
 // rows [0, 64) of a [rows][D] matrix (row stride `stride` elements) into NH 64-column images: 16-byte chunk c of row r is
 // stored at chunk c ^ (r & 6).  Rows whose bit in `rows` is clear, and columns from D on, arrive as zeros.
@@ -94,6 +101,30 @@ __device__ __forceinline__ void ra_store(T* row, const float4v (&t)[2 * KS], flo
   }
 }
 
+// maximum / sum over the four lane groups (lanes l, l ^ 16, l ^ 32, l ^ 48) with register swaps instead of LDS permutes
+__device__ __forceinline__ float ra_other16(float v, float& mine) {
+  const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  mine = __uint_as_float(r[0]);
+  return __uint_as_float(r[1]);
+}
+__device__ __forceinline__ float ra_other32(float v, float& mine) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  mine = __uint_as_float(r[0]);
+  return __uint_as_float(r[1]);
+}
+__device__ __forceinline__ float ra_quad_max(float v) {
+  float a, b = ra_other16(v, a);
+  v = fmaxf(a, b);
+  b = ra_other32(v, a);
+  return fmaxf(a, b);
+}
+__device__ __forceinline__ float ra_quad_sum(float v) {
+  float a, b = ra_other16(v, a);
+  v = a + b;
+  b = ra_other32(v, a);
+  return a + b;
+}
+
 // ---- one (batch, head) of a launch
 struct RaSpan {
   int b, h, n;      // sample, head, length
@@ -144,6 +175,7 @@ __host__ __device__ inline int ra_bias_len(int max_distance) {
   const int n = 2 * ((max_distance + 15) & ~15) + 64 + 16;
   return ((n + 63) & ~63) + 16;  // the copies start 64 bytes apart modulo the 256 bytes of one access
 }
+__host__ __device__ inline int ra_diag_len(int max_distance) { return 2 * ((max_distance + 15) & ~15) + 80; }
 __device__ __forceinline__ int ra_bucket(const PdtRelAttn& p, int d) {
   const int n = d < 0 ? -d : d, half = p.buckets >> 1, exact = half >> 1;
   int b = n;
@@ -161,13 +193,11 @@ __device__ __forceinline__ float ra_table(const PdtRelAttn& p, int bucket, int h
 template <typename T>
 __device__ __forceinline__ RaBias ra_bias_fill(const PdtRelAttn& p, float* mem, int h, int sign, int tid) {
   RaBias t{mem, ra_bias_len(p.max_distance), ra_far(p.max_distance) + 32, ra_far(p.max_distance)};
-  if (p.table) {
-    for (int i = tid; i < t.len + 4; i += RA_THREADS) {
-      const float v = ra_table<T>(p, ra_bucket(p, sign * (i - t.off)), h) * LOG2E;
+  for (int i = tid; i < t.len + 4; i += RA_THREADS) {
+    const float v = p.table ? ra_table<T>(p, ra_bucket(p, sign * (i - t.off)), h) * LOG2E : 0.f;
 #pragma unroll
-      for (int j = 0; j < 4; ++j)
-        if (i - j >= 0 && i - j < t.len) mem[j * t.len + i - j] = v;
-    }
+    for (int j = 0; j < 4; ++j)
+      if (i - j >= 0 && i - j < t.len) mem[j * t.len + i - j] = v;
   }
   return t;
 }
@@ -181,10 +211,16 @@ __device__ __forceinline__ float4v ra_bias4(const RaBias& t, int lane_off, int u
   return *reinterpret_cast<const float4v*>(t.t + lane_off + uc);
 }
 
+// Whether tiles with their offsets in [u0, u1] all lie beyond the near distances: -1 / 1 the side, 0 not all of them.
+// (u - 15 .. u + 15 are the distances of a tile.)
+__device__ __forceinline__ int ra_side(const RaBias& t, int u0, int u1) {
+  return u0 >= t.far + 16 ? 1 : (u1 <= -(t.far + 16) ? -1 : 0);
+}
+
 // ------------------------------------------------------------------------------------------------ forward
 // One wave = 16 QB query rows; online softmax in the log2 domain.
 template <typename T, int KS, int QB, bool DROP>
-__global__ __launch_bounds__(RA_THREADS) void rel_attn_fwd_kernel(PdtRelAttn p) {
+__global__ __launch_bounds__(RA_THREADS) RA_OCC_FWD void rel_attn_fwd_kernel(PdtRelAttn p) {
   constexpr int NH = (KS + 1) / 2, BUF = 2 * NH * RA_IMG;
   extern __shared__ __attribute__((aligned(16))) char smem[];
   const int tid = threadIdx.x, lane = tid & 63, lm = lane & 15, g = lane >> 4;
@@ -219,7 +255,7 @@ __global__ __launch_bounds__(RA_THREADS) void rel_attn_fwd_kernel(PdtRelAttn p) 
   }
   const float k2 = p.scale * LOG2E;
   const uint32_t thr_hi = attn_thr_hi(p.drop_thr), kmul0 = (uint32_t)(4 * g) * ATT_GOLD;
-  float m[QB];
+  float m[QB], bias_lo = 0.f, bias_hi = 0.f;
   float4v l4[QB], o[QB][2 * KS];
 #pragma unroll
   for (int i = 0; i < QB; ++i) {
@@ -232,6 +268,8 @@ __global__ __launch_bounds__(RA_THREADS) void rel_attn_fwd_kernel(PdtRelAttn p) 
     uint64_t wn;
     const int cn = ra_next(p, s, c + 1, nc, wn);
     __syncthreads();  // every wave is done with the other buffer (first time: the bias array is complete)
+    bias_lo = bias.t[0];
+    bias_hi = bias.t[bias.len - 1];
     if (cn < nc) {
       stage(cn, buf ^ 1, wn);
       if (NH == 1) asm volatile("s_waitcnt vmcnt(4)" ::: "memory");
@@ -243,68 +281,78 @@ __global__ __launch_bounds__(RA_THREADS) void rel_attn_fwd_kernel(PdtRelAttn p) 
     if (active) {
       const char* kimg = smem + buf * BUF;
       const char* vimg = kimg + NH * RA_IMG;
-      float4v sc[QB][4];
-#pragma unroll
-      for (int kb = 0; kb < 4; ++kb) {
-#pragma unroll
-        for (int i = 0; i < QB; ++i) sc[i][kb] = splat4(0.f);
-#pragma unroll
-        for (int ks = 0; ks < KS; ++ks) {
-          const short8 kf = ra_row_frag(kimg, kb * 16, ks, lane);
-#pragma unroll
-          for (int i = 0; i < QB; ++i) sc[i][kb] = Half16<T>::mfma(kf, qf[i][ks], sc[i][kb]);
-        }
-      }
-      const bool whole = w == ~0ull;
-#pragma unroll
-      for (int i = 0; i < QB; ++i) {
-        float cmax = -INFINITY;
+      const int u0 = c * RA_CHUNK - q0;
+      const int side = has_bias ? ra_side(bias, u0 - 16 * (QB - 1), u0 + 48) : 1;
+      auto chunk = [&](auto near_tag, auto whole_tag) {
+        constexpr bool NEAR = decltype(near_tag)::value, WHOLE = decltype(whole_tag)::value;
+        const float4v flat = splat4(side < 0 ? bias_lo : bias_hi);
+        float4v sc[QB][4];
 #pragma unroll
         for (int kb = 0; kb < 4; ++kb) {
-          float4v t = sc[i][kb] * k2;
-          if (has_bias) t += ra_bias4(bias, boff, c * RA_CHUNK + kb * 16 - (q0 + 16 * i));
-          if (!whole) {
-            const uint32_t bits = (uint32_t)(w >> (kb * 16 + 4 * g));
 #pragma unroll
-            for (int r = 0; r < 4; ++r) t[r] = (bits >> r) & 1 ? t[r] : -INFINITY;
+          for (int i = 0; i < QB; ++i) sc[i][kb] = splat4(0.f);
+#pragma unroll
+          for (int ks = 0; ks < KS; ++ks) {
+            const short8 kf = ra_row_frag(kimg, kb * 16, ks, lane);
+#pragma unroll
+            for (int i = 0; i < QB; ++i) sc[i][kb] = Half16<T>::mfma(kf, qf[i][ks], sc[i][kb]);
           }
-          cmax = fmaxf(fmaxf(cmax, t[0]), fmaxf(fmaxf(t[1], t[2]), t[3]));
-          sc[i][kb] = t;
         }
-        cmax = quad_max(cmax);
-        const float m_new = fmaxf(m[i], cmax);
-        const float m_use = m_new == -INFINITY ? 0.f : m_new;  // no attended key so far: exp2(-inf - 0) = 0
-        const float alpha = __builtin_amdgcn_exp2f(m[i] - m_use);
-        m[i] = m_new;
-        l4[i] *= alpha;
 #pragma unroll
-        for (int db = 0; db < 2 * KS; ++db) o[i][db] *= alpha;
+        for (int i = 0; i < QB; ++i) {
+          float cmax = -INFINITY;
 #pragma unroll
-        for (int kb = 0; kb < 4; ++kb) {
-          float4v t = sc[i][kb] - m_use;
+          for (int kb = 0; kb < 4; ++kb) {
+            float4v t = sc[i][kb] * k2 + (NEAR ? ra_bias4(bias, boff, u0 + kb * 16 - 16 * i) : flat);
+            if (!WHOLE) {
+              const uint32_t bits = (uint32_t)(w >> (kb * 16 + 4 * g));
 #pragma unroll
-          for (int r = 0; r < 4; ++r) t[r] = __builtin_amdgcn_exp2f(t[r]);
-          l4[i] += t;
-          if (DROP) {
-#pragma unroll
-            for (int r = 0; r < 4; ++r)
-              t[r] *= attn_keep(seed[i], kmul0 + (uint32_t)(c * RA_CHUNK + kb * 16 + r) * ATT_GOLD, thr_hi) ? p.drop_scale : 0.f;
+              for (int r = 0; r < 4; ++r) t[r] = (bits >> r) & 1 ? t[r] : -INFINITY;
+            }
+            cmax = fmaxf(fmaxf(cmax, t[0]), fmaxf(fmaxf(t[1], t[2]), t[3]));
+            sc[i][kb] = t;
           }
-          sc[i][kb] = t;
+          // The accumulators are rescaled only when some row's maximum has grown by more than 2^RA_SLACK since its last
+          // rescale: p then stays below 2^RA_SLACK instead of 1, which 16-bit operands and fp32 sums hold as exactly.
+          if (__any(cmax > m[i] + RA_SLACK)) {
+            const float m_new = fmaxf(m[i], ra_quad_max(cmax));
+            const float alpha = __builtin_amdgcn_exp2f(m[i] - (m_new == -INFINITY ? 0.f : m_new));
+            m[i] = m_new;
+            l4[i] *= alpha;
+#pragma unroll
+            for (int db = 0; db < 2 * KS; ++db) o[i][db] *= alpha;
+          }
+          const float m_use = m[i] == -INFINITY ? 0.f : m[i];  // no attended key so far: exp2(-inf - 0) = 0
+#pragma unroll
+          for (int kb = 0; kb < 4; ++kb) {
+            float4v t = sc[i][kb] - m_use;
+#pragma unroll
+            for (int r = 0; r < 4; ++r) t[r] = __builtin_amdgcn_exp2f(t[r]);
+            l4[i] += t;
+            if (DROP) {
+#pragma unroll
+              for (int r = 0; r < 4; ++r)
+                t[r] *= attn_keep(seed[i], kmul0 + (uint32_t)(c * RA_CHUNK + kb * 16 + r) * ATT_GOLD, thr_hi) ? p.drop_scale : 0.f;
+            }
+            sc[i][kb] = t;
+          }
         }
-      }
 #pragma unroll
-      for (int pb = 0; pb < 2; ++pb) {
-        short8 pf[QB];
+        for (int pb = 0; pb < 2; ++pb) {
+          short8 pf[QB];
 #pragma unroll
-        for (int i = 0; i < QB; ++i) pf[i] = pack_pair<T>(sc[i][2 * pb], sc[i][2 * pb + 1]);
+          for (int i = 0; i < QB; ++i) pf[i] = pack_pair<T>(sc[i][2 * pb], sc[i][2 * pb + 1]);
 #pragma unroll
-        for (int db = 0; db < 2 * KS; ++db) {
-          const short8 vf = ra_tr_frag(vimg, pb * 32, db, lane);
+          for (int db = 0; db < 2 * KS; ++db) {
+            const short8 vf = ra_tr_frag(vimg, pb * 32, db, lane);
 #pragma unroll
-          for (int i = 0; i < QB; ++i) o[i][db] = Half16<T>::mfma(vf, pf[i], o[i][db]);
+            for (int i = 0; i < QB; ++i) o[i][db] = Half16<T>::mfma(vf, pf[i], o[i][db]);
+          }
         }
-      }
+      };
+      if (w != ~0ull) chunk(std::true_type{}, std::false_type{});
+      else if (side) chunk(std::false_type{}, std::true_type{});
+      else chunk(std::true_type{}, std::true_type{});
     }
     c = cn;
     w = wn;
@@ -314,7 +362,7 @@ __global__ __launch_bounds__(RA_THREADS) void rel_attn_fwd_kernel(PdtRelAttn p) 
 #pragma unroll
   for (int i = 0; i < QB; ++i) {
     const int q = q0 + 16 * i + lm;
-    const float l = quad_sum((l4[i][0] + l4[i][1]) + (l4[i][2] + l4[i][3]));
+    const float l = ra_quad_sum((l4[i][0] + l4[i][1]) + (l4[i][2] + l4[i][3]));
     // a row without an attended key has no probability mass: a zero output, and lse = +inf makes every p of backward 0
     // (l is NaN, not 0, when a score was: the output is then NaN as well)
     if (p.lse && g == 0 && q < s.n) p.lse[((int64_t)s.b * p.A + s.h) * p.S + q] = l == 0.f ? INFINITY : m[i] + __log2f(l);
@@ -322,12 +370,11 @@ __global__ __launch_bounds__(RA_THREADS) void rel_attn_fwd_kernel(PdtRelAttn p) 
   }
 }
 
-// Sum of ds over the distances: tile t (lane (lm, g): keys 4 g + r, query lm) of blocks u apart, into diag[u + off + ...].
+// Sum of ds over the distances: tile t (lane (lm, g): keys 4 g + r, query lm) of blocks u apart.
 // N: lane l holds the sum over r of the elements at (4 g + r, l + r), distance u + 4 g - l; W: those with l + r >= 16,
-// i.e. query l + r - 16, distance u + 4 g - l + 16 (lanes 13..15 only).  Lanes l in [4 i, 4 i + 4) of the four groups
-// write different distances, so the array needs one add per i for N and one for W, each to distinct addresses; adds of
-// one wave to its own array execute in order.
-__device__ __forceinline__ void ra_diag_add(float* diag, int at, const float4v& t, int lm, int g) {
+// i.e. query l + r - 16, distance u + 4 g - l + 16 (lanes 13..15 only).  Every lane group has an array of its own, so no two
+// lanes of an add meet; adds of one wave to its own arrays execute in order.
+__device__ __forceinline__ void ra_diag_add(float* d, const float4v& t, int lm) {
   float n = t[0];
   n += dpp_f<0x101>(t[1]);  // row_shl:1
   n += dpp_f<0x102>(t[2]);
@@ -335,17 +382,14 @@ __device__ __forceinline__ void ra_diag_add(float* diag, int at, const float4v& 
   float w = dpp_f<0x11F>(t[1]);  // row_shr:15
   w += dpp_f<0x11E>(t[2]);
   w += dpp_f<0x11D>(t[3]);
-  float* d = diag + at + 4 * g - lm;
-#pragma unroll
-  for (int i = 0; i < 4; ++i)
-    if ((lm >> 2) == i) atomicAdd(d, n);
+  atomicAdd(d, n);
   if (lm >= 13) atomicAdd(d + 16, w);
 }
 
 // ------------------------------------------------------------------------------------------------ dQ and the table gradient
 // One wave = 16 QB query rows, sweeps the keys; also stores delta = rowsum(dO * O) for the dK / dV kernel.
 template <typename T, int KS, int QB, bool DROP>
-__global__ __launch_bounds__(RA_THREADS) void rel_attn_dq_kernel(PdtRelAttn p) {
+__global__ __launch_bounds__(RA_THREADS) RA_OCC_BWD void rel_attn_dq_kernel(PdtRelAttn p) {
   constexpr int NH = (KS + 1) / 2, BUF = 2 * NH * RA_IMG;
   extern __shared__ __attribute__((aligned(16))) char smem[];
   const int tid = threadIdx.x, lane = tid & 63, lm = lane & 15, g = lane >> 4;
@@ -376,10 +420,15 @@ __global__ __launch_bounds__(RA_THREADS) void rel_attn_dq_kernel(PdtRelAttn p) {
   const RaBias bias = ra_bias_fill<T>(p, reinterpret_cast<float*>(smem + 2 * BUF), s.h, 1, tid);
   const int boff = ra_bias_lane(bias, lm, g);
   const bool has_bias = p.table != nullptr, active = q0 < s.n;
-  // diagonal sums of this wave: index 0 is distance -(far + 31)
-  const int dlen = 2 * bias.far + 80;
-  float* diag = bias.t + 4 * bias.len + wave * dlen;
-  for (int i = lane; i < dlen; i += 64) diag[i] = 0.f;
+  // diagonal sums, one array per wave and lane group: entry 0 is distance -(far + 31).  `diag` is where this lane's sum
+  // of a tile at u = 0 belongs.
+  const int dlen = ra_diag_len(p.max_distance);
+  float* const sums = bias.t + 4 * bias.len;
+  float* const diag = sums + (wave * 4 + g) * dlen + bias.far + 31 + 4 * g - lm;
+  if (part)
+    for (int i = tid; i < 4 * RA_WAVES * dlen; i += RA_THREADS) sums[i] = 0.f;
+  float bias_lo = 0.f, bias_hi = 0.f;
+  float4v far_lo = splat4(0.f), far_hi = splat4(0.f);
   short8 qf[QB][KS], df[QB][KS];
   uint32_t seed[QB];
   float nlse[QB], nd[QB];
@@ -396,7 +445,7 @@ __global__ __launch_bounds__(RA_THREADS) void rel_attn_dq_kernel(PdtRelAttn p) {
 #pragma unroll
       for (int j = 0; j < 8; ++j) d += Half16<T>::to_f(df[i][ks][j]) * Half16<T>::to_f(of[j]);
     }
-    d = quad_sum(d);
+    d = ra_quad_sum(d);
     if (g == 0 && q < s.n) p.delta[bh * p.S + q] = d;
     nd[i] = -d;
     nlse[i] = q < s.n ? -p.lse[bh * p.S + q] : -INFINITY;  // rows that are not there: p = 0
@@ -412,7 +461,9 @@ __global__ __launch_bounds__(RA_THREADS) void rel_attn_dq_kernel(PdtRelAttn p) {
   for (int buf = 0; c < nc; buf ^= 1) {
     uint64_t wn;
     const int cn = ra_next(p, s, c + 1, nc, wn);
-    __syncthreads();
+    __syncthreads();  // (first time: the arrays are complete)
+    bias_lo = bias.t[0];
+    bias_hi = bias.t[bias.len - 1];
     if (cn < nc) {
       stage(cn, buf ^ 1, wn);
       if (NH == 1) asm volatile("s_waitcnt vmcnt(4)" ::: "memory");
@@ -424,61 +475,82 @@ __global__ __launch_bounds__(RA_THREADS) void rel_attn_dq_kernel(PdtRelAttn p) {
     if (active) {
       const char* kimg = smem + buf * BUF;
       const char* vimg = kimg + NH * RA_IMG;
-      const bool whole = w == ~0ull;
+      const int u0 = c * RA_CHUNK - q0;
+      const int side = has_bias ? ra_side(bias, u0 - 16 * (QB - 1), u0 + 48) : 1;
+      auto chunk = [&](auto near_tag, auto whole_tag) {
+        constexpr bool NEAR = decltype(near_tag)::value, WHOLE = decltype(whole_tag)::value;
+        float4v flat[QB], ds[QB][4];
 #pragma unroll
-      for (int pb = 0; pb < 2; ++pb) {
-        float4v ds[QB][2];
+        for (int i = 0; i < QB; ++i) flat[i] = splat4((side < 0 ? bias_lo : bias_hi) + nlse[i]);
 #pragma unroll
-        for (int hb = 0; hb < 2; ++hb) {
-          const int kb = 2 * pb + hb;
-          float4v sc[QB], dp[QB];
+        for (int pb = 0; pb < 2; ++pb) {
 #pragma unroll
-          for (int i = 0; i < QB; ++i) { sc[i] = splat4(0.f); dp[i] = splat4(0.f); }
+          for (int hb = 0; hb < 2; ++hb) {
+            const int kb = 2 * pb + hb;
+            float4v sc[QB], dp[QB];
 #pragma unroll
-          for (int ks = 0; ks < KS; ++ks) {
-            const short8 kf = ra_row_frag(kimg, kb * 16, ks, lane), vf = ra_row_frag(vimg, kb * 16, ks, lane);
+            for (int i = 0; i < QB; ++i) { sc[i] = splat4(0.f); dp[i] = splat4(0.f); }
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks) {
+              const short8 kf = ra_row_frag(kimg, kb * 16, ks, lane), vf = ra_row_frag(vimg, kb * 16, ks, lane);
+#pragma unroll
+              for (int i = 0; i < QB; ++i) {
+                sc[i] = Half16<T>::mfma(kf, qf[i][ks], sc[i]);
+                dp[i] = Half16<T>::mfma(vf, df[i][ks], dp[i]);
+              }
+            }
+            const uint32_t bits = (uint32_t)(w >> (kb * 16 + 4 * g));
 #pragma unroll
             for (int i = 0; i < QB; ++i) {
-              sc[i] = Half16<T>::mfma(kf, qf[i][ks], sc[i]);
-              dp[i] = Half16<T>::mfma(vf, df[i][ks], dp[i]);
+              float4v t = sc[i] * k2 + (NEAR ? ra_bias4(bias, boff, u0 + kb * 16 - 16 * i) + nlse[i] : flat[i]);
+#pragma unroll
+              for (int r = 0; r < 4; ++r) t[r] = __builtin_amdgcn_exp2f(t[r]);
+              if (!WHOLE) {
+#pragma unroll
+                for (int r = 0; r < 4; ++r) t[r] = (bits >> r) & 1 ? t[r] : 0.f;
+              }
+              float4v e = dp[i];
+              if (DROP) {
+#pragma unroll
+                for (int r = 0; r < 4; ++r)
+                  e[r] *= attn_keep(seed[i], kmul0 + (uint32_t)(c * RA_CHUNK + kb * 16 + r) * ATT_GOLD, thr_hi) ? p.drop_scale : 0.f;
+              }
+              ds[i][kb] = t * (e + nd[i]);
             }
           }
-          const uint32_t bits = (uint32_t)(w >> (kb * 16 + 4 * g));
+          short8 sf[QB];
 #pragma unroll
-          for (int i = 0; i < QB; ++i) {
-            const int u = c * RA_CHUNK + kb * 16 - (q0 + 16 * i);
-            float4v t = sc[i] * k2 + nlse[i];
-            if (has_bias) t += ra_bias4(bias, boff, u);
+          for (int i = 0; i < QB; ++i) sf[i] = pack_pair<T>(ds[i][2 * pb], ds[i][2 * pb + 1]);
 #pragma unroll
-            for (int r = 0; r < 4; ++r) t[r] = __builtin_amdgcn_exp2f(t[r]);
-            if (!whole) {
+          for (int db = 0; db < 2 * KS; ++db) {
+            const short8 kf = ra_tr_frag(kimg, pb * 32, db, lane);
 #pragma unroll
-              for (int r = 0; r < 4; ++r) t[r] = (bits >> r) & 1 ? t[r] : 0.f;
-            }
-            float4v e = dp[i];
-            if (DROP) {
-#pragma unroll
-              for (int r = 0; r < 4; ++r)
-                e[r] *= attn_keep(seed[i], kmul0 + (uint32_t)(c * RA_CHUNK + kb * 16 + r) * ATT_GOLD, thr_hi) ? p.drop_scale : 0.f;
-            }
-            e = t * (e + nd[i]);
-            if (part) {
-              const int uc = min(max(u, -(bias.far + 16)), bias.far + 16);
-              ra_diag_add(diag, uc + bias.far + 31, e, lm, g);
-            }
-            ds[i][hb] = e;
+            for (int i = 0; i < QB; ++i) dq[i][db] = Half16<T>::mfma(kf, sf[i], dq[i][db]);
           }
         }
-        short8 df_[QB];
+        if (part) {
+          if (NEAR) {  // tiles of the same offset u = u0 + 16 (kb - i) first add up
 #pragma unroll
-        for (int i = 0; i < QB; ++i) df_[i] = pack_pair<T>(ds[i][0], ds[i][1]);
+            for (int j = 1 - QB; j < 4; ++j) {
+              float4v t = splat4(0.f);
 #pragma unroll
-        for (int db = 0; db < 2 * KS; ++db) {
-          const short8 kf = ra_tr_frag(kimg, pb * 32, db, lane);
+              for (int i = 0; i < QB; ++i)
+                if (j + i >= 0 && j + i < 4) t += ds[i][j + i];
+              const int u = min(max(u0 + 16 * j, -(bias.far + 16)), bias.far + 16);
+              ra_diag_add(diag + u, t, lm);
+            }
+          } else {
+            float4v t = splat4(0.f);
 #pragma unroll
-          for (int i = 0; i < QB; ++i) dq[i][db] = Half16<T>::mfma(kf, df_[i], dq[i][db]);
+            for (int i = 0; i < QB; ++i) t += (ds[i][0] + ds[i][1]) + (ds[i][2] + ds[i][3]);
+            if (side < 0) far_lo += t;
+            else far_hi += t;
+          }
         }
-      }
+      };
+      if (w != ~0ull) chunk(std::true_type{}, std::false_type{});
+      else if (side) chunk(std::false_type{}, std::true_type{});
+      else chunk(std::true_type{}, std::true_type{});
     }
     c = cn;
     w = wn;
@@ -491,21 +563,29 @@ __global__ __launch_bounds__(RA_THREADS) void rel_attn_dq_kernel(PdtRelAttn p) {
       ra_store<T, KS>(dqb + (int64_t)q * p.dq.row, dq[i], p.scale, g, p.D, q < s.n);
     }
   }
-  if (part) {  // distances -> buckets: eight lanes per bucket walk its range of distances over the four waves' arrays
+  if (part) {  // the far sums join the ends of their wave's first array; then distances -> buckets
+    const float lo = wave_sum((far_lo[0] + far_lo[1]) + (far_lo[2] + far_lo[3]));
+    const float hi = wave_sum((far_hi[0] + far_hi[1]) + (far_hi[2] + far_hi[3]));
+    if (lane == 0) {
+      sums[wave * 4 * dlen] += lo;
+      sums[wave * 4 * dlen + 2 * bias.far + 62] += hi;
+    }
     __syncthreads();
-    const float* all = bias.t + 4 * bias.len;
+    for (int i = tid; i < dlen; i += RA_THREADS) {  // (the sixteen arrays into the first)
+      float t = 0.f;
+#pragma unroll
+      for (int a = 0; a < 4 * RA_WAVES; ++a) t += sums[a * dlen + i];
+      sums[i] = t;
+    }
+    __syncthreads();
     const int half = p.buckets >> 1, exact = half >> 1, top = bias.far + 31;
-    for (int b0 = 0; b0 < p.buckets; b0 += RA_THREADS / 8) {
+    for (int b0 = 0; b0 < p.buckets; b0 += RA_THREADS / 8) {  // eight lanes per bucket walk its range of distances
       const int b = b0 + (tid >> 3), j = b >= half ? b - half : b;
       float sum = 0.f;
       if (b < p.buckets) {
         int lo = j < exact ? j : p.steps[j - exact], hi = j < exact ? j : (j == half - 1 ? top : p.steps[j + 1 - exact] - 1);
-        if (j < exact && j == half - 1) hi = top;
         if (b >= half) lo = max(lo, 1);
-        for (int n = lo + (tid & 7); n <= hi; n += 8) {
-          const int at = (b >= half ? n : -n) + top;
-          sum += (all[at] + all[dlen + at]) + (all[2 * dlen + at] + all[3 * dlen + at]);
-        }
+        for (int n = lo + (tid & 7); n <= hi; n += 8) sum += sums[(b >= half ? n : -n) + top];
       }
       sum += __shfl_xor(sum, 1, 64);
       sum += __shfl_xor(sum, 2, 64);
@@ -516,15 +596,15 @@ __global__ __launch_bounds__(RA_THREADS) void rel_attn_dq_kernel(PdtRelAttn p) {
 }
 
 // ------------------------------------------------------------------------------------------------ dK, dV
-// One wave = 16 KB keys, sweeps the queries (Q and dO images); lse, delta and dropout seeds of a chunk's queries in LDS.
-template <typename T, int KS, int KB, bool DROP>
-__global__ __launch_bounds__(RA_THREADS) void rel_attn_dkv_kernel(PdtRelAttn p) {
+// One wave = 16 QB keys, sweeps the queries (Q and dO images); lse, delta and dropout seeds of a chunk's queries in LDS.
+template <typename T, int KS, int QB, bool DROP>
+__global__ __launch_bounds__(RA_THREADS) RA_OCC_BWD void rel_attn_dkv_kernel(PdtRelAttn p) {
   constexpr int NH = (KS + 1) / 2, BUF = 2 * NH * RA_IMG + 1024;  // Q | dO | lse, delta, seeds (64 each), 256 spare bytes
   extern __shared__ __attribute__((aligned(16))) char smem[];
   const int tid = threadIdx.x, lane = tid & 63, lm = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const RaSpan s = ra_span(p, blockIdx.x);
-  const int w0 = blockIdx.y * (RA_WAVES * 16 * KB), k0 = w0 + wave * 16 * KB;
+  const int w0 = blockIdx.y * (RA_WAVES * 16 * QB), k0 = w0 + wave * 16 * QB;
   if (w0 >= s.n) return;
   const bool packed = p.cu != nullptr;
   const T* qb_ = ra_base<const T>(p.q, s, packed);
@@ -553,13 +633,15 @@ __global__ __launch_bounds__(RA_THREADS) void rel_attn_dkv_kernel(PdtRelAttn p) 
   const RaBias bias = ra_bias_fill<T>(p, reinterpret_cast<float*>(smem + 2 * BUF), s.h, -1, tid);
   const int boff = ra_bias_lane(bias, lm, g);
   const bool has_bias = p.table != nullptr;
-  short8 kf[KB][KS], vf[KB][KS];
-  bool kok[KB];
-  uint32_t kmul[KB];
+  short8 kf[QB][KS], vf[QB][KS];
+  bool kok[QB];
+  uint32_t kmul[QB];
   const uint64_t kw = k0 < s.n ? ra_word(p, s, k0 / RA_CHUNK) >> (k0 % RA_CHUNK) : 0;
-  const bool active = (kw & (KB == 2 ? 0xFFFFFFFFull : 0xFFFFull)) != 0;  // (a wave's keys lie in one chunk)
+  constexpr uint64_t MINE = QB == 2 ? 0xFFFFFFFFull : 0xFFFFull;  // (a wave's keys lie in one chunk)
+  const bool active = (kw & MINE) != 0, all_keys = (kw & MINE) == MINE;
+  float bias_lo = 0.f, bias_hi = 0.f;
 #pragma unroll
-  for (int i = 0; i < KB; ++i) {
+  for (int i = 0; i < QB; ++i) {
     const int key = k0 + 16 * i + lm;
     kok[i] = (kw >> (16 * i + lm)) & 1;
     kmul[i] = (uint32_t)key * ATT_GOLD;
@@ -571,13 +653,15 @@ __global__ __launch_bounds__(RA_THREADS) void rel_attn_dkv_kernel(PdtRelAttn p) 
   }
   const float k2 = p.scale * LOG2E;
   const uint32_t thr_hi = attn_thr_hi(p.drop_thr);
-  float4v dk_[KB][2 * KS], dv_[KB][2 * KS];
+  float4v dk_[QB][2 * KS], dv_[QB][2 * KS];
 #pragma unroll
-  for (int i = 0; i < KB; ++i)
+  for (int i = 0; i < QB; ++i)
 #pragma unroll
     for (int db = 0; db < 2 * KS; ++db) { dk_[i][db] = splat4(0.f); dv_[i][db] = splat4(0.f); }
   for (int c = 0, buf = 0; c < nc; ++c, buf ^= 1) {
-    __syncthreads();
+    __syncthreads();  // (first time: the bias array is complete)
+    bias_lo = bias.t[0];
+    bias_hi = bias.t[bias.len - 1];
     if (c + 1 < nc) {
       stage(c + 1, buf ^ 1);
       if (NH == 1) asm volatile("s_waitcnt vmcnt(5)" ::: "memory");
@@ -590,21 +674,25 @@ __global__ __launch_bounds__(RA_THREADS) void rel_attn_dkv_kernel(PdtRelAttn p) 
     const char* qimg = smem + buf * BUF;
     const char* gimg = qimg + NH * RA_IMG;
     const float* sc_ = reinterpret_cast<const float*>(gimg + NH * RA_IMG);
-    const int left = s.n - c * RA_CHUNK;
+    const int left = s.n - c * RA_CHUNK, u0 = c * RA_CHUNK - k0;  // (query - key: the array is mirrored)
+    const int side = has_bias ? ra_side(bias, u0 - 16 * (QB - 1), u0 + 48) : 1;
+    auto chunk = [&](auto near_tag, auto whole_tag) {
+    constexpr bool NEAR = decltype(near_tag)::value, WHOLE = decltype(whole_tag)::value;
+    const float flat = side < 0 ? bias_lo : bias_hi;
 #pragma unroll
     for (int pb = 0; pb < 2; ++pb) {
-      float4v pp[KB][2], ds[KB][2];
+      float4v pp[QB][2], ds[QB][2];
 #pragma unroll
       for (int hb = 0; hb < 2; ++hb) {
         const int qb = 2 * pb + hb;
-        float4v sc[KB], dp[KB];
+        float4v sc[QB], dp[QB];
 #pragma unroll
-        for (int i = 0; i < KB; ++i) { sc[i] = splat4(0.f); dp[i] = splat4(0.f); }
+        for (int i = 0; i < QB; ++i) { sc[i] = splat4(0.f); dp[i] = splat4(0.f); }
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks) {
           const short8 qf = ra_row_frag(qimg, qb * 16, ks, lane), gf = ra_row_frag(gimg, qb * 16, ks, lane);
 #pragma unroll
-          for (int i = 0; i < KB; ++i) {
+          for (int i = 0; i < QB; ++i) {
             sc[i] = Half16<T>::mfma(qf, kf[i][ks], sc[i]);
             dp[i] = Half16<T>::mfma(gf, vf[i][ks], dp[i]);
           }
@@ -613,17 +701,17 @@ __global__ __launch_bounds__(RA_THREADS) void rel_attn_dkv_kernel(PdtRelAttn p) 
         const float4v del = *reinterpret_cast<const float4v*>(sc_ + 64 + qb * 16 + 4 * g);
         const uint4v sd = *reinterpret_cast<const uint4v*>(sc_ + 128 + qb * 16 + 4 * g);
 #pragma unroll
-        for (int i = 0; i < KB; ++i) {
-          float4v t = sc[i] * k2 - lse;
-          if (has_bias) t += ra_bias4(bias, boff, c * RA_CHUNK + qb * 16 - (k0 + 16 * i));
-          if (left < RA_CHUNK) {  // queries that are not there
+        for (int i = 0; i < QB; ++i) {
+          float4v t = sc[i] * k2 + ((NEAR ? ra_bias4(bias, boff, u0 + qb * 16 - 16 * i) : splat4(flat)) - lse);
+          if (!WHOLE) {  // queries that are not there
 #pragma unroll
             for (int r = 0; r < 4; ++r) t[r] = qb * 16 + 4 * g + r < left ? t[r] : -INFINITY;
           }
           float4v e = dp[i], pd;
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
-            t[r] = kok[i] ? __builtin_amdgcn_exp2f(t[r]) : 0.f;
+            t[r] = __builtin_amdgcn_exp2f(t[r]);
+            if (!WHOLE) t[r] = kok[i] ? t[r] : 0.f;
             const float keep = !DROP ? 1.f : (attn_keep(sd[r], kmul[i], thr_hi) ? p.drop_scale : 0.f);
             pd[r] = DROP ? t[r] * keep : t[r];
             if (DROP) e[r] *= keep;
@@ -632,24 +720,28 @@ __global__ __launch_bounds__(RA_THREADS) void rel_attn_dkv_kernel(PdtRelAttn p) 
           ds[i][hb] = t * (e - del);
         }
       }
-      short8 pf[KB], sf[KB];
+      short8 pf[QB], sf[QB];
 #pragma unroll
-      for (int i = 0; i < KB; ++i) { pf[i] = pack_pair<T>(pp[i][0], pp[i][1]); sf[i] = pack_pair<T>(ds[i][0], ds[i][1]); }
+      for (int i = 0; i < QB; ++i) { pf[i] = pack_pair<T>(pp[i][0], pp[i][1]); sf[i] = pack_pair<T>(ds[i][0], ds[i][1]); }
 #pragma unroll
       for (int db = 0; db < 2 * KS; ++db) {
         const short8 gf = ra_tr_frag(gimg, pb * 32, db, lane), qf = ra_tr_frag(qimg, pb * 32, db, lane);
 #pragma unroll
-        for (int i = 0; i < KB; ++i) {
+        for (int i = 0; i < QB; ++i) {
           dv_[i][db] = Half16<T>::mfma(gf, pf[i], dv_[i][db]);
           dk_[i][db] = Half16<T>::mfma(qf, sf[i], dk_[i][db]);
         }
       }
     }
+    };
+    if (left < RA_CHUNK || !all_keys) chunk(std::true_type{}, std::false_type{});
+    else if (side) chunk(std::false_type{}, std::true_type{});
+    else chunk(std::true_type{}, std::true_type{});
   }
   T* dkb = ra_base<T>(p.dk, s, packed);
   T* dvb = ra_base<T>(p.dv, s, packed);
 #pragma unroll
-  for (int i = 0; i < KB; ++i) {
+  for (int i = 0; i < QB; ++i) {
     const int key = k0 + 16 * i + lm;
     ra_store<T, KS>(dkb + (int64_t)key * p.dk.row, dk_[i], p.scale, g, p.D, key < s.n);
     ra_store<T, KS>(dvb + (int64_t)key * p.dv.row, dv_[i], 1.0f, g, p.D, key < s.n);
@@ -699,7 +791,15 @@ static int ra_allow_lds(const void* kern, size_t bytes) {
   return 0;
 }
 
-constexpr int RA_QB = 1;  // 16-row blocks per wave
+// 16-row blocks per wave.  Two share every row that a wave reads from LDS, which is what bounds long sequences (2 x 4096
+// tokens, 16 heads, dim 64: forward 266 -> 198 us), but halve the number of workgroups and leave waves without rows when a
+// sequence has fewer than 128: used from two workgroups per CU on (4 x 1001 tokens, 8 heads, dim 128, 256 workgroups: forward
+// 47 us with one block, 61 us with two), and not beyond 64 columns in the backward kernels, whose accumulators would not fit
+// the registers of two waves per SIMD.
+static int ra_blocks(const PdtRelAttn& p, bool backward) {
+  const int64_t len = p.cu ? (p.B ? p.T / p.B : 0) : p.S;  // (packed: the average)
+  return len > 64 && (int64_t)p.B * p.A * ((len + 127) / 128) >= 512 && !(backward && p.D > 64) ? 2 : 1;
+}
 
 static size_t ra_bias_bytes(const PdtRelAttn& p) { return (size_t)4 * ra_bias_len(p.max_distance) * sizeof(float); }
 
@@ -713,15 +813,20 @@ static int ra_launch(KernT kern, const PdtRelAttn& p, int rows_per_block, size_t
 // which: 0 forward, 1 dQ + table gradient, 2 dK / dV
 template <typename T, int KS, bool DROP>
 static int ra_dispatch(int which, const PdtRelAttn& p, hipStream_t st) {
-  constexpr int NH = (KS + 1) / 2;
-  const int rows = RA_WAVES * 16 * RA_QB;
+  constexpr int NH = (KS + 1) / 2, QB2 = KS <= 2 ? 2 : 1;  // (two blocks per wave in the backward kernels)
+  const bool two = ra_blocks(p, which != 0) == 2;
+  const int rows = RA_WAVES * 16 * (two ? 2 : 1);
   const size_t imgs = (size_t)4 * NH * RA_IMG, tab = ra_bias_bytes(p);
-  if (which == 0) return ra_launch(rel_attn_fwd_kernel<T, KS, RA_QB, DROP>, p, rows, imgs + tab, st);
+  if (which == 0)
+    return two ? ra_launch(rel_attn_fwd_kernel<T, KS, 2, DROP>, p, rows, imgs + tab, st)
+               : ra_launch(rel_attn_fwd_kernel<T, KS, 1, DROP>, p, rows, imgs + tab, st);
   if (which == 1) {
-    const size_t diag = (size_t)RA_WAVES * (2 * ((p.max_distance + 15) & ~15) + 80) * sizeof(float);
-    return ra_launch(rel_attn_dq_kernel<T, KS, RA_QB, DROP>, p, rows, imgs + tab + diag, st);
+    const size_t diag = p.dtable_part ? (size_t)4 * RA_WAVES * ra_diag_len(p.max_distance) * sizeof(float) : 0;
+    return two ? ra_launch(rel_attn_dq_kernel<T, KS, QB2, DROP>, p, rows, imgs + tab + diag, st)
+               : ra_launch(rel_attn_dq_kernel<T, KS, 1, DROP>, p, rows, imgs + tab + diag, st);
   }
-  return ra_launch(rel_attn_dkv_kernel<T, KS, RA_QB, DROP>, p, rows, imgs + 2048 + tab, st);
+  return two ? ra_launch(rel_attn_dkv_kernel<T, KS, QB2, DROP>, p, rows, imgs + 2048 + tab, st)
+             : ra_launch(rel_attn_dkv_kernel<T, KS, 1, DROP>, p, rows, imgs + 2048 + tab, st);
 }
 template <typename T>
 static int ra_dispatch_ks(int which, const PdtRelAttn& p, hipStream_t st) {
@@ -786,7 +891,7 @@ extern "C" int pdt_rel_attn_fwd(int dtype, const PdtRelAttn* a, void* stream) {
 }
 
 extern "C" int pdt_rel_attn_dtable_rows(const PdtRelAttn* a) {
-  const int rows = RA_WAVES * 16 * RA_QB;
+  const int rows = RA_WAVES * 16 * ra_blocks(*a, true);
   return a->B * ((a->S + rows - 1) / rows);
 }
 

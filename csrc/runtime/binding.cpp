@@ -550,6 +550,57 @@ std::vector<Tensor> rel_attn_backward(const Tensor& dout, const Tensor& q_in, co
   return {dq, dk, dv, dtable};
 }
 
+// The two calls above as one differentiable operation (in C++: a training pass over short packed batches is bound by the
+// host, and the Python form of this node cost it 30 us more).
+OptTensor opt(const Tensor& t) { return t.defined() ? OptTensor(t) : OptTensor(); }
+struct RelAttnNode : public torch::autograd::Function<RelAttnNode> {
+  static Tensor forward(torch::autograd::AutogradContext* ctx, const Tensor& q, const Tensor& k, const Tensor& v, const OptTensor& table,
+                        int64_t max_distance, std::vector<int64_t> steps, const OptTensor& bits, const OptTensor& cu,
+                        int64_t max_seqlen, double scale, const OptTensor& rng_state, double p, int64_t micro, int64_t site,
+                        const OptTensor& sids, bool wanted) {
+    std::vector<Tensor> r = rel_attn_forward(q, k, v, table, max_distance, steps, bits, cu, max_seqlen, scale, rng_state, p, micro,
+                                             site, sids, wanted);
+    if (wanted) {
+      auto t = [](const OptTensor& x) { return x.has_value() ? *x : Tensor(); };
+      ctx->save_for_backward({q, k, v, t(table), r[0], r[1], t(bits), t(cu), t(rng_state), t(sids)});
+      ctx->saved_data["steps"] = steps;
+      ctx->saved_data["ints"] = std::vector<int64_t>{max_distance, max_seqlen, micro, site};
+      ctx->saved_data["floats"] = std::vector<double>{scale, p};
+    }
+    return r[0];
+  }
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list dout) {
+    TORCH_CHECK(!at::GradMode::is_enabled(), "relative_attention is not twice differentiable");
+    const auto t = ctx->get_saved_variables();
+    const auto ints = ctx->saved_data["ints"].toIntVector();
+    const auto floats = ctx->saved_data["floats"].toDoubleVector();
+    std::vector<Tensor> g = rel_attn_backward(dout[0], t[0], t[1], t[2], t[4], t[5], opt(t[3]), ints[0], ctx->saved_data["steps"].toIntVector(),
+                                              opt(t[6]), opt(t[7]), ints[1], floats[0], opt(t[8]), floats[1], ints[2], ints[3],
+                                              opt(t[9]), t[3].defined() && ctx->needs_input_grad(3));
+    torch::autograd::variable_list out(16);
+    for (int i = 0; i < 3; ++i) out[i] = g[i];
+    if (g[3].defined()) out[3] = g[3].to(t[3].scalar_type());
+    return out;
+  }
+};
+Tensor rel_mask_bits(const Tensor& mask);
+// `key_mask`: [B, S] as rel_mask_bits() takes it, or int64 bits that it made
+Tensor relative_attention(const Tensor& q, const Tensor& k, const Tensor& v, const OptTensor& table, int64_t max_distance,
+                          const std::vector<int64_t>& steps, const OptTensor& key_mask, const OptTensor& cu, int64_t max_seqlen,
+                          double scale, const OptTensor& rng_state, double p, int64_t micro, int64_t site, const OptTensor& sids) {
+  TORCH_CHECK(q.is_cuda(), "q must be on the GPU");
+  OptTensor bits;
+  if (key_mask.has_value()) {
+    same_gpu(*key_mask, q, "key_mask");
+    bits = rel_mask_bits(*key_mask);
+  }
+  const bool wanted = at::GradMode::is_enabled() && (q.requires_grad() || k.requires_grad() || v.requires_grad() ||
+                                                     (table.has_value() && table->requires_grad()));
+  if (!wanted)
+    return rel_attn_forward(q, k, v, table, max_distance, steps, bits, cu, max_seqlen, scale, rng_state, p, micro, site, sids, false)[0];
+  return RelAttnNode::apply(q, k, v, table, max_distance, steps, bits, cu, max_seqlen, scale, rng_state, p, micro, site, sids, true);
+}
+
 // ---- per-head norm + rotation
 struct RopeCall {
   const OptTensor &wq, &wk, &cos, &sin, &pos;
@@ -656,6 +707,41 @@ std::vector<Tensor> qk_rope_backward(const Tensor& dyq, const Tensor& dyk, const
   rope_backward_into(dyq, dyk, q, k, RopeCall{wq, wk, cos, sin, pos, interleaved, eps}, dxq, dxk,
                      dwq.defined() ? dwq.data_ptr<float>() : nullptr, dwk.defined() ? dwk.data_ptr<float>() : nullptr, false);
   return {dxq, dxk, dwq, dwk};
+}
+struct QkRopeNode : public torch::autograd::Function<QkRopeNode> {
+  static torch::autograd::variable_list forward(torch::autograd::AutogradContext* ctx, const Tensor& q, const Tensor& k,
+                                                const OptTensor& wq, const OptTensor& wk, const OptTensor& cos, const OptTensor& sin,
+                                                const OptTensor& pos, bool interleaved, double eps) {
+    std::vector<Tensor> y = qk_rope_forward(q, k, wq, wk, cos, sin, pos, interleaved, eps);
+    auto t = [](const OptTensor& x) { return x.has_value() ? *x : Tensor(); };
+    ctx->save_for_backward({q, k, t(wq), t(wk), t(cos), t(sin), t(pos)});
+    ctx->saved_data["interleaved"] = interleaved;
+    ctx->saved_data["eps"] = eps;
+    return y;
+  }
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list dy) {
+    TORCH_CHECK(!at::GradMode::is_enabled(), "qk_norm_rope is not twice differentiable");
+    const auto t = ctx->get_saved_variables();
+    const bool want_dw = t[2].defined() && (ctx->needs_input_grad(2) || ctx->needs_input_grad(3));
+    std::vector<Tensor> g = qk_rope_backward(dy[0], dy[1], t[0], t[1], opt(t[2]), opt(t[3]), opt(t[4]), opt(t[5]), opt(t[6]),
+                                             ctx->saved_data["interleaved"].toBool(), ctx->saved_data["eps"].toDouble(), want_dw);
+    torch::autograd::variable_list out(9);
+    out[0] = g[0];
+    out[1] = g[1];
+    if (want_dw) {
+      out[2] = g[2].to(t[2].scalar_type());
+      out[3] = g[3].to(t[3].scalar_type());
+    }
+    return out;
+  }
+};
+std::vector<Tensor> qk_norm_rope(const Tensor& q, const Tensor& k, const OptTensor& wq, const OptTensor& wk, const OptTensor& cos,
+                                 const OptTensor& sin, const OptTensor& pos, bool interleaved, double eps) {
+  TORCH_CHECK(q.is_cuda(), "q must be on the GPU");
+  const bool wanted = at::GradMode::is_enabled() && (q.requires_grad() || k.requires_grad() || (wq.has_value() && wq->requires_grad()) ||
+                                                     (wk.has_value() && wk->requires_grad()));
+  if (!wanted) return qk_rope_forward(q, k, wq, wk, cos, sin, pos, interleaved, eps);
+  return QkRopeNode::apply(q, k, wq, wk, cos, sin, pos, interleaved, eps);
 }
 
 // ---------------------------------------------------------------------------------------------------
@@ -1216,6 +1302,8 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("rel_mask_bits", &rel_mask_bits);
   m.def("rel_attn_forward", &rel_attn_forward, nogil());
   m.def("rel_attn_backward", &rel_attn_backward, nogil());
+  m.def("relative_attention", &relative_attention, nogil());
+  m.def("qk_norm_rope", &qk_norm_rope, nogil());
   m.def("qk_rope_forward", &qk_rope_forward, nogil());
   m.def("qk_rope_backward", &qk_rope_backward, nogil());
   m.def("adamw_step", &adamw_step);

@@ -53,30 +53,6 @@ def mask_bits(key_mask: torch.Tensor) -> torch.Tensor:
     return native().rel_mask_bits(key_mask)
 
 
-class _RelAttnFn(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, q, k, v, bias, max_distance, steps, bits, cu, max_seqlen, scale, rng, p, site):
-        state, micro, sids = (rng.state, rng.counter, rng.sample_ids) if rng is not None else (None, 0, None)
-        wanted = any(ctx.needs_input_grad[:4])
-        out, lse = native().rel_attn_forward(q, k, v, bias, max_distance, steps, bits, cu, max_seqlen, scale, state, p, micro,
-                                             site, sids, wanted)
-        if wanted:
-            ctx.save_for_backward(q, k, v, bias, out, lse, bits, cu, state, sids)
-            ctx.meta = (max_distance, steps, max_seqlen, scale, p, micro, site)
-        return out
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, dout):
-        q, k, v, bias, out, lse, bits, cu, state, sids = ctx.saved_tensors
-        max_distance, steps, max_seqlen, scale, p, micro, site = ctx.meta
-        dq, dk, dv, dbias = native().rel_attn_backward(dout, q, k, v, out, lse, bias, max_distance, steps, bits, cu, max_seqlen,
-                                                       scale, state, p, micro, site, sids, ctx.needs_input_grad[3])
-        if dbias is not None:
-            dbias = dbias.to(bias.dtype)
-        return (dq, dk, dv, dbias) + (None,) * 9
-
-
 def relative_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, bias: Optional[torch.Tensor] = None, *,
                        max_distance: int = 128, key_mask: Optional[torch.Tensor] = None,
                        cu_seqlens: Optional[torch.Tensor] = None, max_seqlen: Optional[int] = None,
@@ -105,7 +81,6 @@ def relative_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, bias: 
     """
     if q.dim() not in (3, 4) or (q.dim() == 3) != (cu_seqlens is not None):
         raise ValueError("q, k, v must be [B, S, heads, dim], or packed [T, heads, dim] with cu_seqlens")
-    bits = None
     if cu_seqlens is not None:
         if key_mask is not None:
             raise ValueError("packed rows take no key mask: leave the masked keys out of the rows")
@@ -116,9 +91,8 @@ def relative_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, bias: 
             raise ValueError(f"key_mask must be [B, S] = {tuple(q.shape[:2])}, got {tuple(key_mask.shape)}")
         if key_mask.is_floating_point():
             raise ValueError("key_mask holds truth values (non-zero = attended), not additive scores")
-        if key_mask.device != q.device:
-            raise ValueError("key_mask must be on the device of q")
-        bits = mask_bits(key_mask)
+        if key_mask.dtype == torch.int64:
+            key_mask = key_mask.ne(0)
     steps: Tuple[int, ...] = ()
     if bias is not None:
         if bias.dim() != 2:
@@ -132,8 +106,9 @@ def relative_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, bias: 
         raise ValueError("dropout needs rng, the key of the forward pass")
     if scale is None:
         scale = 1.0 / math.sqrt(q.shape[-1])
-    return _RelAttnFn.apply(q, k, v, bias, max_distance, steps, bits, cu_seqlens, int(max_seqlen or 0), float(scale), rng,
-                            float(dropout_p), int(site))
+    state, micro, sids = (rng.state, rng.counter, rng.sample_ids) if dropout_p > 0.0 else (None, 0, None)
+    return native().relative_attention(q, k, v, bias, max_distance, steps, key_mask, cu_seqlens, int(max_seqlen or 0), scale, state,
+                                       dropout_p, micro, site, sids)
 
 
 def relative_attention_reference(q, k, v, bias=None, *, max_distance=128, key_mask=None, scale=None, dropout_p=0.0, training=False):

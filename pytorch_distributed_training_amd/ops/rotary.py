@@ -18,27 +18,6 @@ def rotary_table(positions: int, dim: int, base: float = 10000.0, device="cuda")
     return angles.cos().float(), angles.sin().float()
 
 
-class _QkRopeFn(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, q, k, wq, wk, cos, sin, pos, interleaved, eps):
-        yq, yk = native().qk_rope_forward(q, k, wq, wk, cos, sin, pos, interleaved, eps)
-        # without a norm the gradient does not depend on the rows
-        ctx.save_for_backward(q, k, wq, wk, cos, sin, pos)
-        ctx.meta = (interleaved, eps)
-        return yq, yk
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, dyq, dyk):
-        q, k, wq, wk, cos, sin, pos = ctx.saved_tensors
-        interleaved, eps = ctx.meta
-        dq, dk, dwq, dwk = native().qk_rope_backward(dyq, dyk, q, k, wq, wk, cos, sin, pos, interleaved, eps,
-                                                     ctx.needs_input_grad[2] or ctx.needs_input_grad[3])
-        if dwq is not None:
-            dwq, dwk = dwq.to(wq.dtype), dwk.to(wk.dtype)
-        return dq, dk, dwq, dwk, None, None, None, None, None
-
-
 def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, q_weight: Optional[torch.Tensor] = None,
                  k_weight: Optional[torch.Tensor] = None, *, rope: Optional[Tuple[torch.Tensor, torch.Tensor]] = None,
                  positions: Optional[torch.Tensor] = None, interleaved: bool = False,
@@ -66,7 +45,8 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, q_weight: Optional[torch.Tens
     for name, t in (("cos", cos), ("sin", sin)):
         if t is not None and t.requires_grad:
             raise ValueError(f"{name} is a table of constants: no gradient is formed for it")
-    return _QkRopeFn.apply(q, k, q_weight, k_weight, cos, sin, positions, bool(interleaved), float(eps))
+    yq, yk = native().qk_norm_rope(q, k, q_weight, k_weight, cos, sin, positions, interleaved, eps)
+    return yq, yk
 
 
 def qk_norm_rope_reference(x: torch.Tensor, weight=None, *, rope=None, positions=None, interleaved=False, eps=1e-6):
