@@ -55,6 +55,17 @@ PER_SOURCE_FLAGS = {"attention.hip": ["-fno-slp-vectorize"],
                     "rel_attention.hip": ["-fno-slp-vectorize", "-mllvm", "-amdgpu-mfma-vgpr-form=1"]}
 
 
+# (no packed fp32 instructions: hipcc -O3 forms v_pk_add / mul / fma_f32 from ordinary float code, and some of their forms
+# have given wrong results on this hardware now and then; the host pass warns that it does not know the feature)
+DEVICE_FLAGS = [f"--offload-arch={ARCH}", "-O3", "-std=c++17", "-fPIC", "-ffp-contract=fast", "-Wno-unused-result",
+                "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
+
+
+def kernel_flags(name: str):
+    """hipcc flags of a kernel source (tests look at the code they produce)."""
+    return DEVICE_FLAGS + PER_SOURCE_FLAGS.get(name, [])
+
+
 def _stamp(paths, flags):
     h = hashlib.sha1(" ".join(flags).encode())
     for p in paths:
@@ -89,10 +100,7 @@ def build(jobs: int = 8, verbose: bool = False, force: bool = False, kernel_defi
     inc, tlib, abi = _torch_paths()
     hip, cpp, hdr = _sources()
     hipcc = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
-    # (no packed fp32 instructions: hipcc -O3 forms v_pk_add / mul / fma_f32 from ordinary float code, and some of their
-    # forms have given wrong results on this hardware now and then; the host pass warns that it does not know the feature)
-    dev_flags = [f"--offload-arch={ARCH}", "-O3", "-std=c++17", "-fPIC", "-ffp-contract=fast", "-Wno-unused-result",
-                 "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
+    dev_flags = list(DEVICE_FLAGS)
     dev_flags += [f"-D{d}" for d in kernel_defines]
     host_flags = ["-O2", "-std=c++17", "-fPIC", "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1",
                   "-DTORCH_EXTENSION_NAME=_C", "-DTORCH_API_INCLUDE_EXTENSION_H",

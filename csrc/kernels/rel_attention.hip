@@ -42,14 +42,14 @@ constexpr float RA_SLACK = 8.0f;
 
 // rows [0, 64) of a [rows][D] matrix (row stride `stride` elements) into NH 64-column images: 16-byte chunk c of row r is
 // stored at chunk c ^ (r & 6).  Rows whose bit in `rows` is clear, and columns from D on, arrive as zeros.
-template <typename T, int NH>
+template <typename T, int NH, int WAVES = RA_WAVES>
 __device__ __forceinline__ void ra_stage(char* img, const T* src, uint32_t stride, uint64_t rows, int D, int lane, int wave) {
   const int4v rsrc = pdt_make_rsrc(src, rows ? (uint32_t)((RA_CHUNK - 1) * stride + D) * 2u : 0u);
 #pragma unroll
   for (int h = 0; h < NH; ++h) {
 #pragma unroll
-    for (int u = 0; u < 2; ++u) {
-      const int piece = u * RA_WAVES + wave, row = piece * 8 + (lane >> 3);
+    for (int u = 0; u < 8 / WAVES; ++u) {
+      const int piece = u * WAVES + wave, row = piece * 8 + (lane >> 3);
       const int col = h * 64 + (((lane & 7) ^ (row & 6)) << 3);
       const bool ok = ((rows >> row) & 1) && col < D;
       pdt_lds_dma16(rsrc, img + h * RA_IMG + piece * 1024, ok ? (row * stride + col) * 2u : 0x80000000u);
@@ -190,10 +190,10 @@ __device__ __forceinline__ float ra_table(const PdtRelAttn& p, int bucket, int h
   const int64_t i = (int64_t)bucket * p.A + h;
   return p.table_f32 ? ((const float*)p.table)[i] : Half16<T>::to_f(((const short*)p.table)[i]);
 }
-template <typename T>
-__device__ __forceinline__ RaBias ra_bias_fill(const PdtRelAttn& p, float* mem, int h, int sign, int tid) {
-  RaBias t{mem, ra_bias_len(p.max_distance), ra_far(p.max_distance) + 32, ra_far(p.max_distance)};
-  for (int i = tid; i < t.len + 4; i += RA_THREADS) {
+template <typename T, int THREADS = RA_THREADS>
+__device__ __forceinline__ RaBias ra_bias_fill(const PdtRelAttn& p, float* mem, int h, int sign, int tid, int max_distance) {
+  RaBias t{mem, ra_bias_len(max_distance), ra_far(max_distance) + 32, ra_far(max_distance)};
+  for (int i = tid; i < t.len + 4; i += THREADS) {
     const float v = p.table ? ra_table<T>(p, ra_bucket(p, sign * (i - t.off)), h) * LOG2E : 0.f;
 #pragma unroll
     for (int j = 0; j < 4; ++j)
@@ -241,7 +241,7 @@ __global__ __launch_bounds__(RA_THREADS) RA_OCC_FWD void rel_attn_fwd_kernel(Pdt
   uint64_t w;
   int c = ra_next(p, s, 0, nc, w);
   if (c < nc) stage(c, 0, w);
-  const RaBias bias = ra_bias_fill<T>(p, reinterpret_cast<float*>(smem + 2 * BUF), s.h, 1, tid);
+  const RaBias bias = ra_bias_fill<T>(p, reinterpret_cast<float*>(smem + 2 * BUF), s.h, 1, tid, p.max_distance);
   const int boff = ra_bias_lane(bias, lm, g);
   const bool has_bias = p.table != nullptr, active = q0 < s.n;
   short8 qf[QB][KS];
@@ -386,6 +386,26 @@ __device__ __forceinline__ void ra_diag_add(float* d, const float4v& t, int lm) 
   if (lm >= 13) atomicAdd(d + 16, w);
 }
 
+// distances -> buckets: sums[top + d] is the sum at distance d, |d| <= top; eight lanes per bucket walk its range
+template <int THREADS>
+__device__ __forceinline__ void ra_bucket_sums(const PdtRelAttn& p, const float* sums, int top, float* part, int tid) {
+  const int half = p.buckets >> 1, exact = half >> 1;
+  for (int b0 = 0; b0 < p.buckets; b0 += THREADS / 8) {
+    const int b = b0 + (tid >> 3), j = b >= half ? b - half : b;
+    float sum = 0.f;
+    if (b < p.buckets) {
+      int lo = j < exact ? j : p.steps[j - exact], hi = j < exact ? j : (j == half - 1 ? top : p.steps[j + 1 - exact] - 1);
+      if (b >= half) lo = max(lo, 1);
+      hi = min(hi, top);
+      for (int n = lo + (tid & 7); n <= hi; n += 8) sum += sums[(b >= half ? n : -n) + top];
+    }
+    sum += __shfl_xor(sum, 1, 64);
+    sum += __shfl_xor(sum, 2, 64);
+    sum += __shfl_xor(sum, 4, 64);
+    if (b < p.buckets && (tid & 7) == 0) part[(int64_t)b * p.A] = sum;
+  }
+}
+
 // ------------------------------------------------------------------------------------------------ dQ and the table gradient
 // One wave = 16 QB query rows, sweeps the keys; also stores delta = rowsum(dO * O) for the dK / dV kernel.
 template <typename T, int KS, int QB, bool DROP>
@@ -417,7 +437,7 @@ __global__ __launch_bounds__(RA_THREADS) RA_OCC_BWD void rel_attn_dq_kernel(PdtR
   uint64_t w;
   int c = ra_next(p, s, 0, nc, w);
   if (c < nc) stage(c, 0, w);
-  const RaBias bias = ra_bias_fill<T>(p, reinterpret_cast<float*>(smem + 2 * BUF), s.h, 1, tid);
+  const RaBias bias = ra_bias_fill<T>(p, reinterpret_cast<float*>(smem + 2 * BUF), s.h, 1, tid, p.max_distance);
   const int boff = ra_bias_lane(bias, lm, g);
   const bool has_bias = p.table != nullptr, active = q0 < s.n;
   // diagonal sums, one array per wave and lane group: entry 0 is distance -(far + 31).  `diag` is where this lane's sum
@@ -578,20 +598,7 @@ __global__ __launch_bounds__(RA_THREADS) RA_OCC_BWD void rel_attn_dq_kernel(PdtR
       sums[i] = t;
     }
     __syncthreads();
-    const int half = p.buckets >> 1, exact = half >> 1, top = bias.far + 31;
-    for (int b0 = 0; b0 < p.buckets; b0 += RA_THREADS / 8) {  // eight lanes per bucket walk its range of distances
-      const int b = b0 + (tid >> 3), j = b >= half ? b - half : b;
-      float sum = 0.f;
-      if (b < p.buckets) {
-        int lo = j < exact ? j : p.steps[j - exact], hi = j < exact ? j : (j == half - 1 ? top : p.steps[j + 1 - exact] - 1);
-        if (b >= half) lo = max(lo, 1);
-        for (int n = lo + (tid & 7); n <= hi; n += 8) sum += sums[(b >= half ? n : -n) + top];
-      }
-      sum += __shfl_xor(sum, 1, 64);
-      sum += __shfl_xor(sum, 2, 64);
-      sum += __shfl_xor(sum, 4, 64);
-      if (b < p.buckets && (tid & 7) == 0) part[(int64_t)b * p.A] = sum;
-    }
+    ra_bucket_sums<RA_THREADS>(p, sums, bias.far + 31, part, tid);
   }
 }
 
@@ -630,7 +637,7 @@ __global__ __launch_bounds__(RA_THREADS) RA_OCC_BWD void rel_attn_dkv_kernel(Pdt
       reinterpret_cast<uint32_t*>(m + 2 * NH * RA_IMG + 512)[tid] = attn_row_seed(dkey, sbh, c * RA_CHUNK + tid);
   };
   stage(0, 0);
-  const RaBias bias = ra_bias_fill<T>(p, reinterpret_cast<float*>(smem + 2 * BUF), s.h, -1, tid);
+  const RaBias bias = ra_bias_fill<T>(p, reinterpret_cast<float*>(smem + 2 * BUF), s.h, -1, tid, p.max_distance);
   const int boff = ra_bias_lane(bias, lm, g);
   const bool has_bias = p.table != nullptr;
   short8 kf[QB][KS], vf[QB][KS];
@@ -748,6 +755,223 @@ __global__ __launch_bounds__(RA_THREADS) RA_OCC_BWD void rel_attn_dkv_kernel(Pdt
   }
 }
 
+// ------------------------------------------------------------------------------------------------ backward, S <= 16 W
+// One workgroup of W waves owns a whole (batch, head): every input is read once and every probability computed once.
+// First each wave takes 16 query rows against all keys, with p and dp of the whole row in registers: delta = sum of p dp is
+// formed from them (neither the output nor its rounding enters), ds follows, and dQ.  Then P and dS go to LDS as 16-bit
+// images in the place of K and V, and each wave takes 16 keys: their columns of P and dS, read transposed, are the operands
+// of dV and dK against the images of dO and Q.  With 64 columns and 128 rows the place holds 64 keys' worth, so this runs in
+// two passes, two waves sharing the columns of 16 keys; otherwise in one.
+// Bound by memory at the training shapes: 7 row reads and writes of 16-bit values per element instead of the two sweeps' 11.
+template <typename T, int KS, int W, bool DROP>
+__global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(KS <= 2 ? 4 : 2, 8))) void rel_attn_bwd_short_kernel(PdtRelAttn p) {
+  constexpr int NH = (KS + 1) / 2, R = 16 * W, NC = R / RA_CHUNK;  // NC 64-row chunks; an image is [NC][NH] chunk images
+  constexpr int IMG = NC * NH * RA_IMG;
+  constexpr int PASSES = NC > NH ? 2 : 1, SPLIT = PASSES;          // key passes; waves that share 16 keys
+  constexpr int CK = NC / PASSES;                                  // 64-key chunks of a pass
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+  char* const qimg = smem;
+  char* const gimg = smem + IMG;
+  char* const kimg = smem + 2 * IMG;  // K | V, later P | dS
+  char* const vimg = smem + 3 * IMG;
+  const int tid = threadIdx.x, lane = tid & 63, lm = lane & 15, g = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const RaSpan s = ra_span(p, blockIdx.x);
+  float* part = p.dtable_part ? p.dtable_part + (int64_t)s.b * p.buckets * p.A + s.h : nullptr;
+  if (s.n == 0) {
+    if (part)
+      for (int i = tid; i < p.buckets; i += 64 * W) part[(int64_t)i * p.A] = 0.f;
+    return;
+  }
+  const bool packed = p.cu != nullptr;
+  uint64_t rows[NC], keys[NC];
+#pragma unroll
+  for (int c = 0; c < NC; ++c) {
+    const int left = s.n - c * RA_CHUNK;
+    rows[c] = left <= 0 ? 0 : (left >= RA_CHUNK ? ~0ull : (1ull << left) - 1);
+    keys[c] = ra_word(p, s, c);
+  }
+  auto stage = [&](char* img, const PdtRelView& v, const uint64_t (&on)[NC]) {
+#pragma unroll
+    for (int c = 0; c < NC; ++c)
+      ra_stage<T, NH, W>(img + c * NH * RA_IMG, ra_base<const T>(v, s, packed) + (int64_t)c * RA_CHUNK * v.row, (uint32_t)v.row, on[c], p.D, lane, wave);
+  };
+  stage(kimg, p.k, keys);
+  stage(vimg, p.v, keys);
+  stage(qimg, p.q, rows);
+  stage(gimg, p.dout, rows);
+  const int q = 16 * wave + lm;
+  const RaBias bias = ra_bias_fill<T, 64 * W>(p, reinterpret_cast<float*>(smem + 4 * IMG), s.h, 1, tid, min(p.max_distance, 128));
+  const float nlse = q < s.n ? -p.lse[((int64_t)s.b * p.A + s.h) * p.S + q] : -INFINITY;  // rows that are not there: p = 0
+  const int boff = ra_bias_lane(bias, lm, g);
+  const uint32_t seed = DROP ? attn_row_seed(drop_key(p.rng), drop_sample(p.rng, s.b) * p.A + s.h, q) : 0u;
+  const uint32_t thr_hi = attn_thr_hi(p.drop_thr), kmul0 = (uint32_t)(4 * g) * ATT_GOLD;
+  const float k2 = p.scale * LOG2E;
+  asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+  __builtin_amdgcn_s_barrier();
+  __builtin_amdgcn_sched_barrier(0);
+
+  // ---- rows: p, dp, delta, ds, dQ.  (Waves up to the end of the last 32 rows take part: their rows are zero.)
+  const bool active = 16 * wave < ((s.n + 31) & ~31);
+  float4v ds[W];
+  short8 pp[W / 2], sf[W / 2];
+#pragma unroll
+  for (int pb = 0; pb < W / 2; ++pb) pp[pb] = sf[pb] = short8{0, 0, 0, 0, 0, 0, 0, 0};
+#pragma unroll
+  for (int kb = 0; kb < W; ++kb) ds[kb] = splat4(0.f);
+  if (active) {
+    short8 qf[KS], df[KS];
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) {
+      qf[ks] = ra_row_frag(qimg + (wave >> 2) * NH * RA_IMG, 16 * (wave & 3), ks, lane);
+      df[ks] = ra_row_frag(gimg + (wave >> 2) * NH * RA_IMG, 16 * (wave & 3), ks, lane);
+    }
+    float4v dp[W], d4 = splat4(0.f);
+#pragma unroll
+    for (int pb = 0; pb < W / 2; ++pb) {
+      float4v pd[2];
+#pragma unroll
+      for (int hb = 0; hb < 2; ++hb) {
+        const int kb = 2 * pb + hb;
+        const uint32_t tile = (uint32_t)(keys[kb >> 2] >> ((kb & 3) * 16)) & 0xFFFFu;  // (wave-uniform)
+        dp[kb] = pd[hb] = splat4(0.f);
+        if (!tile) continue;
+        float4v sc = splat4(0.f), e = splat4(0.f);
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) {
+          sc = Half16<T>::mfma(ra_row_frag(kimg + (kb >> 2) * NH * RA_IMG, (kb & 3) * 16, ks, lane), qf[ks], sc);
+          e = Half16<T>::mfma(ra_row_frag(vimg + (kb >> 2) * NH * RA_IMG, (kb & 3) * 16, ks, lane), df[ks], e);
+        }
+        float4v t = sc * k2 + (ra_bias4(bias, boff, 16 * (kb - wave)) + nlse);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) t[r] = __builtin_amdgcn_exp2f(t[r]);
+        // (selected in every tile: a branch between a product and its use has cost the wait in front of that use, see
+        // tools/mfma_hazards.py)
+        const uint32_t bits = tile >> (4 * g);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) t[r] = (bits >> r) & 1 ? t[r] : 0.f;
+        ds[kb] = pd[hb] = t;
+        if (DROP) {
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            const float keep = attn_keep(seed, kmul0 + (uint32_t)(kb * 16 + r) * ATT_GOLD, thr_hi) ? p.drop_scale : 0.f;
+            pd[hb][r] *= keep;
+            e[r] *= keep;
+          }
+        }
+        d4 += t * e;
+        dp[kb] = e;
+      }
+      pp[pb] = pack_pair<T>(pd[0], pd[1]);
+    }
+    const float delta = ra_quad_sum((d4[0] + d4[1]) + (d4[2] + d4[3]));
+    float4v dq[2 * KS];
+#pragma unroll
+    for (int db = 0; db < 2 * KS; ++db) dq[db] = splat4(0.f);
+#pragma unroll
+    for (int pb = 0; pb < W / 2; ++pb) {
+#pragma unroll
+      for (int hb = 0; hb < 2; ++hb) ds[2 * pb + hb] *= dp[2 * pb + hb] - delta;
+      sf[pb] = pack_pair<T>(ds[2 * pb], ds[2 * pb + 1]);
+      if (((keys[pb >> 1] >> ((pb & 1) * 32)) & 0xFFFFFFFFull) == 0) continue;
+#pragma unroll
+      for (int db = 0; db < 2 * KS; ++db)
+        dq[db] = Half16<T>::mfma(ra_tr_frag(kimg + (pb >> 1) * NH * RA_IMG, (pb & 1) * 32, db, lane), sf[pb], dq[db]);
+    }
+    ra_store<T, KS>(ra_base<T>(p.dq, s, packed) + (int64_t)q * p.dq.row, dq, p.scale, g, p.D, q < s.n);
+  }
+
+  // ---- keys: dV and dK.  A pass: P and dS of its keys as [query][64 keys] images, then 16 keys per wave.
+  T* dkb = ra_base<T>(p.dk, s, packed);
+  T* dvb = ra_base<T>(p.dv, s, packed);
+  const int nqb = (s.n + 31) >> 5;
+#pragma unroll
+  for (int pass = 0; pass < PASSES; ++pass) {
+    const int kblk = pass * 4 * CK + (SPLIT == 2 ? wave & 3 : wave), part_d = SPLIT == 2 ? wave >> 2 : 0;
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // (this wave is done with the place)
+    __builtin_amdgcn_s_barrier();
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int kb = 0; kb < 4 * CK; ++kb) {  // this wave's 16 queries x 4 CK key blocks: four keys (8 bytes) per lane and block
+      const int at = pass * 4 * CK + kb, pos = q & (RA_CHUNK - 1);
+      const int off = ((q >> 6) * CK + (kb >> 2)) * RA_IMG + pos * 128 + (((2 * (kb & 3) + (g >> 1)) ^ (pos & 6)) << 4) + (g & 1) * 8;
+      const int4v a = __builtin_bit_cast(int4v, pp[at >> 1]), c = __builtin_bit_cast(int4v, sf[at >> 1]);
+      *reinterpret_cast<int2v*>(kimg + off) = at & 1 ? int2v{a[2], a[3]} : int2v{a[0], a[1]};
+      *reinterpret_cast<int2v*>(vimg + off) = at & 1 ? int2v{c[2], c[3]} : int2v{c[0], c[1]};
+    }
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    __builtin_amdgcn_sched_barrier(0);
+    const int key = 16 * kblk + lm;
+    constexpr int DB = 2 * KS / SPLIT > 0 ? 2 * KS / SPLIT : 1;  // 16-column blocks of this wave
+    float4v dk_[DB], dv_[DB];
+#pragma unroll
+    for (int i = 0; i < DB; ++i) { dk_[i] = splat4(0.f); dv_[i] = splat4(0.f); }
+    if (((keys[kblk >> 2] >> ((kblk & 3) * 16)) & 0xFFFFu) != 0) {
+      const int kin = kblk - pass * 4 * CK;  // block within the pass
+      for (int qb = 0; qb < nqb; ++qb) {
+        const int base = (qb >> 1), r0 = (qb & 1) * 32;
+        const short8 pf = ra_tr_frag(kimg + (base * CK + (kin >> 2)) * RA_IMG, r0, kin & 3, lane);
+        const short8 tf = ra_tr_frag(vimg + (base * CK + (kin >> 2)) * RA_IMG, r0, kin & 3, lane);
+#pragma unroll
+        for (int i = 0; i < DB; ++i) {
+          const int db = part_d * DB + i;
+          dv_[i] = Half16<T>::mfma(ra_tr_frag(gimg + base * NH * RA_IMG, r0, db, lane), pf, dv_[i]);
+          dk_[i] = Half16<T>::mfma(ra_tr_frag(qimg + base * NH * RA_IMG, r0, db, lane), tf, dk_[i]);
+        }
+      }
+    }
+    if constexpr (DB % 2 == 0) {
+      const int c0 = part_d * DB * 16;
+      ra_store<T, DB / 2>(dkb + (int64_t)key * p.dk.row + c0, dk_, p.scale, g, p.D - c0, key < s.n);
+      ra_store<T, DB / 2>(dvb + (int64_t)key * p.dv.row + c0, dv_, 1.0f, g, p.D - c0, key < s.n);
+    } else {  // one block: four columns (8 bytes) per lane
+      const int col = part_d * 16 + 4 * g;
+      if (key < s.n && col < p.D) {
+        const float4v a = dk_[0] * p.scale, c = dv_[0];
+        *reinterpret_cast<int2v*>(dkb + (int64_t)key * p.dk.row + col) = int2v{cvt_pk<T>(a[0], a[1]), cvt_pk<T>(a[2], a[3])};
+        *reinterpret_cast<int2v*>(dvb + (int64_t)key * p.dv.row + col) = int2v{cvt_pk<T>(c[0], c[1]), cvt_pk<T>(c[2], c[3])};
+      }
+    }
+  }
+
+  // ---- table gradient: the diagonals of this wave's rows (a tile per offset 16 (kb - wave): each entry is written once,
+  // the part W of a tile that belongs to the next offset is carried), then distances -> buckets
+  if (!part) return;
+  constexpr int TOP = R - 1, DLEN = 2 * R + 16;
+  float* const sums = reinterpret_cast<float*>(smem);
+  __syncthreads();
+  for (int i = tid; i < 4 * W * DLEN; i += 64 * W) sums[i] = 0.f;
+  __syncthreads();
+  {
+    float* d = sums + (wave * 4 + g) * DLEN + TOP - 16 * wave + 4 * g - lm;
+    float carry = 0.f;
+#pragma unroll
+    for (int kb = 0; kb < W; ++kb) {
+      const float4v t = ds[kb];
+      float n = t[0];
+      n += dpp_f<0x101>(t[1]);
+      n += dpp_f<0x102>(t[2]);
+      n += dpp_f<0x103>(t[3]);
+      float w = dpp_f<0x11F>(t[1]);
+      w += dpp_f<0x11E>(t[2]);
+      w += dpp_f<0x11D>(t[3]);
+      d[16 * kb] = n + carry;
+      carry = w;
+    }
+    if (lm >= 13) d[16 * W] = carry;
+  }
+  __syncthreads();
+  for (int i = tid; i < DLEN; i += 64 * W) {
+    float t = 0.f;
+#pragma unroll 8
+    for (int a = 0; a < 4 * W; ++a) t += sums[a * DLEN + i];
+    sums[i] = t;
+  }
+  __syncthreads();
+  ra_bucket_sums<64 * W>(p, sums, TOP, part, tid);
+}
+
 // ------------------------------------------------------------------------------------------------ helpers
 // key mask [B][S] (1 or 4 bytes per key, non-zero = attended) -> one bit per key; one wave per 64 keys
 __global__ __launch_bounds__(256) void rel_attn_mask_kernel(const void* mask, int bytes, int64_t stride, int S, int words,
@@ -810,10 +1034,25 @@ static int ra_launch(KernT kern, const PdtRelAttn& p, int rows_per_block, size_t
   return (int)hipGetLastError();
 }
 
-// which: 0 forward, 1 dQ + table gradient, 2 dK / dV
+// sequences that one workgroup of the short backward kernel holds: 64 rows in four waves, 128 in eight
+static int ra_short_rows(const PdtRelAttn& p) { return p.S <= 64 ? 64 : (p.S <= 128 ? 128 : 0); }
+template <typename T, int KS, int W, bool DROP>
+static int ra_launch_short(const PdtRelAttn& p, hipStream_t st) {
+  constexpr int NH = (KS + 1) / 2, R = 16 * W;
+  const size_t work = (size_t)4 * (R / RA_CHUNK) * NH * RA_IMG;
+  static_assert((size_t)4 * W * (2 * R + 16) * sizeof(float) <= (size_t)4 * (R / RA_CHUNK) * NH * RA_IMG, "diagonal sums reuse the images");
+  const size_t lds = work + (size_t)4 * ra_bias_len(p.max_distance < 128 ? p.max_distance : 128) * sizeof(float);
+  auto kern = rel_attn_bwd_short_kernel<T, KS, W, DROP>;
+  if (int e = ra_allow_lds((const void*)kern, lds)) return e;
+  hipLaunchKernelGGL(kern, dim3(p.B * p.A), dim3(64 * W), lds, st, p);
+  return (int)hipGetLastError();
+}
+
+// which: 0 forward, 1 dQ + table gradient, 2 dK / dV, 3 the whole backward of short sequences
 template <typename T, int KS, bool DROP>
 static int ra_dispatch(int which, const PdtRelAttn& p, hipStream_t st) {
   constexpr int NH = (KS + 1) / 2, QB2 = KS <= 2 ? 2 : 1;  // (two blocks per wave in the backward kernels)
+  if (which == 3) return ra_short_rows(p) == 64 ? ra_launch_short<T, KS, 4, DROP>(p, st) : ra_launch_short<T, KS, 8, DROP>(p, st);
   const bool two = ra_blocks(p, which != 0) == 2;
   const int rows = RA_WAVES * 16 * (two ? 2 : 1);
   const size_t imgs = (size_t)4 * NH * RA_IMG, tab = ra_bias_bytes(p);
@@ -891,6 +1130,7 @@ extern "C" int pdt_rel_attn_fwd(int dtype, const PdtRelAttn* a, void* stream) {
 }
 
 extern "C" int pdt_rel_attn_dtable_rows(const PdtRelAttn* a) {
+  if (ra_short_rows(*a)) return a->B;
   const int rows = RA_WAVES * 16 * ra_blocks(*a, true);
   return a->B * ((a->S + rows - 1) / rows);
 }
@@ -905,6 +1145,7 @@ extern "C" int pdt_rel_attn_bwd(int dtype, const PdtRelAttn* a, void* stream) {
   for (const PdtRelView* v : outs)
     if (int e = ra_tail(dtype, *v, *a, st)) return e;
   if (a->B == 0 || a->S == 0) return 0;
+  if (ra_short_rows(*a)) return ra_run(dtype, 3, *a, st);
   if (int e = ra_run(dtype, 1, *a, st)) return e;
   return ra_run(dtype, 2, *a, st);
 }
