@@ -33,26 +33,28 @@ constexpr int RA_IMG = RA_CHUNK * 128;          // bytes of a 64-row x 64-column
 constexpr int RA_MAX_FAR = 512;                 // largest max_distance
 constexpr int RA_MAX_STEPS = 32;                // logarithmic buckets per side
 constexpr float RA_SLACK = 8.0f;
-#ifndef RA_WF
-#define RA_WF 3
-#endif
-// Waves per SIMD that the register allocation of a kernel with QB blocks of KS 32-column steps must allow
-#define RA_OCC_FWD __attribute__((amdgpu_waves_per_eu(KS * QB <= 4 ? RA_WF : 2, 8)))
-#define RA_OCC_BWD __attribute__((amdgpu_waves_per_eu(KS * QB <= 2 ? 3 : 2, 8)))
+// Waves per SIMD that the register allocation of a kernel with QB blocks of KS 32-column steps must allow.  At QB KS = 4:
+// forward and dQ 3 (166 registers; dQ with 2: 83 instead of 75 us at 32 x 512 tokens, 12 heads), dK / dV 2 (with 3 it spills: 86
+// instead of 73 us).
+#define RA_OCC_FWD __attribute__((amdgpu_waves_per_eu(KS * QB <= 4 ? 3 : 2, 8)))
+#define RA_OCC_DQ __attribute__((amdgpu_waves_per_eu(KS * QB <= 4 ? 3 : 2, 8)))
+#define RA_OCC_DKV __attribute__((amdgpu_waves_per_eu(KS * QB <= 2 ? 3 : 2, 8)))
 
 // rows [0, 64) of a [rows][D] matrix (row stride `stride` elements) into NH 64-column images: 16-byte chunk c of row r is
-// stored at chunk c ^ (r & 6).  Rows whose bit in `rows` is clear, and columns from D on, arrive as zeros.
+// stored at chunk c ^ (r & 6).  Rows whose bit in `rows` is clear, and columns from D on, arrive as zeros.  The pieces of a
+// wave lie 8 WAVES rows apart (and 64 columns), which goes into the descriptor: one offset per lane serves all of them.
 template <typename T, int NH, int WAVES = RA_WAVES>
 __device__ __forceinline__ void ra_stage(char* img, const T* src, uint32_t stride, uint64_t rows, int D, int lane, int wave) {
-  const int4v rsrc = pdt_make_rsrc(src, rows ? (uint32_t)((RA_CHUNK - 1) * stride + D) * 2u : 0u);
+  const int row0 = wave * 8 + (lane >> 3), col0 = ((lane & 7) ^ (row0 & 6)) << 3;
+  const uint32_t off = (row0 * stride + col0) * 2u;
 #pragma unroll
   for (int h = 0; h < NH; ++h) {
 #pragma unroll
     for (int u = 0; u < 8 / WAVES; ++u) {
-      const int piece = u * WAVES + wave, row = piece * 8 + (lane >> 3);
-      const int col = h * 64 + (((lane & 7) ^ (row & 6)) << 3);
-      const bool ok = ((rows >> row) & 1) && col < D;
-      pdt_lds_dma16(rsrc, img + h * RA_IMG + piece * 1024, ok ? (row * stride + col) * 2u : 0x80000000u);
+      const int first = u * 8 * WAVES;
+      const int4v rsrc = pdt_make_rsrc(src + (int64_t)first * stride + h * 64, rows ? (uint32_t)((RA_CHUNK - 1 - first) * stride + D - h * 64) * 2u : 0u);
+      const bool ok = ((rows >> (first + row0)) & 1) && col0 + h * 64 < D;
+      pdt_lds_dma16(rsrc, img + h * RA_IMG + (u * WAVES + wave) * 1024, ok ? off : 0x80000000u);
     }
   }
 }
@@ -156,12 +158,52 @@ __device__ __forceinline__ uint64_t ra_word(const PdtRelAttn& p, const RaSpan& s
   if (p.mask_bits) w &= ((const __attribute__((address_space(4))) uint64_t*)p.mask_bits)[(int64_t)s.b * p.mask_words + c];
   return w;
 }
-// next chunk at or after c with an attended key
-__device__ __forceinline__ int ra_next(const PdtRelAttn& p, const RaSpan& s, int c, int nc, uint64_t& w) {
-  w = 0;
-  for (; c < nc; ++c)
-    if ((w = ra_word(p, s, c)) != 0) break;
-  return c;
+// The chunks of a sweep in the order in which a workgroup takes them: first the whole chunks beyond the near distances
+// (`far`: every row of the chunk attended, one bias), then the others that hold any row at all.  Two loops, each with one
+// form of the score arithmetic: three forms in one loop cost 45 to 85 registers more and a wave of occupancy.
+struct RaChunks {
+  int c, nc, lo, hi;  // current chunk; far chunks lie at or below lo or at or above hi
+  int far, left;      // in the first loop; a far chunk was left to the second
+  int buf;            // the LDS buffer it is staged in
+  uint64_t w;         // its attended rows
+  template <typename WordFn>
+  __device__ __forceinline__ void next(WordFn word) {
+    if (far) {
+      for (++c; c < nc; ++c) {
+        if (c > lo && c < hi) {
+          c = hi;
+          if (c >= nc) break;
+        }
+        w = word(c);
+        if (w == ~0ull) return;
+        left |= w != 0;
+      }
+      far = 0;
+      c = left ? -1 : lo;
+      if (!left) nc = min(nc, hi);
+    }
+    for (++c; c < nc; ++c) {
+      w = word(c);
+      if (w != 0 && !(w == ~0ull && (c <= lo || c >= hi))) return;
+    }
+  }
+  __device__ __forceinline__ bool done() const { return c >= nc; }
+};
+// `rows` rows from w0 on against chunks of 64: a chunk is far when all its tiles lie at least `far` beyond all rows
+__device__ __forceinline__ RaChunks ra_chunks(int n, int w0, int rows, int far, bool has_bias, bool any_far) {
+  RaChunks k;
+  k.nc = (n + RA_CHUNK - 1) / RA_CHUNK;
+  // 64 c + 48 - w0 <= -(far + 16)   and   64 c - (w0 + rows - 16) >= far + 16
+  k.lo = w0 - far >= RA_CHUNK ? (w0 - far) / RA_CHUNK - 1 : -1;
+  k.hi = (w0 + rows + far + RA_CHUNK - 1) / RA_CHUNK;
+  if (!has_bias) k.lo = k.nc;
+  if (!any_far) { k.lo = -1; k.hi = k.nc; }
+  k.far = 1;
+  k.left = 0;
+  k.buf = 0;
+  k.c = -1;
+  k.w = 0;
+  return k;
 }
 
 // ---- the bias array: entry i of copy j is the bias (times log2 e) of distance sign * (i + j - off); `off` and the
@@ -172,10 +214,10 @@ struct RaBias {
 };
 __device__ __forceinline__ int ra_far(int max_distance) { return (max_distance + 15) & ~15; }
 __host__ __device__ inline int ra_bias_len(int max_distance) {
-  const int n = 2 * ((max_distance + 15) & ~15) + 64 + 16;
-  return ((n + 63) & ~63) + 16;  // the copies start 64 bytes apart modulo the 256 bytes of one access
+  const int n = 2 * ((max_distance + 15) & ~15) + 64;
+  return (n - 16 + 63) / 64 * 64 + 16;  // the copies start 64 bytes apart modulo the 256 bytes of one access
 }
-__host__ __device__ inline int ra_diag_len(int max_distance) { return 2 * ((max_distance + 15) & ~15) + 80; }
+__host__ __device__ inline int ra_diag_len(int max_distance) { return 2 * ((max_distance + 15) & ~15) + 64; }
 __device__ __forceinline__ int ra_bucket(const PdtRelAttn& p, int d) {
   const int n = d < 0 ? -d : d, half = p.buckets >> 1, exact = half >> 1;
   int b = n;
@@ -211,12 +253,6 @@ __device__ __forceinline__ float4v ra_bias4(const RaBias& t, int lane_off, int u
   return *reinterpret_cast<const float4v*>(t.t + lane_off + uc);
 }
 
-// Whether tiles with their offsets in [u0, u1] all lie beyond the near distances: -1 / 1 the side, 0 not all of them.
-// (u - 15 .. u + 15 are the distances of a tile.)
-__device__ __forceinline__ int ra_side(const RaBias& t, int u0, int u1) {
-  return u0 >= t.far + 16 ? 1 : (u1 <= -(t.far + 16) ? -1 : 0);
-}
-
 // ------------------------------------------------------------------------------------------------ forward
 // One wave = 16 QB query rows; online softmax in the log2 domain.
 template <typename T, int KS, int QB, bool DROP>
@@ -232,18 +268,22 @@ __global__ __launch_bounds__(RA_THREADS) RA_OCC_FWD void rel_attn_fwd_kernel(Pdt
   const T* qb_ = ra_base<const T>(p.q, s, packed);
   const T* kb_ = ra_base<const T>(p.k, s, packed);
   const T* vb_ = ra_base<const T>(p.v, s, packed);
-  const int nc = (s.n + RA_CHUNK - 1) / RA_CHUNK;
+  float* const mb = reinterpret_cast<float*>(smem + 2 * BUF);  // 0 / -inf of the 64 keys of each buffer
   auto stage = [&](int c, int buf, uint64_t w) {
     char* m = smem + buf * BUF;
     ra_stage<T, NH>(m, kb_ + (int64_t)c * RA_CHUNK * p.k.row, (uint32_t)p.k.row, w, p.D, lane, wave);
     ra_stage<T, NH>(m + NH * RA_IMG, vb_ + (int64_t)c * RA_CHUNK * p.v.row, (uint32_t)p.v.row, w, p.D, lane, wave);
+    if (tid < RA_CHUNK) mb[buf * RA_CHUNK + tid] = (w >> tid) & 1 ? 0.f : -INFINITY;
   };
-  uint64_t w;
-  int c = ra_next(p, s, 0, nc, w);
-  if (c < nc) stage(c, 0, w);
-  const RaBias bias = ra_bias_fill<T>(p, reinterpret_cast<float*>(smem + 2 * BUF), s.h, 1, tid, p.max_distance);
+  auto word = [&](int c) { return ra_word(p, s, c); };
+  const float k2 = p.scale * LOG2E;
+  // (the far form takes the maximum of the raw products: not with a negative scale)
+  RaChunks cur = ra_chunks(s.n, w0, RA_WAVES * 16 * QB, ra_far(p.max_distance), p.table != nullptr, k2 > 0.f);
+  cur.next(word);
+  if (!cur.done()) stage(cur.c, 0, cur.w);
+  const RaBias bias = ra_bias_fill<T>(p, mb + 2 * RA_CHUNK, s.h, 1, tid, p.max_distance);
   const int boff = ra_bias_lane(bias, lm, g);
-  const bool has_bias = p.table != nullptr, active = q0 < s.n;
+  const bool active = q0 < s.n;
   short8 qf[QB][KS];
   uint32_t seed[QB];
 #pragma unroll
@@ -253,9 +293,8 @@ __global__ __launch_bounds__(RA_THREADS) RA_OCC_FWD void rel_attn_fwd_kernel(Pdt
     for (int ks = 0; ks < KS; ++ks) qf[i][ks] = ra_gfrag<T>(qb_ + (int64_t)q * p.q.row, ks, p.D, lane, q < s.n);
     seed[i] = DROP ? attn_row_seed(drop_key(p.rng), drop_sample(p.rng, s.b) * p.A + s.h, q) : 0u;
   }
-  const float k2 = p.scale * LOG2E;
   const uint32_t thr_hi = attn_thr_hi(p.drop_thr), kmul0 = (uint32_t)(4 * g) * ATT_GOLD;
-  float m[QB], bias_lo = 0.f, bias_hi = 0.f;
+  float m[QB];
   float4v l4[QB], o[QB][2 * KS];
 #pragma unroll
   for (int i = 0; i < QB; ++i) {
@@ -264,84 +303,83 @@ __global__ __launch_bounds__(RA_THREADS) RA_OCC_FWD void rel_attn_fwd_kernel(Pdt
 #pragma unroll
     for (int db = 0; db < 2 * KS; ++db) o[i][db] = splat4(0.f);
   }
-  for (int buf = 0; c < nc; buf ^= 1) {
-    uint64_t wn;
-    const int cn = ra_next(p, s, c + 1, nc, wn);
-    __syncthreads();  // every wave is done with the other buffer (first time: the bias array is complete)
-    bias_lo = bias.t[0];
-    bias_hi = bias.t[bias.len - 1];
-    if (cn < nc) {
-      stage(cn, buf ^ 1, wn);
-      if (NH == 1) asm volatile("s_waitcnt vmcnt(4)" ::: "memory");
-      else asm volatile("s_waitcnt vmcnt(8)" ::: "memory");
-    } else {
-      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    }
-    __syncthreads();
-    if (active) {
-      const char* kimg = smem + buf * BUF;
-      const char* vimg = kimg + NH * RA_IMG;
-      const int u0 = c * RA_CHUNK - q0;
-      const int side = has_bias ? ra_side(bias, u0 - 16 * (QB - 1), u0 + 48) : 1;
-      auto chunk = [&](auto near_tag, auto whole_tag) {
-        constexpr bool NEAR = decltype(near_tag)::value, WHOLE = decltype(whole_tag)::value;
-        const float4v flat = splat4(side < 0 ? bias_lo : bias_hi);
-        float4v sc[QB][4];
+  __syncthreads();  // the bias array is complete
+  const float bias_lo = bias.t[0], bias_hi = bias.t[bias.len - 1];
+  auto sweep = [&](auto far_tag, RaChunks cur) {
+    constexpr bool FAR = decltype(far_tag)::value;
+    while (!cur.done() && (!FAR || cur.far)) {
+      const int buf = cur.buf;
+      RaChunks nx = cur;
+      nx.next(word);
+      nx.buf ^= 1;
+      __syncthreads();  // every wave is done with the other buffer
+      if (!nx.done()) {
+        stage(nx.c, buf ^ 1, nx.w);
+        if (NH == 1) asm volatile("s_waitcnt vmcnt(4)" ::: "memory");
+        else asm volatile("s_waitcnt vmcnt(8)" ::: "memory");
+      } else {
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+      }
+      __syncthreads();
+      if (active) {
+        const char* kimg = smem + buf * BUF;
+        const char* vimg = kimg + NH * RA_IMG;
+        const int u0 = cur.c * RA_CHUNK - q0;
+        const float flat = cur.c <= cur.lo ? bias_lo : bias_hi;
 #pragma unroll
-        for (int kb = 0; kb < 4; ++kb) {
+        for (int pb = 0; pb < 2; ++pb) {  // 32 keys at a time
+          float4v sc[QB][2];
 #pragma unroll
-          for (int i = 0; i < QB; ++i) sc[i][kb] = splat4(0.f);
+          for (int hb = 0; hb < 2; ++hb) {
 #pragma unroll
-          for (int ks = 0; ks < KS; ++ks) {
-            const short8 kf = ra_row_frag(kimg, kb * 16, ks, lane);
+            for (int i = 0; i < QB; ++i) sc[i][hb] = splat4(0.f);
 #pragma unroll
-            for (int i = 0; i < QB; ++i) sc[i][kb] = Half16<T>::mfma(kf, qf[i][ks], sc[i][kb]);
-          }
-        }
+            for (int ks = 0; ks < KS; ++ks) {
+              const short8 kf = ra_row_frag(kimg, pb * 32 + hb * 16, ks, lane);
 #pragma unroll
-        for (int i = 0; i < QB; ++i) {
-          float cmax = -INFINITY;
-#pragma unroll
-          for (int kb = 0; kb < 4; ++kb) {
-            float4v t = sc[i][kb] * k2 + (NEAR ? ra_bias4(bias, boff, u0 + kb * 16 - 16 * i) : flat);
-            if (!WHOLE) {
-              const uint32_t bits = (uint32_t)(w >> (kb * 16 + 4 * g));
-#pragma unroll
-              for (int r = 0; r < 4; ++r) t[r] = (bits >> r) & 1 ? t[r] : -INFINITY;
+              for (int i = 0; i < QB; ++i) sc[i][hb] = Half16<T>::mfma(kf, qf[i][ks], sc[i][hb]);
             }
-            cmax = fmaxf(fmaxf(cmax, t[0]), fmaxf(fmaxf(t[1], t[2]), t[3]));
-            sc[i][kb] = t;
           }
-          // The accumulators are rescaled only when some row's maximum has grown by more than 2^RA_SLACK since its last
-          // rescale: p then stays below 2^RA_SLACK instead of 1, which 16-bit operands and fp32 sums hold as exactly.
-          if (__any(cmax > m[i] + RA_SLACK)) {
-            const float m_new = fmaxf(m[i], ra_quad_max(cmax));
-            const float alpha = __builtin_amdgcn_exp2f(m[i] - (m_new == -INFINITY ? 0.f : m_new));
-            m[i] = m_new;
-            l4[i] *= alpha;
-#pragma unroll
-            for (int db = 0; db < 2 * KS; ++db) o[i][db] *= alpha;
-          }
-          const float m_use = m[i] == -INFINITY ? 0.f : m[i];  // no attended key so far: exp2(-inf - 0) = 0
-#pragma unroll
-          for (int kb = 0; kb < 4; ++kb) {
-            float4v t = sc[i][kb] - m_use;
-#pragma unroll
-            for (int r = 0; r < 4; ++r) t[r] = __builtin_amdgcn_exp2f(t[r]);
-            l4[i] += t;
-            if (DROP) {
-#pragma unroll
-              for (int r = 0; r < 4; ++r)
-                t[r] *= attn_keep(seed[i], kmul0 + (uint32_t)(c * RA_CHUNK + kb * 16 + r) * ATT_GOLD, thr_hi) ? p.drop_scale : 0.f;
-            }
-            sc[i][kb] = t;
-          }
-        }
-#pragma unroll
-        for (int pb = 0; pb < 2; ++pb) {
           short8 pf[QB];
 #pragma unroll
-          for (int i = 0; i < QB; ++i) pf[i] = pack_pair<T>(sc[i][2 * pb], sc[i][2 * pb + 1]);
+          for (int i = 0; i < QB; ++i) {
+            float cmax = -INFINITY;
+#pragma unroll
+            for (int hb = 0; hb < 2; ++hb) {
+              const int k16 = pb * 32 + hb * 16;
+              if (!FAR)
+                sc[i][hb] = sc[i][hb] * k2 + (ra_bias4(bias, boff, u0 + k16 - 16 * i) +
+                                              *reinterpret_cast<const float4v*>(mb + buf * RA_CHUNK + k16 + 4 * g));
+              const float4v t = sc[i][hb];
+              cmax = fmaxf(fmaxf(cmax, t[0]), fmaxf(fmaxf(t[1], t[2]), t[3]));
+            }
+            if (FAR) cmax = cmax * k2 + flat;
+            // The accumulators are rescaled only when some row's maximum has grown by more than 2^RA_SLACK since its last
+            // rescale: p then stays below 2^RA_SLACK instead of 1, which 16-bit operands and fp32 sums hold as exactly.
+            if (__any(cmax > m[i] + RA_SLACK)) {
+              const float m_new = fmaxf(m[i], ra_quad_max(cmax));
+              const float alpha = __builtin_amdgcn_exp2f(m[i] - (m_new == -INFINITY ? 0.f : m_new));
+              m[i] = m_new;
+              l4[i] *= alpha;
+#pragma unroll
+              for (int db = 0; db < 2 * KS; ++db) o[i][db] *= alpha;
+            }
+            const float m_use = m[i] == -INFINITY ? 0.f : m[i];  // no attended key so far: exp2(-inf - 0) = 0
+#pragma unroll
+            for (int hb = 0; hb < 2; ++hb) {
+              float4v t = FAR ? sc[i][hb] * k2 + (flat - m_use) : sc[i][hb] - m_use;
+#pragma unroll
+              for (int r = 0; r < 4; ++r) t[r] = __builtin_amdgcn_exp2f(t[r]);
+              l4[i] += t;
+              if (DROP) {
+#pragma unroll
+                for (int r = 0; r < 4; ++r)
+                  t[r] *= attn_keep(seed[i], kmul0 + (uint32_t)(cur.c * RA_CHUNK + pb * 32 + hb * 16 + r) * ATT_GOLD, thr_hi) ? p.drop_scale : 0.f;
+              }
+              sc[i][hb] = t;
+            }
+            pf[i] = pack_pair<T>(sc[i][0], sc[i][1]);
+          }
 #pragma unroll
           for (int db = 0; db < 2 * KS; ++db) {
             const short8 vf = ra_tr_frag(vimg, pb * 32, db, lane);
@@ -349,14 +387,12 @@ __global__ __launch_bounds__(RA_THREADS) RA_OCC_FWD void rel_attn_fwd_kernel(Pdt
             for (int i = 0; i < QB; ++i) o[i][db] = Half16<T>::mfma(vf, pf[i], o[i][db]);
           }
         }
-      };
-      if (w != ~0ull) chunk(std::true_type{}, std::false_type{});
-      else if (side) chunk(std::false_type{}, std::true_type{});
-      else chunk(std::true_type{}, std::true_type{});
+      }
+      cur = nx;
     }
-    c = cn;
-    w = wn;
-  }
+    return cur;
+  };
+  sweep(std::false_type{}, sweep(std::true_type{}, cur));
   if (!active) return;
   T* ob = ra_base<T>(p.o, s, packed);
 #pragma unroll
@@ -370,21 +406,59 @@ __global__ __launch_bounds__(RA_THREADS) RA_OCC_FWD void rel_attn_fwd_kernel(Pdt
   }
 }
 
-// Sum of ds over the distances: tile t (lane (lm, g): keys 4 g + r, query lm) of blocks u apart.
-// N: lane l holds the sum over r of the elements at (4 g + r, l + r), distance u + 4 g - l; W: those with l + r >= 16,
-// i.e. query l + r - 16, distance u + 4 g - l + 16 (lanes 13..15 only).  Every lane group has an array of its own, so no two
-// lanes of an add meet; adds of one wave to its own arrays execute in order.
-__device__ __forceinline__ void ra_diag_add(float* d, const float4v& t, int lm) {
+// Sums of ds along its diagonals, from 16x16 tiles (lane (lm, g): keys 4 g + r, query lm) of blocks u apart:
+// N: lane l holds the sum over r of the elements at (4 g + r, l + r), distance u + 4 g - l.  W: those with l + r >= 16, i.e.
+// query l + r - 16, distance u + 4 g - l + 16 (lanes 13..15 only): the place that N of the tile at u + 16 has in the same lane.
+__device__ __forceinline__ float ra_diag_n(const float4v& t) {
   float n = t[0];
   n += dpp_f<0x101>(t[1]);  // row_shl:1
   n += dpp_f<0x102>(t[2]);
   n += dpp_f<0x103>(t[3]);
+  return n;
+}
+__device__ __forceinline__ float ra_diag_w(const float4v& t) {
   float w = dpp_f<0x11F>(t[1]);  // row_shr:15
   w += dpp_f<0x11E>(t[2]);
   w += dpp_f<0x11D>(t[3]);
-  atomicAdd(d, n);
-  if (lm >= 13) atomicAdd(d + 16, w);
+  return w;
 }
+template <int CTRL, int ROWS>
+__device__ __forceinline__ float ra_dpp_rows(float old, float v) {  // the rows in ROWS shifted (zeros come in), the others from old
+  return __int_as_float(__builtin_amdgcn_update_dpp(__float_as_int(old), __float_as_int(v), CTRL, ROWS, 0xF, true));
+}
+// N summed over the lane groups, whose distances are 4 lanes apart: place l' = l + 12 - 4 g has distance u + 12 - l'.  Lanes
+// 0..31 receive the places 0..15 (each twice), lanes 32..63 the places 16..27 (and four zeros).
+__device__ __forceinline__ float ra_diag_fold(float n) {
+  float low = ra_dpp_rows<0x11C, 1>(n, n);  // row_shr:12 of group 0
+  low = ra_dpp_rows<0x118, 2>(low, n);
+  low = ra_dpp_rows<0x114, 4>(low, n);
+  float high = ra_dpp_rows<0x104, 1>(0.f, n);  // what left the row: row_shl:4 of group 0
+  high = ra_dpp_rows<0x108, 2>(high, n);
+  high = ra_dpp_rows<0x10C, 4>(high, n);
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(low), __float_as_uint(high), false, false);
+  float a, b = ra_other16(__uint_as_float(r[0]) + __uint_as_float(r[1]), a);
+  return a + b;
+}
+// The diagonal sums of one wave.  Tiles arrive in ascending order of u; each near u stores its places once (two arrays: places
+// 0..15 and 16..27 of different u fall on the same distances) and hands W to the next.  LDS float atomics instead of this cost
+// 24 us of 134 at 32 x 512 tokens, 12 heads, and four times the arrays.
+struct RaDiag {
+  float* at;    // where this lane stores for u = 0
+  float w;
+  int u;        // the last near tile (a multiple of 16), or NONE
+  static constexpr int NONE = -(1 << 20);
+  __device__ __forceinline__ void store(int v, float n) { at[v] = ra_diag_fold(n); }
+  __device__ __forceinline__ void flush() {
+    if (u != NONE) store(u + 16, w);
+    u = NONE;
+  }
+  __device__ __forceinline__ void add(int v, const float4v& t) {
+    if (u != NONE && u + 16 != v) flush();
+    store(v, ra_diag_n(t) + (u != NONE ? w : 0.f));
+    w = ra_diag_w(t);
+    u = v;
+  }
+};
 
 // distances -> buckets: sums[top + d] is the sum at distance d, |d| <= top; eight lanes per bucket walk its range
 template <int THREADS>
@@ -409,7 +483,7 @@ __device__ __forceinline__ void ra_bucket_sums(const PdtRelAttn& p, const float*
 // ------------------------------------------------------------------------------------------------ dQ and the table gradient
 // One wave = 16 QB query rows, sweeps the keys; also stores delta = rowsum(dO * O) for the dK / dV kernel.
 template <typename T, int KS, int QB, bool DROP>
-__global__ __launch_bounds__(RA_THREADS) RA_OCC_BWD void rel_attn_dq_kernel(PdtRelAttn p) {
+__global__ __launch_bounds__(RA_THREADS) RA_OCC_DQ void rel_attn_dq_kernel(PdtRelAttn p) {
   constexpr int NH = (KS + 1) / 2, BUF = 2 * NH * RA_IMG;
   extern __shared__ __attribute__((aligned(16))) char smem[];
   const int tid = threadIdx.x, lane = tid & 63, lm = lane & 15, g = lane >> 4;
@@ -428,26 +502,28 @@ __global__ __launch_bounds__(RA_THREADS) RA_OCC_BWD void rel_attn_dq_kernel(PdtR
   const T* vb_ = ra_base<const T>(p.v, s, packed);
   const T* ob_ = ra_base<const T>(p.o, s, packed);
   const T* gb_ = ra_base<const T>(p.dout, s, packed);
-  const int nc = (s.n + RA_CHUNK - 1) / RA_CHUNK;
+  float* const mb = reinterpret_cast<float*>(smem + 2 * BUF);  // 0 / -inf of the 64 keys of each buffer
   auto stage = [&](int c, int buf, uint64_t w) {
     char* m = smem + buf * BUF;
     ra_stage<T, NH>(m, kb_ + (int64_t)c * RA_CHUNK * p.k.row, (uint32_t)p.k.row, w, p.D, lane, wave);
     ra_stage<T, NH>(m + NH * RA_IMG, vb_ + (int64_t)c * RA_CHUNK * p.v.row, (uint32_t)p.v.row, w, p.D, lane, wave);
+    if (tid < RA_CHUNK) mb[buf * RA_CHUNK + tid] = (w >> tid) & 1 ? 0.f : -INFINITY;
   };
-  uint64_t w;
-  int c = ra_next(p, s, 0, nc, w);
-  if (c < nc) stage(c, 0, w);
-  const RaBias bias = ra_bias_fill<T>(p, reinterpret_cast<float*>(smem + 2 * BUF), s.h, 1, tid, p.max_distance);
+  auto word = [&](int c) { return ra_word(p, s, c); };
+  RaChunks cur = ra_chunks(s.n, w0, RA_WAVES * 16 * QB, ra_far(p.max_distance), p.table != nullptr, true);
+  cur.next(word);
+  if (!cur.done()) stage(cur.c, 0, cur.w);
+  const RaBias bias = ra_bias_fill<T>(p, mb + 2 * RA_CHUNK, s.h, 1, tid, p.max_distance);
   const int boff = ra_bias_lane(bias, lm, g);
-  const bool has_bias = p.table != nullptr, active = q0 < s.n;
-  // diagonal sums, one array per wave and lane group: entry 0 is distance -(far + 31).  `diag` is where this lane's sum
-  // of a tile at u = 0 belongs.
+  const bool active = q0 < s.n;
+  // diagonal sums, two arrays per wave: entry 0 is distance -(far + 31)
   const int dlen = ra_diag_len(p.max_distance);
   float* const sums = bias.t + 4 * bias.len;
-  float* const diag = sums + (wave * 4 + g) * dlen + bias.far + 31 + 4 * g - lm;
+  RaDiag diag{sums + (wave * 2 + (g >> 1)) * dlen + bias.far + 31 + (g >> 1 ? -4 : 12) - lm, 0.f, RaDiag::NONE};
   if (part)
-    for (int i = tid; i < 4 * RA_WAVES * dlen; i += RA_THREADS) sums[i] = 0.f;
-  float bias_lo = 0.f, bias_hi = 0.f;
+    for (int i = tid; i < 2 * RA_WAVES * dlen; i += RA_THREADS) sums[i] = 0.f;
+  float4v open = splat4(0.f);  // the tile of the last offset, which the next pair of tiles adds to (two blocks per wave)
+  int open_u = RaDiag::NONE;
   float4v far_lo = splat4(0.f), far_hi = splat4(0.f);
   short8 qf[QB][KS], df[QB][KS];
   uint32_t seed[QB];
@@ -478,103 +554,110 @@ __global__ __launch_bounds__(RA_THREADS) RA_OCC_BWD void rel_attn_dq_kernel(PdtR
   for (int i = 0; i < QB; ++i)
 #pragma unroll
     for (int db = 0; db < 2 * KS; ++db) dq[i][db] = splat4(0.f);
-  for (int buf = 0; c < nc; buf ^= 1) {
-    uint64_t wn;
-    const int cn = ra_next(p, s, c + 1, nc, wn);
-    __syncthreads();  // (first time: the arrays are complete)
-    bias_lo = bias.t[0];
-    bias_hi = bias.t[bias.len - 1];
-    if (cn < nc) {
-      stage(cn, buf ^ 1, wn);
-      if (NH == 1) asm volatile("s_waitcnt vmcnt(4)" ::: "memory");
-      else asm volatile("s_waitcnt vmcnt(8)" ::: "memory");
-    } else {
-      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    }
-    __syncthreads();
-    if (active) {
-      const char* kimg = smem + buf * BUF;
-      const char* vimg = kimg + NH * RA_IMG;
-      const int u0 = c * RA_CHUNK - q0;
-      const int side = has_bias ? ra_side(bias, u0 - 16 * (QB - 1), u0 + 48) : 1;
-      auto chunk = [&](auto near_tag, auto whole_tag) {
-        constexpr bool NEAR = decltype(near_tag)::value, WHOLE = decltype(whole_tag)::value;
-        float4v flat[QB], ds[QB][4];
-#pragma unroll
-        for (int i = 0; i < QB; ++i) flat[i] = splat4((side < 0 ? bias_lo : bias_hi) + nlse[i]);
+  __syncthreads();  // the arrays are complete
+  const float bias_lo = bias.t[0], bias_hi = bias.t[bias.len - 1];
+  auto near = [&](int u, const float4v& t) {  // (chunks of the second loop hold far tiles as well)
+    if (u >= bias.far + 16) far_hi += t;
+    else if (u <= -(bias.far + 16)) far_lo += t;
+    else diag.add(u, t);
+  };
+  auto sweep = [&](auto far_tag, RaChunks cur) {
+    constexpr bool FAR = decltype(far_tag)::value;
+    while (!cur.done() && (!FAR || cur.far)) {
+      const int buf = cur.buf;
+      RaChunks nx = cur;
+      nx.next(word);
+      nx.buf ^= 1;
+      __syncthreads();  // every wave is done with the other buffer
+      if (!nx.done()) {
+        stage(nx.c, buf ^ 1, nx.w);
+        if (NH == 1) asm volatile("s_waitcnt vmcnt(4)" ::: "memory");
+        else asm volatile("s_waitcnt vmcnt(8)" ::: "memory");
+      } else {
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+      }
+      __syncthreads();
+      if (active) {
+        const char* kimg = smem + buf * BUF;
+        const char* vimg = kimg + NH * RA_IMG;
+        const int u0 = cur.c * RA_CHUNK - q0;
+        const bool below = cur.c <= cur.lo;
 #pragma unroll
         for (int pb = 0; pb < 2; ++pb) {
+          float4v ds[QB][2];
 #pragma unroll
           for (int hb = 0; hb < 2; ++hb) {
-            const int kb = 2 * pb + hb;
+            const int k16 = pb * 32 + hb * 16;
             float4v sc[QB], dp[QB];
 #pragma unroll
             for (int i = 0; i < QB; ++i) { sc[i] = splat4(0.f); dp[i] = splat4(0.f); }
 #pragma unroll
             for (int ks = 0; ks < KS; ++ks) {
-              const short8 kf = ra_row_frag(kimg, kb * 16, ks, lane), vf = ra_row_frag(vimg, kb * 16, ks, lane);
+              const short8 kf = ra_row_frag(kimg, k16, ks, lane), vf = ra_row_frag(vimg, k16, ks, lane);
 #pragma unroll
               for (int i = 0; i < QB; ++i) {
                 sc[i] = Half16<T>::mfma(kf, qf[i][ks], sc[i]);
                 dp[i] = Half16<T>::mfma(vf, df[i][ks], dp[i]);
               }
             }
-            const uint32_t bits = (uint32_t)(w >> (kb * 16 + 4 * g));
 #pragma unroll
             for (int i = 0; i < QB; ++i) {
-              float4v t = sc[i] * k2 + (NEAR ? ra_bias4(bias, boff, u0 + kb * 16 - 16 * i) + nlse[i] : flat[i]);
+              float4v add = splat4((below ? bias_lo : bias_hi) + nlse[i]);
+              if (!FAR)
+                add = ra_bias4(bias, boff, u0 + k16 - 16 * i) + *reinterpret_cast<const float4v*>(mb + buf * RA_CHUNK + k16 + 4 * g) + nlse[i];
+              float4v t = sc[i] * k2 + add;
 #pragma unroll
               for (int r = 0; r < 4; ++r) t[r] = __builtin_amdgcn_exp2f(t[r]);
-              if (!WHOLE) {
-#pragma unroll
-                for (int r = 0; r < 4; ++r) t[r] = (bits >> r) & 1 ? t[r] : 0.f;
-              }
               float4v e = dp[i];
               if (DROP) {
 #pragma unroll
                 for (int r = 0; r < 4; ++r)
-                  e[r] *= attn_keep(seed[i], kmul0 + (uint32_t)(c * RA_CHUNK + kb * 16 + r) * ATT_GOLD, thr_hi) ? p.drop_scale : 0.f;
+                  e[r] *= attn_keep(seed[i], kmul0 + (uint32_t)(cur.c * RA_CHUNK + k16 + r) * ATT_GOLD, thr_hi) ? p.drop_scale : 0.f;
               }
-              ds[i][kb] = t * (e + nd[i]);
+              ds[i][hb] = t * (e + nd[i]);
             }
           }
           short8 sf[QB];
 #pragma unroll
-          for (int i = 0; i < QB; ++i) sf[i] = pack_pair<T>(ds[i][2 * pb], ds[i][2 * pb + 1]);
+          for (int i = 0; i < QB; ++i) sf[i] = pack_pair<T>(ds[i][0], ds[i][1]);
 #pragma unroll
           for (int db = 0; db < 2 * KS; ++db) {
             const short8 kf = ra_tr_frag(kimg, pb * 32, db, lane);
 #pragma unroll
             for (int i = 0; i < QB; ++i) dq[i][db] = Half16<T>::mfma(kf, sf[i], dq[i][db]);
           }
-        }
-        if (part) {
-          if (NEAR) {  // tiles of the same offset u = u0 + 16 (kb - i) first add up
+          if (part) {
+            if (!FAR) {  // tiles of the same offset u = u0 + 16 (kb - i) first add up
+              const int u = u0 + 32 * pb;
+              if (QB == 2) {
+                if (open_u == u - 16) {
+                  near(u - 16, open + ds[QB - 1][0]);
+                } else {
+                  if (open_u != RaDiag::NONE) near(open_u, open);
+                  near(u - 16, ds[QB - 1][0]);
+                }
+                near(u, ds[0][0] + ds[QB - 1][1]);
+                open = ds[0][1];
+                open_u = u + 16;
+              } else {
+                near(u, ds[0][0]);
+                near(u + 16, ds[0][1]);
+              }
+            } else {
+              float4v t = ds[0][0] + ds[0][1];
 #pragma unroll
-            for (int j = 1 - QB; j < 4; ++j) {
-              float4v t = splat4(0.f);
-#pragma unroll
-              for (int i = 0; i < QB; ++i)
-                if (j + i >= 0 && j + i < 4) t += ds[i][j + i];
-              const int u = min(max(u0 + 16 * j, -(bias.far + 16)), bias.far + 16);
-              ra_diag_add(diag + u, t, lm);
+              for (int i = 1; i < QB; ++i) t += ds[i][0] + ds[i][1];
+              if (below) far_lo += t;
+              else far_hi += t;
             }
-          } else {
-            float4v t = splat4(0.f);
-#pragma unroll
-            for (int i = 0; i < QB; ++i) t += (ds[i][0] + ds[i][1]) + (ds[i][2] + ds[i][3]);
-            if (side < 0) far_lo += t;
-            else far_hi += t;
           }
         }
-      };
-      if (w != ~0ull) chunk(std::true_type{}, std::false_type{});
-      else if (side) chunk(std::false_type{}, std::true_type{});
-      else chunk(std::true_type{}, std::true_type{});
+      }
+      cur = nx;
     }
-    c = cn;
-    w = wn;
-  }
+    return cur;
+  };
+  sweep(std::false_type{}, sweep(std::true_type{}, cur));
   if (active) {
     T* dqb = ra_base<T>(p.dq, s, packed);
 #pragma unroll
@@ -584,17 +667,20 @@ __global__ __launch_bounds__(RA_THREADS) RA_OCC_BWD void rel_attn_dq_kernel(PdtR
     }
   }
   if (part) {  // the far sums join the ends of their wave's first array; then distances -> buckets
+    if (open_u != RaDiag::NONE) near(open_u, open);
+    diag.flush();
     const float lo = wave_sum((far_lo[0] + far_lo[1]) + (far_lo[2] + far_lo[3]));
     const float hi = wave_sum((far_hi[0] + far_hi[1]) + (far_hi[2] + far_hi[3]));
+    float* const mine = sums + wave * 2 * dlen;
     if (lane == 0) {
-      sums[wave * 4 * dlen] += lo;
-      sums[wave * 4 * dlen + 2 * bias.far + 62] += hi;
+      mine[0] += lo;
+      mine[2 * bias.far + 62] += hi;
     }
     __syncthreads();
-    for (int i = tid; i < dlen; i += RA_THREADS) {  // (the sixteen arrays into the first)
+    for (int i = tid; i < dlen; i += RA_THREADS) {  // (the eight arrays into the first)
       float t = 0.f;
 #pragma unroll
-      for (int a = 0; a < 4 * RA_WAVES; ++a) t += sums[a * dlen + i];
+      for (int a = 0; a < 2 * RA_WAVES; ++a) t += sums[a * dlen + i];
       sums[i] = t;
     }
     __syncthreads();
@@ -605,7 +691,7 @@ __global__ __launch_bounds__(RA_THREADS) RA_OCC_BWD void rel_attn_dq_kernel(PdtR
 // ------------------------------------------------------------------------------------------------ dK, dV
 // One wave = 16 QB keys, sweeps the queries (Q and dO images); lse, delta and dropout seeds of a chunk's queries in LDS.
 template <typename T, int KS, int QB, bool DROP>
-__global__ __launch_bounds__(RA_THREADS) RA_OCC_BWD void rel_attn_dkv_kernel(PdtRelAttn p) {
+__global__ __launch_bounds__(RA_THREADS) RA_OCC_DKV void rel_attn_dkv_kernel(PdtRelAttn p) {
   constexpr int NH = (KS + 1) / 2, BUF = 2 * NH * RA_IMG + 1024;  // Q | dO | lse, delta, seeds (64 each), 256 spare bytes
   extern __shared__ __attribute__((aligned(16))) char smem[];
   const int tid = threadIdx.x, lane = tid & 63, lm = lane & 15, g = lane >> 4;
@@ -619,7 +705,6 @@ __global__ __launch_bounds__(RA_THREADS) RA_OCC_BWD void rel_attn_dkv_kernel(Pdt
   const T* vb_ = ra_base<const T>(p.v, s, packed);
   const T* gb_ = ra_base<const T>(p.dout, s, packed);
   const int64_t bh = (int64_t)s.b * p.A + s.h;
-  const int nc = (s.n + RA_CHUNK - 1) / RA_CHUNK;
   const DropKey dkey = drop_key(p.rng);
   const uint32_t sbh = drop_sample(p.rng, s.b) * p.A + s.h;
   auto stage = [&](int c, int buf) {
@@ -636,26 +721,27 @@ __global__ __launch_bounds__(RA_THREADS) RA_OCC_BWD void rel_attn_dkv_kernel(Pdt
     if (DROP && tid < 64)
       reinterpret_cast<uint32_t*>(m + 2 * NH * RA_IMG + 512)[tid] = attn_row_seed(dkey, sbh, c * RA_CHUNK + tid);
   };
-  stage(0, 0);
+  auto word = [&](int c) { return s.n - c * RA_CHUNK >= RA_CHUNK ? ~0ull : (1ull << (s.n - c * RA_CHUNK)) - 1; };  // (queries)
+  RaChunks cur = ra_chunks(s.n, w0, RA_WAVES * 16 * QB, ra_far(p.max_distance), p.table != nullptr, true);
+  cur.next(word);
+  stage(cur.c, 0);
   const RaBias bias = ra_bias_fill<T>(p, reinterpret_cast<float*>(smem + 2 * BUF), s.h, -1, tid, p.max_distance);
   const int boff = ra_bias_lane(bias, lm, g);
-  const bool has_bias = p.table != nullptr;
   short8 kf[QB][KS], vf[QB][KS];
-  bool kok[QB];
+  float kneg[QB];  // -inf for a key that no query attends to
   uint32_t kmul[QB];
   const uint64_t kw = k0 < s.n ? ra_word(p, s, k0 / RA_CHUNK) >> (k0 % RA_CHUNK) : 0;
-  constexpr uint64_t MINE = QB == 2 ? 0xFFFFFFFFull : 0xFFFFull;  // (a wave's keys lie in one chunk)
-  const bool active = (kw & MINE) != 0, all_keys = (kw & MINE) == MINE;
-  float bias_lo = 0.f, bias_hi = 0.f;
+  const bool active = (kw & (QB == 2 ? 0xFFFFFFFFull : 0xFFFFull)) != 0;  // (a wave's keys lie in one chunk)
 #pragma unroll
   for (int i = 0; i < QB; ++i) {
     const int key = k0 + 16 * i + lm;
-    kok[i] = (kw >> (16 * i + lm)) & 1;
+    const bool ok = (kw >> (16 * i + lm)) & 1;
+    kneg[i] = ok ? 0.f : -INFINITY;
     kmul[i] = (uint32_t)key * ATT_GOLD;
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks) {
-      kf[i][ks] = ra_gfrag<T>(kb_ + (int64_t)key * p.k.row, ks, p.D, lane, kok[i]);
-      vf[i][ks] = ra_gfrag<T>(vb_ + (int64_t)key * p.v.row, ks, p.D, lane, kok[i]);
+      kf[i][ks] = ra_gfrag<T>(kb_ + (int64_t)key * p.k.row, ks, p.D, lane, ok);
+      vf[i][ks] = ra_gfrag<T>(vb_ + (int64_t)key * p.v.row, ks, p.D, lane, ok);
     }
   }
   const float k2 = p.scale * LOG2E;
@@ -665,86 +751,87 @@ __global__ __launch_bounds__(RA_THREADS) RA_OCC_BWD void rel_attn_dkv_kernel(Pdt
   for (int i = 0; i < QB; ++i)
 #pragma unroll
     for (int db = 0; db < 2 * KS; ++db) { dk_[i][db] = splat4(0.f); dv_[i][db] = splat4(0.f); }
-  for (int c = 0, buf = 0; c < nc; ++c, buf ^= 1) {
-    __syncthreads();  // (first time: the bias array is complete)
-    bias_lo = bias.t[0];
-    bias_hi = bias.t[bias.len - 1];
-    if (c + 1 < nc) {
-      stage(c + 1, buf ^ 1);
-      if (NH == 1) asm volatile("s_waitcnt vmcnt(5)" ::: "memory");
-      else asm volatile("s_waitcnt vmcnt(9)" ::: "memory");
-    } else {
-      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    }
-    __syncthreads();
-    if (!active) continue;
-    const char* qimg = smem + buf * BUF;
-    const char* gimg = qimg + NH * RA_IMG;
-    const float* sc_ = reinterpret_cast<const float*>(gimg + NH * RA_IMG);
-    const int left = s.n - c * RA_CHUNK, u0 = c * RA_CHUNK - k0;  // (query - key: the array is mirrored)
-    const int side = has_bias ? ra_side(bias, u0 - 16 * (QB - 1), u0 + 48) : 1;
-    auto chunk = [&](auto near_tag, auto whole_tag) {
-    constexpr bool NEAR = decltype(near_tag)::value, WHOLE = decltype(whole_tag)::value;
-    const float flat = side < 0 ? bias_lo : bias_hi;
+  __syncthreads();  // the bias array is complete
+  const float bias_lo = bias.t[0], bias_hi = bias.t[bias.len - 1];
+  auto sweep = [&](auto far_tag, RaChunks cur) {
+    constexpr bool FAR = decltype(far_tag)::value;
+    while (!cur.done() && (!FAR || cur.far)) {
+      const int buf = cur.buf;
+      RaChunks nx = cur;
+      nx.next(word);
+      nx.buf ^= 1;
+      __syncthreads();  // every wave is done with the other buffer
+      if (!nx.done()) {
+        stage(nx.c, buf ^ 1);
+        if (NH == 1) asm volatile("s_waitcnt vmcnt(5)" ::: "memory");
+        else asm volatile("s_waitcnt vmcnt(9)" ::: "memory");
+      } else {
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+      }
+      const char* qimg = smem + buf * BUF;
+      const char* gimg = qimg + NH * RA_IMG;
+      float* const sc_ = reinterpret_cast<float*>(smem + buf * BUF + 2 * NH * RA_IMG);
+      // queries that are not there: p = 0 (their lse has arrived as 0)
+      if (!FAR && wave == 0 && cur.c * RA_CHUNK + lane >= s.n) sc_[lane] = INFINITY;
+      __syncthreads();
+      if (active) {
+        const int u0 = cur.c * RA_CHUNK - k0;  // query - key: the bias array is mirrored
+        const float flat = cur.c <= cur.lo ? bias_lo : bias_hi;
 #pragma unroll
-    for (int pb = 0; pb < 2; ++pb) {
-      float4v pp[QB][2], ds[QB][2];
+        for (int pb = 0; pb < 2; ++pb) {
+          float4v pp[QB][2], ds[QB][2];
 #pragma unroll
-      for (int hb = 0; hb < 2; ++hb) {
-        const int qb = 2 * pb + hb;
-        float4v sc[QB], dp[QB];
+          for (int hb = 0; hb < 2; ++hb) {
+            const int q16 = pb * 32 + hb * 16;
+            float4v sc[QB], dp[QB];
 #pragma unroll
-        for (int i = 0; i < QB; ++i) { sc[i] = splat4(0.f); dp[i] = splat4(0.f); }
+            for (int i = 0; i < QB; ++i) { sc[i] = splat4(0.f); dp[i] = splat4(0.f); }
 #pragma unroll
-        for (int ks = 0; ks < KS; ++ks) {
-          const short8 qf = ra_row_frag(qimg, qb * 16, ks, lane), gf = ra_row_frag(gimg, qb * 16, ks, lane);
+            for (int ks = 0; ks < KS; ++ks) {
+              const short8 qf = ra_row_frag(qimg, q16, ks, lane), gf = ra_row_frag(gimg, q16, ks, lane);
 #pragma unroll
-          for (int i = 0; i < QB; ++i) {
-            sc[i] = Half16<T>::mfma(qf, kf[i][ks], sc[i]);
-            dp[i] = Half16<T>::mfma(gf, vf[i][ks], dp[i]);
+              for (int i = 0; i < QB; ++i) {
+                sc[i] = Half16<T>::mfma(qf, kf[i][ks], sc[i]);
+                dp[i] = Half16<T>::mfma(gf, vf[i][ks], dp[i]);
+              }
+            }
+            const float4v lse = *reinterpret_cast<const float4v*>(sc_ + q16 + 4 * g);
+            const float4v del = *reinterpret_cast<const float4v*>(sc_ + 64 + q16 + 4 * g);
+            const uint4v sd = *reinterpret_cast<const uint4v*>(sc_ + 128 + q16 + 4 * g);
+#pragma unroll
+            for (int i = 0; i < QB; ++i) {
+              float4v t = sc[i] * k2 + ((FAR ? splat4(flat + kneg[i]) : ra_bias4(bias, boff, u0 + q16 - 16 * i) + kneg[i]) - lse);
+              float4v e = dp[i], pd;
+#pragma unroll
+              for (int r = 0; r < 4; ++r) {
+                t[r] = __builtin_amdgcn_exp2f(t[r]);
+                const float keep = !DROP ? 1.f : (attn_keep(sd[r], kmul[i], thr_hi) ? p.drop_scale : 0.f);
+                pd[r] = DROP ? t[r] * keep : t[r];
+                if (DROP) e[r] *= keep;
+              }
+              pp[i][hb] = pd;
+              ds[i][hb] = t * (e - del);
+            }
           }
-        }
-        const float4v lse = *reinterpret_cast<const float4v*>(sc_ + qb * 16 + 4 * g);
-        const float4v del = *reinterpret_cast<const float4v*>(sc_ + 64 + qb * 16 + 4 * g);
-        const uint4v sd = *reinterpret_cast<const uint4v*>(sc_ + 128 + qb * 16 + 4 * g);
+          short8 pf[QB], sf[QB];
 #pragma unroll
-        for (int i = 0; i < QB; ++i) {
-          float4v t = sc[i] * k2 + ((NEAR ? ra_bias4(bias, boff, u0 + qb * 16 - 16 * i) : splat4(flat)) - lse);
-          if (!WHOLE) {  // queries that are not there
+          for (int i = 0; i < QB; ++i) { pf[i] = pack_pair<T>(pp[i][0], pp[i][1]); sf[i] = pack_pair<T>(ds[i][0], ds[i][1]); }
 #pragma unroll
-            for (int r = 0; r < 4; ++r) t[r] = qb * 16 + 4 * g + r < left ? t[r] : -INFINITY;
+          for (int db = 0; db < 2 * KS; ++db) {
+            const short8 gf = ra_tr_frag(gimg, pb * 32, db, lane), qf = ra_tr_frag(qimg, pb * 32, db, lane);
+#pragma unroll
+            for (int i = 0; i < QB; ++i) {
+              dv_[i][db] = Half16<T>::mfma(gf, pf[i], dv_[i][db]);
+              dk_[i][db] = Half16<T>::mfma(qf, sf[i], dk_[i][db]);
+            }
           }
-          float4v e = dp[i], pd;
-#pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            t[r] = __builtin_amdgcn_exp2f(t[r]);
-            if (!WHOLE) t[r] = kok[i] ? t[r] : 0.f;
-            const float keep = !DROP ? 1.f : (attn_keep(sd[r], kmul[i], thr_hi) ? p.drop_scale : 0.f);
-            pd[r] = DROP ? t[r] * keep : t[r];
-            if (DROP) e[r] *= keep;
-          }
-          pp[i][hb] = pd;
-          ds[i][hb] = t * (e - del);
         }
       }
-      short8 pf[QB], sf[QB];
-#pragma unroll
-      for (int i = 0; i < QB; ++i) { pf[i] = pack_pair<T>(pp[i][0], pp[i][1]); sf[i] = pack_pair<T>(ds[i][0], ds[i][1]); }
-#pragma unroll
-      for (int db = 0; db < 2 * KS; ++db) {
-        const short8 gf = ra_tr_frag(gimg, pb * 32, db, lane), qf = ra_tr_frag(qimg, pb * 32, db, lane);
-#pragma unroll
-        for (int i = 0; i < QB; ++i) {
-          dv_[i][db] = Half16<T>::mfma(gf, pf[i], dv_[i][db]);
-          dk_[i][db] = Half16<T>::mfma(qf, sf[i], dk_[i][db]);
-        }
-      }
+      cur = nx;
     }
-    };
-    if (left < RA_CHUNK || !all_keys) chunk(std::true_type{}, std::false_type{});
-    else if (side) chunk(std::false_type{}, std::true_type{});
-    else chunk(std::true_type{}, std::true_type{});
-  }
+    return cur;
+  };
+  sweep(std::false_type{}, sweep(std::true_type{}, cur));
   T* dkb = ra_base<T>(p.dk, s, packed);
   T* dvb = ra_base<T>(p.dv, s, packed);
 #pragma unroll
@@ -949,13 +1036,7 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(KS <= 2 
 #pragma unroll
     for (int kb = 0; kb < W; ++kb) {
       const float4v t = ds[kb];
-      float n = t[0];
-      n += dpp_f<0x101>(t[1]);
-      n += dpp_f<0x102>(t[2]);
-      n += dpp_f<0x103>(t[3]);
-      float w = dpp_f<0x11F>(t[1]);
-      w += dpp_f<0x11E>(t[2]);
-      w += dpp_f<0x11D>(t[3]);
+      const float n = ra_diag_n(t), w = ra_diag_w(t);
       d[16 * kb] = n + carry;
       carry = w;
     }
@@ -1057,12 +1138,12 @@ static int ra_dispatch(int which, const PdtRelAttn& p, hipStream_t st) {
   const int rows = RA_WAVES * 16 * (two ? 2 : 1);
   const size_t imgs = (size_t)4 * NH * RA_IMG, tab = ra_bias_bytes(p);
   if (which == 0)
-    return two ? ra_launch(rel_attn_fwd_kernel<T, KS, 2, DROP>, p, rows, imgs + tab, st)
-               : ra_launch(rel_attn_fwd_kernel<T, KS, 1, DROP>, p, rows, imgs + tab, st);
+    return two ? ra_launch(rel_attn_fwd_kernel<T, KS, 2, DROP>, p, rows, imgs + 512 + tab, st)
+               : ra_launch(rel_attn_fwd_kernel<T, KS, 1, DROP>, p, rows, imgs + 512 + tab, st);
   if (which == 1) {
-    const size_t diag = p.dtable_part ? (size_t)4 * RA_WAVES * ra_diag_len(p.max_distance) * sizeof(float) : 0;
-    return two ? ra_launch(rel_attn_dq_kernel<T, KS, QB2, DROP>, p, rows, imgs + tab + diag, st)
-               : ra_launch(rel_attn_dq_kernel<T, KS, 1, DROP>, p, rows, imgs + tab + diag, st);
+    const size_t diag = p.dtable_part ? (size_t)2 * RA_WAVES * ra_diag_len(p.max_distance) * sizeof(float) : 0;
+    return two ? ra_launch(rel_attn_dq_kernel<T, KS, QB2, DROP>, p, rows, imgs + 512 + tab + diag, st)
+               : ra_launch(rel_attn_dq_kernel<T, KS, 1, DROP>, p, rows, imgs + 512 + tab + diag, st);
   }
   return two ? ra_launch(rel_attn_dkv_kernel<T, KS, QB2, DROP>, p, rows, imgs + 2048 + tab, st)
              : ra_launch(rel_attn_dkv_kernel<T, KS, 1, DROP>, p, rows, imgs + 2048 + tab, st);
