@@ -180,6 +180,9 @@ typedef struct PdtRelView {  // element (b, i, h, c) at p[b * batch + i * row + 
 } PdtRelView;
 typedef struct PdtRelAttn {
   PdtRelView q, k, v, o;        // 16-byte aligned, strides multiples of 8 elements
+  PdtRelView o_lo;              // null, or what rounding took from o, as a second 16-bit tensor: written by the forward, read by
+                                // the backward of sequences longer than 128 (pdt_rel_attn_uses_low), whose rowsum(dO * O) - and
+                                // with it every gradient - would otherwise carry the rounding of o
   PdtRelView dout, dq, dk, dv;  // backward
   float* lse;                   // fp32 [B, A, S], log2 domain (forward: null = not wanted)
   float* delta;                 // fp32 [B, A, S] scratch of the backward
@@ -187,7 +190,7 @@ typedef struct PdtRelAttn {
   float* dtable_part;           // null, or fp32 [pdt_rel_attn_dtable_rows()][buckets][A]: partial sums of the table gradient
                                 // (finish with pdt_colsum_finish(part, rows, buckets * A, 1, ...))
   int table_f32, buckets, max_distance;
-  int steps[33];
+  int steps[40];                // entries behind the last: INT_MAX
   const uint64_t* mask_bits;    // null, or one bit per key [B][mask_words], mask_words = ceil(S / 64) (pdt_rel_attn_mask)
   int mask_words;
   const int32_t* cu;            // null, or first rows of the samples in packed [T, ...] tensors, int32 [B + 1]; rows from
@@ -200,6 +203,7 @@ typedef struct PdtRelAttn {
 // key mask [B, S] (`bytes` = 1 or 4 per key, `stride` keys from sample to sample; non-zero = attended) -> bits
 int pdt_rel_attn_mask(const void* mask, int bytes, int64_t stride, int B, int S, uint64_t* bits, void* stream);
 int pdt_rel_attn_fwd(int dtype, const PdtRelAttn* a, void* stream);
+int pdt_rel_attn_uses_low(int S);
 int pdt_rel_attn_dtable_rows(const PdtRelAttn* a);
 int pdt_rel_attn_bwd(int dtype, const PdtRelAttn* a, void* stream);
 

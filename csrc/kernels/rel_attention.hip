@@ -158,36 +158,20 @@ __device__ __forceinline__ uint64_t ra_word(const PdtRelAttn& p, const RaSpan& s
   if (p.mask_bits) w &= ((const __attribute__((address_space(4))) uint64_t*)p.mask_bits)[(int64_t)s.b * p.mask_words + c];
   return w;
 }
-// The chunks of a sweep in the order in which a workgroup takes them: first the whole chunks beyond the near distances
-// (`far`: every row of the chunk attended, one bias), then the others that hold any row at all.  Two loops, each with one
-// form of the score arithmetic: three forms in one loop cost 45 to 85 registers more and a wave of occupancy.
+// The chunks of a sweep that hold an attended row, in ascending order.  A whole chunk beyond the near distances (every row
+// attended, one bias) is `far`: runs of far and of other chunks take turns in two loops, each with one form of the score
+// arithmetic.  The forms as branches of one loop cost 45 to 85 registers more, and a wave of occupancy with them.
 struct RaChunks {
   int c, nc, lo, hi;  // current chunk; far chunks lie at or below lo or at or above hi
-  int far, left;      // in the first loop; a far chunk was left to the second
   int buf;            // the LDS buffer it is staged in
   uint64_t w;         // its attended rows
   template <typename WordFn>
   __device__ __forceinline__ void next(WordFn word) {
-    if (far) {
-      for (++c; c < nc; ++c) {
-        if (c > lo && c < hi) {
-          c = hi;
-          if (c >= nc) break;
-        }
-        w = word(c);
-        if (w == ~0ull) return;
-        left |= w != 0;
-      }
-      far = 0;
-      c = left ? -1 : lo;
-      if (!left) nc = min(nc, hi);
-    }
-    for (++c; c < nc; ++c) {
-      w = word(c);
-      if (w != 0 && !(w == ~0ull && (c <= lo || c >= hi))) return;
-    }
+    for (++c; c < nc; ++c)
+      if ((w = word(c)) != 0) break;
   }
   __device__ __forceinline__ bool done() const { return c >= nc; }
+  __device__ __forceinline__ bool far() const { return w == ~0ull && (c <= lo || c >= hi); }
 };
 // `rows` rows from w0 on against chunks of 64: a chunk is far when all its tiles lie at least `far` beyond all rows
 __device__ __forceinline__ RaChunks ra_chunks(int n, int w0, int rows, int far, bool has_bias, bool any_far) {
@@ -198,10 +182,8 @@ __device__ __forceinline__ RaChunks ra_chunks(int n, int w0, int rows, int far, 
   k.hi = (w0 + rows + far + RA_CHUNK - 1) / RA_CHUNK;
   if (!has_bias) k.lo = k.nc;
   if (!any_far) { k.lo = -1; k.hi = k.nc; }
-  k.far = 1;
-  k.left = 0;
-  k.buf = 0;
   k.c = -1;
+  k.buf = 0;
   k.w = 0;
   return k;
 }
@@ -223,7 +205,10 @@ __device__ __forceinline__ int ra_bucket(const PdtRelAttn& p, int d) {
   int b = n;
   if (n >= exact) {
     b = exact;
-    for (int j = 1; j < half - exact; ++j) b += n >= p.steps[j] ? 1 : 0;
+    for (int j0 = 1; j0 < half - exact; j0 += 8) {  // (eight at a time: one scalar load; the entries behind the last are INT_MAX)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) b += n >= p.steps[j0 + j] ? 1 : 0;
+    }
   }
   return b + (d > 0 ? half : 0);
 }
@@ -254,15 +239,17 @@ __device__ __forceinline__ float4v ra_bias4(const RaBias& t, int lane_off, int u
 }
 
 // ------------------------------------------------------------------------------------------------ forward
-// One wave = 16 QB query rows; online softmax in the log2 domain.
-template <typename T, int KS, int QB, bool DROP>
+// One wave = 16 QB query rows against all keys, or (SPLIT 2) against half of every chunk; online softmax in the log2 domain.
+template <typename T, int KS, int QB, int SPLIT, bool DROP>
 __global__ __launch_bounds__(RA_THREADS) RA_OCC_FWD void rel_attn_fwd_kernel(PdtRelAttn p) {
   constexpr int NH = (KS + 1) / 2, BUF = 2 * NH * RA_IMG;
   extern __shared__ __attribute__((aligned(16))) char smem[];
   const int tid = threadIdx.x, lane = tid & 63, lm = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const RaSpan s = ra_span(p, blockIdx.x);
-  const int w0 = blockIdx.y * (RA_WAVES * 16 * QB), q0 = w0 + wave * 16 * QB;
+  constexpr int ROWS = RA_WAVES / SPLIT * 16 * QB;
+  const int group = SPLIT == 2 ? wave & 1 : wave, half = SPLIT == 2 ? wave >> 1 : 0;
+  const int w0 = blockIdx.y * ROWS, q0 = w0 + group * 16 * QB;
   if (w0 >= s.n) return;
   const bool packed = p.cu != nullptr;
   const T* qb_ = ra_base<const T>(p.q, s, packed);
@@ -278,21 +265,22 @@ __global__ __launch_bounds__(RA_THREADS) RA_OCC_FWD void rel_attn_fwd_kernel(Pdt
   auto word = [&](int c) { return ra_word(p, s, c); };
   const float k2 = p.scale * LOG2E;
   // (the far form takes the maximum of the raw products: not with a negative scale)
-  RaChunks cur = ra_chunks(s.n, w0, RA_WAVES * 16 * QB, ra_far(p.max_distance), p.table != nullptr, k2 > 0.f);
+  RaChunks cur = ra_chunks(s.n, w0, ROWS, ra_far(p.max_distance), p.table != nullptr, k2 > 0.f);
   cur.next(word);
+  const bool active = q0 < s.n;
+  short8 qf[QB][KS];
+#pragma unroll
+  for (int i = 0; i < QB; ++i)
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks)
+      qf[i][ks] = ra_gfrag<T>(qb_ + (int64_t)(q0 + 16 * i + lm) * p.q.row, ks, p.D, lane, q0 + 16 * i + lm < s.n);
   if (!cur.done()) stage(cur.c, 0, cur.w);
   const RaBias bias = ra_bias_fill<T>(p, mb + 2 * RA_CHUNK, s.h, 1, tid, p.max_distance);
   const int boff = ra_bias_lane(bias, lm, g);
-  const bool active = q0 < s.n;
-  short8 qf[QB][KS];
   uint32_t seed[QB];
 #pragma unroll
-  for (int i = 0; i < QB; ++i) {
-    const int q = q0 + 16 * i + lm;
-#pragma unroll
-    for (int ks = 0; ks < KS; ++ks) qf[i][ks] = ra_gfrag<T>(qb_ + (int64_t)q * p.q.row, ks, p.D, lane, q < s.n);
-    seed[i] = DROP ? attn_row_seed(drop_key(p.rng), drop_sample(p.rng, s.b) * p.A + s.h, q) : 0u;
-  }
+  for (int i = 0; i < QB; ++i)
+    seed[i] = DROP ? attn_row_seed(drop_key(p.rng), drop_sample(p.rng, s.b) * p.A + s.h, q0 + 16 * i + lm) : 0u;
   const uint32_t thr_hi = attn_thr_hi(p.drop_thr), kmul0 = (uint32_t)(4 * g) * ATT_GOLD;
   float m[QB];
   float4v l4[QB], o[QB][2 * KS];
@@ -307,7 +295,7 @@ __global__ __launch_bounds__(RA_THREADS) RA_OCC_FWD void rel_attn_fwd_kernel(Pdt
   const float bias_lo = bias.t[0], bias_hi = bias.t[bias.len - 1];
   auto sweep = [&](auto far_tag, RaChunks cur) {
     constexpr bool FAR = decltype(far_tag)::value;
-    while (!cur.done() && (!FAR || cur.far)) {
+    while (!cur.done() && cur.far() == FAR) {
       const int buf = cur.buf;
       RaChunks nx = cur;
       nx.next(word);
@@ -327,7 +315,8 @@ __global__ __launch_bounds__(RA_THREADS) RA_OCC_FWD void rel_attn_fwd_kernel(Pdt
         const int u0 = cur.c * RA_CHUNK - q0;
         const float flat = cur.c <= cur.lo ? bias_lo : bias_hi;
 #pragma unroll
-        for (int pb = 0; pb < 2; ++pb) {  // 32 keys at a time
+        for (int pi = 0; pi < 2 / SPLIT; ++pi) {  // 32 keys at a time
+          const int pb = SPLIT == 2 ? half : pi;
           float4v sc[QB][2];
 #pragma unroll
           for (int hb = 0; hb < 2; ++hb) {
@@ -392,17 +381,60 @@ __global__ __launch_bounds__(RA_THREADS) RA_OCC_FWD void rel_attn_fwd_kernel(Pdt
     }
     return cur;
   };
-  sweep(std::false_type{}, sweep(std::true_type{}, cur));
+  while (!cur.done()) cur = sweep(std::false_type{}, sweep(std::true_type{}, cur));
+  float l[QB];
+#pragma unroll
+  for (int i = 0; i < QB; ++i) l[i] = (l4[i][0] + l4[i][1]) + (l4[i][2] + l4[i][3]);
+  if (SPLIT == 2) {  // the two waves of a row group join their halves of the keys
+    constexpr int F = QB * (8 * KS + 2);
+    static_assert(2 * F * 64 * (int)sizeof(float) <= 2 * BUF, "the join reuses the images");
+    float* x = reinterpret_cast<float*>(smem) + group * F * 64 + lane;
+    __syncthreads();
+    if (half == 1 && active) {
+#pragma unroll
+      for (int i = 0; i < QB; ++i) {
+        float* y = x + i * (8 * KS + 2) * 64;
+#pragma unroll
+        for (int e = 0; e < 8 * KS; ++e) y[e * 64] = o[i][e >> 2][e & 3];
+        y[8 * KS * 64] = m[i];
+        y[(8 * KS + 1) * 64] = l[i];
+      }
+    }
+    __syncthreads();
+    if (half == 1) return;
+#pragma unroll
+    for (int i = 0; i < QB; ++i) {
+      const float* y = x + i * (8 * KS + 2) * 64;
+      if (!active) break;
+      const float m2 = y[8 * KS * 64], top = fmaxf(m[i], m2), use = top == -INFINITY ? 0.f : top;
+      const float a = __builtin_amdgcn_exp2f(m[i] - use), b = __builtin_amdgcn_exp2f(m2 - use);
+      m[i] = top;
+      l[i] = l[i] * a + y[(8 * KS + 1) * 64] * b;
+#pragma unroll
+      for (int e = 0; e < 8 * KS; ++e) o[i][e >> 2][e & 3] = o[i][e >> 2][e & 3] * a + y[e * 64] * b;
+    }
+  }
   if (!active) return;
   T* ob = ra_base<T>(p.o, s, packed);
 #pragma unroll
   for (int i = 0; i < QB; ++i) {
     const int q = q0 + 16 * i + lm;
-    const float l = ra_quad_sum((l4[i][0] + l4[i][1]) + (l4[i][2] + l4[i][3]));
+    const float total = ra_quad_sum(l[i]);
     // a row without an attended key has no probability mass: a zero output, and lse = +inf makes every p of backward 0
-    // (l is NaN, not 0, when a score was: the output is then NaN as well)
-    if (p.lse && g == 0 && q < s.n) p.lse[((int64_t)s.b * p.A + s.h) * p.S + q] = l == 0.f ? INFINITY : m[i] + __log2f(l);
-    ra_store<T, KS>(ob + (int64_t)q * p.o.row, o[i], l == 0.f ? 0.f : 1.0f / l, g, p.D, q < s.n);
+    // (the sum is NaN, not 0, when a score was: the output is then NaN as well)
+    if (p.lse && g == 0 && q < s.n) p.lse[((int64_t)s.b * p.A + s.h) * p.S + q] = total == 0.f ? INFINITY : m[i] + __log2f(total);
+    const float inv = total == 0.f ? 0.f : 1.0f / total;
+    ra_store<T, KS>(ob + (int64_t)q * p.o.row, o[i], inv, g, p.D, q < s.n);
+    if (p.o_lo.p) {
+#pragma unroll
+      for (int db = 0; db < 2 * KS; ++db)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const float v = o[i][db][r] * inv;
+          o[i][db][r] = v - Half16<T>::to_f(Half16<T>::from_f(v));
+        }
+      ra_store<T, KS>(ra_base<T>(p.o_lo, s, packed) + (int64_t)q * p.o_lo.row, o[i], 1.0f, g, p.D, q < s.n);
+    }
   }
 }
 
@@ -481,15 +513,17 @@ __device__ __forceinline__ void ra_bucket_sums(const PdtRelAttn& p, const float*
 }
 
 // ------------------------------------------------------------------------------------------------ dQ and the table gradient
-// One wave = 16 QB query rows, sweeps the keys; also stores delta = rowsum(dO * O) for the dK / dV kernel.
-template <typename T, int KS, int QB, bool DROP>
+// One wave = 16 QB query rows, sweeps the keys (SPLIT 2: half of every chunk); also stores delta = rowsum(dO * O) for the dK / dV kernel.
+template <typename T, int KS, int QB, int SPLIT, bool DROP>
 __global__ __launch_bounds__(RA_THREADS) RA_OCC_DQ void rel_attn_dq_kernel(PdtRelAttn p) {
   constexpr int NH = (KS + 1) / 2, BUF = 2 * NH * RA_IMG;
   extern __shared__ __attribute__((aligned(16))) char smem[];
   const int tid = threadIdx.x, lane = tid & 63, lm = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const RaSpan s = ra_span(p, blockIdx.x);
-  const int w0 = blockIdx.y * (RA_WAVES * 16 * QB), q0 = w0 + wave * 16 * QB;
+  constexpr int ROWS = RA_WAVES / SPLIT * 16 * QB;
+  const int group = SPLIT == 2 ? wave & 1 : wave, half = SPLIT == 2 ? wave >> 1 : 0;
+  const int w0 = blockIdx.y * ROWS, q0 = w0 + group * 16 * QB;
   float* part = p.dtable_part ? p.dtable_part + ((int64_t)s.b * gridDim.y + blockIdx.y) * p.buckets * p.A + s.h : nullptr;
   if (w0 >= s.n) {
     if (part)
@@ -501,6 +535,7 @@ __global__ __launch_bounds__(RA_THREADS) RA_OCC_DQ void rel_attn_dq_kernel(PdtRe
   const T* kb_ = ra_base<const T>(p.k, s, packed);
   const T* vb_ = ra_base<const T>(p.v, s, packed);
   const T* ob_ = ra_base<const T>(p.o, s, packed);
+  const T* lb_ = ra_base<const T>(p.o_lo, s, packed);
   const T* gb_ = ra_base<const T>(p.dout, s, packed);
   float* const mb = reinterpret_cast<float*>(smem + 2 * BUF);  // 0 / -inf of the 64 keys of each buffer
   auto stage = [&](int c, int buf, uint64_t w) {
@@ -510,12 +545,27 @@ __global__ __launch_bounds__(RA_THREADS) RA_OCC_DQ void rel_attn_dq_kernel(PdtRe
     if (tid < RA_CHUNK) mb[buf * RA_CHUNK + tid] = (w >> tid) & 1 ? 0.f : -INFINITY;
   };
   auto word = [&](int c) { return ra_word(p, s, c); };
-  RaChunks cur = ra_chunks(s.n, w0, RA_WAVES * 16 * QB, ra_far(p.max_distance), p.table != nullptr, true);
+  RaChunks cur = ra_chunks(s.n, w0, ROWS, ra_far(p.max_distance), p.table != nullptr, true);
   cur.next(word);
+  const bool active = q0 < s.n;
+  const int64_t bh = (int64_t)s.b * p.A + s.h;
+  short8 qf[QB][KS], df[QB][KS], of[QB][KS], lf[QB][KS];
+  float nlse[QB], nd[QB];
+#pragma unroll
+  for (int i = 0; i < QB; ++i) {
+    const int q = q0 + 16 * i + lm;
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) {
+      qf[i][ks] = ra_gfrag<T>(qb_ + (int64_t)q * p.q.row, ks, p.D, lane, q < s.n);
+      df[i][ks] = ra_gfrag<T>(gb_ + (int64_t)q * p.dout.row, ks, p.D, lane, q < s.n);
+      of[i][ks] = ra_gfrag<T>(ob_ + (int64_t)q * p.o.row, ks, p.D, lane, q < s.n);
+      lf[i][ks] = ra_gfrag<T>(lb_ + (int64_t)q * p.o_lo.row, ks, p.D, lane, q < s.n && p.o_lo.p);
+    }
+    nlse[i] = q < s.n ? -p.lse[bh * p.S + q] : -INFINITY;  // rows that are not there: p = 0
+  }
   if (!cur.done()) stage(cur.c, 0, cur.w);
   const RaBias bias = ra_bias_fill<T>(p, mb + 2 * RA_CHUNK, s.h, 1, tid, p.max_distance);
   const int boff = ra_bias_lane(bias, lm, g);
-  const bool active = q0 < s.n;
   // diagonal sums, two arrays per wave: entry 0 is distance -(far + 31)
   const int dlen = ra_diag_len(p.max_distance);
   float* const sums = bias.t + 4 * bias.len;
@@ -524,27 +574,20 @@ __global__ __launch_bounds__(RA_THREADS) RA_OCC_DQ void rel_attn_dq_kernel(PdtRe
     for (int i = tid; i < 2 * RA_WAVES * dlen; i += RA_THREADS) sums[i] = 0.f;
   float4v open = splat4(0.f);  // the tile of the last offset, which the next pair of tiles adds to (two blocks per wave)
   int open_u = RaDiag::NONE;
-  float4v far_lo = splat4(0.f), far_hi = splat4(0.f);
-  short8 qf[QB][KS], df[QB][KS];
+  float far_lo = 0.f, far_hi = 0.f;
   uint32_t seed[QB];
-  float nlse[QB], nd[QB];
-  const int64_t bh = (int64_t)s.b * p.A + s.h;
 #pragma unroll
   for (int i = 0; i < QB; ++i) {
     const int q = q0 + 16 * i + lm;
     float d = 0.f;
 #pragma unroll
-    for (int ks = 0; ks < KS; ++ks) {
-      qf[i][ks] = ra_gfrag<T>(qb_ + (int64_t)q * p.q.row, ks, p.D, lane, q < s.n);
-      df[i][ks] = ra_gfrag<T>(gb_ + (int64_t)q * p.dout.row, ks, p.D, lane, q < s.n);
-      const short8 of = ra_gfrag<T>(ob_ + (int64_t)q * p.o.row, ks, p.D, lane, q < s.n);
+    for (int ks = 0; ks < KS; ++ks)
 #pragma unroll
-      for (int j = 0; j < 8; ++j) d += Half16<T>::to_f(df[i][ks][j]) * Half16<T>::to_f(of[j]);
-    }
+      for (int j = 0; j < 8; ++j)
+        d += Half16<T>::to_f(df[i][ks][j]) * (Half16<T>::to_f(of[i][ks][j]) + Half16<T>::to_f(lf[i][ks][j]));
     d = ra_quad_sum(d);
-    if (g == 0 && q < s.n) p.delta[bh * p.S + q] = d;
+    if (half == 0 && g == 0 && q < s.n) p.delta[bh * p.S + q] = d;
     nd[i] = -d;
-    nlse[i] = q < s.n ? -p.lse[bh * p.S + q] : -INFINITY;  // rows that are not there: p = 0
     seed[i] = DROP ? attn_row_seed(drop_key(p.rng), drop_sample(p.rng, s.b) * p.A + s.h, q) : 0u;
   }
   const float k2 = p.scale * LOG2E;
@@ -556,14 +599,14 @@ __global__ __launch_bounds__(RA_THREADS) RA_OCC_DQ void rel_attn_dq_kernel(PdtRe
     for (int db = 0; db < 2 * KS; ++db) dq[i][db] = splat4(0.f);
   __syncthreads();  // the arrays are complete
   const float bias_lo = bias.t[0], bias_hi = bias.t[bias.len - 1];
-  auto near = [&](int u, const float4v& t) {  // (chunks of the second loop hold far tiles as well)
-    if (u >= bias.far + 16) far_hi += t;
-    else if (u <= -(bias.far + 16)) far_lo += t;
+  auto near = [&](int u, const float4v& t) {  // (a chunk that is not far may hold far tiles)
+    if (u >= bias.far + 16) far_hi += (t[0] + t[1]) + (t[2] + t[3]);
+    else if (u <= -(bias.far + 16)) far_lo += (t[0] + t[1]) + (t[2] + t[3]);
     else diag.add(u, t);
   };
   auto sweep = [&](auto far_tag, RaChunks cur) {
     constexpr bool FAR = decltype(far_tag)::value;
-    while (!cur.done() && (!FAR || cur.far)) {
+    while (!cur.done() && cur.far() == FAR) {
       const int buf = cur.buf;
       RaChunks nx = cur;
       nx.next(word);
@@ -583,7 +626,8 @@ __global__ __launch_bounds__(RA_THREADS) RA_OCC_DQ void rel_attn_dq_kernel(PdtRe
         const int u0 = cur.c * RA_CHUNK - q0;
         const bool below = cur.c <= cur.lo;
 #pragma unroll
-        for (int pb = 0; pb < 2; ++pb) {
+        for (int pi = 0; pi < 2 / SPLIT; ++pi) {
+          const int pb = SPLIT == 2 ? half : pi;
           float4v ds[QB][2];
 #pragma unroll
           for (int hb = 0; hb < 2; ++hb) {
@@ -647,8 +691,9 @@ __global__ __launch_bounds__(RA_THREADS) RA_OCC_DQ void rel_attn_dq_kernel(PdtRe
               float4v t = ds[0][0] + ds[0][1];
 #pragma unroll
               for (int i = 1; i < QB; ++i) t += ds[i][0] + ds[i][1];
-              if (below) far_lo += t;
-              else far_hi += t;
+              const float sum = (t[0] + t[1]) + (t[2] + t[3]);
+              if (below) far_lo += sum;
+              else far_hi += sum;
             }
           }
         }
@@ -657,8 +702,23 @@ __global__ __launch_bounds__(RA_THREADS) RA_OCC_DQ void rel_attn_dq_kernel(PdtRe
     }
     return cur;
   };
-  sweep(std::false_type{}, sweep(std::true_type{}, cur));
-  if (active) {
+  while (!cur.done()) cur = sweep(std::false_type{}, sweep(std::true_type{}, cur));
+  if (SPLIT == 2) {  // the two waves of a row group add up their halves of the keys
+    constexpr int F = QB * 8 * KS;
+    static_assert(2 * F * 64 * (int)sizeof(float) <= 2 * BUF, "the join reuses the images");
+    float* x = reinterpret_cast<float*>(smem) + group * F * 64 + lane;
+    __syncthreads();
+    if (half == 1 && active) {
+#pragma unroll
+      for (int e = 0; e < F; ++e) x[e * 64] = dq[e / (8 * KS)][(e / 4) % (2 * KS)][e & 3];
+    }
+    __syncthreads();
+    if (half == 0 && active) {
+#pragma unroll
+      for (int e = 0; e < F; ++e) dq[e / (8 * KS)][(e / 4) % (2 * KS)][e & 3] += x[e * 64];
+    }
+  }
+  if (active && half == 0) {
     T* dqb = ra_base<T>(p.dq, s, packed);
 #pragma unroll
     for (int i = 0; i < QB; ++i) {
@@ -669,8 +729,8 @@ __global__ __launch_bounds__(RA_THREADS) RA_OCC_DQ void rel_attn_dq_kernel(PdtRe
   if (part) {  // the far sums join the ends of their wave's first array; then distances -> buckets
     if (open_u != RaDiag::NONE) near(open_u, open);
     diag.flush();
-    const float lo = wave_sum((far_lo[0] + far_lo[1]) + (far_lo[2] + far_lo[3]));
-    const float hi = wave_sum((far_hi[0] + far_hi[1]) + (far_hi[2] + far_hi[3]));
+    const float lo = wave_sum(far_lo);
+    const float hi = wave_sum(far_hi);
     float* const mine = sums + wave * 2 * dlen;
     if (lane == 0) {
       mine[0] += lo;
@@ -689,15 +749,17 @@ __global__ __launch_bounds__(RA_THREADS) RA_OCC_DQ void rel_attn_dq_kernel(PdtRe
 }
 
 // ------------------------------------------------------------------------------------------------ dK, dV
-// One wave = 16 QB keys, sweeps the queries (Q and dO images); lse, delta and dropout seeds of a chunk's queries in LDS.
-template <typename T, int KS, int QB, bool DROP>
+// One wave = 16 QB keys, sweeps the queries (Q and dO images; SPLIT 2: half of every chunk); lse, delta and dropout seeds of a chunk's queries in LDS.
+template <typename T, int KS, int QB, int SPLIT, bool DROP>
 __global__ __launch_bounds__(RA_THREADS) RA_OCC_DKV void rel_attn_dkv_kernel(PdtRelAttn p) {
   constexpr int NH = (KS + 1) / 2, BUF = 2 * NH * RA_IMG + 1024;  // Q | dO | lse, delta, seeds (64 each), 256 spare bytes
   extern __shared__ __attribute__((aligned(16))) char smem[];
   const int tid = threadIdx.x, lane = tid & 63, lm = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const RaSpan s = ra_span(p, blockIdx.x);
-  const int w0 = blockIdx.y * (RA_WAVES * 16 * QB), k0 = w0 + wave * 16 * QB;
+  constexpr int ROWS = RA_WAVES / SPLIT * 16 * QB;
+  const int group = SPLIT == 2 ? wave & 1 : wave, half = SPLIT == 2 ? wave >> 1 : 0;
+  const int w0 = blockIdx.y * ROWS, k0 = w0 + group * 16 * QB;
   if (w0 >= s.n) return;
   const bool packed = p.cu != nullptr;
   const T* qb_ = ra_base<const T>(p.q, s, packed);
@@ -722,11 +784,8 @@ __global__ __launch_bounds__(RA_THREADS) RA_OCC_DKV void rel_attn_dkv_kernel(Pdt
       reinterpret_cast<uint32_t*>(m + 2 * NH * RA_IMG + 512)[tid] = attn_row_seed(dkey, sbh, c * RA_CHUNK + tid);
   };
   auto word = [&](int c) { return s.n - c * RA_CHUNK >= RA_CHUNK ? ~0ull : (1ull << (s.n - c * RA_CHUNK)) - 1; };  // (queries)
-  RaChunks cur = ra_chunks(s.n, w0, RA_WAVES * 16 * QB, ra_far(p.max_distance), p.table != nullptr, true);
+  RaChunks cur = ra_chunks(s.n, w0, ROWS, ra_far(p.max_distance), p.table != nullptr, true);
   cur.next(word);
-  stage(cur.c, 0);
-  const RaBias bias = ra_bias_fill<T>(p, reinterpret_cast<float*>(smem + 2 * BUF), s.h, -1, tid, p.max_distance);
-  const int boff = ra_bias_lane(bias, lm, g);
   short8 kf[QB][KS], vf[QB][KS];
   float kneg[QB];  // -inf for a key that no query attends to
   uint32_t kmul[QB];
@@ -744,6 +803,9 @@ __global__ __launch_bounds__(RA_THREADS) RA_OCC_DKV void rel_attn_dkv_kernel(Pdt
       vf[i][ks] = ra_gfrag<T>(vb_ + (int64_t)key * p.v.row, ks, p.D, lane, ok);
     }
   }
+  stage(cur.c, 0);
+  const RaBias bias = ra_bias_fill<T>(p, reinterpret_cast<float*>(smem + 2 * BUF), s.h, -1, tid, p.max_distance);
+  const int boff = ra_bias_lane(bias, lm, g);
   const float k2 = p.scale * LOG2E;
   const uint32_t thr_hi = attn_thr_hi(p.drop_thr);
   float4v dk_[QB][2 * KS], dv_[QB][2 * KS];
@@ -755,7 +817,7 @@ __global__ __launch_bounds__(RA_THREADS) RA_OCC_DKV void rel_attn_dkv_kernel(Pdt
   const float bias_lo = bias.t[0], bias_hi = bias.t[bias.len - 1];
   auto sweep = [&](auto far_tag, RaChunks cur) {
     constexpr bool FAR = decltype(far_tag)::value;
-    while (!cur.done() && (!FAR || cur.far)) {
+    while (!cur.done() && cur.far() == FAR) {
       const int buf = cur.buf;
       RaChunks nx = cur;
       nx.next(word);
@@ -778,7 +840,8 @@ __global__ __launch_bounds__(RA_THREADS) RA_OCC_DKV void rel_attn_dkv_kernel(Pdt
         const int u0 = cur.c * RA_CHUNK - k0;  // query - key: the bias array is mirrored
         const float flat = cur.c <= cur.lo ? bias_lo : bias_hi;
 #pragma unroll
-        for (int pb = 0; pb < 2; ++pb) {
+        for (int pi = 0; pi < 2 / SPLIT; ++pi) {
+          const int pb = SPLIT == 2 ? half : pi;
           float4v pp[QB][2], ds[QB][2];
 #pragma unroll
           for (int hb = 0; hb < 2; ++hb) {
@@ -831,7 +894,29 @@ __global__ __launch_bounds__(RA_THREADS) RA_OCC_DKV void rel_attn_dkv_kernel(Pdt
     }
     return cur;
   };
-  sweep(std::false_type{}, sweep(std::true_type{}, cur));
+  while (!cur.done()) cur = sweep(std::false_type{}, sweep(std::true_type{}, cur));
+  if (SPLIT == 2) {  // the two waves of a key group add up their halves of the queries
+    constexpr int F = QB * 8 * KS;
+    static_assert(4 * F * 64 * (int)sizeof(float) <= 2 * BUF, "the join reuses the images");
+    float* x = reinterpret_cast<float*>(smem) + group * 2 * F * 64 + lane;
+    __syncthreads();
+    if (half == 1 && active) {
+#pragma unroll
+      for (int e = 0; e < F; ++e) {
+        x[e * 64] = dk_[e / (8 * KS)][(e / 4) % (2 * KS)][e & 3];
+        x[(F + e) * 64] = dv_[e / (8 * KS)][(e / 4) % (2 * KS)][e & 3];
+      }
+    }
+    __syncthreads();
+    if (half == 1) return;
+    if (active) {
+#pragma unroll
+      for (int e = 0; e < F; ++e) {
+        dk_[e / (8 * KS)][(e / 4) % (2 * KS)][e & 3] += x[e * 64];
+        dv_[e / (8 * KS)][(e / 4) % (2 * KS)][e & 3] += x[(F + e) * 64];
+      }
+    }
+  }
   T* dkb = ra_base<T>(p.dk, s, packed);
   T* dvb = ra_base<T>(p.dv, s, packed);
 #pragma unroll
@@ -1096,14 +1181,12 @@ static int ra_allow_lds(const void* kern, size_t bytes) {
   return 0;
 }
 
-// 16-row blocks per wave.  Two share every row that a wave reads from LDS, which is what bounds long sequences (2 x 4096
-// tokens, 16 heads, dim 64: forward 266 -> 198 us), but halve the number of workgroups and leave waves without rows when a
-// sequence has fewer than 128: used from two workgroups per CU on (4 x 1001 tokens, 8 heads, dim 128, 256 workgroups: forward
-// 47 us with one block, 61 us with two), and not beyond 64 columns in the backward kernels, whose accumulators would not fit
-// the registers of two waves per SIMD.
-static int ra_blocks(const PdtRelAttn& p, bool backward) {
+// Shape of a workgroup.  A wave takes two 16-row blocks, so that both use every row it reads from LDS.  128 rows: four waves
+// with 32 rows each.  64 rows: two pairs of waves, a pair shares 32 rows and splits every chunk; twice the workgroups, and
+// sequences of up to 64 rows keep all waves busy.  128 rows from two workgroups per CU on.
+static int ra_rows(const PdtRelAttn& p) {
   const int64_t len = p.cu ? (p.B ? p.T / p.B : 0) : p.S;  // (packed: the average)
-  return len > 64 && (int64_t)p.B * p.A * ((len + 127) / 128) >= 512 && !(backward && p.D > 64) ? 2 : 1;
+  return len > 64 && (int64_t)p.B * p.A * ((len + 127) / 128) >= 512 ? 128 : 64;
 }
 
 static size_t ra_bias_bytes(const PdtRelAttn& p) { return (size_t)4 * ra_bias_len(p.max_distance) * sizeof(float); }
@@ -1132,21 +1215,23 @@ static int ra_launch_short(const PdtRelAttn& p, hipStream_t st) {
 // which: 0 forward, 1 dQ + table gradient, 2 dK / dV, 3 the whole backward of short sequences
 template <typename T, int KS, bool DROP>
 static int ra_dispatch(int which, const PdtRelAttn& p, hipStream_t st) {
-  constexpr int NH = (KS + 1) / 2, QB2 = KS <= 2 ? 2 : 1;  // (two blocks per wave in the backward kernels)
+  constexpr int NH = (KS + 1) / 2;
   if (which == 3) return ra_short_rows(p) == 64 ? ra_launch_short<T, KS, 4, DROP>(p, st) : ra_launch_short<T, KS, 8, DROP>(p, st);
-  const bool two = ra_blocks(p, which != 0) == 2;
-  const int rows = RA_WAVES * 16 * (two ? 2 : 1);
+  const int rows = ra_rows(p);
   const size_t imgs = (size_t)4 * NH * RA_IMG, tab = ra_bias_bytes(p);
   if (which == 0)
-    return two ? ra_launch(rel_attn_fwd_kernel<T, KS, 2, DROP>, p, rows, imgs + 512 + tab, st)
-               : ra_launch(rel_attn_fwd_kernel<T, KS, 1, DROP>, p, rows, imgs + 512 + tab, st);
+    return rows == 128 ? ra_launch(rel_attn_fwd_kernel<T, KS, 2, 1, DROP>, p, rows, imgs + 512 + tab, st)
+                       : ra_launch(rel_attn_fwd_kernel<T, KS, 2, 2, DROP>, p, rows, imgs + 512 + tab, st);
   if (which == 1) {
     const size_t diag = p.dtable_part ? (size_t)2 * RA_WAVES * ra_diag_len(p.max_distance) * sizeof(float) : 0;
-    return two ? ra_launch(rel_attn_dq_kernel<T, KS, QB2, DROP>, p, rows, imgs + 512 + tab + diag, st)
-               : ra_launch(rel_attn_dq_kernel<T, KS, 1, DROP>, p, rows, imgs + 512 + tab + diag, st);
+    return rows == 128 ? ra_launch(rel_attn_dq_kernel<T, KS, 2, 1, DROP>, p, rows, imgs + 512 + tab + diag, st)
+                       : ra_launch(rel_attn_dq_kernel<T, KS, 2, 2, DROP>, p, rows, imgs + 512 + tab + diag, st);
   }
-  return two ? ra_launch(rel_attn_dkv_kernel<T, KS, QB2, DROP>, p, rows, imgs + 2048 + tab, st)
-             : ra_launch(rel_attn_dkv_kernel<T, KS, 1, DROP>, p, rows, imgs + 2048 + tab, st);
+  // (beyond 64 columns the accumulators of two blocks of dK and dV do not fit the registers: one block per wave)
+  if constexpr (KS > 2) return ra_launch(rel_attn_dkv_kernel<T, KS, 1, 1, DROP>, p, 64, imgs + 2048 + tab, st);
+  else
+    return rows == 128 ? ra_launch(rel_attn_dkv_kernel<T, KS, 2, 1, DROP>, p, rows, imgs + 2048 + tab, st)
+                       : ra_launch(rel_attn_dkv_kernel<T, KS, 2, 2, DROP>, p, rows, imgs + 2048 + tab, st);
 }
 template <typename T>
 static int ra_dispatch_ks(int which, const PdtRelAttn& p, hipStream_t st) {
@@ -1167,7 +1252,7 @@ static int ra_check(int dtype, const PdtRelAttn& p) {
   if (dtype != PDT_F16 && dtype != PDT_BF16) return -1;
   if (p.B < 0 || p.S < 0 || p.A <= 0 || p.D <= 0 || p.D > 128 || p.D % 8) return -3;
   if ((int64_t)p.B * p.A > 0x7FFFFFFF || (p.S + RA_CHUNK - 1) / RA_CHUNK > 65535) return -3;
-  const PdtRelView* views[9] = {&p.q, &p.k, &p.v, &p.o, &p.dout, &p.dq, &p.dk, &p.dv, nullptr};
+  const PdtRelView* views[] = {&p.q, &p.k, &p.v, &p.o, &p.o_lo, &p.dout, &p.dq, &p.dk, &p.dv, nullptr};
   for (int i = 0; views[i]; ++i)  // 16-byte rows, and 64 rows within the 31-bit window of a transfer
     if (views[i]->p && (views[i]->row % 8 || views[i]->head % 8 || views[i]->batch % 8 || views[i]->row < 0 ||
                         views[i]->row > (1 << 23) || (uintptr_t)views[i]->p % 16))
@@ -1210,9 +1295,11 @@ extern "C" int pdt_rel_attn_fwd(int dtype, const PdtRelAttn* a, void* stream) {
   return ra_run(dtype, 0, *a, st);
 }
 
+extern "C" int pdt_rel_attn_uses_low(int S) { return S > 128 ? 1 : 0; }
+
 extern "C" int pdt_rel_attn_dtable_rows(const PdtRelAttn* a) {
   if (ra_short_rows(*a)) return a->B;
-  const int rows = RA_WAVES * 16 * ra_blocks(*a, true);
+  const int rows = ra_rows(*a);
   return a->B * ((a->S + rows - 1) / rows);
 }
 

@@ -7,6 +7,7 @@
 #include <ATen/hip/HIPEvent.h>
 
 #include <algorithm>
+#include <climits>
 #include <cmath>
 #include <cstdlib>
 #include <memory>
@@ -450,6 +451,7 @@ PdtRelAttn rel_args(const Tensor& q, const Tensor& k, const Tensor& v, const Ten
     a.table_f32 = t.scalar_type() == at::kFloat;
     a.buckets = (int)t.size(0);
     a.max_distance = (int)c.max_distance;
+    std::fill(std::begin(a.steps), std::end(a.steps), INT_MAX);
     for (size_t i = 0; i < c.steps.size(); ++i) {
       TORCH_CHECK(c.steps[i] >= (i ? c.steps[i - 1] : half / 2) && c.steps[i] <= c.max_distance, "steps must ascend up to max_distance");
       a.steps[i] = (int)c.steps[i];
@@ -485,7 +487,7 @@ PdtRng rel_rng(const OptTensor& state, double p, int64_t micro, int64_t site, co
   // (the masks derive from (sample, head, query, key): the sequence length plays no part)
   return make_rng(*state, micro, site, sids, 1, B);
 }
-// -> o, lse (lse only when wanted)
+// -> o, lse, o_lo (what a backward pass needs only when wanted; o_lo for long sequences only, see PdtRelAttn)
 std::vector<Tensor> rel_attn_forward(const Tensor& q_in, const Tensor& k_in, const Tensor& v_in, const OptTensor& table,
                                      int64_t max_distance, const std::vector<int64_t>& steps, const OptTensor& bits,
                                      const OptTensor& cu, int64_t max_seqlen, double scale, const OptTensor& rng_state,
@@ -497,18 +499,22 @@ std::vector<Tensor> rel_attn_forward(const Tensor& q_in, const Tensor& k_in, con
   const RelCall c{table, bits, cu, steps, max_distance, max_seqlen, scale, p};
   PdtRelAttn a = rel_args(q, k, v, o, c, PdtRng{});
   a.rng = rel_rng(rng_state, p, micro, site, sids, a.B);
-  if (q.numel() == 0) return {o, want_lse ? at::empty({a.B, a.A, a.S}, q.options().dtype(at::kFloat)) : Tensor()};
-  Tensor lse;
+  if (q.numel() == 0) return {o, want_lse ? at::empty({a.B, a.A, a.S}, q.options().dtype(at::kFloat)) : Tensor(), Tensor()};
+  Tensor lse, low;
   if (want_lse) {
     lse = at::empty({a.B, a.A, a.S}, q.options().dtype(at::kFloat));
     a.lse = lse.data_ptr<float>();
+    if (pdt_rel_attn_uses_low(a.S)) {
+      low = at::empty(q.sizes(), q.options());
+      a.o_lo = rel_view(low);
+    }
   }
   check(pdt_rel_attn_fwd(dt_code(q), &a, cur_stream()), "rel_attn_fwd");
-  return {o, lse};
+  return {o, lse, low};
 }
 // dq, dk, dv into the given tensors; the table gradient (fp32 [buckets, A]) into `dtable` (+= when accumulate)
 void rel_attn_backward_into(const Tensor& dout_in, const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& o,
-                            const Tensor& lse, const RelCall& c, const PdtRng& rng, Tensor dq, Tensor dk, Tensor dv,
+                            const Tensor& low, const Tensor& lse, const RelCall& c, const PdtRng& rng, Tensor dq, Tensor dk, Tensor dv,
                             float* dtable, bool accumulate) {
   PdtRelAttn a = rel_args(q, k, v, o, c, rng);
   const Tensor dout = head_rows(dout_in, "dout");
@@ -516,6 +522,10 @@ void rel_attn_backward_into(const Tensor& dout_in, const Tensor& q, const Tensor
   chkf32(lse, "lse");
   TORCH_CHECK(lse.dim() == 3 && lse.size(0) == a.B && lse.size(1) == a.A && lse.size(2) == a.S, "lse must be [B, heads, S]");
   Tensor delta = at::empty_like(lse), part;
+  if (low.defined()) {
+    TORCH_CHECK(low.sizes() == o.sizes() && low.scalar_type() == o.scalar_type(), "low must have o's shape and dtype");
+    a.o_lo = rel_view(low);
+  }
   a.dout = rel_view(dout); a.dq = rel_view(dq); a.dk = rel_view(dk); a.dv = rel_view(dv);
   a.lse = lse.data_ptr<float>(); a.delta = delta.data_ptr<float>();
   const int rows = pdt_rel_attn_dtable_rows(&a);
@@ -529,7 +539,7 @@ void rel_attn_backward_into(const Tensor& dout_in, const Tensor& q, const Tensor
                             cur_stream()), "colsum_finish");
 }
 std::vector<Tensor> rel_attn_backward(const Tensor& dout, const Tensor& q_in, const Tensor& k_in, const Tensor& v_in, const Tensor& o,
-                                      const Tensor& lse, const OptTensor& table, int64_t max_distance,
+                                      const Tensor& lse, const OptTensor& low, const OptTensor& table, int64_t max_distance,
                                       const std::vector<int64_t>& steps, const OptTensor& bits, const OptTensor& cu,
                                       int64_t max_seqlen, double scale, const OptTensor& rng_state, double p, int64_t micro,
                                       int64_t site, const OptTensor& sids, bool want_dtable) {
@@ -545,7 +555,7 @@ std::vector<Tensor> rel_attn_backward(const Tensor& dout, const Tensor& q_in, co
   }
   if (want_dtable) dtable = at::empty(table->sizes(), q.options().dtype(at::kFloat));
   const RelCall c{table, bits, cu, steps, max_distance, max_seqlen, scale, p};
-  rel_attn_backward_into(dout, q, k, v, o, lse, c, rel_rng(rng_state, p, micro, site, sids, lse.size(0)), dq, dk, dv,
+  rel_attn_backward_into(dout, q, k, v, o, low.has_value() ? *low : Tensor(), lse, c, rel_rng(rng_state, p, micro, site, sids, lse.size(0)), dq, dk, dv,
                          want_dtable ? dtable.data_ptr<float>() : nullptr, false);
   return {dq, dk, dv, dtable};
 }
@@ -562,7 +572,7 @@ struct RelAttnNode : public torch::autograd::Function<RelAttnNode> {
                                              site, sids, wanted);
     if (wanted) {
       auto t = [](const OptTensor& x) { return x.has_value() ? *x : Tensor(); };
-      ctx->save_for_backward({q, k, v, t(table), r[0], r[1], t(bits), t(cu), t(rng_state), t(sids)});
+      ctx->save_for_backward({q, k, v, t(table), r[0], r[1], t(bits), t(cu), t(rng_state), t(sids), r[2]});
       ctx->saved_data["steps"] = steps;
       ctx->saved_data["ints"] = std::vector<int64_t>{max_distance, max_seqlen, micro, site};
       ctx->saved_data["floats"] = std::vector<double>{scale, p};
@@ -574,7 +584,7 @@ struct RelAttnNode : public torch::autograd::Function<RelAttnNode> {
     const auto t = ctx->get_saved_variables();
     const auto ints = ctx->saved_data["ints"].toIntVector();
     const auto floats = ctx->saved_data["floats"].toDoubleVector();
-    std::vector<Tensor> g = rel_attn_backward(dout[0], t[0], t[1], t[2], t[4], t[5], opt(t[3]), ints[0], ctx->saved_data["steps"].toIntVector(),
+    std::vector<Tensor> g = rel_attn_backward(dout[0], t[0], t[1], t[2], t[4], t[5], opt(t[10]), opt(t[3]), ints[0], ctx->saved_data["steps"].toIntVector(),
                                               opt(t[6]), opt(t[7]), ints[1], floats[0], opt(t[8]), floats[1], ints[2], ints[3],
                                               opt(t[9]), t[3].defined() && ctx->needs_input_grad(3));
     torch::autograd::variable_list out(16);
@@ -804,7 +814,7 @@ void position_attention_backward(const LayerPosition& pos, const Tensor& qkv, co
   const RelCall c{pos.table, bits, cu, pos.steps, pos.max_distance, S, 0.125, p};
   const Tensor dqk = turns ? at::empty_like(qk) : dqkv;
   rel_attn_backward_into(head_view(dctx, B, S, A, packed), third(turns ? qk : qkv, 0), third(turns ? qk : qkv, 1), third(qkv, 2),
-                         head_view(ctx, B, S, A, packed), lse, c, rng, third(dqk, 0), third(dqk, 1), third(dqkv, 2), dtable, accumulate);
+                         head_view(ctx, B, S, A, packed), Tensor(), lse, c, rng, third(dqk, 0), third(dqk, 1), third(dqkv, 2), dtable, accumulate);
   if (turns)
     rope_backward_into(third(dqk, 0), third(dqk, 1), third(qkv, 0), third(qkv, 1),
                        RopeCall{pos.wq, pos.wk, pos.cos, pos.sin, positions, false, pos.eps}, third(dqkv, 0), third(dqkv, 1),
