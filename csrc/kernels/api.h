@@ -118,6 +118,8 @@ int pdt_layernorm_bwd_max_blocks(void);
 // partial is [nblk][nseg][H]; out_j[c] (+)= sum_b partial[b][j][c] for each non-null out_j (nseg <= 4)
 int pdt_colsum_finish(const float* partial, int nblk, int H, int nseg, float* o0, float* o1, float* o2, float* o3,
                       int accumulate, void* stream);
+// the same for one or two 16-bit outputs, without accumulation
+int pdt_colsum_finish16(int dtype, const float* partial, int nblk, int H, int nseg, void* o0, void* o1, void* stream);
 // Several finishing jobs in ONE launch (a layer's backward produces four sets of partial sums; with short micro-batches
 // the launches, not the sums, are what they cost).  Job j is pdt_colsum_finish(partial, nblk, H, nseg, out..., accumulate).
 typedef struct PdtColsumJob {

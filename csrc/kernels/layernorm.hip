@@ -159,12 +159,10 @@ struct ColsumOuts { float* out[4]; };
 // Each block owns 32 columns: 32 row groups x 32 columns; a thread sums every 32nd partial row of its column
 // (coalesced 128-B reads across the 32 lanes, 4 independent accumulators to keep loads in flight), then the
 // row groups are combined in a fixed order through LDS.
-__device__ __forceinline__ void colsum_finish_body(const float* __restrict__ partial, int nblk, int H, int nseg,
-                                                   float* const (&out)[4], int accumulate, int block) {
+// sum over the partial rows of column idx, in the threads with threadIdx.x < 32 (a fixed order of additions)
+__device__ __forceinline__ float colsum_finish_sum(const float* __restrict__ partial, int nblk, int total, int idx) {
   __shared__ float red[32][33];
   const int cg = threadIdx.x & 31, rg = threadIdx.x >> 5;
-  const int total = nseg * H;
-  const int idx = block * 32 + cg;
   float s0 = 0.f, s1 = 0.f, s2 = 0.f, s3 = 0.f;
   if (idx < total) {
     int b = rg;
@@ -178,10 +176,18 @@ __device__ __forceinline__ void colsum_finish_body(const float* __restrict__ par
   }
   red[rg][cg] = (s0 + s1) + (s2 + s3);
   __syncthreads();
-  if (rg == 0 && idx < total) {
-    float t = 0.f;
+  float t = 0.f;
+  if (rg == 0) {
 #pragma unroll
     for (int r = 0; r < 32; ++r) t += red[r][cg];
+  }
+  return t;
+}
+__device__ __forceinline__ void colsum_finish_body(const float* __restrict__ partial, int nblk, int H, int nseg,
+                                                   float* const (&out)[4], int accumulate, int block) {
+  const int total = nseg * H, idx = block * 32 + (threadIdx.x & 31);
+  const float t = colsum_finish_sum(partial, nblk, total, idx);
+  if (threadIdx.x < 32 && idx < total) {
     const int seg = idx / H, c = idx % H;
     float* o = seg == 0 ? out[0] : (seg == 1 ? out[1] : (seg == 2 ? out[2] : out[3]));
     if (o) o[c] = accumulate ? o[c] + t : t;
@@ -191,6 +197,15 @@ __device__ __forceinline__ void colsum_finish_body(const float* __restrict__ par
 __global__ __launch_bounds__(1024) void colsum_finish_kernel(const float* __restrict__ partial, int nblk, int H,
                                                              int nseg, ColsumOuts outs, int accumulate) {
   colsum_finish_body(partial, nblk, H, nseg, outs.out, accumulate, blockIdx.x);
+}
+
+// the same into 16-bit outputs (gradients of 16-bit parameters outside the arena)
+template <typename T>
+__global__ __launch_bounds__(1024) void colsum_finish16_kernel(const float* __restrict__ partial, int nblk, int H, int nseg,
+                                                               short* o0, short* o1) {
+  const int total = nseg * H, idx = blockIdx.x * 32 + (threadIdx.x & 31);
+  const float t = colsum_finish_sum(partial, nblk, total, idx);
+  if (threadIdx.x < 32 && idx < total) (idx < H ? o0 : o1)[idx < H ? idx : idx - H] = Half16<T>::from_f(t);
 }
 
 // several jobs in one launch: block -> job through the running block counts (first[j] = first block of job j)
@@ -304,6 +319,16 @@ extern "C" int pdt_colsum_finish(const float* partial, int nblk, int H, int nseg
   const int total = nseg * H;
   hipLaunchKernelGGL(colsum_finish_kernel, dim3((total + 31) / 32), dim3(1024), 0, (hipStream_t)stream, partial, nblk,
                      H, nseg, outs, accumulate);
+  return (int)hipGetLastError();
+}
+
+extern "C" int pdt_colsum_finish16(int dtype, const float* partial, int nblk, int H, int nseg, void* o0, void* o1, void* stream) {
+  if (H <= 0 || nseg < 1 || nseg > 2 || !o0 || (nseg == 2 && !o1) || nblk < 0) return -2;
+  const dim3 grid((nseg * H + 31) / 32);
+  if (dtype == PDT_F16)
+    hipLaunchKernelGGL(colsum_finish16_kernel<_Float16>, grid, dim3(1024), 0, (hipStream_t)stream, partial, nblk, H, nseg, (short*)o0, (short*)o1);
+  else
+    hipLaunchKernelGGL(colsum_finish16_kernel<__bf16>, grid, dim3(1024), 0, (hipStream_t)stream, partial, nblk, H, nseg, (short*)o0, (short*)o1);
   return (int)hipGetLastError();
 }
 

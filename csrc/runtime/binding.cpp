@@ -512,10 +512,23 @@ std::vector<Tensor> rel_attn_forward(const Tensor& q_in, const Tensor& k_in, con
   check(pdt_rel_attn_fwd(dt_code(q), &a, cur_stream()), "rel_attn_fwd");
   return {o, lse, low};
 }
-// dq, dk, dv into the given tensors; the table gradient (fp32 [buckets, A]) into `dtable` (+= when accumulate)
+// Where a call's parameter gradients go: fp32 (possibly added to what is there), or 16-bit
+struct GradOut {
+  void* p = nullptr;
+  bool half = false, accumulate = false;
+};
+GradOut grad_out(const Tensor& t) { return t.defined() ? GradOut{t.data_ptr(), t.scalar_type() != at::kFloat, false} : GradOut{}; }
+void finish_columns(int dtype, const Tensor& part, int rows, int H, int nseg, const GradOut& a, const GradOut& b) {
+  const float* p = rows ? part.data_ptr<float>() : nullptr;
+  if (a.half)
+    check(pdt_colsum_finish16(dtype, p, rows, H, nseg, a.p, b.p, cur_stream()), "colsum_finish16");
+  else
+    check(pdt_colsum_finish(p, rows, H, nseg, (float*)a.p, (float*)b.p, nullptr, nullptr, a.accumulate ? 1 : 0, cur_stream()), "colsum_finish");
+}
+// dq, dk, dv into the given tensors; the table gradient [buckets, A] where `dtable` says
 void rel_attn_backward_into(const Tensor& dout_in, const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& o,
                             const Tensor& low, const Tensor& lse, const RelCall& c, const PdtRng& rng, Tensor dq, Tensor dk, Tensor dv,
-                            float* dtable, bool accumulate) {
+                            const GradOut& dtable) {
   PdtRelAttn a = rel_args(q, k, v, o, c, rng);
   const Tensor dout = head_rows(dout_in, "dout");
   TORCH_CHECK(dout.sizes() == q.sizes() && dout.scalar_type() == q.scalar_type(), "dout must have q's shape and dtype");
@@ -529,14 +542,12 @@ void rel_attn_backward_into(const Tensor& dout_in, const Tensor& q, const Tensor
   a.dout = rel_view(dout); a.dq = rel_view(dq); a.dk = rel_view(dk); a.dv = rel_view(dv);
   a.lse = lse.data_ptr<float>(); a.delta = delta.data_ptr<float>();
   const int rows = pdt_rel_attn_dtable_rows(&a);
-  if (dtable) {
+  if (dtable.p) {
     part = at::empty({rows, (int64_t)a.buckets * a.A}, lse.options());
     a.dtable_part = part.data_ptr<float>();
   }
   check(pdt_rel_attn_bwd(dt_code(q), &a, cur_stream()), "rel_attn_bwd");
-  if (dtable)
-    check(pdt_colsum_finish(a.dtable_part, rows, a.buckets * a.A, 1, dtable, nullptr, nullptr, nullptr, accumulate ? 1 : 0,
-                            cur_stream()), "colsum_finish");
+  if (dtable.p) finish_columns(dt_code(q), part, rows, a.buckets * a.A, 1, dtable, GradOut{});
 }
 std::vector<Tensor> rel_attn_backward(const Tensor& dout, const Tensor& q_in, const Tensor& k_in, const Tensor& v_in, const Tensor& o,
                                       const Tensor& lse, const OptTensor& low, const OptTensor& table, int64_t max_distance,
@@ -550,13 +561,13 @@ std::vector<Tensor> rel_attn_backward(const Tensor& dout, const Tensor& q_in, co
   Tensor dtable;
   want_dtable = want_dtable && table.has_value();
   if (q.numel() == 0) {
-    if (want_dtable) dtable = at::zeros(table->sizes(), q.options().dtype(at::kFloat));
+    if (want_dtable) dtable = at::zeros(table->sizes(), table->options());
     return {dq, dk, dv, dtable};
   }
-  if (want_dtable) dtable = at::empty(table->sizes(), q.options().dtype(at::kFloat));
+  if (want_dtable) dtable = at::empty(table->sizes(), table->options());
   const RelCall c{table, bits, cu, steps, max_distance, max_seqlen, scale, p};
   rel_attn_backward_into(dout, q, k, v, o, low.has_value() ? *low : Tensor(), lse, c, rel_rng(rng_state, p, micro, site, sids, lse.size(0)), dq, dk, dv,
-                         want_dtable ? dtable.data_ptr<float>() : nullptr, false);
+                         grad_out(dtable));
   return {dq, dk, dv, dtable};
 }
 
@@ -588,8 +599,7 @@ struct RelAttnNode : public torch::autograd::Function<RelAttnNode> {
                                               opt(t[6]), opt(t[7]), ints[1], floats[0], opt(t[8]), floats[1], ints[2], ints[3],
                                               opt(t[9]), t[3].defined() && ctx->needs_input_grad(3));
     torch::autograd::variable_list out(16);
-    for (int i = 0; i < 3; ++i) out[i] = g[i];
-    if (g[3].defined()) out[3] = g[3].to(t[3].scalar_type());
+    for (int i = 0; i < 4; ++i) out[i] = g[i];
     return out;
   }
 };
@@ -677,9 +687,9 @@ void rope_forward_into(const Tensor& q, const Tensor& k, const RopeCall& c, Tens
   a.y[0] = rel_view(yq); a.y[1] = rel_view(yk);
   check(pdt_qk_rope_fwd(dt_code(q), &a, cur_stream()), "qk_rope_fwd");
 }
-// dxq, dxk into the given tensors; weight gradients (fp32 [D]) into dwq / dwk (+= when accumulate) unless null
+// dxq, dxk into the given tensors; the weight gradients [D] where dwq / dwk say (both or neither)
 void rope_backward_into(const Tensor& dyq_in, const Tensor& dyk_in, const Tensor& q, const Tensor& k, const RopeCall& c, Tensor dxq,
-                        Tensor dxk, float* dwq, float* dwk, bool accumulate) {
+                        Tensor dxk, const GradOut& dwq, const GradOut& dwk) {
   PdtQkRope a = rope_args(q, k, c);
   const Tensor dyq = head_rows(dyq_in, "dq"), dyk = head_rows(dyk_in, "dk");
   TORCH_CHECK(dyq.sizes() == q.sizes() && dyk.sizes() == k.sizes() && dyq.scalar_type() == q.scalar_type() &&
@@ -688,11 +698,9 @@ void rope_backward_into(const Tensor& dyq_in, const Tensor& dyk_in, const Tensor
   a.dx[0] = rel_view(dxq); a.dx[1] = rel_view(dxk);
   Tensor part;
   const int blocks = pdt_qk_rope_bwd_blocks(&a);
-  if (dwq || dwk) part = at::empty({blocks, 2 * (int64_t)a.D}, q.options().dtype(at::kFloat));
+  if (dwq.p) part = at::empty({blocks, 2 * (int64_t)a.D}, q.options().dtype(at::kFloat));
   check(pdt_qk_rope_bwd(dt_code(q), &a, part.defined() ? part.data_ptr<float>() : nullptr, cur_stream()), "qk_rope_bwd");
-  if (part.defined())
-    check(pdt_colsum_finish(part.data_ptr<float>(), blocks, a.D, 2, dwq, dwk, nullptr, nullptr, accumulate ? 1 : 0, cur_stream()),
-          "colsum_finish");
+  if (part.defined()) finish_columns(dt_code(q), part, blocks, a.D, 2, dwq, dwk);
 }
 std::vector<Tensor> qk_rope_forward(const Tensor& q_in, const Tensor& k_in, const OptTensor& wq, const OptTensor& wk,
                                     const OptTensor& cos, const OptTensor& sin, const OptTensor& pos, bool interleaved, double eps) {
@@ -711,11 +719,11 @@ std::vector<Tensor> qk_rope_backward(const Tensor& dyq, const Tensor& dyk, const
   const Tensor q = head_rows(q_in, "q"), k = head_rows(k_in, "k");
   Tensor dxq = at::empty(q.sizes(), q.options()), dxk = at::empty(k.sizes(), k.options()), dwq, dwk;
   if (want_dw && wq.has_value()) {
-    dwq = at::empty({q.size(-1)}, q.options().dtype(at::kFloat));
-    dwk = at::empty({q.size(-1)}, q.options().dtype(at::kFloat));
+    dwq = at::empty({q.size(-1)}, wq->options());
+    dwk = at::empty({q.size(-1)}, wk->options());
   }
   rope_backward_into(dyq, dyk, q, k, RopeCall{wq, wk, cos, sin, pos, interleaved, eps}, dxq, dxk,
-                     dwq.defined() ? dwq.data_ptr<float>() : nullptr, dwk.defined() ? dwk.data_ptr<float>() : nullptr, false);
+                     grad_out(dwq), grad_out(dwk));
   return {dxq, dxk, dwq, dwk};
 }
 struct QkRopeNode : public torch::autograd::Function<QkRopeNode> {
@@ -739,8 +747,8 @@ struct QkRopeNode : public torch::autograd::Function<QkRopeNode> {
     out[0] = g[0];
     out[1] = g[1];
     if (want_dw) {
-      out[2] = g[2].to(t[2].scalar_type());
-      out[3] = g[3].to(t[3].scalar_type());
+      out[2] = g[2];
+      out[3] = g[3];
     }
     return out;
   }
@@ -810,16 +818,15 @@ void position_attention_backward(const LayerPosition& pos, const Tensor& qkv, co
   const bool turns = pos.turns();
   TORCH_CHECK((int)gr.size() == 12 + (pos.table.has_value() ? 1 : 0) + (pos.wq.has_value() ? 2 : 0), "layer_backward: gradients of the position parameters missing");
   size_t at = 12;
-  float* dtable = pos.table.has_value() ? gr[at++].data_ptr<float>() : nullptr;
+  auto grad = [&](bool there) { return there ? GradOut{gr[at++].data_ptr<float>(), false, accumulate} : GradOut{}; };
+  const GradOut dtable = grad(pos.table.has_value()), dwq = grad(pos.wq.has_value()), dwk = grad(pos.wq.has_value());
   const RelCall c{pos.table, bits, cu, pos.steps, pos.max_distance, S, 0.125, p};
   const Tensor dqk = turns ? at::empty_like(qk) : dqkv;
   rel_attn_backward_into(head_view(dctx, B, S, A, packed), third(turns ? qk : qkv, 0), third(turns ? qk : qkv, 1), third(qkv, 2),
-                         head_view(ctx, B, S, A, packed), Tensor(), lse, c, rng, third(dqk, 0), third(dqk, 1), third(dqkv, 2), dtable, accumulate);
+                         head_view(ctx, B, S, A, packed), Tensor(), lse, c, rng, third(dqk, 0), third(dqk, 1), third(dqkv, 2), dtable);
   if (turns)
     rope_backward_into(third(dqk, 0), third(dqk, 1), third(qkv, 0), third(qkv, 1),
-                       RopeCall{pos.wq, pos.wk, pos.cos, pos.sin, positions, false, pos.eps}, third(dqkv, 0), third(dqkv, 1),
-                       pos.wq.has_value() ? gr[at].data_ptr<float>() : nullptr, pos.wq.has_value() ? gr[at + 1].data_ptr<float>() : nullptr,
-                       accumulate);
+                       RopeCall{pos.wq, pos.wk, pos.cos, pos.sin, positions, false, pos.eps}, third(dqkv, 0), third(dqkv, 1), dwq, dwk);
 }
 struct LayerDims { int B, S, A; double p_attn, p_hidden, eps; int64_t micro, layer; };
 
