@@ -32,7 +32,7 @@ constexpr int RA_CHUNK = 64;                    // rows per LDS image
 constexpr int RA_IMG = RA_CHUNK * 128;          // bytes of a 64-row x 64-column image
 constexpr int RA_MAX_FAR = 512;                 // largest max_distance
 constexpr int RA_MAX_STEPS = 32;                // logarithmic buckets per side
-constexpr float RA_SLACK = 8.0f;
+constexpr float RA_SLACK = 8.0f, RA_SLACK_DROP = 4.0f;  // (with dropout p is divided by the share kept as well)
 // Waves per SIMD that the register allocation of a kernel with QB blocks of KS 32-column steps must allow.  At QB KS = 4:
 // forward and dQ 3 (166 registers; dQ with 2: 83 instead of 75 us at 32 x 512 tokens, 12 heads), dK / dV 2 (with 3 it spills: 86
 // instead of 73 us).
@@ -158,9 +158,12 @@ __device__ __forceinline__ uint64_t ra_word(const PdtRelAttn& p, const RaSpan& s
   if (p.mask_bits) w &= ((const __attribute__((address_space(4))) uint64_t*)p.mask_bits)[(int64_t)s.b * p.mask_words + c];
   return w;
 }
-// The chunks of a sweep that hold an attended row, in ascending order.  A whole chunk beyond the near distances (every row
-// attended, one bias) is `far`: runs of far and of other chunks take turns in two loops, each with one form of the score
-// arithmetic.  The forms as branches of one loop cost 45 to 85 registers more, and a wave of occupancy with them.
+// The chunks of a sweep that hold an attended row, in ascending order.  Whole chunks (every row attended) beyond the near
+// distances have one bias, whole near ones look theirs up, the others mask rows as well: runs of each kind take turns in
+// three loops with one form of the score arithmetic each.  The forms as branches of one loop cost 45 to 85 registers more, and
+// a wave of occupancy with them.
+enum { RA_FARAWAY, RA_NEAR, RA_PARTIAL };
+template <int K> using RaKind = std::integral_constant<int, K>;
 struct RaChunks {
   int c, nc, lo, hi;  // current chunk; far chunks lie at or below lo or at or above hi
   int buf;            // the LDS buffer it is staged in
@@ -171,17 +174,16 @@ struct RaChunks {
       if ((w = word(c)) != 0) break;
   }
   __device__ __forceinline__ bool done() const { return c >= nc; }
-  __device__ __forceinline__ bool far() const { return w == ~0ull && (c <= lo || c >= hi); }
+  __device__ __forceinline__ int kind() const { return w != ~0ull ? RA_PARTIAL : (c <= lo || c >= hi ? RA_FARAWAY : RA_NEAR); }
 };
 // `rows` rows from w0 on against chunks of 64: a chunk is far when all its tiles lie at least `far` beyond all rows
-__device__ __forceinline__ RaChunks ra_chunks(int n, int w0, int rows, int far, bool has_bias, bool any_far) {
+__device__ __forceinline__ RaChunks ra_chunks(int n, int w0, int rows, int far, bool has_bias) {
   RaChunks k;
   k.nc = (n + RA_CHUNK - 1) / RA_CHUNK;
   // 64 c + 48 - w0 <= -(far + 16)   and   64 c - (w0 + rows - 16) >= far + 16
   k.lo = w0 - far >= RA_CHUNK ? (w0 - far) / RA_CHUNK - 1 : -1;
   k.hi = (w0 + rows + far + RA_CHUNK - 1) / RA_CHUNK;
   if (!has_bias) k.lo = k.nc;
-  if (!any_far) { k.lo = -1; k.hi = k.nc; }
   k.c = -1;
   k.buf = 0;
   k.w = 0;
@@ -264,8 +266,7 @@ __global__ __launch_bounds__(RA_THREADS) RA_OCC_FWD void rel_attn_fwd_kernel(Pdt
   };
   auto word = [&](int c) { return ra_word(p, s, c); };
   const float k2 = p.scale * LOG2E;
-  // (the far form takes the maximum of the raw products: not with a negative scale)
-  RaChunks cur = ra_chunks(s.n, w0, ROWS, ra_far(p.max_distance), p.table != nullptr, k2 > 0.f);
+  RaChunks cur = ra_chunks(s.n, w0, ROWS, ra_far(p.max_distance), p.table != nullptr);
   cur.next(word);
   const bool active = q0 < s.n;
   short8 qf[QB][KS];
@@ -282,20 +283,24 @@ __global__ __launch_bounds__(RA_THREADS) RA_OCC_FWD void rel_attn_fwd_kernel(Pdt
   for (int i = 0; i < QB; ++i)
     seed[i] = DROP ? attn_row_seed(drop_key(p.rng), drop_sample(p.rng, s.b) * p.A + s.h, q0 + 16 * i + lm) : 0u;
   const uint32_t thr_hi = attn_thr_hi(p.drop_thr), kmul0 = (uint32_t)(4 * g) * ATT_GOLD;
+  // Running maximum m of a row (log2 domain), and what the products start from: c0 = -m / k2, so that the scores come out of
+  // the matrix unit with the maximum subtracted.  m = -inf: no attended key so far (the products then start from 0).
+  const float inv_k2 = 1.0f / k2;
   float m[QB];
-  float4v l4[QB], o[QB][2 * KS];
+  float4v c0[QB], l4[QB], o[QB][2 * KS];
 #pragma unroll
   for (int i = 0; i < QB; ++i) {
     m[i] = -INFINITY;
-    l4[i] = splat4(0.f);
+    c0[i] = l4[i] = splat4(0.f);
 #pragma unroll
     for (int db = 0; db < 2 * KS; ++db) o[i][db] = splat4(0.f);
   }
   __syncthreads();  // the bias array is complete
   const float bias_lo = bias.t[0], bias_hi = bias.t[bias.len - 1];
-  auto sweep = [&](auto far_tag, RaChunks cur) {
-    constexpr bool FAR = decltype(far_tag)::value;
-    while (!cur.done() && cur.far() == FAR) {
+  auto sweep = [&](auto kind, RaChunks cur) {
+    constexpr int KIND = decltype(kind)::value;
+    constexpr float SLACK = DROP ? RA_SLACK_DROP : RA_SLACK;
+    while (!cur.done() && cur.kind() == KIND) {
       const int buf = cur.buf;
       RaChunks nx = cur;
       nx.next(word);
@@ -321,7 +326,7 @@ __global__ __launch_bounds__(RA_THREADS) RA_OCC_FWD void rel_attn_fwd_kernel(Pdt
 #pragma unroll
           for (int hb = 0; hb < 2; ++hb) {
 #pragma unroll
-            for (int i = 0; i < QB; ++i) sc[i][hb] = splat4(0.f);
+            for (int i = 0; i < QB; ++i) sc[i][hb] = c0[i];
 #pragma unroll
             for (int ks = 0; ks < KS; ++ks) {
               const short8 kf = ra_row_frag(kimg, pb * 32 + hb * 16, ks, lane);
@@ -336,27 +341,30 @@ __global__ __launch_bounds__(RA_THREADS) RA_OCC_FWD void rel_attn_fwd_kernel(Pdt
 #pragma unroll
             for (int hb = 0; hb < 2; ++hb) {
               const int k16 = pb * 32 + hb * 16;
-              if (!FAR)
-                sc[i][hb] = sc[i][hb] * k2 + (ra_bias4(bias, boff, u0 + k16 - 16 * i) +
-                                              *reinterpret_cast<const float4v*>(mb + buf * RA_CHUNK + k16 + 4 * g));
-              const float4v t = sc[i][hb];
+              float4v b = splat4(flat);
+              if (KIND != RA_FARAWAY) b = ra_bias4(bias, boff, u0 + k16 - 16 * i);
+              if (KIND == RA_PARTIAL) b += *reinterpret_cast<const float4v*>(mb + buf * RA_CHUNK + k16 + 4 * g);
+              const float4v t = sc[i][hb] * k2 + b;
               cmax = fmaxf(fmaxf(cmax, t[0]), fmaxf(fmaxf(t[1], t[2]), t[3]));
+              sc[i][hb] = t;
             }
-            if (FAR) cmax = cmax * k2 + flat;
-            // The accumulators are rescaled only when some row's maximum has grown by more than 2^RA_SLACK since its last
-            // rescale: p then stays below 2^RA_SLACK instead of 1, which 16-bit operands and fp32 sums hold as exactly.
-            if (__any(cmax > m[i] + RA_SLACK)) {
-              const float m_new = fmaxf(m[i], ra_quad_max(cmax));
-              const float alpha = __builtin_amdgcn_exp2f(m[i] - (m_new == -INFINITY ? 0.f : m_new));
+            // The accumulators are rescaled only when some row's maximum has grown by more than 2^SLACK since its last
+            // rescale: p then stays below 2^SLACK instead of 1, which 16-bit operands and fp32 sums hold as exactly.
+            if (__any(cmax > (m[i] == -INFINITY ? -INFINITY : SLACK))) {
+              const float used = m[i] == -INFINITY ? 0.f : m[i], m_new = fmaxf(m[i], ra_quad_max(cmax) + used);
+              const float now = m_new == -INFINITY ? 0.f : m_new;
+              const float alpha = __builtin_amdgcn_exp2f(m[i] - now);
               m[i] = m_new;
+              c0[i] = splat4(-now * inv_k2);
+              sc[i][0] += used - now;
+              sc[i][1] += used - now;
               l4[i] *= alpha;
 #pragma unroll
               for (int db = 0; db < 2 * KS; ++db) o[i][db] *= alpha;
             }
-            const float m_use = m[i] == -INFINITY ? 0.f : m[i];  // no attended key so far: exp2(-inf - 0) = 0
 #pragma unroll
             for (int hb = 0; hb < 2; ++hb) {
-              float4v t = FAR ? sc[i][hb] * k2 + (flat - m_use) : sc[i][hb] - m_use;
+              float4v t = sc[i][hb];
 #pragma unroll
               for (int r = 0; r < 4; ++r) t[r] = __builtin_amdgcn_exp2f(t[r]);
               l4[i] += t;
@@ -381,7 +389,7 @@ __global__ __launch_bounds__(RA_THREADS) RA_OCC_FWD void rel_attn_fwd_kernel(Pdt
     }
     return cur;
   };
-  while (!cur.done()) cur = sweep(std::false_type{}, sweep(std::true_type{}, cur));
+  while (!cur.done()) cur = sweep(RaKind<RA_PARTIAL>{}, sweep(RaKind<RA_NEAR>{}, sweep(RaKind<RA_FARAWAY>{}, cur)));
   float l[QB];
 #pragma unroll
   for (int i = 0; i < QB; ++i) l[i] = (l4[i][0] + l4[i][1]) + (l4[i][2] + l4[i][3]);
@@ -545,11 +553,12 @@ __global__ __launch_bounds__(RA_THREADS) RA_OCC_DQ void rel_attn_dq_kernel(PdtRe
     if (tid < RA_CHUNK) mb[buf * RA_CHUNK + tid] = (w >> tid) & 1 ? 0.f : -INFINITY;
   };
   auto word = [&](int c) { return ra_word(p, s, c); };
-  RaChunks cur = ra_chunks(s.n, w0, ROWS, ra_far(p.max_distance), p.table != nullptr, true);
+  RaChunks cur = ra_chunks(s.n, w0, ROWS, ra_far(p.max_distance), p.table != nullptr);
   cur.next(word);
   const bool active = q0 < s.n;
   const int64_t bh = (int64_t)s.b * p.A + s.h;
   short8 qf[QB][KS], df[QB][KS], of[QB][KS], lf[QB][KS];
+  const float k2 = p.scale * LOG2E;
   float nlse[QB], nd[QB];
 #pragma unroll
   for (int i = 0; i < QB; ++i) {
@@ -561,7 +570,8 @@ __global__ __launch_bounds__(RA_THREADS) RA_OCC_DQ void rel_attn_dq_kernel(PdtRe
       of[i][ks] = ra_gfrag<T>(ob_ + (int64_t)q * p.o.row, ks, p.D, lane, q < s.n);
       lf[i][ks] = ra_gfrag<T>(lb_ + (int64_t)q * p.o_lo.row, ks, p.D, lane, q < s.n && p.o_lo.p);
     }
-    nlse[i] = q < s.n ? -p.lse[bh * p.S + q] : -INFINITY;  // rows that are not there: p = 0
+    // what the products start from, so that scores come out with lse subtracted (rows that are not there: p = 0)
+    nlse[i] = (q < s.n ? -p.lse[bh * p.S + q] : -INFINITY) / k2;
   }
   if (!cur.done()) stage(cur.c, 0, cur.w);
   const RaBias bias = ra_bias_fill<T>(p, mb + 2 * RA_CHUNK, s.h, 1, tid, p.max_distance);
@@ -586,11 +596,13 @@ __global__ __launch_bounds__(RA_THREADS) RA_OCC_DQ void rel_attn_dq_kernel(PdtRe
       for (int j = 0; j < 8; ++j)
         d += Half16<T>::to_f(df[i][ks][j]) * (Half16<T>::to_f(of[i][ks][j]) + Half16<T>::to_f(lf[i][ks][j]));
     d = ra_quad_sum(d);
-    if (half == 0 && g == 0 && q < s.n) p.delta[bh * p.S + q] = d;
     nd[i] = -d;
+    if (half == 0 && g == 0 && q < s.n) {  // (for the dK / dV kernel)
+      p.delta[bh * p.S + q] = -d;
+      p.delta[((int64_t)p.B * p.A + bh) * p.S + q] = nlse[i];
+    }
     seed[i] = DROP ? attn_row_seed(drop_key(p.rng), drop_sample(p.rng, s.b) * p.A + s.h, q) : 0u;
   }
-  const float k2 = p.scale * LOG2E;
   const uint32_t thr_hi = attn_thr_hi(p.drop_thr), kmul0 = (uint32_t)(4 * g) * ATT_GOLD;
   float4v dq[QB][2 * KS];
 #pragma unroll
@@ -604,9 +616,9 @@ __global__ __launch_bounds__(RA_THREADS) RA_OCC_DQ void rel_attn_dq_kernel(PdtRe
     else if (u <= -(bias.far + 16)) far_lo += (t[0] + t[1]) + (t[2] + t[3]);
     else diag.add(u, t);
   };
-  auto sweep = [&](auto far_tag, RaChunks cur) {
-    constexpr bool FAR = decltype(far_tag)::value;
-    while (!cur.done() && cur.far() == FAR) {
+  auto sweep = [&](auto kind, RaChunks cur) {
+    constexpr int KIND = decltype(kind)::value;
+    while (!cur.done() && cur.kind() == KIND) {
       const int buf = cur.buf;
       RaChunks nx = cur;
       nx.next(word);
@@ -634,7 +646,7 @@ __global__ __launch_bounds__(RA_THREADS) RA_OCC_DQ void rel_attn_dq_kernel(PdtRe
             const int k16 = pb * 32 + hb * 16;
             float4v sc[QB], dp[QB];
 #pragma unroll
-            for (int i = 0; i < QB; ++i) { sc[i] = splat4(0.f); dp[i] = splat4(0.f); }
+            for (int i = 0; i < QB; ++i) { sc[i] = splat4(nlse[i]); dp[i] = splat4(DROP ? 0.f : nd[i]); }
 #pragma unroll
             for (int ks = 0; ks < KS; ++ks) {
               const short8 kf = ra_row_frag(kimg, k16, ks, lane), vf = ra_row_frag(vimg, k16, ks, lane);
@@ -646,10 +658,10 @@ __global__ __launch_bounds__(RA_THREADS) RA_OCC_DQ void rel_attn_dq_kernel(PdtRe
             }
 #pragma unroll
             for (int i = 0; i < QB; ++i) {
-              float4v add = splat4((below ? bias_lo : bias_hi) + nlse[i]);
-              if (!FAR)
-                add = ra_bias4(bias, boff, u0 + k16 - 16 * i) + *reinterpret_cast<const float4v*>(mb + buf * RA_CHUNK + k16 + 4 * g) + nlse[i];
-              float4v t = sc[i] * k2 + add;
+              float4v b = splat4(below ? bias_lo : bias_hi);
+              if (KIND != RA_FARAWAY) b = ra_bias4(bias, boff, u0 + k16 - 16 * i);
+              if (KIND == RA_PARTIAL) b += *reinterpret_cast<const float4v*>(mb + buf * RA_CHUNK + k16 + 4 * g);
+              float4v t = sc[i] * k2 + b;
 #pragma unroll
               for (int r = 0; r < 4; ++r) t[r] = __builtin_amdgcn_exp2f(t[r]);
               float4v e = dp[i];
@@ -658,7 +670,7 @@ __global__ __launch_bounds__(RA_THREADS) RA_OCC_DQ void rel_attn_dq_kernel(PdtRe
                 for (int r = 0; r < 4; ++r)
                   e[r] *= attn_keep(seed[i], kmul0 + (uint32_t)(cur.c * RA_CHUNK + k16 + r) * ATT_GOLD, thr_hi) ? p.drop_scale : 0.f;
               }
-              ds[i][hb] = t * (e + nd[i]);
+              ds[i][hb] = DROP ? t * (e + nd[i]) : t * e;
             }
           }
           short8 sf[QB];
@@ -671,7 +683,7 @@ __global__ __launch_bounds__(RA_THREADS) RA_OCC_DQ void rel_attn_dq_kernel(PdtRe
             for (int i = 0; i < QB; ++i) dq[i][db] = Half16<T>::mfma(kf, sf[i], dq[i][db]);
           }
           if (part) {
-            if (!FAR) {  // tiles of the same offset u = u0 + 16 (kb - i) first add up
+            if (KIND != RA_FARAWAY) {  // tiles of the same offset u = u0 + 16 (kb - i) first add up
               const int u = u0 + 32 * pb;
               if (QB == 2) {
                 if (open_u == u - 16) {
@@ -702,7 +714,7 @@ __global__ __launch_bounds__(RA_THREADS) RA_OCC_DQ void rel_attn_dq_kernel(PdtRe
     }
     return cur;
   };
-  while (!cur.done()) cur = sweep(std::false_type{}, sweep(std::true_type{}, cur));
+  while (!cur.done()) cur = sweep(RaKind<RA_PARTIAL>{}, sweep(RaKind<RA_NEAR>{}, sweep(RaKind<RA_FARAWAY>{}, cur)));
   if (SPLIT == 2) {  // the two waves of a row group add up their halves of the keys
     constexpr int F = QB * 8 * KS;
     static_assert(2 * F * 64 * (int)sizeof(float) <= 2 * BUF, "the join reuses the images");
@@ -749,7 +761,8 @@ __global__ __launch_bounds__(RA_THREADS) RA_OCC_DQ void rel_attn_dq_kernel(PdtRe
 }
 
 // ------------------------------------------------------------------------------------------------ dK, dV
-// One wave = 16 QB keys, sweeps the queries (Q and dO images; SPLIT 2: half of every chunk); lse, delta and dropout seeds of a chunk's queries in LDS.
+// One wave = 16 QB keys, sweeps the queries (Q and dO images; SPLIT 2: half of every chunk); the start values of the products and the dropout seeds
+// of a chunk's queries in LDS.
 template <typename T, int KS, int QB, int SPLIT, bool DROP>
 __global__ __launch_bounds__(RA_THREADS) RA_OCC_DKV void rel_attn_dkv_kernel(PdtRelAttn p) {
   constexpr int NH = (KS + 1) / 2, BUF = 2 * NH * RA_IMG + 1024;  // Q | dO | lse, delta, seeds (64 each), 256 spare bytes
@@ -775,19 +788,19 @@ __global__ __launch_bounds__(RA_THREADS) RA_OCC_DKV void rel_attn_dkv_kernel(Pdt
     const uint64_t rows = left >= RA_CHUNK ? ~0ull : (1ull << left) - 1;
     ra_stage<T, NH>(m, qb_ + (int64_t)c * RA_CHUNK * p.q.row, (uint32_t)p.q.row, rows, p.D, lane, wave);
     ra_stage<T, NH>(m + NH * RA_IMG, gb_ + (int64_t)c * RA_CHUNK * p.dout.row, (uint32_t)p.dout.row, rows, p.D, lane, wave);
-    // lse (wave 0) and delta (wave 1) of the chunk; waves 2 and 3 read delta again into the spare bytes, so that every
+    // -lse / k2 (wave 0) and -delta (wave 1) of the chunk's queries; waves 2 and 3 read delta again into the spare bytes, so that every
     // wave has the same number of transfers in flight.
-    const float* src = (wave == 0 ? p.lse : p.delta) + bh * p.S + (int64_t)c * RA_CHUNK;
+    const float* src = p.delta + ((wave == 0 ? (int64_t)p.B * p.A : 0) + bh) * p.S + (int64_t)c * RA_CHUNK;
     const int slot = wave == 0 ? 0 : (wave == 1 ? 1 : 3);
     pdt_lds_dma4(pdt_make_rsrc(src, 256u), m + 2 * NH * RA_IMG + slot * 256, lane < left ? lane * 4u : 0x80000000u);
     if (DROP && tid < 64)
       reinterpret_cast<uint32_t*>(m + 2 * NH * RA_IMG + 512)[tid] = attn_row_seed(dkey, sbh, c * RA_CHUNK + tid);
   };
   auto word = [&](int c) { return s.n - c * RA_CHUNK >= RA_CHUNK ? ~0ull : (1ull << (s.n - c * RA_CHUNK)) - 1; };  // (queries)
-  RaChunks cur = ra_chunks(s.n, w0, ROWS, ra_far(p.max_distance), p.table != nullptr, true);
+  RaChunks cur = ra_chunks(s.n, w0, ROWS, ra_far(p.max_distance), p.table != nullptr);
   cur.next(word);
   short8 kf[QB][KS], vf[QB][KS];
-  float kneg[QB];  // -inf for a key that no query attends to
+  bool kok[QB];  // (what a lane computes for a key that no query attends to is dropped at the end)
   uint32_t kmul[QB];
   const uint64_t kw = k0 < s.n ? ra_word(p, s, k0 / RA_CHUNK) >> (k0 % RA_CHUNK) : 0;
   const bool active = (kw & (QB == 2 ? 0xFFFFFFFFull : 0xFFFFull)) != 0;  // (a wave's keys lie in one chunk)
@@ -795,7 +808,7 @@ __global__ __launch_bounds__(RA_THREADS) RA_OCC_DKV void rel_attn_dkv_kernel(Pdt
   for (int i = 0; i < QB; ++i) {
     const int key = k0 + 16 * i + lm;
     const bool ok = (kw >> (16 * i + lm)) & 1;
-    kneg[i] = ok ? 0.f : -INFINITY;
+    kok[i] = ok;
     kmul[i] = (uint32_t)key * ATT_GOLD;
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks) {
@@ -815,9 +828,9 @@ __global__ __launch_bounds__(RA_THREADS) RA_OCC_DKV void rel_attn_dkv_kernel(Pdt
     for (int db = 0; db < 2 * KS; ++db) { dk_[i][db] = splat4(0.f); dv_[i][db] = splat4(0.f); }
   __syncthreads();  // the bias array is complete
   const float bias_lo = bias.t[0], bias_hi = bias.t[bias.len - 1];
-  auto sweep = [&](auto far_tag, RaChunks cur) {
-    constexpr bool FAR = decltype(far_tag)::value;
-    while (!cur.done() && cur.far() == FAR) {
+  auto sweep = [&](auto kind, RaChunks cur) {
+    constexpr int KIND = decltype(kind)::value;
+    while (!cur.done() && cur.kind() == KIND) {
       const int buf = cur.buf;
       RaChunks nx = cur;
       nx.next(word);
@@ -833,8 +846,8 @@ __global__ __launch_bounds__(RA_THREADS) RA_OCC_DKV void rel_attn_dkv_kernel(Pdt
       const char* qimg = smem + buf * BUF;
       const char* gimg = qimg + NH * RA_IMG;
       float* const sc_ = reinterpret_cast<float*>(smem + buf * BUF + 2 * NH * RA_IMG);
-      // queries that are not there: p = 0 (their lse has arrived as 0)
-      if (!FAR && wave == 0 && cur.c * RA_CHUNK + lane >= s.n) sc_[lane] = INFINITY;
+      // queries that are not there: p = 0 (their start value has arrived as 0)
+      if (KIND == RA_PARTIAL && wave == 0 && cur.c * RA_CHUNK + lane >= s.n) sc_[lane] = k2 > 0.f ? -INFINITY : INFINITY;
       __syncthreads();
       if (active) {
         const int u0 = cur.c * RA_CHUNK - k0;  // query - key: the bias array is mirrored
@@ -846,9 +859,12 @@ __global__ __launch_bounds__(RA_THREADS) RA_OCC_DKV void rel_attn_dkv_kernel(Pdt
 #pragma unroll
           for (int hb = 0; hb < 2; ++hb) {
             const int q16 = pb * 32 + hb * 16;
+            const float4v lse = *reinterpret_cast<const float4v*>(sc_ + q16 + 4 * g);
+            const float4v del = *reinterpret_cast<const float4v*>(sc_ + 64 + q16 + 4 * g);
+            const uint4v sd = *reinterpret_cast<const uint4v*>(sc_ + 128 + q16 + 4 * g);
             float4v sc[QB], dp[QB];
 #pragma unroll
-            for (int i = 0; i < QB; ++i) { sc[i] = splat4(0.f); dp[i] = splat4(0.f); }
+            for (int i = 0; i < QB; ++i) { sc[i] = lse; dp[i] = DROP ? splat4(0.f) : del; }
 #pragma unroll
             for (int ks = 0; ks < KS; ++ks) {
               const short8 qf = ra_row_frag(qimg, q16, ks, lane), gf = ra_row_frag(gimg, q16, ks, lane);
@@ -858,12 +874,9 @@ __global__ __launch_bounds__(RA_THREADS) RA_OCC_DKV void rel_attn_dkv_kernel(Pdt
                 dp[i] = Half16<T>::mfma(gf, vf[i][ks], dp[i]);
               }
             }
-            const float4v lse = *reinterpret_cast<const float4v*>(sc_ + q16 + 4 * g);
-            const float4v del = *reinterpret_cast<const float4v*>(sc_ + 64 + q16 + 4 * g);
-            const uint4v sd = *reinterpret_cast<const uint4v*>(sc_ + 128 + q16 + 4 * g);
 #pragma unroll
             for (int i = 0; i < QB; ++i) {
-              float4v t = sc[i] * k2 + ((FAR ? splat4(flat + kneg[i]) : ra_bias4(bias, boff, u0 + q16 - 16 * i) + kneg[i]) - lse);
+              float4v t = sc[i] * k2 + (KIND == RA_FARAWAY ? splat4(flat) : ra_bias4(bias, boff, u0 + q16 - 16 * i));
               float4v e = dp[i], pd;
 #pragma unroll
               for (int r = 0; r < 4; ++r) {
@@ -873,7 +886,7 @@ __global__ __launch_bounds__(RA_THREADS) RA_OCC_DKV void rel_attn_dkv_kernel(Pdt
                 if (DROP) e[r] *= keep;
               }
               pp[i][hb] = pd;
-              ds[i][hb] = t * (e - del);
+              ds[i][hb] = DROP ? t * (e + del) : t * e;
             }
           }
           short8 pf[QB], sf[QB];
@@ -894,7 +907,7 @@ __global__ __launch_bounds__(RA_THREADS) RA_OCC_DKV void rel_attn_dkv_kernel(Pdt
     }
     return cur;
   };
-  while (!cur.done()) cur = sweep(std::false_type{}, sweep(std::true_type{}, cur));
+  while (!cur.done()) cur = sweep(RaKind<RA_PARTIAL>{}, sweep(RaKind<RA_NEAR>{}, sweep(RaKind<RA_FARAWAY>{}, cur)));
   if (SPLIT == 2) {  // the two waves of a key group add up their halves of the queries
     constexpr int F = QB * 8 * KS;
     static_assert(4 * F * 64 * (int)sizeof(float) <= 2 * BUF, "the join reuses the images");
@@ -922,6 +935,10 @@ __global__ __launch_bounds__(RA_THREADS) RA_OCC_DKV void rel_attn_dkv_kernel(Pdt
 #pragma unroll
   for (int i = 0; i < QB; ++i) {
     const int key = k0 + 16 * i + lm;
+    if (!kok[i]) {
+#pragma unroll
+      for (int db = 0; db < 2 * KS; ++db) dk_[i][db] = dv_[i][db] = splat4(0.f);
+    }
     ra_store<T, KS>(dkb + (int64_t)key * p.dk.row, dk_[i], p.scale, g, p.D, key < s.n);
     ra_store<T, KS>(dvb + (int64_t)key * p.dv.row, dv_[i], 1.0f, g, p.D, key < s.n);
   }
@@ -974,11 +991,12 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(KS <= 2 
   stage(gimg, p.dout, rows);
   const int q = 16 * wave + lm;
   const RaBias bias = ra_bias_fill<T, 64 * W>(p, reinterpret_cast<float*>(smem + 4 * IMG), s.h, 1, tid, min(p.max_distance, 128));
-  const float nlse = q < s.n ? -p.lse[((int64_t)s.b * p.A + s.h) * p.S + q] : -INFINITY;  // rows that are not there: p = 0
+  const float k2 = p.scale * LOG2E;
+  // what the products start from, so that scores come out with lse subtracted (rows that are not there: p = 0)
+  const float nlse = (q < s.n ? -p.lse[((int64_t)s.b * p.A + s.h) * p.S + q] : -INFINITY) / k2;
   const int boff = ra_bias_lane(bias, lm, g);
   const uint32_t seed = DROP ? attn_row_seed(drop_key(p.rng), drop_sample(p.rng, s.b) * p.A + s.h, q) : 0u;
   const uint32_t thr_hi = attn_thr_hi(p.drop_thr), kmul0 = (uint32_t)(4 * g) * ATT_GOLD;
-  const float k2 = p.scale * LOG2E;
   asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
   __builtin_amdgcn_s_barrier();
   __builtin_amdgcn_sched_barrier(0);
@@ -1008,13 +1026,13 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(KS <= 2 
         const uint32_t tile = (uint32_t)(keys[kb >> 2] >> ((kb & 3) * 16)) & 0xFFFFu;  // (wave-uniform)
         dp[kb] = pd[hb] = splat4(0.f);
         if (!tile) continue;
-        float4v sc = splat4(0.f), e = splat4(0.f);
+        float4v sc = splat4(nlse), e = splat4(0.f);
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks) {
           sc = Half16<T>::mfma(ra_row_frag(kimg + (kb >> 2) * NH * RA_IMG, (kb & 3) * 16, ks, lane), qf[ks], sc);
           e = Half16<T>::mfma(ra_row_frag(vimg + (kb >> 2) * NH * RA_IMG, (kb & 3) * 16, ks, lane), df[ks], e);
         }
-        float4v t = sc * k2 + (ra_bias4(bias, boff, 16 * (kb - wave)) + nlse);
+        float4v t = sc * k2 + ra_bias4(bias, boff, 16 * (kb - wave));
 #pragma unroll
         for (int r = 0; r < 4; ++r) t[r] = __builtin_amdgcn_exp2f(t[r]);
         // (selected in every tile: a branch between a product and its use has cost the wait in front of that use, see
@@ -1182,11 +1200,17 @@ static int ra_allow_lds(const void* kern, size_t bytes) {
 }
 
 // Shape of a workgroup.  A wave takes two 16-row blocks, so that both use every row it reads from LDS.  128 rows: four waves
-// with 32 rows each.  64 rows: two pairs of waves, a pair shares 32 rows and splits every chunk; twice the workgroups, and
-// sequences of up to 64 rows keep all waves busy.  128 rows from two workgroups per CU on.
-static int ra_rows(const PdtRelAttn& p) {
+// with 32 rows each.  64 rows: two pairs of waves, a pair shares 32 rows and splits every chunk - up to half as slow again per
+// row in long sequences (2 x 4096 tokens, 16 heads: forward 231 against 189 us), but sequences of up to 64 rows keep all waves
+// busy, and small batches reach more CUs (12 heads, 1 x 300 tokens: backward 29.5 against 35.0 us, 1 x 2000: 100 against
+// 119 us).  Compared by rounds over the `slots` workgroups that run at a time.
+enum { RA_FWD, RA_DQ, RA_DKV, RA_SHORT };
+static int ra_rows(const PdtRelAttn& p, int which) {
   const int64_t len = p.cu ? (p.B ? p.T / p.B : 0) : p.S;  // (packed: the average)
-  return len > 64 && (int64_t)p.B * p.A * ((len + 127) / 128) >= 512 ? 128 : 64;
+  if (len <= 64) return 64;
+  const int64_t slots = 256 * (which == RA_DKV || p.D > 64 ? 2 : 3), heads = (int64_t)p.B * p.A;
+  const int64_t full = (heads * ((len + 127) / 128) + slots - 1) / slots, half = (heads * ((len + 63) / 64) + slots - 1) / slots;
+  return half * 4 < full * 5 ? 64 : 128;
 }
 
 static size_t ra_bias_bytes(const PdtRelAttn& p) { return (size_t)4 * ra_bias_len(p.max_distance) * sizeof(float); }
@@ -1212,17 +1236,16 @@ static int ra_launch_short(const PdtRelAttn& p, hipStream_t st) {
   return (int)hipGetLastError();
 }
 
-// which: 0 forward, 1 dQ + table gradient, 2 dK / dV, 3 the whole backward of short sequences
 template <typename T, int KS, bool DROP>
 static int ra_dispatch(int which, const PdtRelAttn& p, hipStream_t st) {
   constexpr int NH = (KS + 1) / 2;
-  if (which == 3) return ra_short_rows(p) == 64 ? ra_launch_short<T, KS, 4, DROP>(p, st) : ra_launch_short<T, KS, 8, DROP>(p, st);
-  const int rows = ra_rows(p);
+  if (which == RA_SHORT) return ra_short_rows(p) == 64 ? ra_launch_short<T, KS, 4, DROP>(p, st) : ra_launch_short<T, KS, 8, DROP>(p, st);
+  const int rows = ra_rows(p, which);
   const size_t imgs = (size_t)4 * NH * RA_IMG, tab = ra_bias_bytes(p);
-  if (which == 0)
+  if (which == RA_FWD)
     return rows == 128 ? ra_launch(rel_attn_fwd_kernel<T, KS, 2, 1, DROP>, p, rows, imgs + 512 + tab, st)
                        : ra_launch(rel_attn_fwd_kernel<T, KS, 2, 2, DROP>, p, rows, imgs + 512 + tab, st);
-  if (which == 1) {
+  if (which == RA_DQ) {
     const size_t diag = p.dtable_part ? (size_t)2 * RA_WAVES * ra_diag_len(p.max_distance) * sizeof(float) : 0;
     return rows == 128 ? ra_launch(rel_attn_dq_kernel<T, KS, 2, 1, DROP>, p, rows, imgs + 512 + tab + diag, st)
                        : ra_launch(rel_attn_dq_kernel<T, KS, 2, 2, DROP>, p, rows, imgs + 512 + tab + diag, st);
@@ -1292,14 +1315,14 @@ extern "C" int pdt_rel_attn_fwd(int dtype, const PdtRelAttn* a, void* stream) {
   hipStream_t st = (hipStream_t)stream;
   if (int e = ra_tail(dtype, a->o, *a, st)) return e;
   if (a->B == 0 || a->S == 0) return 0;
-  return ra_run(dtype, 0, *a, st);
+  return ra_run(dtype, RA_FWD, *a, st);
 }
 
 extern "C" int pdt_rel_attn_uses_low(int S) { return S > 128 ? 1 : 0; }
 
 extern "C" int pdt_rel_attn_dtable_rows(const PdtRelAttn* a) {
   if (ra_short_rows(*a)) return a->B;
-  const int rows = ra_rows(*a);
+  const int rows = ra_rows(*a, RA_DQ);
   return a->B * ((a->S + rows - 1) / rows);
 }
 
@@ -1313,7 +1336,7 @@ extern "C" int pdt_rel_attn_bwd(int dtype, const PdtRelAttn* a, void* stream) {
   for (const PdtRelView* v : outs)
     if (int e = ra_tail(dtype, *v, *a, st)) return e;
   if (a->B == 0 || a->S == 0) return 0;
-  if (ra_short_rows(*a)) return ra_run(dtype, 3, *a, st);
-  if (int e = ra_run(dtype, 1, *a, st)) return e;
-  return ra_run(dtype, 2, *a, st);
+  if (ra_short_rows(*a)) return ra_run(dtype, RA_SHORT, *a, st);
+  if (int e = ra_run(dtype, RA_DQ, *a, st)) return e;
+  return ra_run(dtype, RA_DKV, *a, st);
 }

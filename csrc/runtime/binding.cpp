@@ -457,6 +457,7 @@ PdtRelAttn rel_args(const Tensor& q, const Tensor& k, const Tensor& v, const Ten
       a.steps[i] = (int)c.steps[i];
     }
   }
+  TORCH_CHECK(std::isfinite(c.scale) && c.scale != 0.0, "scale must be finite and not zero");
   a.scale = (float)c.scale;
   a.drop_thr = thr16(c.p);
   a.drop_scale = keep_scale(c.p);
@@ -483,7 +484,7 @@ PdtRng rel_rng(const OptTensor& state, double p, int64_t micro, int64_t site, co
     TORCH_CHECK(p <= 0.0, "dropout needs a generator state");
     return PdtRng{nullptr, 0, 0, nullptr, 1u, 0u, nullptr};
   }
-  TORCH_CHECK(p < 1.0, "the dropout probability must be below 1");
+  TORCH_CHECK(p <= 0.99, "the dropout probability must be at most 0.99");  // (16-bit probabilities divided by the share kept)
   // (the masks derive from (sample, head, query, key): the sequence length plays no part)
   return make_rng(*state, micro, site, sids, 1, B);
 }
@@ -534,7 +535,7 @@ void rel_attn_backward_into(const Tensor& dout_in, const Tensor& q, const Tensor
   TORCH_CHECK(dout.sizes() == q.sizes() && dout.scalar_type() == q.scalar_type(), "dout must have q's shape and dtype");
   chkf32(lse, "lse");
   TORCH_CHECK(lse.dim() == 3 && lse.size(0) == a.B && lse.size(1) == a.A && lse.size(2) == a.S, "lse must be [B, heads, S]");
-  Tensor delta = at::empty_like(lse), part;
+  Tensor delta = at::empty({2, lse.size(0), lse.size(1), lse.size(2)}, lse.options()), part;
   if (low.defined()) {
     TORCH_CHECK(low.sizes() == o.sizes() && low.scalar_type() == o.scalar_type(), "low must have o's shape and dtype");
     a.o_lo = rel_view(low);

@@ -72,7 +72,7 @@ def relative_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, bias: 
     whatever its row holds (infinities and NaN included) and gets zero gradients.  A query without any attended key has a
     zero output and no gradient.  An additive float mask is refused.
 
-    ``dropout_p`` with ``rng`` (an :class:`~.fused.RngKey`) and ``site``: dropout on the probabilities with the framework's
+    ``dropout_p`` (at most 0.99) with ``rng`` (an :class:`~.fused.RngKey`) and ``site``: dropout on the probabilities with the framework's
     counter-based masks.
 
     Returns a contiguous tensor of q's shape and dtype.  Probabilities and their gradients are rounded to q's dtype as
@@ -102,10 +102,14 @@ def relative_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, bias: 
             bias = bias.contiguous()
     else:
         max_distance = 0
+    if not 0.0 <= dropout_p <= 0.99:
+        raise ValueError(f"dropout_p must be from 0 to 0.99 (got {dropout_p})")
     if dropout_p > 0.0 and rng is None:
         raise ValueError("dropout needs rng, the key of the forward pass")
     if scale is None:
         scale = 1.0 / math.sqrt(q.shape[-1])
+    if not math.isfinite(scale) or scale == 0.0:
+        raise ValueError("scale must be finite and not zero")
     state, micro, sids = (rng.state, rng.counter, rng.sample_ids) if dropout_p > 0.0 else (None, 0, None)
     return native().relative_attention(q, k, v, bias, max_distance, steps, key_mask, cu_seqlens, int(max_seqlen or 0), scale, state,
                                        dropout_p, micro, site, sids)

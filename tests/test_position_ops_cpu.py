@@ -56,6 +56,10 @@ def _qkv(*shape, dtype=torch.float16):
     (dict(bias=torch.zeros(32)), (1, 4, 2, 64), "buckets, heads"),
     (dict(bias=torch.zeros(32, 2), max_distance=600), (1, 4, 2, 64), "max_distance"),
     (dict(dropout_p=0.1), (1, 4, 2, 64), "rng"),
+    (dict(dropout_p=-0.1), (1, 4, 2, 64), "dropout_p"),
+    (dict(dropout_p=0.995), (1, 4, 2, 64), "dropout_p"),
+    (dict(scale=0.0), (1, 4, 2, 64), "scale"),
+    (dict(scale=math.inf), (1, 4, 2, 64), "scale"),
 ])
 def test_relative_attention_refusals(kwargs, shape, what):
     with pytest.raises(ValueError, match=what):
