@@ -195,8 +195,11 @@ typedef struct PdtRelAttn {
   int steps[40];                // entries behind the last: INT_MAX
   const uint64_t* mask_bits;    // null, or one bit per key [B][mask_words], mask_words = ceil(S / 64) (pdt_rel_attn_mask)
   int mask_words;
+  const void* mask;             // instead of mask_bits: the mask itself, `mask_bytes` (1 or 4) per key, `mask_stride` keys from
+  int mask_bytes;               // sample to sample (a load per 64 keys and workgroup: for short sequences, where packing it
+  int64_t mask_stride;          // first would cost a launch)
   const int32_t* cu;            // null, or first rows of the samples in packed [T, ...] tensors, int32 [B + 1]; rows from
-                                // cu[B] on become zero.  S is then the longest sample.
+                                // cu[B] on become zero (B >= 1; without samples nothing is written).  S is then the longest sample.
   int B, S, A, D, T;
   float scale, drop_scale;
   uint32_t drop_thr;

@@ -150,11 +150,29 @@ template <typename T>
 __device__ __forceinline__ T* ra_base(const PdtRelView& v, const RaSpan& s, bool packed) {
   return (T*)v.p + (packed ? s.row0 * v.row : (int64_t)s.b * v.batch) + (int64_t)s.h * v.head;
 }
+// Rows from cu[B] on of a packed output belong to no sample and become zero: the workgroups of the last sample share them.
+template <typename T>
+__device__ __forceinline__ void ra_tail(const PdtRelAttn& p, const RaSpan& s, const PdtRelView& v, int tid, int threads) {
+  if (!p.cu || s.b != p.B - 1) return;
+  const int first = min(max(uniform_load_i32(p.cu, p.B), 0), p.T), per = p.D >> 3;
+  const int64_t n = (int64_t)(p.T - first) * per;
+  for (int64_t i = (int64_t)blockIdx.y * threads + tid; i < n; i += (int64_t)gridDim.y * threads) {
+    const int r = (int)(i / per), c = (int)(i - (int64_t)r * per);
+    *reinterpret_cast<int4v*>((T*)v.p + (int64_t)(first + r) * v.row + (int64_t)s.h * v.head + c * 8) = int4v{0, 0, 0, 0};
+  }
+}
 // attended keys of chunk c, one bit each
 __device__ __forceinline__ uint64_t ra_word(const PdtRelAttn& p, const RaSpan& s, int c) {
   const int left = s.n - c * RA_CHUNK;
   if (left <= 0) return 0;
   uint64_t w = left >= RA_CHUNK ? ~0ull : (1ull << left) - 1;
+  if (p.mask) {  // (the whole wave comes here together)
+    const int k = c * RA_CHUNK + (threadIdx.x & 63);
+    const int64_t at = (int64_t)s.b * p.mask_stride + k;
+    bool on = false;
+    if (k < s.n) on = p.mask_bytes == 1 ? ((const uint8_t*)p.mask)[at] != 0 : ((const int32_t*)p.mask)[at] != 0;
+    w &= __ballot(on);
+  }
   if (p.mask_bits) w &= ((const __attribute__((address_space(4))) uint64_t*)p.mask_bits)[(int64_t)s.b * p.mask_words + c];
   return w;
 }
@@ -252,6 +270,7 @@ __global__ __launch_bounds__(RA_THREADS) RA_OCC_FWD void rel_attn_fwd_kernel(Pdt
   constexpr int ROWS = RA_WAVES / SPLIT * 16 * QB;
   const int group = SPLIT == 2 ? wave & 1 : wave, half = SPLIT == 2 ? wave >> 1 : 0;
   const int w0 = blockIdx.y * ROWS, q0 = w0 + group * 16 * QB;
+  ra_tail<T>(p, s, p.o, tid, RA_THREADS);
   if (w0 >= s.n) return;
   const bool packed = p.cu != nullptr;
   const T* qb_ = ra_base<const T>(p.q, s, packed);
@@ -533,6 +552,7 @@ __global__ __launch_bounds__(RA_THREADS) RA_OCC_DQ void rel_attn_dq_kernel(PdtRe
   const int group = SPLIT == 2 ? wave & 1 : wave, half = SPLIT == 2 ? wave >> 1 : 0;
   const int w0 = blockIdx.y * ROWS, q0 = w0 + group * 16 * QB;
   float* part = p.dtable_part ? p.dtable_part + ((int64_t)s.b * gridDim.y + blockIdx.y) * p.buckets * p.A + s.h : nullptr;
+  ra_tail<T>(p, s, p.dq, tid, RA_THREADS);
   if (w0 >= s.n) {
     if (part)
       for (int i = tid; i < p.buckets; i += RA_THREADS) part[(int64_t)i * p.A] = 0.f;
@@ -773,6 +793,8 @@ __global__ __launch_bounds__(RA_THREADS) RA_OCC_DKV void rel_attn_dkv_kernel(Pdt
   constexpr int ROWS = RA_WAVES / SPLIT * 16 * QB;
   const int group = SPLIT == 2 ? wave & 1 : wave, half = SPLIT == 2 ? wave >> 1 : 0;
   const int w0 = blockIdx.y * ROWS, k0 = w0 + group * 16 * QB;
+  ra_tail<T>(p, s, p.dk, tid, RA_THREADS);
+  ra_tail<T>(p, s, p.dv, tid, RA_THREADS);
   if (w0 >= s.n) return;
   const bool packed = p.cu != nullptr;
   const T* qb_ = ra_base<const T>(p.q, s, packed);
@@ -967,6 +989,9 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(KS <= 2 
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const RaSpan s = ra_span(p, blockIdx.x);
   float* part = p.dtable_part ? p.dtable_part + (int64_t)s.b * p.buckets * p.A + s.h : nullptr;
+  ra_tail<T>(p, s, p.dq, tid, 64 * W);
+  ra_tail<T>(p, s, p.dk, tid, 64 * W);
+  ra_tail<T>(p, s, p.dv, tid, 64 * W);
   if (s.n == 0) {
     if (part)
       for (int i = tid; i < p.buckets; i += 64 * W) part[(int64_t)i * p.A] = 0.f;
@@ -1172,17 +1197,6 @@ __global__ __launch_bounds__(256) void rel_attn_mask_kernel(const void* mask, in
   if (lane == 0) bits[i] = w;
 }
 
-// rows [cu[B], T) of a packed output: no sample owns them, they are zero
-template <typename T>
-__global__ __launch_bounds__(256) void rel_attn_tail_kernel(PdtRelView v, const int32_t* cu, int B, int T_, int A, int D) {
-  const int first = min(max(cu[B], 0), T_), per = A * (D >> 3);
-  const int64_t n = (int64_t)(T_ - first) * per;
-  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
-    const int r = (int)(i / per), rest = (int)(i - (int64_t)r * per), h = rest / (D >> 3), c = rest - h * (D >> 3);
-    *reinterpret_cast<int4v*>((T*)v.p + (int64_t)(first + r) * v.row + (int64_t)h * v.head + c * 8) = int4v{0, 0, 0, 0};
-  }
-}
-
 // more dynamic LDS than 64 KiB needs the attribute; set once per kernel and device (not a stream operation: done at the
 // first launch, i.e. in the warm-up of a step that is captured later)
 static int ra_allow_lds(const void* kern, size_t bytes) {
@@ -1281,18 +1295,12 @@ static int ra_check(int dtype, const PdtRelAttn& p) {
                         views[i]->row > (1 << 23) || (uintptr_t)views[i]->p % 16))
       return -4;
   if (!p.q.p || !p.k.p || !p.v.p || !p.o.p) return -2;
+  if (p.mask && ((p.mask_bytes != 1 && p.mask_bytes != 4) || p.mask_bits)) return -2;
   if (p.table && (p.buckets < 4 || p.buckets % 2 || p.buckets > 4 * RA_MAX_STEPS || p.max_distance <= p.buckets / 4 ||
                   p.max_distance > RA_MAX_FAR))
     return -5;
   if (!p.table && p.max_distance != 0) return -5;
   return 0;
-}
-
-static int ra_tail(int dtype, const PdtRelView& v, const PdtRelAttn& p, hipStream_t st) {
-  if (!p.cu) return 0;
-  if (dtype == PDT_F16) hipLaunchKernelGGL(rel_attn_tail_kernel<_Float16>, dim3(64), dim3(256), 0, st, v, p.cu, p.B, p.T, p.A, p.D);
-  else hipLaunchKernelGGL(rel_attn_tail_kernel<__bf16>, dim3(64), dim3(256), 0, st, v, p.cu, p.B, p.T, p.A, p.D);
-  return (int)hipGetLastError();
 }
 
 }  // namespace pdt
@@ -1313,7 +1321,6 @@ extern "C" int pdt_rel_attn_mask(const void* mask, int bytes, int64_t stride, in
 extern "C" int pdt_rel_attn_fwd(int dtype, const PdtRelAttn* a, void* stream) {
   if (int e = ra_check(dtype, *a)) return e;
   hipStream_t st = (hipStream_t)stream;
-  if (int e = ra_tail(dtype, a->o, *a, st)) return e;
   if (a->B == 0 || a->S == 0) return 0;
   return ra_run(dtype, RA_FWD, *a, st);
 }
@@ -1332,9 +1339,6 @@ extern "C" int pdt_rel_attn_bwd(int dtype, const PdtRelAttn* a, void* stream) {
   if (a->B > 0 && a->S > 0 && (!a->lse || !a->delta)) return -2;
   if (a->dtable_part && !a->table) return -2;
   hipStream_t st = (hipStream_t)stream;
-  const PdtRelView* outs[3] = {&a->dq, &a->dk, &a->dv};
-  for (const PdtRelView* v : outs)
-    if (int e = ra_tail(dtype, *v, *a, st)) return e;
   if (a->B == 0 || a->S == 0) return 0;
   if (ra_short_rows(*a)) return ra_run(dtype, RA_SHORT, *a, st);
   if (int e = ra_run(dtype, RA_DQ, *a, st)) return e;

@@ -400,7 +400,7 @@ void same_gpu(const Tensor& t, const Tensor& as, const char* name) {
   TORCH_CHECK(t.device() == as.device(), name, " must be on the device of q");
 }
 
-// What the three kernels of one call share.  q, k, v come from head_rows().
+// What the three kernels of one call share.  q, k, v come from head_rows().  `bits`: int64 mask bits, or the mask itself.
 struct RelCall {
   const OptTensor &table, &bits, &cu;
   const std::vector<int64_t>& steps;
@@ -430,7 +430,14 @@ PdtRelAttn rel_args(const Tensor& q, const Tensor& k, const Tensor& v, const Ten
     a.T = (int)q.size(0);
   } else {
     a.B = (int)q.size(0); a.S = (int)q.size(1);
-    if (c.bits.has_value()) {
+    if (c.bits.has_value() && c.bits->scalar_type() != at::kLong) {  // (a mask as key_mask_tensor() leaves it)
+      const Tensor& m = *c.bits;
+      TORCH_CHECK(m.dim() == 2 && m.size(0) == a.B && m.size(1) == a.S && (a.S <= 1 || m.stride(1) == 1), "key_mask must be [B, S]");
+      same_gpu(m, q, "key_mask");
+      a.mask = m.data_ptr();
+      a.mask_bytes = m.scalar_type() == at::kInt ? 4 : 1;
+      a.mask_stride = a.B <= 1 ? 0 : m.stride(0);
+    } else if (c.bits.has_value()) {
       TORCH_CHECK(c.bits->scalar_type() == at::kLong && c.bits->is_contiguous() && c.bits->dim() == 2 &&
                   c.bits->size(0) == a.B && c.bits->size(1) == (a.S + 63) / 64, "mask bits must be int64 [B, ceil(S / 64)]");
       same_gpu(*c.bits, q, "mask bits");
@@ -464,18 +471,22 @@ PdtRelAttn rel_args(const Tensor& q, const Tensor& k, const Tensor& v, const Ten
   a.rng = rng;
   return a;
 }
-// key mask [B, S] (bool, uint8 or int32; non-zero = attended) -> one bit per key, int64 [B, ceil(S / 64)]
-Tensor rel_mask_bits(const Tensor& mask) {
+// key mask [B, S] (bool, uint8 or int32; non-zero = attended) with neighbouring keys
+Tensor key_mask_tensor(const Tensor& mask) {
   TORCH_CHECK(mask.is_cuda() && mask.dim() == 2, "the key mask must be a [B, S] GPU tensor");
-  DeviceGuard guard(mask.device());
   const auto st = mask.scalar_type();
   TORCH_CHECK(st == at::kBool || st == at::kByte || st == at::kInt, "the key mask must be bool, uint8 or int32 (non-zero = attended), got ", st);
-  const int64_t B = mask.size(0), S = mask.size(1);
-  TORCH_CHECK(B <= 0x7FFFFFFF && S <= 0x7FFFFFFF, "the key mask is too large");
-  const Tensor m = S <= 1 || mask.stride(1) == 1 ? mask : mask.contiguous();
-  Tensor bits = at::empty({B, (S + 63) / 64}, mask.options().dtype(at::kLong));
+  TORCH_CHECK(mask.size(0) <= 0x7FFFFFFF && mask.size(1) <= 0x7FFFFFFF, "the key mask is too large");
+  return mask.size(1) <= 1 || mask.stride(1) == 1 ? mask : mask.contiguous();
+}
+// -> one bit per key, int64 [B, ceil(S / 64)]
+Tensor rel_mask_bits(const Tensor& mask) {
+  const Tensor m = key_mask_tensor(mask);
+  DeviceGuard guard(m.device());
+  const int64_t B = m.size(0), S = m.size(1);
+  Tensor bits = at::empty({B, (S + 63) / 64}, m.options().dtype(at::kLong));
   if (bits.numel())
-    check(pdt_rel_attn_mask(m.data_ptr(), st == at::kInt ? 4 : 1, B <= 1 ? 0 : m.stride(0), (int)B, (int)S,
+    check(pdt_rel_attn_mask(m.data_ptr(), m.scalar_type() == at::kInt ? 4 : 1, B <= 1 ? 0 : m.stride(0), (int)B, (int)S,
                             reinterpret_cast<uint64_t*>(bits.data_ptr<int64_t>()), cur_stream()), "rel_attn_mask");
   return bits;
 }
@@ -510,6 +521,7 @@ std::vector<Tensor> rel_attn_forward(const Tensor& q_in, const Tensor& k_in, con
       a.o_lo = rel_view(low);
     }
   }
+  if (a.B == 0) o.zero_();  // (rows, but no sequences)
   check(pdt_rel_attn_fwd(dt_code(q), &a, cur_stream()), "rel_attn_fwd");
   return {o, lse, low};
 }
@@ -547,6 +559,8 @@ void rel_attn_backward_into(const Tensor& dout_in, const Tensor& q, const Tensor
     part = at::empty({rows, (int64_t)a.buckets * a.A}, lse.options());
     a.dtable_part = part.data_ptr<float>();
   }
+  if (a.B == 0)
+    for (Tensor t : {dq, dk, dv}) t.zero_();
   check(pdt_rel_attn_bwd(dt_code(q), &a, cur_stream()), "rel_attn_bwd");
   if (dtable.p) finish_columns(dt_code(q), part, rows, a.buckets * a.A, 1, dtable, GradOut{});
 }
@@ -604,8 +618,7 @@ struct RelAttnNode : public torch::autograd::Function<RelAttnNode> {
     return out;
   }
 };
-Tensor rel_mask_bits(const Tensor& mask);
-// `key_mask`: [B, S] as rel_mask_bits() takes it, or int64 bits that it made
+// `key_mask`: [B, S] as key_mask_tensor() takes it
 Tensor relative_attention(const Tensor& q, const Tensor& k, const Tensor& v, const OptTensor& table, int64_t max_distance,
                           const std::vector<int64_t>& steps, const OptTensor& key_mask, const OptTensor& cu, int64_t max_seqlen,
                           double scale, const OptTensor& rng_state, double p, int64_t micro, int64_t site, const OptTensor& sids) {
@@ -613,7 +626,7 @@ Tensor relative_attention(const Tensor& q, const Tensor& k, const Tensor& v, con
   OptTensor bits;
   if (key_mask.has_value()) {
     same_gpu(*key_mask, q, "key_mask");
-    bits = rel_mask_bits(*key_mask);
+    bits = key_mask->dim() == 2 && key_mask->size(1) <= 128 ? key_mask_tensor(*key_mask) : rel_mask_bits(*key_mask);
   }
   const bool wanted = at::GradMode::is_enabled() && (q.requires_grad() || k.requires_grad() || v.requires_grad() ||
                                                      (table.has_value() && table->requires_grad()));
