@@ -5,6 +5,8 @@
 // pieces; sums are fp32.  A row (one head of one token) belongs to L neighbouring lanes, and a lane holds the two 8-element
 // chunks that the rotation pairs up (i and i + R/2, or two neighbouring chunks), so that turning a pair never crosses lanes
 // and only the sum of squares does.  A wave keeps the angles of its token(s) in registers while it walks over their heads.
+// Forward, 131072 tokens of 16 heads of 64, queries and keys in bf16 (1.07 GB): 212 us, 5.1 TB/s, the rate of a large copy;
+// 20000 tokens of 8 + 1 heads of 128 at positions up to 2^20: 30 us.
 #include "common.hpp"
 
 namespace pdt {
@@ -34,10 +36,16 @@ __device__ __forceinline__ QrLane qr_lane(const PdtQkRope& p, int slot) {
   return l;
 }
 template <typename T>
-__device__ __forceinline__ void qr_load(const T* row, const QrLane& l, float (&a)[8], float (&b)[8]) {
-  short8 va = {0, 0, 0, 0, 0, 0, 0, 0}, vb = va;
+__device__ __forceinline__ void qr_fetch(const T* row, const QrLane& l, short8& va, short8& vb) {
+  const short8 none = {0, 0, 0, 0, 0, 0, 0, 0};
+  va = vb = none;
   if (l.ok0) va = *reinterpret_cast<const short8*>(row + l.c0 * 8);
   if (l.ok1) vb = *reinterpret_cast<const short8*>(row + l.c1 * 8);
+}
+template <typename T>
+__device__ __forceinline__ void qr_load(const T* row, const QrLane& l, float (&a)[8], float (&b)[8]) {
+  short8 va, vb;
+  qr_fetch<T>(row, l, va, vb);
   unpack8<T>(va, a);
   unpack8<T>(vb, b);
 }
@@ -149,86 +157,92 @@ __global__ __launch_bounds__(64 * QR_WAVES) void qk_rope_fwd_kernel(PdtQkRope p,
   }
 }
 
-// Grid-stride over the tokens, so that the weight gradients stay in registers: a lane adds up its 16 columns of both
-// sides, the workgroup writes one partial row.
+// Grid-stride over the tokens, so that the weight gradient stays in registers: a lane adds up its 16 columns, the workgroup
+// writes one partial row.  blockIdx.y = side: with both sides in one workgroup the two weights and two sums cost 64 registers
+// more.  The 144 to 166 registers (forced under 128 they spill: 530 us) leave 3 waves per SIMD, so loads run one item ahead,
+// and the grid is what fits the card at once, 768 workgroups over both sides.  131072 tokens of 16 heads of 64 (1.61 GB):
+// 326 us, 4.9 TB/s.  Loading one item at a time took 390 us, 1024 workgroups (one round and a third) 378 us.
+constexpr int QR_BWD_BLOCKS = 384;
 template <typename T, int L, int MODE>
 __global__ __launch_bounds__(64 * QR_WAVES) void qk_rope_bwd_kernel(PdtQkRope p, int gt, float* __restrict__ partial) {
-  __shared__ float red[QR_WAVES][2][256];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, grp = lane / L;
+  __shared__ float red[QR_WAVES][256];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, grp = lane / L, side = blockIdx.y;
   const int per_wave = (64 / L) / gt;
   const QrLane l = qr_lane<MODE>(p, lane & (L - 1));
-  float acc[2][16];
+  const bool normed = p.w[side] != nullptr;
+  float acc_a[8], acc_b[8], wa[8], wb[8];
 #pragma unroll
-  for (int i = 0; i < 16; ++i) acc[0][i] = acc[1][i] = 0.f;
-  float w[2][16];
-#pragma unroll
-  for (int side = 0; side < 2; ++side) {
-    float wa[8], wb[8];
-    qr_weight<T>(p, side, l, wa, wb);
-#pragma unroll
-    for (int e = 0; e < 8; ++e) { w[side][e] = wa[e]; w[side][8 + e] = wb[e]; }
-  }
-  const int step = gridDim.x * QR_WAVES * per_wave;
-  for (int t = (blockIdx.x * QR_WAVES + wave) * per_wave + grp / gt; t < p.T; t += step) {
+  for (int e = 0; e < 8; ++e) acc_a[e] = acc_b[e] = 0.f;
+  qr_weight<T>(p, side, l, wa, wb);
+  // one (token, head) after the other; the next one's rows and position are on their way while this one is worked on
+  const int step = gridDim.x * QR_WAVES * per_wave, heads = p.heads[side], h0 = grp & (gt - 1);
+  int t = h0 < heads ? (blockIdx.x * QR_WAVES + wave) * per_wave + grp / gt : p.T, h = h0, turned = -1;
+  short8 x0, x1, g0, g1;
+  int64_t pos = 0;
+  const auto fetch = [&](int tn, int hn) {
+    const int b = tn / p.seq, at = tn - b * p.seq;
+    if (normed) qr_fetch<T>(qr_row<const T>(p.x[side], b, at) + (int64_t)hn * p.x[side].head, l, x0, x1);
+    qr_fetch<T>(qr_row<const T>(p.y[side], b, at) + (int64_t)hn * p.y[side].head, l, g0, g1);
+    if (MODE) pos = qr_pos(p, tn, at);
+  };
+  if (t < p.T) fetch(t, h);
+  float cs[8], sn[8];
+  while (t < p.T) {
+    float xa[8], xb[8], ga[8], gb[8];
+    unpack8<T>(g0, ga);
+    unpack8<T>(g1, gb);
+    if (normed) {
+      unpack8<T>(x0, xa);
+      unpack8<T>(x1, xb);
+    }
+    if (MODE && turned != t) qr_angles<MODE>(p, l, pos, cs, sn);
+    turned = t;
     const int b = t / p.seq, at = t - b * p.seq;
-    float cs[8], sn[8];
-    if (MODE) qr_angles<MODE>(p, l, qr_pos(p, t, at), cs, sn);
+    T* dx = qr_row<T>(p.dx[side], b, at) + (int64_t)h * p.dx[side].head;
+    h += gt;
+    if (h >= heads) { h = h0; t += step; }
+    if (t < p.T) fetch(t, h);
+    qr_turn<MODE, -1>(ga, gb, cs, sn);
+    if (normed) {
+      float ss = 0.f, dot = 0.f;
 #pragma unroll
-    for (int side = 0; side < 2; ++side) {
-      const T* x = qr_row<const T>(p.x[side], b, at);
-      const T* dy = qr_row<const T>(p.y[side], b, at);
-      T* dx = qr_row<T>(p.dx[side], b, at);
-      for (int h = grp & (gt - 1); h < p.heads[side]; h += gt) {
-        float ga[8], gb[8];
-        qr_load<T>(dy + (int64_t)h * p.y[side].head, l, ga, gb);
-        if (p.w[side]) {
-          float xa[8], xb[8];
-          qr_load<T>(x + (int64_t)h * p.x[side].head, l, xa, xb);
-          qr_turn<MODE, -1>(ga, gb, cs, sn);
-          float ss = 0.f, dot = 0.f;
+      for (int e = 0; e < 8; ++e) {
+        ss += xa[e] * xa[e] + xb[e] * xb[e];
+        dot += ga[e] * wa[e] * xa[e] + gb[e] * wb[e] * xb[e];
+      }
+      const float r = rsqrtf(qr_sum<L>(ss) / p.D + p.eps);
+      const float m = qr_sum<L>(dot) * r * r / p.D;  // mean(h x r) r
 #pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            ss += xa[e] * xa[e] + xb[e] * xb[e];
-            dot += ga[e] * w[side][e] * xa[e] + gb[e] * w[side][8 + e] * xb[e];
-          }
-          const float r = rsqrtf(qr_sum<L>(ss) / p.D + p.eps);
-          const float m = qr_sum<L>(dot) * r * r / p.D;  // mean(h x r) r
-#pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            acc[side][e] += ga[e] * xa[e] * r;
-            acc[side][8 + e] += gb[e] * xb[e] * r;
-            ga[e] = r * (ga[e] * w[side][e] - xa[e] * m);
-            gb[e] = r * (gb[e] * w[side][8 + e] - xb[e] * m);
-          }
-        } else {
-          qr_turn<MODE, -1>(ga, gb, cs, sn);
-        }
-        qr_store<T>(dx + (int64_t)h * p.dx[side].head, l, ga, gb);
+      for (int e = 0; e < 8; ++e) {
+        acc_a[e] += ga[e] * xa[e] * r;
+        acc_b[e] += gb[e] * xb[e] * r;
+        ga[e] = r * (ga[e] * wa[e] - xa[e] * m);
+        gb[e] = r * (gb[e] * wb[e] - xb[e] * m);
       }
     }
+    qr_store<T>(dx, l, ga, gb);
   }
   if (!partial) return;
 #pragma unroll
-  for (int side = 0; side < 2; ++side) {
+  for (int e = 0; e < 8; ++e)
 #pragma unroll
-    for (int i = 0; i < 16; ++i)
+    for (int o = 32; o >= L; o >>= 1) {
+      acc_a[e] += __shfl_xor(acc_a[e], o, 64);
+      acc_b[e] += __shfl_xor(acc_b[e], o, 64);
+    }
+  if (lane < L) {
 #pragma unroll
-      for (int o = 32; o >= L; o >>= 1) acc[side][i] += __shfl_xor(acc[side][i], o, 64);
-    if (lane < L) {
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        if (l.ok0) red[wave][side][l.c0 * 8 + e] = acc[side][e];
-        if (l.ok1) red[wave][side][l.c1 * 8 + e] = acc[side][8 + e];
-      }
+    for (int e = 0; e < 8; ++e) {
+      if (l.ok0) red[wave][l.c0 * 8 + e] = acc_a[e];
+      if (l.ok1) red[wave][l.c1 * 8 + e] = acc_b[e];
     }
   }
   __syncthreads();
-  for (int i = threadIdx.x; i < 2 * p.D; i += 64 * QR_WAVES) {
-    const int side = i >= p.D, c = i - side * p.D;
+  for (int c = threadIdx.x; c < p.D; c += 64 * QR_WAVES) {
     float s = 0.f;
 #pragma unroll
-    for (int v = 0; v < QR_WAVES; ++v) s += red[v][side][c];
-    partial[(int64_t)blockIdx.x * 2 * p.D + i] = s;
+    for (int v = 0; v < QR_WAVES; ++v) s += red[v][c];
+    partial[((int64_t)blockIdx.x * 2 + side) * p.D + c] = s;
   }
 }
 
@@ -268,7 +282,7 @@ template <typename T, int L>
 static int qr_launch(const PdtQkRope& p, bool bwd, float* partial, hipStream_t st) {
   const int gt = qr_groups(p, L), mode = p.R == 0 ? 0 : (p.interleaved ? 2 : 1);
   if (bwd) {
-    const dim3 grid(pdt_qk_rope_bwd_blocks(&p));
+    const dim3 grid(pdt_qk_rope_bwd_blocks(&p), 2);
     if (mode == 0) hipLaunchKernelGGL((qk_rope_bwd_kernel<T, L, 0>), grid, dim3(64 * QR_WAVES), 0, st, p, gt, partial);
     else if (mode == 1) hipLaunchKernelGGL((qk_rope_bwd_kernel<T, L, 1>), grid, dim3(64 * QR_WAVES), 0, st, p, gt, partial);
     else hipLaunchKernelGGL((qk_rope_bwd_kernel<T, L, 2>), grid, dim3(64 * QR_WAVES), 0, st, p, gt, partial);
@@ -304,7 +318,7 @@ extern "C" int pdt_qk_rope_fwd(int dtype, const PdtQkRope* a, void* stream) {
 }
 extern "C" int pdt_qk_rope_bwd_blocks(const PdtQkRope* a) {
   const int n = qr_blocks_for(*a);
-  return n < 1 ? 1 : (n > 1024 ? 1024 : n);
+  return n < 1 ? 1 : (n > QR_BWD_BLOCKS ? QR_BWD_BLOCKS : n);
 }
 extern "C" int pdt_qk_rope_bwd(int dtype, const PdtQkRope* a, float* partial, void* stream) {
   if (int e = qr_check(dtype, *a, true)) return e;
