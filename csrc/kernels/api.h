@@ -187,6 +187,9 @@ typedef struct PdtRelAttn {
                                 // with it every gradient - would otherwise carry the rounding of o
   PdtRelView dout, dq, dk, dv;  // backward
   float* lse;                   // fp32 [B, A, S], log2 domain (forward: null = not wanted)
+  float* mass;                  // null, or fp32 [2, B, A, S]: how much of a row's softmax lies in chunks of keys beyond the last
+                                // bucket's distance, before and behind the row; written by the forward, read for the table gradient
+                                // (where pdt_rel_attn_uses_low)
   float* delta;                 // fp32 [2, B, A, S] scratch of the backward
   const void* table;            // [buckets, A], 16-bit or (table_f32) fp32; null: no bias (buckets = max_distance = 0)
   float* dtable_part;           // null, or fp32 [pdt_rel_attn_dtable_rows()][buckets][A]: partial sums of the table gradient

@@ -305,6 +305,8 @@ __global__ __launch_bounds__(RA_THREADS) RA_OCC_FWD void rel_attn_fwd_kernel(Pdt
   // Running maximum m of a row (log2 domain), and what the products start from: c0 = -m / k2, so that the scores come out of
   // the matrix unit with the maximum subtracted.  m = -inf: no attended key so far (the products then start from 0).
   const float inv_k2 = 1.0f / k2;
+  constexpr int ZONE = RA_WAVES * 16 * QB;
+  float* const zone = bias.t + 4 * bias.len + wave * 16 * QB + lm;  // [2][ZONE]: log2 of the rows' sums at the near chunks' ends
   float m[QB];
   float4v c0[QB], l4[QB], o[QB][2 * KS];
 #pragma unroll
@@ -316,10 +318,10 @@ __global__ __launch_bounds__(RA_THREADS) RA_OCC_FWD void rel_attn_fwd_kernel(Pdt
   }
   __syncthreads();  // the bias array is complete
   const float bias_lo = bias.t[0], bias_hi = bias.t[bias.len - 1];
-  auto sweep = [&](auto kind, RaChunks cur) {
+  auto sweep = [&](auto kind, RaChunks cur, int stop) {
     constexpr int KIND = decltype(kind)::value;
     constexpr float SLACK = DROP ? RA_SLACK_DROP : RA_SLACK;
-    while (!cur.done() && cur.kind() == KIND) {
+    while (cur.c < stop && cur.kind() == KIND) {
       const int buf = cur.buf;
       RaChunks nx = cur;
       nx.next(word);
@@ -408,7 +410,19 @@ __global__ __launch_bounds__(RA_THREADS) RA_OCC_FWD void rel_attn_fwd_kernel(Pdt
     }
     return cur;
   };
-  while (!cur.done()) cur = sweep(RaKind<RA_PARTIAL>{}, sweep(RaKind<RA_NEAR>{}, sweep(RaKind<RA_FARAWAY>{}, cur)));
+#pragma unroll 1
+  for (int z = 0; z < 3; ++z) {  // the chunks below the near ones, the near ones, those above
+    const int stop = p.mass && z < 2 ? min(z ? cur.hi : cur.lo + 1, cur.nc) : cur.nc;
+    while (cur.c < stop)
+      cur = sweep(RaKind<RA_PARTIAL>{}, sweep(RaKind<RA_NEAR>{}, sweep(RaKind<RA_FARAWAY>{}, cur, stop), stop), stop);
+    if (!p.mass) break;
+    if (z == 2) break;
+#pragma unroll
+    for (int i = 0; i < QB; ++i) {
+      const float t = ra_quad_sum((l4[i][0] + l4[i][1]) + (l4[i][2] + l4[i][3]));
+      if (g == 0) zone[z * ZONE + 16 * i] = m[i] + __log2f(t);  // (-inf where nothing was summed)
+    }
+  }
   float l[QB];
 #pragma unroll
   for (int i = 0; i < QB; ++i) l[i] = (l4[i][0] + l4[i][1]) + (l4[i][2] + l4[i][3]);
@@ -449,7 +463,18 @@ __global__ __launch_bounds__(RA_THREADS) RA_OCC_FWD void rel_attn_fwd_kernel(Pdt
     const float total = ra_quad_sum(l[i]);
     // a row without an attended key has no probability mass: a zero output, and lse = +inf makes every p of backward 0
     // (the sum is NaN, not 0, when a score was: the output is then NaN as well)
-    if (p.lse && g == 0 && q < s.n) p.lse[((int64_t)s.b * p.A + s.h) * p.S + q] = total == 0.f ? INFINITY : m[i] + __log2f(total);
+    const int64_t row = ((int64_t)s.b * p.A + s.h) * p.S + q;
+    const float lse = total == 0.f ? INFINITY : m[i] + __log2f(total);
+    if (p.lse && g == 0 && q < s.n) p.lse[row] = lse;
+    if (p.mass && g == 0 && q < s.n) {
+      float lo = __builtin_amdgcn_exp2f(zone[16 * i] - lse), in = __builtin_amdgcn_exp2f(zone[ZONE + 16 * i] - lse);
+      if (SPLIT == 2) {
+        lo += __builtin_amdgcn_exp2f(zone[16 * (i + 2 * QB)] - lse);
+        in += __builtin_amdgcn_exp2f(zone[ZONE + 16 * (i + 2 * QB)] - lse);
+      }
+      p.mass[row] = cur.lo < 0 ? 0.f : lo;
+      p.mass[(int64_t)p.B * p.A * p.S + row] = cur.hi >= cur.nc || 1.f - in < 0x1p-16f ? 0.f : 1.f - in;  // (less is the rounding of `in`)
+    }
     const float inv = total == 0.f ? 0.f : 1.0f / total;
     ra_store<T, KS>(ob + (int64_t)q * p.o.row, o[i], inv, g, p.D, q < s.n);
     if (p.o_lo.p) {
@@ -518,6 +543,14 @@ struct RaDiag {
     u = v;
   }
 };
+
+template <int N>
+__device__ __forceinline__ float ra_sum(const float (&v)[N]) {
+  float s = v[0];
+#pragma unroll
+  for (int i = 1; i < N; ++i) s += v[i];
+  return s;
+}
 
 // distances -> buckets: sums[top + d] is the sum at distance d, |d| <= top; eight lanes per bucket walk its range
 template <int THREADS>
@@ -604,12 +637,16 @@ __global__ __launch_bounds__(RA_THREADS) RA_OCC_DQ void rel_attn_dq_kernel(PdtRe
     for (int i = tid; i < 2 * RA_WAVES * dlen; i += RA_THREADS) sums[i] = 0.f;
   float4v open = splat4(0.f);  // the tile of the last offset, which the next pair of tiles adds to (two blocks per wave)
   int open_u = RaDiag::NONE;
-  float far_lo = 0.f, far_hi = 0.f;
+  // A row's ds add up to 0 but for the roundings that its output carries.  Most distances of a long sequence fall into the two
+  // far buckets, where ds nearly cancels and these remainders would show (2 x 4096 tokens: 3.3e-3 of the table gradient, now
+  // 2.4e-3, for 239 -> 247 us).  The remainder e is what delta is off by, so far sums give back e times their share of the row
+  // (p.mass: chunks that are far as a whole; the far tiles of a row's near chunks keep theirs).
+  float far_lo = 0.f, far_hi = 0.f, e_all[QB];
   uint32_t seed[QB];
 #pragma unroll
   for (int i = 0; i < QB; ++i) {
     const int q = q0 + 16 * i + lm;
-    float d = 0.f;
+    float d = e_all[i] = 0.f;
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks)
 #pragma unroll
@@ -638,7 +675,9 @@ __global__ __launch_bounds__(RA_THREADS) RA_OCC_DQ void rel_attn_dq_kernel(PdtRe
   };
   auto sweep = [&](auto kind, RaChunks cur) {
     constexpr int KIND = decltype(kind)::value;
-    while (!cur.done() && cur.kind() == KIND) {
+    const bool below = cur.c <= cur.lo;  // (a run of far chunks stays on one side)
+    const float before = ra_sum(e_all);
+    while (!cur.done() && cur.kind() == KIND && (KIND != RA_FARAWAY || (cur.c <= cur.lo) == below)) {
       const int buf = cur.buf;
       RaChunks nx = cur;
       nx.next(word);
@@ -656,7 +695,6 @@ __global__ __launch_bounds__(RA_THREADS) RA_OCC_DQ void rel_attn_dq_kernel(PdtRe
         const char* kimg = smem + buf * BUF;
         const char* vimg = kimg + NH * RA_IMG;
         const int u0 = cur.c * RA_CHUNK - q0;
-        const bool below = cur.c <= cur.lo;
 #pragma unroll
         for (int pi = 0; pi < 2 / SPLIT; ++pi) {
           const int pb = SPLIT == 2 ? half : pi;
@@ -703,6 +741,11 @@ __global__ __launch_bounds__(RA_THREADS) RA_OCC_DQ void rel_attn_dq_kernel(PdtRe
             for (int i = 0; i < QB; ++i) dq[i][db] = Half16<T>::mfma(kf, sf[i], dq[i][db]);
           }
           if (part) {
+#pragma unroll
+            for (int i = 0; i < QB; ++i) {
+              const float4v t = ds[i][0] + ds[i][1];
+              e_all[i] += (t[0] + t[1]) + (t[2] + t[3]);
+            }
             if (KIND != RA_FARAWAY) {  // tiles of the same offset u = u0 + 16 (kb - i) first add up
               const int u = u0 + 32 * pb;
               if (QB == 2) {
@@ -719,27 +762,27 @@ __global__ __launch_bounds__(RA_THREADS) RA_OCC_DQ void rel_attn_dq_kernel(PdtRe
                 near(u, ds[0][0]);
                 near(u + 16, ds[0][1]);
               }
-            } else {
-              float4v t = ds[0][0] + ds[0][1];
-#pragma unroll
-              for (int i = 1; i < QB; ++i) t += ds[i][0] + ds[i][1];
-              const float sum = (t[0] + t[1]) + (t[2] + t[3]);
-              if (below) far_lo += sum;
-              else far_hi += sum;
             }
           }
         }
       }
       cur = nx;
     }
+    if (KIND == RA_FARAWAY) {
+      far_lo += below ? ra_sum(e_all) - before : 0.f;
+      far_hi += below ? 0.f : ra_sum(e_all) - before;
+    }
     return cur;
   };
   while (!cur.done()) cur = sweep(RaKind<RA_PARTIAL>{}, sweep(RaKind<RA_NEAR>{}, sweep(RaKind<RA_FARAWAY>{}, cur)));
   if (SPLIT == 2) {  // the two waves of a row group add up their halves of the keys
     constexpr int F = QB * 8 * KS;
-    static_assert(2 * F * 64 * (int)sizeof(float) <= 2 * BUF, "the join reuses the images");
+    static_assert((2 * F + 4 * QB) * 64 * (int)sizeof(float) <= 2 * BUF, "the join reuses the images");
     float* x = reinterpret_cast<float*>(smem) + group * F * 64 + lane;
+    float* y = reinterpret_cast<float*>(smem) + (2 * F + group * 2 * QB) * 64 + lane;
     __syncthreads();
+#pragma unroll
+    for (int i = 0; i < QB; ++i) y[(half * QB + i) * 64] = e_all[i];
     if (half == 1 && active) {
 #pragma unroll
       for (int e = 0; e < F; ++e) x[e * 64] = dq[e / (8 * KS)][(e / 4) % (2 * KS)][e & 3];
@@ -749,6 +792,8 @@ __global__ __launch_bounds__(RA_THREADS) RA_OCC_DQ void rel_attn_dq_kernel(PdtRe
 #pragma unroll
       for (int e = 0; e < F; ++e) dq[e / (8 * KS)][(e / 4) % (2 * KS)][e & 3] += x[e * 64];
     }
+#pragma unroll
+    for (int i = 0; i < QB; ++i) e_all[i] += y[((half ^ 1) * QB + i) * 64];
   }
   if (active && half == 0) {
     T* dqb = ra_base<T>(p.dq, s, packed);
@@ -761,6 +806,18 @@ __global__ __launch_bounds__(RA_THREADS) RA_OCC_DQ void rel_attn_dq_kernel(PdtRe
   if (part) {  // the far sums join the ends of their wave's first array; then distances -> buckets
     if (open_u != RaDiag::NONE) near(open_u, open);
     diag.flush();
+    if (p.mass) {
+#pragma unroll
+      for (int i = 0; i < QB; ++i) {
+        const int q = q0 + 16 * i + lm;
+        const float e = ra_quad_sum(e_all[i]);
+        if (half == 0 && g == 0 && q < s.n) {  // once per row; a share of 0 takes nothing, not even NaN
+          const float ml = p.mass[bh * p.S + q], mh = p.mass[((int64_t)p.B * p.A + bh) * p.S + q];
+          far_lo -= ml != 0.f ? e * ml : 0.f;
+          far_hi -= mh != 0.f ? e * mh : 0.f;
+        }
+      }
+    }
     const float lo = wave_sum(far_lo);
     const float hi = wave_sum(far_hi);
     float* const mine = sums + wave * 2 * dlen;
@@ -1256,9 +1313,11 @@ static int ra_dispatch(int which, const PdtRelAttn& p, hipStream_t st) {
   if (which == RA_SHORT) return ra_short_rows(p) == 64 ? ra_launch_short<T, KS, 4, DROP>(p, st) : ra_launch_short<T, KS, 8, DROP>(p, st);
   const int rows = ra_rows(p, which);
   const size_t imgs = (size_t)4 * NH * RA_IMG, tab = ra_bias_bytes(p);
-  if (which == RA_FWD)
-    return rows == 128 ? ra_launch(rel_attn_fwd_kernel<T, KS, 2, 1, DROP>, p, rows, imgs + 512 + tab, st)
-                       : ra_launch(rel_attn_fwd_kernel<T, KS, 2, 2, DROP>, p, rows, imgs + 512 + tab, st);
+  if (which == RA_FWD) {
+    const size_t zones = p.mass ? (size_t)2 * RA_WAVES * 32 * sizeof(float) : 0;
+    return rows == 128 ? ra_launch(rel_attn_fwd_kernel<T, KS, 2, 1, DROP>, p, rows, imgs + 512 + tab + zones, st)
+                       : ra_launch(rel_attn_fwd_kernel<T, KS, 2, 2, DROP>, p, rows, imgs + 512 + tab + zones, st);
+  }
   if (which == RA_DQ) {
     const size_t diag = p.dtable_part ? (size_t)2 * RA_WAVES * ra_diag_len(p.max_distance) * sizeof(float) : 0;
     return rows == 128 ? ra_launch(rel_attn_dq_kernel<T, KS, 2, 1, DROP>, p, rows, imgs + 512 + tab + diag, st)

@@ -499,6 +499,18 @@ PdtRng rel_rng(const OptTensor& state, double p, int64_t micro, int64_t site, co
   // (the masks derive from (sample, head, query, key): the sequence length plays no part)
   return make_rng(*state, micro, site, sids, 1, B);
 }
+// log-sum-exps [B, heads, S], or [3, B, heads, S] with the far shares of long rows behind them (PdtRelAttn.mass)
+Tensor rel_row_sums(int64_t B, int64_t A, int64_t S, bool table, const at::TensorOptions& f32) {
+  return table && pdt_rel_attn_uses_low((int)S) ? at::empty({3, B, A, S}, f32) : at::empty({B, A, S}, f32);
+}
+void set_row_sums(PdtRelAttn& a, const Tensor& lse) {
+  chkf32(lse, "lse");
+  const int64_t d = lse.dim() - 3;
+  TORCH_CHECK((d == 0 || (d == 1 && lse.size(0) == 3)) && lse.size(d) == a.B && lse.size(d + 1) == a.A && lse.size(d + 2) == a.S,
+              "lse must be [B, heads, S] or [3, B, heads, S]");
+  a.lse = lse.data_ptr<float>();
+  a.mass = d ? a.lse + (int64_t)a.B * a.A * a.S : nullptr;
+}
 // -> o, lse, o_lo (what a backward pass needs only when wanted; o_lo for long sequences only, see PdtRelAttn)
 std::vector<Tensor> rel_attn_forward(const Tensor& q_in, const Tensor& k_in, const Tensor& v_in, const OptTensor& table,
                                      int64_t max_distance, const std::vector<int64_t>& steps, const OptTensor& bits,
@@ -514,8 +526,8 @@ std::vector<Tensor> rel_attn_forward(const Tensor& q_in, const Tensor& k_in, con
   if (q.numel() == 0) return {o, want_lse ? at::empty({a.B, a.A, a.S}, q.options().dtype(at::kFloat)) : Tensor(), Tensor()};
   Tensor lse, low;
   if (want_lse) {
-    lse = at::empty({a.B, a.A, a.S}, q.options().dtype(at::kFloat));
-    a.lse = lse.data_ptr<float>();
+    lse = rel_row_sums(a.B, a.A, a.S, table.has_value(), q.options().dtype(at::kFloat));
+    set_row_sums(a, lse);
     if (pdt_rel_attn_uses_low(a.S)) {
       low = at::empty(q.sizes(), q.options());
       a.o_lo = rel_view(low);
@@ -545,15 +557,14 @@ void rel_attn_backward_into(const Tensor& dout_in, const Tensor& q, const Tensor
   PdtRelAttn a = rel_args(q, k, v, o, c, rng);
   const Tensor dout = head_rows(dout_in, "dout");
   TORCH_CHECK(dout.sizes() == q.sizes() && dout.scalar_type() == q.scalar_type(), "dout must have q's shape and dtype");
-  chkf32(lse, "lse");
-  TORCH_CHECK(lse.dim() == 3 && lse.size(0) == a.B && lse.size(1) == a.A && lse.size(2) == a.S, "lse must be [B, heads, S]");
-  Tensor delta = at::empty({2, lse.size(0), lse.size(1), lse.size(2)}, lse.options()), part;
+  set_row_sums(a, lse);
+  Tensor delta = at::empty({2, a.B, a.A, a.S}, lse.options()), part;
   if (low.defined()) {
     TORCH_CHECK(low.sizes() == o.sizes() && low.scalar_type() == o.scalar_type(), "low must have o's shape and dtype");
     a.o_lo = rel_view(low);
   }
   a.dout = rel_view(dout); a.dq = rel_view(dq); a.dk = rel_view(dk); a.dv = rel_view(dv);
-  a.lse = lse.data_ptr<float>(); a.delta = delta.data_ptr<float>();
+  a.delta = delta.data_ptr<float>();
   const int rows = pdt_rel_attn_dtable_rows(&a);
   if (dtable.p) {
     part = at::empty({rows, (int64_t)a.buckets * a.A}, lse.options());
@@ -581,7 +592,7 @@ std::vector<Tensor> rel_attn_backward(const Tensor& dout, const Tensor& q_in, co
   }
   if (want_dtable) dtable = at::empty(table->sizes(), table->options());
   const RelCall c{table, bits, cu, steps, max_distance, max_seqlen, scale, p};
-  rel_attn_backward_into(dout, q, k, v, o, low.has_value() ? *low : Tensor(), lse, c, rel_rng(rng_state, p, micro, site, sids, lse.size(0)), dq, dk, dv,
+  rel_attn_backward_into(dout, q, k, v, o, low.has_value() ? *low : Tensor(), lse, c, rel_rng(rng_state, p, micro, site, sids, lse.size(-3)), dq, dk, dv,
                          grad_out(dtable));
   return {dq, dk, dv, dtable};
 }
@@ -818,8 +829,7 @@ Tensor position_attention_forward(const LayerPosition& pos, const Tensor& qkv, T
   const Tensor o = head_view(ctx, B, S, A, packed);
   const RelCall c{pos.table, bits, cu, pos.steps, pos.max_distance, S, 0.125, p};
   PdtRelAttn a = rel_args(q, k, v, o, c, rng);
-  TORCH_CHECK(lse.numel() >= (int64_t)a.B * a.A * a.S, "lse is too small");
-  a.lse = lse.data_ptr<float>();
+  set_row_sums(a, lse);
   if (qkv.size(0)) check(pdt_rel_attn_fwd(dt_code(qkv), &a, cur_stream()), "rel_attn_fwd");
   return qk;
 }
@@ -873,7 +883,7 @@ std::vector<Tensor> layer_forward(const Tensor& x, const Tensor& mask, const Ten
   Tensor ctx = at::empty({T, H}, x.options());
   Tensor qk;
   // (the position kernels count packed rows by the longest sample there can be: no more than the rows there are)
-  Tensor lse = at::empty({B, A, pos && cup ? std::min<int64_t>(S, T) : S}, f32);
+  Tensor lse = pos ? rel_row_sums(B, A, cup ? std::min<int64_t>(S, T) : S, pos->table.has_value(), f32) : at::empty({B, A, S}, f32);
   if (pos)
     qk = position_attention_forward(*pos, qkv, ctx, lse, positions, bits, cu, B, S, A, p_attn,
                                     make_rng(rng_state, micro, site + 0, sids, S, B));

@@ -549,3 +549,42 @@ def test_rotated_attention_depends_on_relative_positions_only():
     u, _ = half_step(torch.float16)
     top = qkv[:, :, 2].double().abs().max()
     assert (outs[0] - outs[1]).abs().max() <= 2 * (math.exp(4 * 16 * u) - 1) * top + 6 * u * top
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_relative_attention_far_buckets_give_back_the_rounding_of_p(dtype):
+    """Scores of two levels, whose probabilities round the same way in every row, and values that follow them: the forward's
+    output is off by the same e = u p / (1 + p) in every row (p = 0.5 (1 + 0.9 u) is stored as 0.5).  Without giving it back,
+    the far buckets would add up e times their share of the row over all rows, S e / 2 each; what may remain is the share of
+    the keys that lie in a far bucket but not in chunks that are far as a whole: the buckets' ends, the workgroup's rows and two
+    chunks, in all no more than 64 + 128 + 2 * 64 keys on a side."""
+    S, u = 2048, half_step(dtype)[0]
+    p = 0.5 * (1 + 0.9 * u)
+    q = torch.zeros(1, S, 1, 64, dtype=dtype, device="cuda")
+    k, v, dout = torch.zeros_like(q), torch.zeros_like(q), torch.zeros_like(q)
+    q[..., :3] = 1
+    left = math.log(p) * 8  # the scale is 1 / 8; the score in three parts, each of the dtype
+    for i in range(3):
+        part = torch.tensor(left, dtype=torch.float64).to(dtype)
+        k[:, 1::2, :, i] = part
+        left -= float(part)
+    v[:, 0::2, :, 5] = 1
+    v[:, 1::2, :, 5] = -1
+    dout[..., 5] = 1
+    bias = torch.zeros(32, 1, device="cuda", requires_grad=True)
+    for t in (q, k, v):
+        t.requires_grad_()
+    ops().relative_attention(q, k, v, bias, max_distance=128).backward(dout)
+    score = (q.detach().double()[0, :, 0] @ k.detach().double()[0, :, 0].T) / 8
+    prob = score.softmax(-1)
+    dp = torch.ones(S, 1, dtype=torch.float64, device="cuda") * v.detach().double()[0, :, 0, 5]
+    ds = prob * (dp - (prob * dp).sum(-1, keepdim=True))
+    gap = torch.arange(S, device="cuda")
+    bucket = bucket_rule(gap[None, :] - gap[:, None], 32, 128)
+    true = torch.zeros(32, dtype=torch.float64, device="cuda").index_add_(0, bucket.flatten(), ds.flatten())
+    e = 0.45 * u / (1 + p)
+    for b in (15, 31):
+        off = abs(float(bias.grad[b, 0]) - float(true[b]))
+        left_over = S * e * (64 + 128 + 2 * 64) / S * 1.05 + F32 * S  # (1.05: the keys of either level)
+        assert off < left_over, (b, off, left_over, S * e / 2)
+        assert dtype == torch.float16 or left_over < 0.4 * S * e
