@@ -75,6 +75,10 @@ def relative_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, bias: 
     ``dropout_p`` (at most 0.99) with ``rng`` (an :class:`~.fused.RngKey`) and ``site``: dropout on the probabilities with the framework's
     counter-based masks.
 
+    Forward and backward may be captured into a graph; masks and ``cu_seqlens`` are then read at every replay (``max_seqlen`` and
+    the shapes are those of the capture).  As with any operator, let no eager autograd graph of the same leaves live meanwhile:
+    their gradients would be accumulated on its stream, outside the capture.
+
     Returns a contiguous tensor of q's shape and dtype.  Probabilities and their gradients are rounded to q's dtype as
     operands of the matrix products; scores, softmax statistics and all sums are fp32.  The gradient of ``bias`` is summed in
     fp32 in a fixed order, so it is the same in every run.

@@ -588,3 +588,87 @@ def test_relative_attention_far_buckets_give_back_the_rounding_of_p(dtype):
         left_over = S * e * (64 + 128 + 2 * 64) / S * 1.05 + F32 * S  # (1.05: the keys of either level)
         assert off < left_over, (b, off, left_over, S * e / 2)
         assert dtype == torch.float16 or left_over < 0.4 * S * e
+
+
+@pytest.mark.parametrize("form", ["short mask", "long mask", "packed"])
+def test_captured_passes_read_the_lengths_and_masks_of_each_replay(form):
+    """A captured training pass with its buffers refilled between replays: other masks, other sequence borders."""
+    A, D, T = 2, 64, 400
+    S = {"short mask": 100, "long mask": 200, "packed": 0}[form]
+    lengths = [[S, 0], [1, S], [S // 2, 65]] if S else [[300, 0, 64], [5, 130, 1], [0, 399, 1]]
+    gen = torch.Generator(device="cuda").manual_seed(S)
+    shape = (2, S, A, D) if S else (T, A, D)
+    q, k, v = ((torch.randn(shape, generator=gen, device="cuda")).half().requires_grad_() for _ in range(3))
+    bias = torch.randn(32, A, generator=gen, device="cuda").requires_grad_()
+    dout = torch.randn(shape, generator=gen, device="cuda").half()
+
+    def where(lens):
+        lens = torch.tensor(lens, device="cuda")
+        if S:
+            return torch.arange(S, device="cuda")[None, :] < lens[:, None]
+        return torch.cat([lens.new_zeros(1), lens.cumsum(0)]).int()
+
+    def step(at):
+        more = {"key_mask": at} if S else {"cu_seqlens": at, "max_seqlen": 399}
+        out = ops().relative_attention(q, k, v, bias, **more)
+        return (out, *torch.autograd.grad(out, (q, k, v, bias), dout))
+
+    held = where(lengths[0])
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step(held)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        res = step(held)
+    for lens in lengths + lengths[:1]:
+        held.copy_(where(lens))
+        graph.replay()
+        torch.cuda.synchronize()
+        want = step(where(lens))
+        assert all(torch.equal(a, b) for a, b in zip(res, want)), lens
+
+
+@pytest.mark.parametrize("S", [60, 300])
+def test_relative_attention_of_one_tensor_and_with_a_frozen_table(S):
+    """The same tensor as queries, keys and values: its gradient is the sum of the three; a table that takes no gradient."""
+    (x, y, z), bias, dout, _ = padded_case(torch.bfloat16, 2, S, 2, 64, seed=S)
+    parts = [x.detach().clone().requires_grad_() for _ in range(3)]
+    out = ops().relative_attention(*parts, bias)
+    apart = torch.autograd.grad(out, (*parts, bias), dout)
+    x = x.detach().clone().requires_grad_()
+    frozen = bias.detach()
+    same = ops().relative_attention(x, x, x, frozen)
+    assert torch.equal(same, out)
+    (g,) = torch.autograd.grad(same, x, dout)
+    u = half_step(torch.bfloat16)[0]
+    total = sum(t.double() for t in apart[:3])
+    bound = 2 * u * (apart[0].double().abs() + apart[1].double().abs() + apart[2].double().abs())  # two sums of 16-bit terms
+    assert ((g.double() - total).abs() <= bound * (1 + u) + 1e-30).all()
+
+
+def test_two_calls_at_once_on_two_streams():
+    """Calls of both operators on two streams, backward passes included, as eager results one after the other."""
+    cases = [padded_case(torch.float16, 2, S, 2, 64, lens=[S, S // 3], seed=S) for S in (120, 450)]
+    rope = ops().rotary_table(512, 64)
+    w = [(torch.rand(64, device="cuda") + 0.5).requires_grad_() for _ in range(2)]
+
+    def step(case):
+        (q, k, v), bias, dout, valid = case
+        a, b = ops().qk_norm_rope(q, k, *w, rope=rope)
+        out = ops().relative_attention(a, b, v, bias, key_mask=valid)
+        return (out, *torch.autograd.grad(out, (q, k, v, bias, *w), dout))
+
+    want = [step(c) for c in cases]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in cases]
+    for _ in range(5):
+        got = []
+        for c, s in zip(cases, streams):
+            s.wait_stream(torch.cuda.current_stream())
+            with torch.cuda.stream(s):
+                got.append(step(c))
+        torch.cuda.synchronize()
+        for a, b in zip(want, got):
+            assert all(torch.equal(x, y) for x, y in zip(a, b))
