@@ -202,7 +202,8 @@ typedef struct PdtRelAttn {
   int mask_bytes;               // sample to sample (a load per 64 keys and workgroup: for short sequences, where packing it
   int64_t mask_stride;          // first would cost a launch)
   const int32_t* cu;            // null, or first rows of the samples in packed [T, ...] tensors, int32 [B + 1]; rows from
-                                // cu[B] on become zero (B >= 1; without samples nothing is written).  S is then the longest sample.
+                                // cu[B] on become zero, as do those of a sample from S on, the longest length announced (B >= 1;
+                                // without samples nothing is written)
   int B, S, A, D, T;
   float scale, drop_scale;
   uint32_t drop_thr;

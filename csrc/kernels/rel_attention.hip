@@ -159,16 +159,21 @@ template <typename T>
 __device__ __forceinline__ T* ra_base(const PdtRelView& v, const RaSpan& s, bool packed) {
   return (T*)v.p + (packed ? s.row0 * v.row : (int64_t)s.b * v.batch) + (int64_t)s.h * v.head;
 }
-// Rows from cu[B] on of a packed output belong to no sample and become zero: the workgroups of the last sample share them.
+// Rows of a packed output that no sample takes in become zero: those from cu[B] on (by the last sample's workgroups), those
+// before cu[0] (by the first's) and what of a sample lies beyond the longest length announced (by its own).
 template <typename T>
 __device__ __forceinline__ void ra_tail(const PdtRelAttn& p, const RaSpan& s, const PdtRelView& v, int tid, int threads) {
-  if (!p.cu || s.b != p.B - 1) return;
-  const int first = min(max(uniform_load_i32(p.cu, p.B), 0), p.T), per = p.D >> 3;
-  const int64_t n = (int64_t)(p.T - first) * per;
-  for (int64_t i = (int64_t)blockIdx.y * threads + tid; i < n; i += (int64_t)gridDim.y * threads) {
-    const int r = (int)(i / per), c = (int)(i - (int64_t)r * per);
-    *reinterpret_cast<int4v*>((T*)v.p + (int64_t)(first + r) * v.row + (int64_t)s.h * v.head + c * 8) = int4v{0, 0, 0, 0};
-  }
+  if (!p.cu) return;
+  const int per = p.D >> 3;
+  auto zero = [&](int64_t first, int64_t end) {
+    const int64_t n = (end - first) * per;
+    for (int64_t i = (int64_t)blockIdx.y * threads + tid; i < n; i += (int64_t)gridDim.y * threads) {
+      const int64_t r = i / per, c = i - r * per;
+      *reinterpret_cast<int4v*>((T*)v.p + (first + r) * v.row + (int64_t)s.h * v.head + c * 8) = int4v{0, 0, 0, 0};
+    }
+  };
+  zero(s.row0 + s.n, s.b == p.B - 1 ? p.T : min(max(uniform_load_i32(p.cu, s.b + 1), 0), p.T));
+  if (s.b == 0) zero(0, s.row0);
 }
 // attended keys of chunk c, one bit each
 __device__ __forceinline__ uint64_t ra_word(const PdtRelAttn& p, const RaSpan& s, int c) {

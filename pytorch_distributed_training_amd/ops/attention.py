@@ -63,7 +63,8 @@ def relative_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, bias: 
     into a fused projection are read in place (unit inner stride, other strides multiples of 8 elements, 16-byte aligned -
     anything else is copied first).  With ``cu_seqlens`` (int32 ``[B + 1]`` on the GPU, ascending from 0) they are the packed rows
     ``[T, heads, dim]`` of sequences of different lengths instead, ``max_seqlen`` the longest of them; rows from
-    ``cu_seqlens[-1]`` on belong to no sequence, their outputs and gradients are zero.
+    ``cu_seqlens[-1]`` on belong to no sequence, their outputs and gradients are zero.  So are those of rows beyond
+    ``max_seqlen`` in a sequence that is longer after all: the sequence is cut there.
 
     ``bias``: ``[buckets, heads]``, fp32 or of q's dtype; ``None`` leaves it out.  ``max_distance`` (at most 512): where the
     last bucket of each side begins at the latest, see :func:`bucket_steps`.

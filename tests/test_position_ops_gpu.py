@@ -672,3 +672,26 @@ def test_two_calls_at_once_on_two_streams():
         torch.cuda.synchronize()
         for a, b in zip(want, got):
             assert all(torch.equal(x, y) for x, y in zip(a, b))
+
+
+@pytest.mark.parametrize("limit", [50, 100, 130])
+def test_relative_attention_cuts_packed_sequences_at_the_length_announced(limit):
+    """Sequences longer than max_seqlen count up to it; rows before the first and behind the last one belong to none."""
+    lead, lens, tail, A, D = 3, [20, 150, 1, 131], 9, 2, 64
+    T = lead + sum(lens) + tail
+    gen = torch.Generator(device="cuda").manual_seed(limit)
+    q, k, v = (torch.randn(T, A, D, generator=gen, device="cuda").half().requires_grad_() for _ in range(3))
+    bias = torch.randn(32, A, generator=gen, device="cuda").requires_grad_()
+    dout = (torch.randn(T, A, D, generator=gen, device="cuda") * 0.25).half()
+    cu = torch.tensor([lead] + lens, device="cuda").cumsum(0).int()
+    junk = [torch.full((T, A, D), 7.0, dtype=torch.float16, device="cuda") for _ in range(8)]  # (what the outputs' memory held)
+    del junk
+    out = ops().relative_attention(q, k, v, bias, cu_seqlens=cu, max_seqlen=limit)
+    grads = torch.autograd.grad(out, (q, k, v, bias), dout)
+    spans = [(lo, min(hi, lo + limit)) for lo, hi in zip(cu.tolist()[:-1], cu.tolist()[1:])]
+    check_attention(q, k, v, bias, dout, spans=spans, got=(out, *grads))
+    outside = torch.ones(T, dtype=torch.bool, device="cuda")
+    for lo, hi in spans:
+        outside[lo:hi] = False
+    for t in (out, *grads[:3]):
+        assert t[outside].abs().sum() == 0
