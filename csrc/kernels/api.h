@@ -25,7 +25,7 @@ typedef struct PdtRng {
   uint32_t seq;           // tokens per sample of the activation the kernel works on (1 for [B, H] tensors)
   uint32_t seq_magic;     // ceil(2^32 / seq): row / seq == umulhi(row, seq_magic) for row * seq < 2^32
   // Unpadded (packed) activations [T, H], where a row's sample and position do not follow from its index: the
-  // dropout row of every row, precomputed (sample id * 512 + position; device, uint32 [T]).  Takes precedence over
+  // dropout row of every row, precomputed (as drop_row() forms it; device, uint32 [T]).  Takes precedence over
   // the (sample_ids, seq) rule for row-wise tensors; per-sample tensors and attention still use sample_ids.
   const uint32_t* row_table;
 } PdtRng;

@@ -150,7 +150,8 @@ __device__ __forceinline__ DropKey drop_key(const RngArgs& r) {
   return k;
 }
 // Row of a [B*seq, H] activation -> the row its dropout counters are derived from (see PdtRng::sample_ids):
-// global sample id * 512 + position inside the sample (512 = the longest sequence the position table allows).
+// sample id * 512 + position inside the sample.  (Where the position table allows more than 512 tokens, the ids handed in are
+// multiples of the number of 512-row blocks that the longest sequence takes.)
 __device__ __forceinline__ uint32_t drop_row(const RngArgs& r, uint32_t row) {
   if (r.row_table) return r.row_table[row];
   if (!r.sample_ids) return row;

@@ -186,9 +186,11 @@ PdtRng make_rng(const Tensor& state, int64_t micro, int64_t site, const OptTenso
   if (sids.has_value()) {
     TORCH_CHECK(sids->is_cuda() && sids->scalar_type() == at::kInt && sids->is_contiguous() && sids->dim() == 1,
                 "sample_ids must be a contiguous int32 [B] GPU tensor");
-    TORCH_CHECK(seq >= 1 && seq <= 512, "sample-keyed dropout: at most 512 tokens per sample");
+    // (a sample has the 512 rows from id * 512 on: ids of longer samples come in steps of several, NativeRuntime.sample_blocks)
+    TORCH_CHECK(seq >= 1, "sample-keyed dropout: at least one token per sample");
     TORCH_CHECK(batch < 0 || sids->numel() == batch, "sample_ids has ", sids->numel(), " entries for a batch of ", batch);
-    TORCH_CHECK(sids->numel() * seq < (int64_t(1) << 23), "sample-keyed dropout: too many rows for the exact row / seq trick");
+    TORCH_CHECK(sids->numel() * seq < std::min(int64_t(1) << 23, (int64_t(1) << 32) / seq),
+                "sample-keyed dropout: too many rows for the exact row / seq trick");
     r.sample_ids = sids->data_ptr<int32_t>();
     r.seq = (uint32_t)seq;
     r.seq_magic = seq == 1 ? 0u : (uint32_t)(((uint64_t(1) << 32) + (uint64_t)seq - 1) / (uint64_t)seq);

@@ -65,7 +65,7 @@ class MaskInfo:
                  positions=None):
         """`cu_seqlens` / `rowmap` / `positions`: an UNPADDED batch (native path only) - the hidden states are the packed
         [T, H] rows of the real tokens, sample b owns rows cu_seqlens[b] .. cu_seqlens[b+1], `seq` is the longest sample,
-        `rowmap[t]` the dropout row (sample id * 512 + position) of packed row t and `positions[t]` (int64) its position."""
+        `rowmap[t]` the dropout row (sample id * 512 dropout_blocks + position) of packed row t and `positions[t]` (int64) its position."""
         self.batch, self.seq = batch, seq
         self.cu, self.rowmap, self.positions = cu_seqlens, rowmap, positions
         self._all_attended = mask is None
@@ -411,6 +411,7 @@ class _ClassifierBase(nn.Module):
         if cfg.head_dim != 64:
             raise ValueError("native attention kernels are specialised for head_dim == 64")
         rt = runtime or fused.NativeRuntime(arena, seed, global_seed)
+        rt.sample_blocks = max(rt.sample_blocks, cfg.dropout_blocks)
         self.arena, self.runtime = arena, rt
         base = self.base_model
         bp = f"{prefix}{self.base_model_prefix}."
@@ -464,7 +465,7 @@ class _ClassifierBase(nn.Module):
         tok = token_index
         b_of = torch.div(tok, S, rounding_mode="floor")
         sid = sample_ids.reshape(-1).to(torch.int64)[b_of] if sample_ids is not None else b_of
-        rowmap = (sid * 512 + (tok - b_of * S)).to(torch.int32)
+        rowmap = (sid * (512 * self.config.dropout_blocks) + (tok - b_of * S)).to(torch.int32)
         cu = cu_seqlens.to(torch.int32)
         mask = MaskInfo(None, B, S, tok.device, cu_seqlens=cu, rowmap=rowmap,
                         positions=tok - b_of * S if self.config.rotary_dim else None)

@@ -51,6 +51,13 @@ class EncoderConfig:
         return bool(self.relative_attention_num_buckets or self.qk_norm or self.rotary_dim)
 
     @property
+    def dropout_blocks(self) -> int:
+        """Rows that the dropout counters set aside for a sample, in blocks of 512: enough for the longest sequence that the
+        position table allows (RoBERTa's positions start behind the padding index), so that no two samples share a row."""
+        longest = self.max_position_embeddings - (self.pad_token_id + 1 if self.model_type == "roberta" else 0)
+        return max(1, -(-longest // 512))
+
+    @property
     def head_dim(self) -> int:
         return self.hidden_size // self.num_attention_heads
 

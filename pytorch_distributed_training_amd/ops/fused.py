@@ -53,6 +53,9 @@ class NativeRuntime:
         gs = seed if global_seed is None else global_seed
         self.rng_state_global = torch.tensor([gs ^ 0x5BD1E995, 0], dtype=torch.int64, device=arena.device)
         self.micro = 0  # per-rank micro-batch counter (the no-ids keying)
+        # The kernels give a sample id 512 dropout rows; a model with longer sequences hands them ids in steps of so many
+        # (EncoderConfig.dropout_blocks), so that the next sample's rows begin behind its own.
+        self.sample_blocks = 1
         self.key = RngKey(self.rng_state, 0, None)  # of the forward pass in progress
         self.segment_done: Optional[Callable[[int], None]] = None  # set by the DP reducer wrapper
         # segments whose completion is reported later, by release(): a segment that gets part of its gradient outside
@@ -93,6 +96,8 @@ class NativeRuntime:
             self.next_micro()
         else:
             ids = sample_ids.reshape(-1).to(device=self.arena.device, dtype=torch.int32).contiguous()
+            if self.sample_blocks > 1:
+                ids = ids * self.sample_blocks
             # (the window counter advances with every zero_grad(), i.e. once per optimizer step on every rank)
             self.key = RngKey(self.rng_state_global, self.arena.window & 0x7FFFFFFF, ids)
         return self.key
@@ -218,8 +223,15 @@ def _position_inputs(nat: LayerNative, mask):
     return (mask.positions, mask.bits()) if nat.position is not None else (None, None)
 
 
+def _check_length(cfg, seq: int) -> None:
+    """Longer sequences would run into the dropout rows of the next sample (and have no position of their own)."""
+    if seq > 512 * cfg.dropout_blocks:
+        raise ValueError(f"sequences of {seq} tokens are longer than the configuration's positions allow")
+
+
 def encoder_layer_forward(layer, hidden, mask, rng=None):
     nat = layer._native
+    _check_length(layer.cfg, mask.seq)
     if hidden.dtype != nat.w[0].dtype:
         hidden = hidden.to(nat.w[0].dtype)
     if hidden.dim() == 2 and mask.cu is None:
@@ -291,6 +303,7 @@ def encoder_stack_forward(layers, hidden, mask, rng=None):
     PDT_LAYER_NODES=1 keeps one node per layer."""
     if not layers:
         return hidden
+    _check_length(layers[0].cfg, mask.seq)
     # (without a tape - evaluation - the layers run one by one: every layer's saved tensors die with its call, whereas the
     # one-call form returns those of the whole stack at once)
     if len(layers) == 1 or not torch.is_grad_enabled() or os.environ.get("PDT_LAYER_NODES") == "1":
