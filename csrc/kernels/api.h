@@ -191,6 +191,8 @@ typedef struct PdtRelAttn {
                                 // bucket's distance, before and behind the row; written by the forward, read for the table gradient
                                 // (where pdt_rel_attn_uses_low)
   float* delta;                 // fp32 [2, B, A, S] scratch of the backward
+  uint32_t* peaks;              // uint32 [pdt_rel_attn_peaks()] scratch of its fp16 form for S > 128 (0 entries: unused)
+  int peak_rows;                // (set by pdt_rel_attn_bwd)
   const void* table;            // [buckets, A], 16-bit or (table_f32) fp32; null: no bias (buckets = max_distance = 0)
   float* dtable_part;           // null, or fp32 [pdt_rel_attn_dtable_rows()][buckets][A]: partial sums of the table gradient
                                 // (finish with pdt_colsum_finish(part, rows, buckets * A, 1, ...))
@@ -214,6 +216,7 @@ int pdt_rel_attn_mask(const void* mask, int bytes, int64_t stride, int B, int S,
 int pdt_rel_attn_fwd(int dtype, const PdtRelAttn* a, void* stream);
 int pdt_rel_attn_uses_low(int S);
 int pdt_rel_attn_dtable_rows(const PdtRelAttn* a);
+int64_t pdt_rel_attn_peaks(int dtype, const PdtRelAttn* a);
 int pdt_rel_attn_bwd(int dtype, const PdtRelAttn* a, void* stream);
 
 // ---- Per-head RMS norm of queries and keys with the position rotation -----------------------------------

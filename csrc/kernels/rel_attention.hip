@@ -136,6 +136,35 @@ __device__ __forceinline__ float ra_quad_sum(float v) {
   return a + b;
 }
 
+// ---- the lift of an fp16 backward pass
+// P and ds are operands of 16 bits.  ds has the size of P times the output gradients, 1e-7 for 1000 keys and gradients of 1e-4,
+// and as it stands fp16 would round it to steps of 6e-8 (1000 keys, gradients of 1e-4: an error of 9.9e-3 of dQ, where relative
+// roundings leave 5.1e-4; 2100 keys and 1e-3: 2.2e-3 and 4.1e-4).  So P enters the products as 2^lift P, with the power of two that brings the largest |dout| of
+// the rows that share it to [1/2, 1), and the results are multiplied by 2^-lift: the factor rides on the exponent of P and on
+// final scales that are there anyway.  2^lift P over the share kept stays below 2^15; |ds| 2^lift stays below what output
+// gradients of size one give without a lift, half the sum of |v| over a row (p (1 - p) times the spread of dp) but for
+// dropout's factor.  bf16 has fp32's exponents: no lift.
+template <typename T> constexpr bool RA_LIFTS = std::is_same<T, _Float16>::value;
+// the largest of the bits of |x| over eight 16-bit values (ordered like the values; infinities and NaN are larger than all numbers)
+__device__ __forceinline__ uint32_t ra_top(uint32_t top, const short8& x) {
+#pragma unroll
+  for (int j = 0; j < 8; ++j) top = max(top, (uint32_t)x[j] & 0x7FFFu);
+  return top;
+}
+template <int CTRL>
+__device__ __forceinline__ uint32_t ra_ror_max(uint32_t v) {
+  return max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, 0xF, 0xF, false));
+}
+__device__ __forceinline__ uint32_t ra_wave_max(uint32_t v) {  // (wave-uniform; no LDS permutes, whose addresses would stay in registers)
+  v = ra_ror_max<0x121>(ra_ror_max<0x122>(ra_ror_max<0x124>(ra_ror_max<0x128>(v))));  // row_ror:8, 4, 2, 1
+  const auto at = [&](int lane) { return (uint32_t)__builtin_amdgcn_readlane((int)v, lane); };
+  return max(max(at(0), at(16)), max(at(32), at(48)));
+}
+__device__ __forceinline__ int ra_lift(uint32_t top, float drop_scale) {
+  const int room = 14 - ((int)(__float_as_uint(drop_scale) >> 23) - 127);  // (the share kept: at most 2^room / 2^15)
+  return min(max(14 - (int)(top >> 10), 0), room);
+}
+
 // ---- one (batch, head) of a launch
 struct RaSpan {
   int b, h, n;      // sample, head, length
@@ -222,8 +251,8 @@ __device__ __forceinline__ RaChunks ra_chunks(int n, int w0, int rows, int far, 
   return k;
 }
 
-// ---- the bias array: entry i of copy j is the bias (times log2 e) of distance sign * (i + j - off); `off` and the
-// clamp leave room so that a tile beyond the near distances reads the constant part.
+// ---- the bias array: entry i of copy j is the bias (times log2 e, `plus` a constant) of distance sign * (i + j - off); `off`
+// and the clamp leave room so that a tile beyond the near distances reads the constant part.
 struct RaBias {
   float* t;
   int len, off, far;  // far: max_distance rounded up to the tile size
@@ -252,10 +281,10 @@ __device__ __forceinline__ float ra_table(const PdtRelAttn& p, int bucket, int h
   return p.table_f32 ? ((const float*)p.table)[i] : Half16<T>::to_f(((const short*)p.table)[i]);
 }
 template <typename T, int THREADS = RA_THREADS>
-__device__ __forceinline__ RaBias ra_bias_fill(const PdtRelAttn& p, float* mem, int h, int sign, int tid, int max_distance) {
+__device__ __forceinline__ RaBias ra_bias_fill(const PdtRelAttn& p, float* mem, int h, int sign, int tid, int max_distance, float plus = 0.f) {
   RaBias t{mem, ra_bias_len(max_distance), ra_far(max_distance) + 32, ra_far(max_distance)};
   for (int i = tid; i < t.len + 4; i += THREADS) {
-    const float v = p.table ? ra_table<T>(p, ra_bucket(p, sign * (i - t.off)), h) * LOG2E : 0.f;
+    const float v = (p.table ? ra_table<T>(p, ra_bucket(p, sign * (i - t.off)), h) * LOG2E : 0.f) + plus;
 #pragma unroll
     for (int j = 0; j < 4; ++j)
       if (i - j >= 0 && i - j < t.len) mem[j * t.len + i - j] = v;
@@ -640,6 +669,19 @@ __global__ __launch_bounds__(RA_THREADS) RA_OCC_DQ void rel_attn_dq_kernel(PdtRe
     // what the products start from, so that scores come out with lse subtracted (rows that are not there: p = 0)
     nlse[i] = (q < s.n ? -p.lse[bh * p.S + q] : -INFINITY) / k2;
   }
+  int lift = 0;  // (of the wave's own rows)
+  if constexpr (RA_LIFTS<T>) {
+    uint32_t top = 0;
+#pragma unroll
+    for (int i = 0; i < QB; ++i)
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks) top = ra_top(top, df[i][ks]);
+    top = ra_wave_max(top);
+    lift = ra_lift(top, p.drop_scale);
+    // for the dK / dV kernel, whose sums run over all rows (two waves of a pair hold the same rows and write the same)
+    if (lane == 0) p.peaks[(bh * gridDim.y + blockIdx.y) * RA_WAVES + wave] = top;
+  }
+  const float drop_lift = RA_LIFTS<T> ? __uint_as_float((uint32_t)(127 - lift) << 23) : 1.0f;  // 2^-lift
   if (!cur.done()) stage(cur.c, 0, cur.w);
   const RaBias bias = ra_bias_fill<T>(p, mb + 2 * RA_CHUNK, s.h, 1, tid, p.max_distance);
   const int boff = ra_bias_lane(bias, lm, g);
@@ -672,6 +714,7 @@ __global__ __launch_bounds__(RA_THREADS) RA_OCC_DQ void rel_attn_dq_kernel(PdtRe
       p.delta[bh * p.S + q] = -d;
       p.delta[((int64_t)p.B * p.A + bh) * p.S + q] = nlse[i];
     }
+    if (RA_LIFTS<T>) nlse[i] += lift / k2;
     seed[i] = DROP ? attn_row_seed(drop_key(p.rng), drop_sample(p.rng, s.b) * p.A + s.h, q) : 0u;
   }
   const uint32_t thr_hi = attn_thr_hi(p.drop_thr), kmul0 = (uint32_t)(4 * g) * ATT_GOLD;
@@ -814,7 +857,7 @@ __global__ __launch_bounds__(RA_THREADS) RA_OCC_DQ void rel_attn_dq_kernel(PdtRe
 #pragma unroll
     for (int i = 0; i < QB; ++i) {
       const int q = q0 + 16 * i + lm;
-      ra_store<T, KS>(dqb + (int64_t)q * p.dq.row, dq[i], p.scale, g, p.D, q < s.n);
+      ra_store<T, KS>(dqb + (int64_t)q * p.dq.row, dq[i], p.scale * drop_lift, g, p.D, q < s.n);
     }
   }
   if (part) {  // the far sums join the ends of their wave's first array; then distances -> buckets
@@ -835,15 +878,17 @@ __global__ __launch_bounds__(RA_THREADS) RA_OCC_DQ void rel_attn_dq_kernel(PdtRe
     const float lo = wave_sum(far_lo);
     const float hi = wave_sum(far_hi);
     float* const mine = sums + wave * 2 * dlen;
+    float* const drops = sums + 2 * RA_WAVES * dlen;
     if (lane == 0) {
       mine[0] += lo;
       mine[2 * bias.far + 62] += hi;
+      if (RA_LIFTS<T>) drops[wave] = drop_lift;
     }
     __syncthreads();
     for (int i = tid; i < dlen; i += RA_THREADS) {  // (the eight arrays into the first)
       float t = 0.f;
 #pragma unroll
-      for (int a = 0; a < 2 * RA_WAVES; ++a) t += sums[a * dlen + i];
+      for (int a = 0; a < 2 * RA_WAVES; ++a) t += sums[a * dlen + i] * (RA_LIFTS<T> ? drops[a >> 1] : 1.0f);
       sums[i] = t;
     }
     __syncthreads();
@@ -910,7 +955,16 @@ __global__ __launch_bounds__(RA_THREADS) RA_OCC_DKV void rel_attn_dkv_kernel(Pdt
     }
   }
   stage(cur.c, 0);
-  const RaBias bias = ra_bias_fill<T>(p, reinterpret_cast<float*>(smem + 2 * BUF), s.h, -1, tid, p.max_distance);
+  int lift = 0;  // (one for all queries: it goes into P through the bias array)
+  if constexpr (RA_LIFTS<T>) {
+    const int blocks = (p.S + p.peak_rows - 1) / p.peak_rows, there = (s.n + p.peak_rows - 1) / p.peak_rows * RA_WAVES;
+    const uint32_t* const peaks = p.peaks + bh * blocks * RA_WAVES;
+    uint32_t top = 0;
+    for (int i = lane; i < there; i += 64) top = max(top, peaks[i]);
+    lift = ra_lift(ra_wave_max(top), p.drop_scale);
+  }
+  const float drop_lift = RA_LIFTS<T> ? __uint_as_float((uint32_t)(127 - lift) << 23) : 1.0f;  // 2^-lift
+  const RaBias bias = ra_bias_fill<T>(p, reinterpret_cast<float*>(smem + 2 * BUF), s.h, -1, tid, p.max_distance, (float)lift);
   const int boff = ra_bias_lane(bias, lm, g);
   const float k2 = p.scale * LOG2E;
   const uint32_t thr_hi = attn_thr_hi(p.drop_thr);
@@ -1032,8 +1086,8 @@ __global__ __launch_bounds__(RA_THREADS) RA_OCC_DKV void rel_attn_dkv_kernel(Pdt
 #pragma unroll
       for (int db = 0; db < 2 * KS; ++db) dk_[i][db] = dv_[i][db] = splat4(0.f);
     }
-    ra_store<T, KS>(dkb + (int64_t)key * p.dk.row, dk_[i], p.scale, g, p.D, key < s.n);
-    ra_store<T, KS>(dvb + (int64_t)key * p.dv.row, dv_[i], 1.0f, g, p.D, key < s.n);
+    ra_store<T, KS>(dkb + (int64_t)key * p.dk.row, dk_[i], p.scale * drop_lift, g, p.D, key < s.n);
+    ra_store<T, KS>(dvb + (int64_t)key * p.dv.row, dv_[i], drop_lift, g, p.D, key < s.n);
   }
 }
 
@@ -1089,13 +1143,33 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(KS <= 2 
   const RaBias bias = ra_bias_fill<T, 64 * W>(p, reinterpret_cast<float*>(smem + 4 * IMG), s.h, 1, tid, min(p.max_distance, 128));
   const float k2 = p.scale * LOG2E;
   // what the products start from, so that scores come out with lse subtracted (rows that are not there: p = 0)
-  const float nlse = (q < s.n ? -p.lse[((int64_t)s.b * p.A + s.h) * p.S + q] : -INFINITY) / k2;
+  float nlse = (q < s.n ? -p.lse[((int64_t)s.b * p.A + s.h) * p.S + q] : -INFINITY) / k2;
   const int boff = ra_bias_lane(bias, lm, g);
   const uint32_t seed = DROP ? attn_row_seed(drop_key(p.rng), drop_sample(p.rng, s.b) * p.A + s.h, q) : 0u;
   const uint32_t thr_hi = attn_thr_hi(p.drop_thr), kmul0 = (uint32_t)(4 * g) * ATT_GOLD;
   asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+  uint32_t* const tops = reinterpret_cast<uint32_t*>(bias.t + 4 * bias.len);
+  if constexpr (RA_LIFTS<T>) {  // the largest |dout|, over what this wave has staged
+    uint32_t top = 0;
+#pragma unroll
+    for (int i = 0; i < NC * NH; ++i)
+#pragma unroll
+      for (int u = 0; u < 8 / W; ++u) top = ra_top(top, *reinterpret_cast<const short8*>(gimg + i * RA_IMG + (u * W + wave) * 1024 + lane * 16));
+    top = ra_wave_max(top);
+    if (lane == 0) tops[wave] = top;
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+  }
   __builtin_amdgcn_s_barrier();
   __builtin_amdgcn_sched_barrier(0);
+  int lift = 0;
+  if constexpr (RA_LIFTS<T>) {
+    uint32_t top = 0;
+#pragma unroll
+    for (int i = 0; i < W; ++i) top = max(top, tops[i]);
+    lift = __builtin_amdgcn_readfirstlane(ra_lift(top, p.drop_scale));
+    nlse += lift / k2;
+  }
+  const float drop_lift = RA_LIFTS<T> ? __uint_as_float((uint32_t)(127 - lift) << 23) : 1.0f;  // 2^-lift
 
   // ---- rows: p, dp, delta, ds, dQ.  (Waves up to the end of the last 32 rows take part: their rows are zero.)
   const bool active = 16 * wave < ((s.n + 31) & ~31);
@@ -1150,7 +1224,7 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(KS <= 2 
       }
       pp[pb] = pack_pair<T>(pd[0], pd[1]);
     }
-    const float delta = ra_quad_sum((d4[0] + d4[1]) + (d4[2] + d4[3]));
+    const float delta = ra_quad_sum((d4[0] + d4[1]) + (d4[2] + d4[3])) * drop_lift;  // (d4: with the lift of p)
     float4v dq[2 * KS];
 #pragma unroll
     for (int db = 0; db < 2 * KS; ++db) dq[db] = splat4(0.f);
@@ -1164,7 +1238,7 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(KS <= 2 
       for (int db = 0; db < 2 * KS; ++db)
         dq[db] = Half16<T>::mfma(ra_tr_frag(kimg + (pb >> 1) * NH * RA_IMG, (pb & 1) * 32, db, lane), sf[pb], dq[db]);
     }
-    ra_store<T, KS>(ra_base<T>(p.dq, s, packed) + (int64_t)q * p.dq.row, dq, p.scale, g, p.D, q < s.n);
+    ra_store<T, KS>(ra_base<T>(p.dq, s, packed) + (int64_t)q * p.dq.row, dq, p.scale * drop_lift, g, p.D, q < s.n);
   }
 
   // ---- keys: dV and dK.  A pass: P and dS of its keys as [query][64 keys] images, then 16 keys per wave.
@@ -1209,12 +1283,12 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(KS <= 2 
     }
     if constexpr (DB % 2 == 0) {
       const int c0 = part_d * DB * 16;
-      ra_store<T, DB / 2>(dkb + (int64_t)key * p.dk.row + c0, dk_, p.scale, g, p.D - c0, key < s.n);
-      ra_store<T, DB / 2>(dvb + (int64_t)key * p.dv.row + c0, dv_, 1.0f, g, p.D - c0, key < s.n);
+      ra_store<T, DB / 2>(dkb + (int64_t)key * p.dk.row + c0, dk_, p.scale * drop_lift, g, p.D - c0, key < s.n);
+      ra_store<T, DB / 2>(dvb + (int64_t)key * p.dv.row + c0, dv_, drop_lift, g, p.D - c0, key < s.n);
     } else {  // one block: four columns (8 bytes) per lane
       const int col = part_d * 16 + 4 * g;
       if (key < s.n && col < p.D) {
-        const float4v a = dk_[0] * p.scale, c = dv_[0];
+        const float4v a = dk_[0] * (p.scale * drop_lift), c = dv_[0] * drop_lift;
         *reinterpret_cast<int2v*>(dkb + (int64_t)key * p.dk.row + col) = int2v{cvt_pk<T>(a[0], a[1]), cvt_pk<T>(a[2], a[3])};
         *reinterpret_cast<int2v*>(dvb + (int64_t)key * p.dv.row + col) = int2v{cvt_pk<T>(c[0], c[1]), cvt_pk<T>(c[2], c[3])};
       }
@@ -1246,7 +1320,7 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(KS <= 2 
     float t = 0.f;
 #pragma unroll 8
     for (int a = 0; a < 4 * W; ++a) t += sums[a * DLEN + i];
-    sums[i] = t;
+    sums[i] = t * drop_lift;
   }
   __syncthreads();
   ra_bucket_sums<64 * W>(p, sums, TOP, part, tid);
@@ -1314,7 +1388,7 @@ static int ra_launch_short(const PdtRelAttn& p, hipStream_t st) {
   constexpr int NH = (KS + 1) / 2, R = 16 * W;
   const size_t work = (size_t)4 * (R / RA_CHUNK) * NH * RA_IMG;
   static_assert((size_t)4 * W * (2 * R + 16) * sizeof(float) <= (size_t)4 * (R / RA_CHUNK) * NH * RA_IMG, "diagonal sums reuse the images");
-  const size_t lds = work + (size_t)4 * ra_bias_len(p.max_distance < 128 ? p.max_distance : 128) * sizeof(float);
+  const size_t lds = work + (size_t)4 * ra_bias_len(p.max_distance < 128 ? p.max_distance : 128) * sizeof(float) + W * sizeof(uint32_t);
   auto kern = rel_attn_bwd_short_kernel<T, KS, W, DROP>;
   if (int e = ra_allow_lds((const void*)kern, lds)) return e;
   hipLaunchKernelGGL(kern, dim3(p.B * p.A), dim3(64 * W), lds, st, p);
@@ -1333,7 +1407,7 @@ static int ra_dispatch(int which, const PdtRelAttn& p, hipStream_t st) {
                        : ra_launch(rel_attn_fwd_kernel<T, KS, 2, 2, DROP>, p, rows, imgs + 512 + tab + zones, st);
   }
   if (which == RA_DQ) {
-    const size_t diag = p.dtable_part ? (size_t)2 * RA_WAVES * ra_diag_len(p.max_distance) * sizeof(float) : 0;
+    const size_t diag = p.dtable_part ? (size_t)RA_WAVES * (2 * ra_diag_len(p.max_distance) + 1) * sizeof(float) : 0;
     return rows == 128 ? ra_launch(rel_attn_dq_kernel<T, KS, 2, 1, DROP>, p, rows, imgs + 512 + tab + diag, st)
                        : ra_launch(rel_attn_dq_kernel<T, KS, 2, 2, DROP>, p, rows, imgs + 512 + tab + diag, st);
   }
@@ -1406,6 +1480,12 @@ extern "C" int pdt_rel_attn_dtable_rows(const PdtRelAttn* a) {
   return a->B * ((a->S + rows - 1) / rows);
 }
 
+extern "C" int64_t pdt_rel_attn_peaks(int dtype, const PdtRelAttn* a) {  // one entry per wave of dQ
+  if (dtype != PDT_F16 || ra_short_rows(*a)) return 0;
+  const int rows = ra_rows(*a, RA_DQ);
+  return (int64_t)a->B * a->A * ((a->S + rows - 1) / rows) * RA_WAVES;
+}
+
 extern "C" int pdt_rel_attn_bwd(int dtype, const PdtRelAttn* a, void* stream) {
   if (int e = ra_check(dtype, *a)) return e;
   if (!a->dout.p || !a->dq.p || !a->dk.p || !a->dv.p) return -2;
@@ -1414,6 +1494,9 @@ extern "C" int pdt_rel_attn_bwd(int dtype, const PdtRelAttn* a, void* stream) {
   hipStream_t st = (hipStream_t)stream;
   if (a->B == 0 || a->S == 0) return 0;
   if (ra_short_rows(*a)) return ra_run(dtype, RA_SHORT, *a, st);
-  if (int e = ra_run(dtype, RA_DQ, *a, st)) return e;
-  return ra_run(dtype, RA_DKV, *a, st);
+  if (pdt_rel_attn_peaks(dtype, a) && !a->peaks) return -2;
+  PdtRelAttn p = *a;
+  p.peak_rows = ra_rows(p, RA_DQ);
+  if (int e = ra_run(dtype, RA_DQ, p, st)) return e;
+  return ra_run(dtype, RA_DKV, p, st);
 }

@@ -567,6 +567,11 @@ void rel_attn_backward_into(const Tensor& dout_in, const Tensor& q, const Tensor
   }
   a.dout = rel_view(dout); a.dq = rel_view(dq); a.dk = rel_view(dk); a.dv = rel_view(dv);
   a.delta = delta.data_ptr<float>();
+  Tensor peaks;
+  if (const int64_t n = pdt_rel_attn_peaks(dt_code(q), &a)) {
+    peaks = at::empty({n}, q.options().dtype(at::kInt));
+    a.peaks = reinterpret_cast<uint32_t*>(peaks.data_ptr<int32_t>());
+  }
   const int rows = pdt_rel_attn_dtable_rows(&a);
   if (dtable.p) {
     part = at::empty({rows, (int64_t)a.buckets * a.A}, lse.options());

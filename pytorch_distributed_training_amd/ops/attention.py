@@ -81,7 +81,8 @@ def relative_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, bias: 
     their gradients would be accumulated on its stream, outside the capture.
 
     Returns a contiguous tensor of q's shape and dtype.  Probabilities and their gradients are rounded to q's dtype as
-    operands of the matrix products; scores, softmax statistics and all sums are fp32.  The gradient of ``bias`` is summed in
+    operands of the matrix products (in fp16 by a power of two above their size, so that small gradients of the output keep
+    their digits); scores, softmax statistics and all sums are fp32.  The gradient of ``bias`` is summed in
     fp32 in a fixed order, so it is the same in every run.
     """
     if q.dim() not in (3, 4) or (q.dim() == 3) != (cu_seqlens is not None):
