@@ -48,7 +48,7 @@ def direct():
         h = x
         t0 = time.perf_counter()
         for i, l in enumerate(layers):
-            outs = C.layer_forward(h, mask, kvl, l._native.w, state, B, S, A, 0.1, 0.1, 1e-12, 1, i, None, None, None, None, None, None)
+            outs = C.layer_forward(h, mask, kvl, l._native.w, state, B, S, A, 0.1, 0.1, 1e-12, 1, i, None, None, None, None, None, None, True)
             saved.append((h, outs[1:]))
             h = outs[0]
         t1 = time.perf_counter()

@@ -798,8 +798,8 @@ std::vector<Tensor> qk_norm_rope(const Tensor& q, const Tensor& k, const OptTens
 // Encoder layer.  Weight list order (16-bit compute copies):
 //   0 wqkv[3H,H] 1 bqkv[3H] 2 wo[H,H] 3 bo[H] 4 ln1_g 5 ln1_b 6 w1[F,H] 7 b1[F] 8 w2[H,F] 9 b2[H] 10 ln2_g 11 ln2_b
 // Gradient list: the same order, fp32 views of the gradient arena.
-// Saved list: 0 qkv 1 ctx 2 lse 3 z1 4 stats1 5 x1 6 u 7 gact 8 z2 9 stats2 (10 normalised / rotated queries and keys
-// [T, 2, A, 64] of a layer with such a position option)
+// Saved list: 0 qkv 1 ctx 2 lse 3 z1 4 stats1 5 x1 6 u 7 gact 8 z2 9 stats2, then of a layer with position options the normalised /
+// rotated queries and keys [T, 2, A, 64], if it has such, and beyond 128 tokens what rounding took from ctx (PdtRelAttn.o_lo)
 // ---------------------------------------------------------------------------------------------------
 // What a layer's attention does with positions: a bias table and / or a norm and rotation of its queries and keys.  The
 // gradients of `table`, `wq`, `wk` (those that are there) follow the twelve of the gradient list, in this order.
@@ -820,8 +820,9 @@ Tensor head_third(const Tensor& qkv, int i, int64_t B, int64_t S, int64_t A, boo
 Tensor head_view(const Tensor& x, int64_t B, int64_t S, int64_t A, bool packed) {
   return packed ? x.view({x.size(0), A, 64}) : x.view({B, S, A, 64});
 }
-// attention of a layer with position options: ctx and lse are filled; returns the normalised / rotated queries and keys
-Tensor position_attention_forward(const LayerPosition& pos, const Tensor& qkv, Tensor ctx, Tensor lse, const OptTensor& positions,
+// attention of a layer with position options: ctx, lse and (where a backward pass wants it) low are filled; returns the normalised /
+// rotated queries and keys
+Tensor position_attention_forward(const LayerPosition& pos, const Tensor& qkv, Tensor ctx, Tensor lse, const Tensor& low, const OptTensor& positions,
                                   const OptTensor& bits, const OptTensor& cu, int64_t B, int64_t S, int64_t A, double p, const PdtRng& rng) {
   const bool packed = cu.has_value();
   TORCH_CHECK(!packed || !pos.cos.has_value() || positions.has_value(), "packed rows need their positions for the rotation");
@@ -837,10 +838,11 @@ Tensor position_attention_forward(const LayerPosition& pos, const Tensor& qkv, T
   const RelCall c{pos.table, bits, cu, pos.steps, pos.max_distance, S, 0.125, p};
   PdtRelAttn a = rel_args(q, k, v, o, c, rng);
   set_row_sums(a, lse);
+  if (low.defined()) a.o_lo = rel_view(head_view(low, B, S, A, packed));
   if (qkv.size(0)) check(pdt_rel_attn_fwd(dt_code(qkv), &a, cur_stream()), "rel_attn_fwd");
   return qk;
 }
-void position_attention_backward(const LayerPosition& pos, const Tensor& qkv, const Tensor& qk, const Tensor& ctx, const Tensor& dctx,
+void position_attention_backward(const LayerPosition& pos, const Tensor& qkv, const Tensor& qk, const Tensor& ctx, const Tensor& low, const Tensor& dctx,
                                  const Tensor& lse, Tensor dqkv, const std::vector<Tensor>& gr, const OptTensor& positions,
                                  const OptTensor& bits, const OptTensor& cu, int64_t B, int64_t S, int64_t A, double p,
                                  const PdtRng& rng, bool accumulate) {
@@ -854,7 +856,7 @@ void position_attention_backward(const LayerPosition& pos, const Tensor& qkv, co
   const RelCall c{pos.table, bits, cu, pos.steps, pos.max_distance, S, 0.125, p};
   const Tensor dqk = turns ? at::empty_like(qk) : dqkv;
   rel_attn_backward_into(head_view(dctx, B, S, A, packed), third(turns ? qk : qkv, 0), third(turns ? qk : qkv, 1), third(qkv, 2),
-                         head_view(ctx, B, S, A, packed), Tensor(), lse, c, rng, third(dqk, 0), third(dqk, 1), third(dqkv, 2), dtable);
+                         head_view(ctx, B, S, A, packed), low.defined() ? head_view(low, B, S, A, packed) : Tensor(), lse, c, rng, third(dqk, 0), third(dqk, 1), third(dqkv, 2), dtable);
   if (turns)
     rope_backward_into(third(dqk, 0), third(dqk, 1), third(qkv, 0), third(qkv, 1),
                        RopeCall{pos.wq, pos.wk, pos.cos, pos.sin, positions, false, pos.eps}, third(dqkv, 0), third(dqkv, 1), dwq, dwk);
@@ -865,7 +867,7 @@ std::vector<Tensor> layer_forward(const Tensor& x, const Tensor& mask, const Ten
                                   const std::vector<Tensor>& w, const Tensor& rng_state, int64_t B, int64_t S, int64_t A,
                                   double p_attn, double p_hidden, double eps, int64_t micro, int64_t layer,
                                   const OptTensor& sids, const OptTensor& cu, const OptTensor& rowmap,
-                                  const LayerPositionPtr& pos, const OptTensor& positions, const OptTensor& bits) {
+                                  const LayerPositionPtr& pos, const OptTensor& positions, const OptTensor& bits, bool tape) {
   DeviceGuard guard(x.device());
   chk16(x, "x");
   TORCH_CHECK(w.size() == 12, "layer_forward: 12 weight tensors expected");
@@ -888,11 +890,13 @@ std::vector<Tensor> layer_forward(const Tensor& x, const Tensor& mask, const Ten
   Tensor qkv = gemm_nt(x, w[0], e_bias);
 
   Tensor ctx = at::empty({T, H}, x.options());
-  Tensor qk;
+  Tensor qk, low;
   // (the position kernels count packed rows by the longest sample there can be: no more than the rows there are)
-  Tensor lse = pos ? rel_row_sums(B, A, cup ? std::min<int64_t>(S, T) : S, pos->table.has_value(), f32) : at::empty({B, A, S}, f32);
+  const int64_t longest = cup ? std::min<int64_t>(S, T) : S;
+  Tensor lse = pos ? rel_row_sums(B, A, longest, pos->table.has_value(), f32) : at::empty({B, A, S}, f32);
+  if (pos && tape && pdt_rel_attn_uses_low((int)longest)) low = at::empty({T, H}, x.options());
   if (pos)
-    qk = position_attention_forward(*pos, qkv, ctx, lse, positions, bits, cu, B, S, A, p_attn,
+    qk = position_attention_forward(*pos, qkv, ctx, lse, low, positions, bits, cu, B, S, A, p_attn,
                                     make_rng(rng_state, micro, site + 0, sids, S, B));
   else
     check(pdt_attn_fwd(dt_code(x), qkv.data_ptr(), mask.data_ptr<int32_t>(), kv_len.data_ptr<int32_t>(), cup, ctx.data_ptr(),
@@ -916,6 +920,7 @@ std::vector<Tensor> layer_forward(const Tensor& x, const Tensor& mask, const Ten
   Tensor x2 = ln_fwd(z2, w[10], w[11], stats2, eps);
   std::vector<Tensor> out = {x2, qkv, ctx, lse, z1, stats1, x1, u, gact, z2, stats2};
   if (qk.defined()) out.push_back(qk);
+  if (low.defined()) out.push_back(low);
   return out;
 }
 
@@ -926,7 +931,8 @@ Tensor layer_backward(const Tensor& dy_in, const Tensor& x, const std::vector<Te
                       const OptTensor& rowmap, const LayerPositionPtr& pos, const OptTensor& positions, const OptTensor& bits) {
   DeviceGuard guard(x.device());
   const int32_t* cup = cu.has_value() ? cu->data_ptr<int32_t>() : nullptr;
-  TORCH_CHECK(sv.size() == (pos && pos->turns() ? 11u : 10u) && w.size() == 12 && (pos || gr.size() == 12), "layer_backward: bad list sizes");
+  const size_t turns = pos && pos->turns(), lows = pos && pdt_rel_attn_uses_low((int)(cup ? std::min<int64_t>(S, x.size(0)) : S));
+  TORCH_CHECK(sv.size() == 10 + turns + lows && w.size() == 12 && (pos || gr.size() == 12), "layer_backward: bad list sizes");
   const Tensor dy = dy_in.contiguous();
   chk16(dy, "dy");
   const Tensor &qkv = sv[0], &ctx = sv[1], &lse = sv[2], &z1 = sv[3], &stats1 = sv[4], &x1 = sv[5], &u = sv[6],
@@ -962,7 +968,7 @@ Tensor layer_backward(const Tensor& dy_in, const Tensor& x, const std::vector<Te
   const int db_rows = pdt_attn_bwd_dbias_rows((int)B, (int)S);
   Tensor db_part = fused_db ? at::empty({(int64_t)db_rows, 3 * (int64_t)H}, lse.options()) : Tensor();
   if (pos)
-    position_attention_backward(*pos, qkv, pos->turns() ? sv[10] : Tensor(), ctx, dctx, lse, dqkv, gr, positions, bits, cu, B, S, A,
+    position_attention_backward(*pos, qkv, turns ? sv[10] : Tensor(), ctx, lows ? sv[10 + turns] : Tensor(), dctx, lse, dqkv, gr, positions, bits, cu, B, S, A,
                                 p_attn, make_rng(rng_state, micro, site + 0, sids, S, B), accumulate);
   else
     check(pdt_attn_bwd(dt_code(x), qkv.data_ptr(), mask.data_ptr<int32_t>(), kv_len.data_ptr<int32_t>(), cup, ctx.data_ptr(),
@@ -1000,18 +1006,18 @@ std::vector<Tensor> stack_forward(const Tensor& x, const Tensor& mask, const Ten
                                   const OptTensor& bits) {
   TORCH_CHECK(!w.empty() && w.size() == layer_ids.size() && pos.size() == w.size(), "stack_forward: one weight list and one id per layer");
   std::vector<Tensor> all;
-  all.reserve(w.size() * 12);
+  all.reserve(w.size() * 13);
   Tensor h = x;
   for (size_t l = 0; l < w.size(); ++l) {
     std::vector<Tensor> o = layer_forward(h, mask, kv_len, w[l], rng_state, B, S, A, p_attn, p_hidden, eps, micro,
-                                          layer_ids[l], sids, cu, rowmap, pos[l], positions, bits);
+                                          layer_ids[l], sids, cu, rowmap, pos[l], positions, bits, true);
     h = o[0];
     for (auto& t : o) all.push_back(std::move(t));
   }
   return all;
 }
 
-// Backward of the run, last layer first.  `saved[l]` = the 11 (12) tensors stack_forward returned for layer l;
+// Backward of the run, last layer first.  `saved[l]` = the 11 to 13 tensors stack_forward returned for layer l;
 // `accumulate[l]`: add to layer l's gradients instead of overwriting them.  After every layer its saved tensors
 // are dropped and `layer_done(l)` is called with the GIL held (the Python side drops ITS references there and
 // reports the layer's gradient segment as complete: bucket all-reduce, gradient-lane merge).

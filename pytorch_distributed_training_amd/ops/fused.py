@@ -142,7 +142,6 @@ class LayerNative:
         # what attention does with positions besides the plain softmax: the layer's table and norm weights (fp32 masters)
         # and their gradients, which follow the twelve above in the gradient list
         self.position = None
-        self.saved = 11  # tensors the layer's forward returns
         if cfg.position_ops:
             from .attention import bucket_steps
 
@@ -159,8 +158,6 @@ class LayerNative:
                 pos.eps = cfg.qk_norm_eps
             if cfg.rotary_dim:
                 pos.cos, pos.sin = runtime.rotary_table(cfg)
-            if cfg.qk_norm or cfg.rotary_dim:
-                self.saved = 12
             spec = spec + extra
             self.g += [arena.gview(n, s) for n, s in extra]
             self.position = pos
@@ -193,7 +190,7 @@ class _LayerFn(torch.autograd.Function):
             x2, m, kvl, nat.w, key.state, B, S, cfg.num_attention_heads,
             cfg.attention_probs_dropout_prob if train else 0.0, cfg.hidden_dropout_prob if train else 0.0,
             cfg.layer_norm_eps, key.counter, layer.index + nat.site_offset, key.sample_ids, mask.cu, mask.rowmap,
-            nat.position, *_position_inputs(nat, mask))
+            nat.position, *_position_inputs(nat, mask), ctx.needs_input_grad[0])
         ctx.layer, ctx.mask, ctx.x2, ctx.saved = layer, (m, kvl, mask.cu, mask.rowmap), x2, outs[1:]
         ctx.position_inputs = _position_inputs(nat, mask)
         ctx.meta = (B, S, H, train, key, packed)
@@ -267,7 +264,7 @@ class _StackFn(torch.autograd.Function):
             [l._native.position for l in layers], *_position_inputs(first._native, mask))
         ctx.layers, ctx.mask, ctx.x2, ctx.ids = layers, (m, kvl, mask.cu, mask.rowmap), x2, ids
         ctx.position_inputs = _position_inputs(first._native, mask)
-        n = first._native.saved
+        n = len(outs) // len(layers)
         ctx.saved = [outs[i * n:(i + 1) * n] for i in range(len(layers))]
         ctx.meta = (B, S, H, train, key, packed)
         ctx.lane = first._native.rt.lane
