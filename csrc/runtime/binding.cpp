@@ -5,6 +5,8 @@
 #include <ATen/hip/impl/HIPGuardImplMasqueradingAsCUDA.h>
 #include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
 #include <ATen/hip/HIPEvent.h>
+#include <c10/core/impl/TorchDispatchModeTLS.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 
 #include <algorithm>
 #include <climits>
@@ -398,6 +400,20 @@ PdtRelView rel_view(const Tensor& t) {
   auto st = [&](int64_t i) { return t.size(i) <= 1 ? (int64_t)0 : t.stride(i); };
   return PdtRelView{t.data_ptr(), d == 4 ? st(0) : 0, st(d - 3), st(d - 2)};
 }
+// The operators' nodes know the backward pass only.  What else follows a tensor's data - a tangent of forward-mode
+// differentiation, a trace that records operations - does not see the kernels and would be lost without a word.
+void plain_call(std::initializer_list<const Tensor*> tensors, std::initializer_list<const OptTensor*> more, const char* name) {
+  using Modes = c10::impl::TorchDispatchModeTLS;
+  using Key = c10::impl::TorchDispatchModeKey;
+  TORCH_CHECK(!torch::jit::tracer::isTracing() && !Modes::get_mode(Key::PROXY).has_value() && !Modes::get_mode(Key::FAKE).has_value(),
+              name, " cannot be traced: a trace would hold its empty output tensor");
+  const auto plain = [&](const Tensor& t) {
+    TORCH_CHECK(!t.defined() || !t._fw_grad(0).defined(), name, " has no forward-mode derivative: the tangent would be dropped");
+  };
+  for (const Tensor* t : tensors) plain(*t);
+  for (const OptTensor* t : more)
+    if (t->has_value()) plain(**t);
+}
 void same_gpu(const Tensor& t, const Tensor& as, const char* name) {
   TORCH_CHECK(t.device() == as.device(), name, " must be on the device of q");
 }
@@ -640,6 +656,7 @@ struct RelAttnNode : public torch::autograd::Function<RelAttnNode> {
 Tensor relative_attention(const Tensor& q, const Tensor& k, const Tensor& v, const OptTensor& table, int64_t max_distance,
                           const std::vector<int64_t>& steps, const OptTensor& key_mask, const OptTensor& cu, int64_t max_seqlen,
                           double scale, const OptTensor& rng_state, double p, int64_t micro, int64_t site, const OptTensor& sids) {
+  plain_call({&q, &k, &v}, {&table}, "relative_attention");
   TORCH_CHECK(q.is_cuda(), "q must be on the GPU");
   OptTensor bits;
   if (key_mask.has_value()) {
@@ -787,6 +804,7 @@ struct QkRopeNode : public torch::autograd::Function<QkRopeNode> {
 };
 std::vector<Tensor> qk_norm_rope(const Tensor& q, const Tensor& k, const OptTensor& wq, const OptTensor& wk, const OptTensor& cos,
                                  const OptTensor& sin, const OptTensor& pos, bool interleaved, double eps) {
+  plain_call({&q, &k}, {&wq, &wk, &cos, &sin}, "qk_norm_rope");
   TORCH_CHECK(q.is_cuda(), "q must be on the GPU");
   const bool wanted = at::GradMode::is_enabled() && (q.requires_grad() || k.requires_grad() || (wq.has_value() && wq->requires_grad()) ||
                                                      (wk.has_value() && wk->requires_grad()));

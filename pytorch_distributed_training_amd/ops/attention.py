@@ -80,11 +80,15 @@ def relative_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, bias: 
     the shapes are those of the capture).  As with any operator, let no eager autograd graph of the same leaves live meanwhile:
     their gradients would be accumulated on its stream, outside the capture.
 
+    Forward-mode differentiation, a second derivative and traces are refused.
+
     Returns a contiguous tensor of q's shape and dtype.  Probabilities and their gradients are rounded to q's dtype as
     operands of the matrix products (in fp16 by a power of two above their size, so that small gradients of the output keep
     their digits); scores, softmax statistics and all sums are fp32.  The gradient of ``bias`` is summed in
     fp32 in a fixed order, so it is the same in every run.
     """
+    if torch._C._is_tracing():  # (sizes are tensors there, and bucket_steps() would keep them)
+        raise RuntimeError("relative_attention cannot be traced: a trace would hold its empty output tensor")
     if q.dim() not in (3, 4) or (q.dim() == 3) != (cu_seqlens is not None):
         raise ValueError("q, k, v must be [B, S, heads, dim], or packed [T, heads, dim] with cu_seqlens")
     if cu_seqlens is not None:

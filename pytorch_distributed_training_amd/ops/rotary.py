@@ -37,7 +37,8 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, q_weight: Optional[torch.Tens
     outside the table is clamped into it.  By default a token's position is its place in the sequence ``S`` (or ``T``).
 
     Returns contiguous tensors of the shapes and dtype of q and k.  All arithmetic is fp32, rounded once at the end; the
-    weight gradients are summed in fp32 in a fixed order.
+    weight gradients are summed in fp32 in a fixed order.  Forward-mode differentiation, a second derivative and traces are
+    refused.
     """
     if rope is None and positions is not None:
         raise ValueError("positions mean something only with rope")
