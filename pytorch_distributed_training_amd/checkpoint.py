@@ -17,6 +17,7 @@ from __future__ import annotations
 
 import json
 import os
+from dataclasses import replace
 from typing import Dict, Optional
 
 import torch
@@ -54,7 +55,22 @@ def save_pretrained(model: nn.Module, directory: str, suffix: str = "", write_co
     return path
 
 
-POSITION_PARAMS = (".relative_attention_bias.weight", ".query_norm.weight", ".key_norm.weight")
+TABLE_PARAMS = (".relative_attention_bias.weight",)
+NORM_PARAMS = (".query_norm.weight", ".key_norm.weight")
+
+
+def switched_on(own, saved_cfg: EncoderConfig, cfg: EncoderConfig) -> set:
+    """Those of the parameter names `own` that belong to a position option that `cfg` switches on over `saved_cfg`: weights saved
+    under `saved_cfg` lack them, and they keep the values they are built with - bias tables of zero, which change nothing until
+    they are trained, and norm weights of one, which do normalise every query and key."""
+    fresh = ()
+    if cfg.relative_attention_num_buckets and not saved_cfg.relative_attention_num_buckets:
+        fresh += TABLE_PARAMS
+    if cfg.qk_norm and not saved_cfg.qk_norm:
+        fresh += NORM_PARAMS
+    return {k for k in own if k.endswith(fresh)} if fresh else set()
+
+
 _LEGACY = ((".LayerNorm.gamma", ".LayerNorm.weight"), (".LayerNorm.beta", ".LayerNorm.bias"))
 
 
@@ -81,14 +97,14 @@ def _read_weights(directory: str) -> Dict[str, torch.Tensor]:
     return out
 
 
-def load_state_dict_into(model: nn.Module, sd: Dict[str, torch.Tensor], strict: bool = True):
-    """Copy `sd` into the model's (possibly arena-backed) parameters, then refresh the 16-bit copy."""
+def load_state_dict_into(model: nn.Module, sd: Dict[str, torch.Tensor], strict: bool = True, fresh=()):
+    """Copy `sd` into the model's (possibly arena-backed) parameters, then refresh the 16-bit copy.  `fresh`: parameters that
+    may be missing besides the head's and keep their values (see :func:`switched_on`)."""
     m = _unwrap(model)
     own = dict(m.named_parameters())
     missing = [k for k in own if k not in sd]
     unexpected = [k for k in sd if k not in own]
-    # (the tables and norm weights of the position options start neutral: a checkpoint from before they were switched on may lack them)
-    head_only = all(k.startswith("classifier") or ".pooler." in k or k.endswith(POSITION_PARAMS) for k in missing)
+    head_only = all(k.startswith("classifier") or ".pooler." in k or k in fresh for k in missing)
     if strict and (unexpected or (missing and not head_only)):
         raise KeyError(f"state_dict mismatch: missing {missing[:4]}, unexpected {unexpected[:4]}")
     with torch.no_grad():
@@ -105,14 +121,16 @@ def load_state_dict_into(model: nn.Module, sd: Dict[str, torch.Tensor], strict: 
 
 def load_pretrained(directory: str, num_labels: Optional[int] = None, **overrides) -> nn.Module:
     """``AutoModelForSequenceClassification.from_pretrained(directory)``: config + weights from disk.  A
-    checkpoint without a classification head (pre-training weights) gets a freshly initialised one."""
-    cfg = EncoderConfig.load(directory)
-    if num_labels is not None:
-        cfg.num_labels = num_labels
+    checkpoint without a classification head (pre-training weights) gets a freshly initialised one, and so do the parameters
+    of a position option that `overrides` switch on."""
+    saved = EncoderConfig.load(directory)
+    cfg = replace(saved) if num_labels is None else replace(saved, num_labels=num_labels)
     for k, v in overrides.items():
         setattr(cfg, k, v)
+    cfg.validate()
     model = build_model(cfg)
-    load_state_dict_into(model, _read_weights(directory), strict=True)
+    load_state_dict_into(model, _read_weights(directory), strict=True,
+                         fresh=switched_on(dict(model.named_parameters()), saved, cfg))
     return model
 
 
@@ -121,11 +139,14 @@ def from_transformers(hf_model, **overrides) -> nn.Module:
     reference builds with ``AutoModelForSequenceClassification.from_pretrained``,
     /root/reference/test_data_parallelism.py:112): same configuration, same weights - parameter names are the HF names,
     so the state dict is taken as it is."""
-    cfg = EncoderConfig.from_hf_dict(hf_model.config.to_dict())
+    saved = EncoderConfig.from_hf_dict(hf_model.config.to_dict())
+    cfg = replace(saved)
     for k, v in overrides.items():
         setattr(cfg, k, v)
+    cfg.validate()
     model = build_model(cfg)
-    load_state_dict_into(model, {k: v.detach() for k, v in hf_model.state_dict().items()}, strict=True)
+    load_state_dict_into(model, {k: v.detach() for k, v in hf_model.state_dict().items()}, strict=True,
+                         fresh=switched_on(dict(model.named_parameters()), saved, cfg))
     return model
 
 

@@ -17,6 +17,7 @@ from __future__ import annotations
 
 import os
 import time
+from dataclasses import replace
 from typing import Dict, List, Optional, Tuple
 
 import torch
@@ -41,11 +42,13 @@ def split_layers(num_layers: int, stages: int) -> List[Tuple[int, int]]:
 
 
 def build_stage(model_cfg, stage: int, stages: int, full_state: Optional[Dict[str, torch.Tensor]] = None,
-                seed: Optional[int] = None) -> nn.Module:
+                seed: Optional[int] = None, saved_cfg=None) -> nn.Module:
     """Module of one pipeline stage.  Its initial weights are the corresponding slice of the FULL model
     built from `seed` (or of `full_state`), so a pipelined run starts from the same point as a
-    single-process run - a precondition for matching loss curves."""
-    from ..checkpoint import POSITION_PARAMS
+    single-process run - a precondition for matching loss curves.  `saved_cfg`: the configuration that `full_state` was saved
+    with; parameters of a position option that `model_cfg` switches on over it start as they are built.  Without it an
+    option counts as off there if the state has none of its parameters in any layer."""
+    from ..checkpoint import NORM_PARAMS, TABLE_PARAMS, switched_on
     from ..models.bert import build_model
 
     lo, hi = split_layers(model_cfg.num_hidden_layers, stages)[stage]
@@ -55,8 +58,13 @@ def build_stage(model_cfg, stage: int, stages: int, full_state: Optional[Dict[st
         full_state = build_model(model_cfg).state_dict()
     part = build_model(model_cfg, layer_range=(lo, hi), with_embeddings=stage == 0, with_head=stage == stages - 1)
     own = part.state_dict()
-    # (tables and norm weights of position options that the full state was saved without keep their neutral start)
-    fresh = {k for k in own if k not in full_state and k.endswith(POSITION_PARAMS)}
+    if saved_cfg is None:
+        saved_cfg = replace(model_cfg)
+        if not any(k.endswith(TABLE_PARAMS) for k in full_state):
+            saved_cfg.relative_attention_num_buckets = 0
+        if not any(k.endswith(NORM_PARAMS) for k in full_state):
+            saved_cfg.qk_norm = False
+    fresh = {k for k in switched_on(own, saved_cfg, model_cfg) if k not in full_state}
     missing = [k for k in own if k not in full_state and k not in fresh]
     if missing:
         raise KeyError(f"stage {stage}: parameters missing from the full state dict: {missing[:4]}")
@@ -301,7 +309,8 @@ def run_pipeline_training(rank: int, world_size: int, cfg) -> dict:
     train_dl, eval_dl = model_parallel_loaders(cfg, train_ds, val_ds, collate, mesh, micro_bs * accum)
     set_seed(cfg.seed)
     full_state = ckpt._read_weights(cfg.init_from) if cfg.init_from else None
-    stage_model = build_stage(model_cfg, mesh.stage, 2, full_state, seed=cfg.seed)
+    stage_model = build_stage(model_cfg, mesh.stage, 2, full_state, seed=cfg.seed,
+                              saved_cfg=ckpt.EncoderConfig.load(cfg.init_from) if cfg.init_from else None)
     print(f"[RANK: {rank}] Initialized model (stage {mesh.stage}, replica {mesh.replica}).")
     optimizer = AdamW(params=stage_model.parameters(), lr=cfg.lr, correct_bias=cfg.correct_bias)
     print(f"[RANK: {rank}] Initialized optimizer.")
