@@ -304,6 +304,11 @@ def load_training_state(directory: str, model: nn.Module, optimizer=None, schedu
     if tag is None:
         raise FileNotFoundError(f"no published checkpoint in {directory}")
     sub = os.path.join(directory, f"checkpoint-{tag}")
+    cfg = getattr(_unwrap(model), "config", None)
+    if isinstance(cfg, EncoderConfig) and os.path.exists(os.path.join(sub, "config.json")):
+        saved = EncoderConfig.load(sub).position_fields()  # (a rotation has no weights that would be missing or left over)
+        if saved != cfg.position_fields():
+            raise ValueError(f"the run was saved with the position options {saved}, this model has {cfg.position_fields()}")
     load_state_dict_into(model, load_file(os.path.join(sub, wname)), strict=True)
     state = torch.load(os.path.join(sub, sname), map_location="cpu", weights_only=True)
     opt = getattr(optimizer, "optimizer", optimizer)

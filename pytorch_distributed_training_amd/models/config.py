@@ -50,6 +50,18 @@ class EncoderConfig:
         """Whether the encoder layers use any of the position options (relative bias, query / key norm, rotation)."""
         return bool(self.relative_attention_num_buckets or self.qk_norm or self.rotary_dim)
 
+    def position_fields(self) -> Dict:
+        """The position options that change what a layer computes (those of an option that is off are left out)."""
+        out = {}
+        if self.relative_attention_num_buckets:
+            out.update(relative_attention_num_buckets=self.relative_attention_num_buckets,
+                       relative_attention_max_distance=self.relative_attention_max_distance)
+        if self.qk_norm:
+            out.update(qk_norm=True, qk_norm_eps=self.qk_norm_eps)
+        if self.rotary_dim:
+            out.update(rotary_dim=self.rotary_dim, rotary_base=self.rotary_base)
+        return out
+
     @property
     def dropout_blocks(self) -> int:
         """Rows that the dropout counters set aside for a sample, in blocks of 512: enough for the longest sequence that the

@@ -51,6 +51,19 @@ def test_a_resumed_run_does_not_start_parameters_afresh(tmp_path, name):
         load_training_state(str(tmp_path), _trained())
 
 
+@pytest.mark.parametrize("change", [dict(rotary_dim=0), dict(rotary_dim=64), dict(rotary_base=500.0), dict(qk_norm_eps=1e-3),
+                                    dict(relative_attention_max_distance=60), dict(qk_norm=False), dict(relative_attention_num_buckets=0)])
+def test_a_resumed_run_keeps_its_position_options(tmp_path, change):
+    save_training_state(str(tmp_path), _trained(), extra={"global_step": 3})
+    with pytest.raises(ValueError, match="position options"):
+        load_training_state(str(tmp_path), _trained(**change))
+
+
+def test_options_off_do_not_count():
+    a, b = preset("bert-tiny", relative_attention_max_distance=64, qk_norm_eps=1e-3, rotary_base=5.0), preset("bert-tiny")
+    assert a.position_fields() == b.position_fields() == {}
+
+
 def test_options_are_switched_on_over_a_plain_checkpoint(tmp_path):
     plain = build_model("bert-tiny-nodrop")
     save_pretrained(plain, str(tmp_path))
