@@ -6,7 +6,8 @@ never saves anything, so an elastic restart recomputes from scratch.  Here:
 * :func:`save_pretrained` / :func:`load_pretrained` write / read the HF directory layout
   (``config.json`` + ``model.safetensors``; ``pytorch_model.bin`` is accepted on load with
   ``weights_only=True``).  Parameter names are HF's, so a directory written here loads into
-  ``transformers.BertForSequenceClassification`` and vice versa.  Legacy ``bert.embeddings.position_ids``
+  ``transformers.BertForSequenceClassification`` and vice versa - but for models with position options, which
+  ``transformers`` does not know and leaves out.  Legacy ``bert.embeddings.position_ids``
   buffers and ``LayerNorm.gamma/beta`` spellings are tolerated on load.
 * :func:`save_training_state` / :func:`load_training_state` add the sidecar needed to resume exactly:
   optimizer moments, step count, loss scale, LR-schedule position, epoch / in-epoch batch offset, RNG counters.
@@ -152,10 +153,12 @@ def from_transformers(hf_model, **overrides) -> nn.Module:
 
 def to_transformers(model: nn.Module):
     """The inverse of :func:`from_transformers`: a ``transformers`` model of the matching architecture holding this
-    model's (master, fp32) weights."""
+    model's (master, fp32) weights.  Models with position options are refused."""
+    inner = _unwrap(model)
+    if inner.config.position_ops:
+        raise ValueError(f"transformers' models do not have the position options {inner.config.position_fields()}")
     import transformers
 
-    inner = _unwrap(model)
     hf_cfg = transformers.AutoConfig.for_model(**inner.config.to_hf_dict())
     hf = transformers.AutoModelForSequenceClassification.from_config(hf_cfg)
     missing, unexpected = hf.load_state_dict(_hf_state_dict(model), strict=False)

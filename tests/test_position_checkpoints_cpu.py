@@ -90,3 +90,12 @@ def test_stages_of_a_state_that_lacks_some_layers_are_refused(name, told):
         with pytest.raises(KeyError):
             build_stage(cfg, 0, 2, plain, saved_cfg=cfg)
         build_stage(cfg, 0, 2, plain, saved_cfg=preset("bert-tiny-nodrop"))
+
+
+@pytest.mark.parametrize("change", [dict(rotary_dim=32), dict(qk_norm=True), dict(relative_attention_num_buckets=16)])
+def test_models_with_position_options_are_not_handed_to_transformers(change):
+    """transformers would build the plain architecture and compute something else (a rotation has no weights to be left over)."""
+    from pytorch_distributed_training_amd.checkpoint import to_transformers
+
+    with pytest.raises(ValueError, match="position options"):
+        to_transformers(build_model("bert-tiny-nodrop", **change))
