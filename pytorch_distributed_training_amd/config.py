@@ -97,7 +97,7 @@ class TrainConfig:
         16-GB cards) on the CPU and with ``--compat``; on a GPU as many samples as fit a budget of half the free HBM
         and at most 131072 tokens (the shape the kernels are tuned for), counting a sample at the longest length the
         collator can produce and ~34 bytes of saved activations per token, layer and hidden unit (measured: 106 GB
-        for 131072 tokens of BERT-large).
+        for 131072 tokens of BERT-large; `EncoderConfig.saved_bytes` with the position options).
 
         Free memory is a per-rank reading (a co-tenant, several ranks rehearsing on one card), but the micro-batch
         decides the loaders' batch size, the number of optimizer steps per epoch and the pipeline's message shapes, so
@@ -113,8 +113,8 @@ class TrainConfig:
             import torch
 
             free_bytes, _total = torch.cuda.mem_get_info(device)
-        per_token = 34 * model_cfg.num_hidden_layers * model_cfg.hidden_size
         seq = self.max_length or model_cfg.max_position_embeddings
+        per_token = model_cfg.saved_bytes(seq) * model_cfg.num_hidden_layers * model_cfg.hidden_size
         tokens = min(131072, int(0.5 * free_bytes) // per_token)
         cap = max(8, tokens // max(1, seq))
         agreed = agree_min(cap, device if hasattr(device, "index") else None)

@@ -62,6 +62,12 @@ class EncoderConfig:
             out.update(rotary_dim=self.rotary_dim, rotary_base=self.rotary_base)
         return out
 
+    def saved_bytes(self, seq: int) -> int:
+        """Bytes that a layer's forward keeps for its backward, per token and hidden unit: 34, with normalised or rotated queries
+        and keys 4 more, and with any position option beyond 128 tokens 2 for the low part of the attention's output and one for
+        the far shares of its rows (8 bytes for each head of 64)."""
+        return 34 + (4 if self.qk_norm or self.rotary_dim else 0) + (3 if self.position_ops and seq > 128 else 0)
+
     @property
     def dropout_blocks(self) -> int:
         """Rows that the dropout counters set aside for a sample, in blocks of 512: enough for the longest sequence that the
