@@ -11,6 +11,7 @@ from . import native
 
 MAX_BUCKETS = 128
 MAX_DISTANCE = 512
+MASK_DTYPES = (torch.bool, torch.uint8, torch.int32)  # read in place; other whole numbers are compared with 0 first
 
 
 @functools.lru_cache(maxsize=None)
@@ -48,7 +49,7 @@ def relative_bucket(distance: torch.Tensor, num_buckets: int, max_distance: int)
 
 def mask_bits(key_mask: torch.Tensor) -> torch.Tensor:
     """A key mask ``[B, S]`` as the kernels read it: one bit per key, int64 ``[B, ceil(S / 64)]``."""
-    if key_mask.dtype == torch.int64:
+    if key_mask.dtype not in MASK_DTYPES:
         key_mask = key_mask.ne(0)
     return native().rel_mask_bits(key_mask)
 
@@ -99,9 +100,9 @@ def relative_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, bias: 
     elif key_mask is not None:
         if tuple(key_mask.shape) != tuple(q.shape[:2]):
             raise ValueError(f"key_mask must be [B, S] = {tuple(q.shape[:2])}, got {tuple(key_mask.shape)}")
-        if key_mask.is_floating_point():
+        if key_mask.is_floating_point() or key_mask.is_complex():
             raise ValueError("key_mask holds truth values (non-zero = attended), not additive scores")
-        if key_mask.dtype == torch.int64:
+        if key_mask.dtype not in MASK_DTYPES:
             key_mask = key_mask.ne(0)
     steps: Tuple[int, ...] = ()
     if bias is not None:
