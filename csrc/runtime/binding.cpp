@@ -482,7 +482,7 @@ PdtRelAttn rel_args(const Tensor& q, const Tensor& k, const Tensor& v, const Ten
       a.steps[i] = (int)c.steps[i];
     }
   }
-  TORCH_CHECK(std::isfinite(c.scale) && c.scale != 0.0, "scale must be finite and not zero");
+  TORCH_CHECK(std::abs(c.scale) >= 0x1p-64 && std::abs(c.scale) <= 0x1p64, "the size of scale must be from 2^-64 to 2^64");
   a.scale = (float)c.scale;
   a.drop_thr = thr16(c.p);
   a.drop_scale = keep_scale(c.p);

@@ -74,6 +74,8 @@ def relative_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, bias: 
     whatever its row holds (infinities and NaN included) and gets zero gradients.  A query without any attended key has a
     zero output and no gradient.  An additive float mask is refused.
 
+    ``scale`` (``1 / sqrt(dim)`` by default): not zero, of a size from 2^-64 to 2^64.
+
     ``dropout_p`` (at most 0.99) with ``rng`` (an :class:`~.fused.RngKey`) and ``site``: dropout on the probabilities with the framework's
     counter-based masks.
 
@@ -119,8 +121,8 @@ def relative_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, bias: 
         raise ValueError("dropout needs rng, the key of the forward pass")
     if scale is None:
         scale = 1.0 / math.sqrt(q.shape[-1])
-    if not math.isfinite(scale) or scale == 0.0:
-        raise ValueError("scale must be finite and not zero")
+    if not 2.0 ** -64 <= abs(scale) <= 2.0 ** 64:  # (fp32 holds the scale, its reciprocal and their products with the scores)
+        raise ValueError(f"the size of scale must be from 2^-64 to 2^64 (got {scale})")
     state, micro, sids = (rng.state, rng.counter, rng.sample_ids) if dropout_p > 0.0 else (None, 0, None)
     return native().relative_attention(q, k, v, bias, max_distance, steps, key_mask, cu_seqlens, int(max_seqlen or 0), scale, state,
                                        dropout_p, micro, site, sids)

@@ -25,3 +25,42 @@ def test_complex_masks_are_refused():
     q = torch.zeros(1, 4, 2, 64, dtype=torch.float16)
     with pytest.raises(ValueError, match="truth values"):
         relative_attention(q, q, q, key_mask=torch.ones(1, 4, dtype=torch.complex64))
+
+
+@pytest.mark.parametrize("scale", [1e-20, -1e-20, 1e-40, 1e-60, 1e20, -1e30, 1e39, math.nan])
+def test_scales_that_fp32_cannot_work_with_are_refused(scale):
+    q = torch.zeros(1, 4, 2, 64, dtype=torch.float16)
+    with pytest.raises(ValueError, match="scale"):
+        relative_attention(q, q, q, scale=scale)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("S", [60, 300])
+@pytest.mark.parametrize("a,b", [(-30, -33), (20, 20), (-64, 3)])
+def test_scales_of_either_end(S, a, b):
+    """Powers of two moved between q, k and the scale change no digit of the scores (bf16 and fp32 hold all of them)."""
+    gen = torch.Generator(device="cuda").manual_seed(S)
+    q, k, v = (torch.randn(2, S, 2, 64, generator=gen, device="cuda").bfloat16().requires_grad_() for _ in range(3))
+    bias = torch.randn(32, 2, generator=gen, device="cuda").requires_grad_()
+    dout = torch.randn(2, S, 2, 64, generator=gen, device="cuda").bfloat16()
+    want = relative_attention(q, k, v, bias, scale=0.125)
+    ref = torch.autograd.grad(want, (q, k, v, bias), dout)
+    x = [(q.detach().double() * 2.0 ** a).bfloat16().requires_grad_(), (k.detach().double() * 2.0 ** b).bfloat16().requires_grad_(), v, bias]
+    out = relative_attention(*x, scale=2.0 ** (-3 - a - b))
+    got = torch.autograd.grad(out, x, dout)
+    torch.testing.assert_close(out, want, rtol=2 ** -7, atol=1e-6)
+    for g, w, e in zip(got, ref, (a, b, 0, 0)):
+        d = (g.double() * 2.0 ** e - w.double()).norm() / w.double().norm()
+        assert d < 2 ** -8, float(d)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("sign", [1, -1])
+def test_the_smallest_scale_leaves_the_table(sign):
+    S = 200
+    gen = torch.Generator(device="cuda").manual_seed(S)
+    q, k, v = (torch.randn(1, S, 2, 64, generator=gen, device="cuda").half() for _ in range(3))
+    bias = torch.randn(32, 2, generator=gen, device="cuda") * 5
+    a = relative_attention(q, k, v, bias, scale=sign * 2.0 ** -64)
+    b = relative_attention(torch.zeros_like(q), k, v, bias)
+    assert torch.isfinite(a).all() and (a.float() - b.float()).abs().max() <= 2e-3 * v.abs().max()
