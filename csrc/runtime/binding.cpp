@@ -508,12 +508,14 @@ Tensor rel_mask_bits(const Tensor& mask) {
                             reinterpret_cast<uint64_t*>(bits.data_ptr<int64_t>()), cur_stream()), "rel_attn_mask");
   return bits;
 }
-PdtRng rel_rng(const OptTensor& state, double p, int64_t micro, int64_t site, const OptTensor& sids, int64_t B) {
+PdtRng rel_rng(const OptTensor& state, double p, int64_t micro, int64_t site, const OptTensor& sids, int64_t B, const Tensor& q) {
   if (p <= 0.0 || !state.has_value()) {
     TORCH_CHECK(p <= 0.0, "dropout needs a generator state");
     return PdtRng{nullptr, 0, 0, nullptr, 1u, 0u, nullptr};
   }
   TORCH_CHECK(p <= 0.99, "the dropout probability must be at most 0.99");  // (16-bit probabilities divided by the share kept)
+  same_gpu(*state, q, "the generator state");
+  if (sids.has_value()) same_gpu(*sids, q, "sample_ids");
   // (the masks derive from (sample, head, query, key): the sequence length plays no part)
   return make_rng(*state, micro, site, sids, 1, B);
 }
@@ -540,7 +542,7 @@ std::vector<Tensor> rel_attn_forward(const Tensor& q_in, const Tensor& k_in, con
   Tensor o = at::empty(q.sizes(), q.options());
   const RelCall c{table, bits, cu, steps, max_distance, max_seqlen, scale, p};
   PdtRelAttn a = rel_args(q, k, v, o, c, PdtRng{});
-  a.rng = rel_rng(rng_state, p, micro, site, sids, a.B);
+  a.rng = rel_rng(rng_state, p, micro, site, sids, a.B, q);
   if (q.numel() == 0) return {o, want_lse ? at::empty({a.B, a.A, a.S}, q.options().dtype(at::kFloat)) : Tensor(), Tensor()};
   Tensor lse, low;
   if (want_lse) {
@@ -615,7 +617,7 @@ std::vector<Tensor> rel_attn_backward(const Tensor& dout, const Tensor& q_in, co
   }
   if (want_dtable) dtable = at::empty(table->sizes(), table->options());
   const RelCall c{table, bits, cu, steps, max_distance, max_seqlen, scale, p};
-  rel_attn_backward_into(dout, q, k, v, o, low.has_value() ? *low : Tensor(), lse, c, rel_rng(rng_state, p, micro, site, sids, lse.size(-3)), dq, dk, dv,
+  rel_attn_backward_into(dout, q, k, v, o, low.has_value() ? *low : Tensor(), lse, c, rel_rng(rng_state, p, micro, site, sids, lse.size(-3), q), dq, dk, dv,
                          grad_out(dtable));
   return {dq, dk, dv, dtable};
 }

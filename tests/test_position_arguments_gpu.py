@@ -64,3 +64,19 @@ def test_the_smallest_scale_leaves_the_table(sign):
     a = relative_attention(q, k, v, bias, scale=sign * 2.0 ** -64)
     b = relative_attention(torch.zeros_like(q), k, v, bias)
     assert torch.isfinite(a).all() and (a.float() - b.float()).abs().max() <= 2e-3 * v.abs().max()
+
+
+@pytest.mark.gpu
+def test_generator_states_of_another_device_are_refused():
+    from pytorch_distributed_training_amd.ops.fused import RngKey
+
+    q = torch.zeros(1, 4, 2, 64, dtype=torch.float16, device="cuda")
+    state = torch.zeros(2, dtype=torch.int64, device="cuda")
+    with pytest.raises(RuntimeError, match="rng state|device of q"):
+        relative_attention(q, q, q, dropout_p=0.1, rng=RngKey(state.cpu(), 0, None))
+    with pytest.raises(RuntimeError, match="device of q"):
+        relative_attention(q, q, q, dropout_p=0.1, rng=RngKey(state, 0, torch.zeros(1, dtype=torch.int32)))
+    if torch.cuda.device_count() > 1:
+        other = RngKey(state.to("cuda:1"), 0, None)
+        with pytest.raises(RuntimeError, match="device of q"):
+            relative_attention(q, q, q, dropout_p=0.1, rng=other)
