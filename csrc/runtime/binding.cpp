@@ -395,6 +395,11 @@ Tensor head_rows(const Tensor& t, const char* name) {
     ok = ok && (t.size(i) <= 1 || (t.stride(i) % 8 == 0 && t.stride(i) >= 0 && (i != t.dim() - 3 || t.stride(i) <= (1 << 23))));
   return ok ? t : t.clone(at::MemoryFormat::Contiguous);
 }
+// weights, tables, positions and borders as the kernels read them: contiguous and on the 16-byte grid, copied if they are not
+OptTensor dense(const OptTensor& t) {
+  if (!t.has_value() || (t->is_contiguous() && (!t->has_storage() || (reinterpret_cast<uintptr_t>(t->data_ptr()) & 15) == 0))) return t;
+  return t->clone(at::MemoryFormat::Contiguous);
+}
 PdtRelView rel_view(const Tensor& t) {
   const int64_t d = t.dim();
   auto st = [&](int64_t i) { return t.size(i) <= 1 ? (int64_t)0 : t.stride(i); };
@@ -656,10 +661,11 @@ struct RelAttnNode : public torch::autograd::Function<RelAttnNode> {
 };
 // `key_mask`: [B, S] as key_mask_tensor() takes it
 Tensor relative_attention(const Tensor& q, const Tensor& k, const Tensor& v, const OptTensor& table, int64_t max_distance,
-                          const std::vector<int64_t>& steps, const OptTensor& key_mask, const OptTensor& cu, int64_t max_seqlen,
+                          const std::vector<int64_t>& steps, const OptTensor& key_mask, const OptTensor& cu_in, int64_t max_seqlen,
                           double scale, const OptTensor& rng_state, double p, int64_t micro, int64_t site, const OptTensor& sids) {
   plain_call({&q, &k, &v}, {&table}, "relative_attention");
   TORCH_CHECK(q.is_cuda(), "q must be on the GPU");
+  const OptTensor cu = cu_in.has_value() && !cu_in->is_contiguous() ? OptTensor(cu_in->contiguous()) : cu_in;
   OptTensor bits;
   if (key_mask.has_value()) {
     same_gpu(*key_mask, q, "key_mask");
@@ -804,10 +810,11 @@ struct QkRopeNode : public torch::autograd::Function<QkRopeNode> {
     return out;
   }
 };
-std::vector<Tensor> qk_norm_rope(const Tensor& q, const Tensor& k, const OptTensor& wq, const OptTensor& wk, const OptTensor& cos,
-                                 const OptTensor& sin, const OptTensor& pos, bool interleaved, double eps) {
-  plain_call({&q, &k}, {&wq, &wk, &cos, &sin}, "qk_norm_rope");
+std::vector<Tensor> qk_norm_rope(const Tensor& q, const Tensor& k, const OptTensor& wq_in, const OptTensor& wk_in, const OptTensor& cos_in,
+                                 const OptTensor& sin_in, const OptTensor& pos_in, bool interleaved, double eps) {
+  plain_call({&q, &k}, {&wq_in, &wk_in, &cos_in, &sin_in}, "qk_norm_rope");
   TORCH_CHECK(q.is_cuda(), "q must be on the GPU");
+  const OptTensor wq = dense(wq_in), wk = dense(wk_in), cos = dense(cos_in), sin = dense(sin_in), pos = dense(pos_in);
   const bool wanted = at::GradMode::is_enabled() && (q.requires_grad() || k.requires_grad() || (wq.has_value() && wq->requires_grad()) ||
                                                      (wk.has_value() && wk->requires_grad()));
   if (!wanted) return qk_rope_forward(q, k, wq, wk, cos, sin, pos, interleaved, eps);

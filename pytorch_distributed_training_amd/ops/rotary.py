@@ -27,7 +27,7 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, q_weight: Optional[torch.Tens
 
     ``q``, ``k``: fp16 or bf16 ``[B, S, heads, dim]`` or ``[T, heads, dim]``, ``dim`` a multiple of 8 up to 256; they may
     differ in the number of heads.  Views into a fused projection are read in place (unit inner stride, other strides
-    multiples of 8 elements, 16-byte aligned - anything else is copied first).
+    multiples of 8 elements, 16-byte aligned - anything else, here and below, is copied first).
 
     ``q_weight``, ``k_weight``: ``[dim]``, fp32 or of q's dtype, shared by the heads of a side; without them there is no norm.
 

@@ -80,3 +80,31 @@ def test_generator_states_of_another_device_are_refused():
         other = RngKey(state.to("cuda:1"), 0, None)
         with pytest.raises(RuntimeError, match="device of q"):
             relative_attention(q, q, q, dropout_p=0.1, rng=other)
+
+
+@pytest.mark.gpu
+def test_weights_tables_positions_and_borders_of_any_layout():
+    gen = torch.Generator(device="cuda").manual_seed(0)
+    B, S, A, D = 3, 20, 2, 64
+    q, k, v = (torch.randn(B, S, A, D, generator=gen, device="cuda").half().requires_grad_() for _ in range(3))
+    w = [torch.rand(D, generator=gen, device="cuda").add(0.5).requires_grad_() for _ in range(2)]
+    from pytorch_distributed_training_amd.ops import qk_norm_rope, rotary_table
+
+    cos, sin = rotary_table(100, D)
+    pos = torch.arange(S, device="cuda")[None] + 5
+
+    def run(w, rope, pos):
+        y = qk_norm_rope(q, k, *w, rope=rope, positions=pos)
+        return (*y, *torch.autograd.grad(y, (q, k, *w), [torch.ones_like(t) for t in y]))
+
+    want = run(w, (cos, sin), pos.repeat(B, 1))
+    spread = [t.detach().repeat_interleave(3)[::3].requires_grad_() for t in w]
+    shifted = [torch.cat([t.detach()[:1], t.detach()])[1:].requires_grad_() for t in w]  # (off the 16-byte grid)
+    wide = [torch.cat([t, t], 1)[:, :D // 2] for t in (cos, sin)]
+    for args in ((w, (cos, sin), pos.expand(B, S)), (spread, (cos, sin), pos.repeat(B, 2)[:, :S]), (shifted, wide, pos.repeat(B, 1)),
+                 (w, [torch.cat([t.flatten()[:1], t.flatten()])[1:].view(t.shape) for t in (cos, sin)], pos.repeat(B, 1))):
+        assert all(torch.equal(a, b) for a, b in zip(run(*args), want))
+    rows = [t.detach().reshape(B * S, A, D) for t in (q, k, v)]
+    cu = torch.tensor([0, 7, 30, 60], dtype=torch.int32, device="cuda")
+    want = relative_attention(*rows, cu_seqlens=cu, max_seqlen=30)
+    assert torch.equal(relative_attention(*rows, cu_seqlens=cu.repeat_interleave(2)[::2], max_seqlen=30), want)
