@@ -287,6 +287,7 @@ static int qr_launch(const PdtQkRope& p, bool bwd, float* partial, hipStream_t s
     else if (mode == 1) hipLaunchKernelGGL((qk_rope_bwd_kernel<T, L, 1>), grid, dim3(64 * QR_WAVES), 0, st, p, gt, partial);
     else hipLaunchKernelGGL((qk_rope_bwd_kernel<T, L, 2>), grid, dim3(64 * QR_WAVES), 0, st, p, gt, partial);
   } else {
+    if ((int64_t)qr_blocks_for(p) * 64 * QR_WAVES > 0xFFFFFFFFll) return -3;  // (a launch counts its threads in 32 bits)
     const dim3 grid(qr_blocks_for(p));
     if (mode == 0) hipLaunchKernelGGL((qk_rope_fwd_kernel<T, L, 0>), grid, dim3(64 * QR_WAVES), 0, st, p, gt);
     else if (mode == 1) hipLaunchKernelGGL((qk_rope_fwd_kernel<T, L, 1>), grid, dim3(64 * QR_WAVES), 0, st, p, gt);

@@ -1374,8 +1374,12 @@ static int ra_rows(const PdtRelAttn& p, int which) {
 
 static size_t ra_bias_bytes(const PdtRelAttn& p) { return (size_t)4 * ra_bias_len(p.max_distance) * sizeof(float); }
 
+// (a launch counts its threads along x in 32 bits)
+static bool ra_too_many(const PdtRelAttn& p, int threads) { return (int64_t)p.B * p.A * threads > 0xFFFFFFFFll; }
+
 template <typename KernT>
 static int ra_launch(KernT kern, const PdtRelAttn& p, int rows_per_block, size_t lds, hipStream_t stream) {
+  if (ra_too_many(p, RA_THREADS)) return -3;
   if (int e = ra_allow_lds((const void*)kern, lds)) return e;
   hipLaunchKernelGGL(kern, dim3(p.B * p.A, (p.S + rows_per_block - 1) / rows_per_block), dim3(RA_THREADS), lds, stream, p);
   return (int)hipGetLastError();
@@ -1390,6 +1394,7 @@ static int ra_launch_short(const PdtRelAttn& p, hipStream_t st) {
   static_assert((size_t)4 * W * (2 * R + 16) * sizeof(float) <= (size_t)4 * (R / RA_CHUNK) * NH * RA_IMG, "diagonal sums reuse the images");
   const size_t lds = work + (size_t)4 * ra_bias_len(p.max_distance < 128 ? p.max_distance : 128) * sizeof(float) + W * sizeof(uint32_t);
   auto kern = rel_attn_bwd_short_kernel<T, KS, W, DROP>;
+  if (ra_too_many(p, 64 * W)) return -3;
   if (int e = ra_allow_lds((const void*)kern, lds)) return e;
   hipLaunchKernelGGL(kern, dim3(p.B * p.A), dim3(64 * W), lds, st, p);
   return (int)hipGetLastError();

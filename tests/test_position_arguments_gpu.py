@@ -108,3 +108,14 @@ def test_weights_tables_positions_and_borders_of_any_layout():
     cu = torch.tensor([0, 7, 30, 60], dtype=torch.int32, device="cuda")
     want = relative_attention(*rows, cu_seqlens=cu, max_seqlen=30)
     assert torch.equal(relative_attention(*rows, cu_seqlens=cu.repeat_interleave(2)[::2], max_seqlen=30), want)
+
+
+@pytest.mark.gpu
+def test_more_heads_than_a_launch_holds_are_refused():
+    """Expanded rows: the grid of (sample, head) pairs passes 2^32 threads while the output is 270 MB."""
+    one = torch.zeros(1, 1, 16, 8, dtype=torch.float16, device="cuda")
+    q = one.expand((1 << 20) + 1, 1, 16, 8)
+    with pytest.raises(RuntimeError, match="argument check"):
+        relative_attention(q, q, q)
+    q = one.expand(1 << 19, 1, 16, 8)
+    assert relative_attention(q, q, q).abs().max() == 0
