@@ -46,9 +46,9 @@ def _sources():
     return hip, cpp, hdr
 
 
-# the attention kernels write their fp32 math as explicit vector operations; the SLP vectoriser on top of that pairs up the
-# scalar adds of the DPP row reductions (v_mov_b32_dpp + v_pk_add_f32, 6 instructions per 4 values and step) where the
-# un-paired adds fold into v_add_f32_dpp (4 instructions)
+# the attention kernels write their fp32 math as explicit vector operations.  With packed fp32 instructions the SLP vectoriser
+# would pair up the scalar adds of the DPP row reductions on top of that (v_mov_b32_dpp + v_pk_add_f32 instead of v_add_f32_dpp);
+# without them, as built here, both settings give the same instructions but for the order of some conversions
 # rel_attention.hip: matrix products accumulate in ordinary registers (the other form moves every accumulator that is not a
 # pure sum through v_accvgpr_read / write: 416 of 2726 instructions of the forward kernel)
 PER_SOURCE_FLAGS = {"attention.hip": ["-fno-slp-vectorize"],

@@ -241,7 +241,7 @@ __global__ __launch_bounds__(ATT_THREADS) PDT_ATT_FWD_OCC void attn_fwd_kernel(A
         if (FULL || pb < nb) {
 #pragma unroll
           for (int hb = 0; hb < 2; ++hb) {
-            float4v p = packed4(s[2 * pb + hb] + nm4);
+            float4v p = s[2 * pb + hb] + nm4;
 #pragma unroll
             for (int r = 0; r < 4; ++r) p[r] = __builtin_amdgcn_exp2f(p[r]);
             l4 += p;
@@ -344,7 +344,7 @@ __global__ __launch_bounds__(ATT_THREADS) void attn_bwd_dq_kernel(AttnArgs a, fl
           dp = Half16<T>::mfma(row_frag(vimg, kb16, 0, lane), df0, dp);
           dp = Half16<T>::mfma(row_frag(vimg, kb16, 1, lane), df1, dp);
           const float4v mb = *reinterpret_cast<const float4v*>(mbias + c0 + kb16 + 4 * g);
-          float4v ps = packed4(sc * k2v + (mb + nlse4));
+          float4v ps = sc * k2v + (mb + nlse4);
 #pragma unroll
           for (int r = 0; r < 4; ++r) ps[r] = __builtin_amdgcn_exp2f(ps[r]);
           float4v e = dp + nd4;
@@ -458,7 +458,7 @@ __global__ __launch_bounds__(ATT_THREADS) void attn_bwd_dkv_kernel(AttnArgs a, f
             const float4v ls = *reinterpret_cast<const float4v*>(lse_s + c0 + q16 + 4 * g);
             const float4v nde = *reinterpret_cast<const float4v*>(del_s + c0 + q16 + 4 * g);
             const uint4v sd = *reinterpret_cast<const uint4v*>(seed_s + c0 + q16 + 4 * g);
-            float4v p = packed4(sc * k2v + (mb4 + ls));
+            float4v p = sc * k2v + (mb4 + ls);
 #pragma unroll
             for (int r = 0; r < 4; ++r) p[r] = __builtin_amdgcn_exp2f(p[r]);
             float4v pd = p, e = dp * a.scale + nde;
@@ -648,7 +648,7 @@ void attn_bwd_fused128_kernel(AttnArgs a, float* __restrict__ dbias) {
           dp = Half16<T>::mfma(row_frag(img1, kb16, 0, lane), df0, dp);
           dp = Half16<T>::mfma(row_frag(img1, kb16, 1, lane), df1, dp);
           const float4v mb = *reinterpret_cast<const float4v*>(mbias + kb16 + 4 * g);
-          float4v ps = packed4(sc * k2v + (mb + nlse4));
+          float4v ps = sc * k2v + (mb + nlse4);
 #pragma unroll
           for (int r = 0; r < 4; ++r) ps[r] = __builtin_amdgcn_exp2f(ps[r]);
           float4v e = dp + nd4;
@@ -719,7 +719,7 @@ void attn_bwd_fused128_kernel(AttnArgs a, float* __restrict__ dbias) {
           const float4v ls = *reinterpret_cast<const float4v*>(lse_s + q16 + 4 * g);
           const float4v nde = *reinterpret_cast<const float4v*>(del_s + q16 + 4 * g) * (-a.scale);
           const uint4v sd = *reinterpret_cast<const uint4v*>(seed_s + q16 + 4 * g);
-          float4v p = packed4(sc * k2v + (mb4 + ls));
+          float4v p = sc * k2v + (mb4 + ls);
 #pragma unroll
           for (int r = 0; r < 4; ++r) p[r] = __builtin_amdgcn_exp2f(p[r]);
           float4v pd = p, e = dp * a.scale + nde;

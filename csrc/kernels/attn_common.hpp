@@ -31,9 +31,7 @@ __device__ __forceinline__ uint32_t attn_thr_hi(uint32_t thr) { return (thr > 65
 // maximum, dropout factor, dS = P * (dP - delta)).  The build switches packed fp32 instructions off (build_ext.py), so an
 // operation on 4-vectors is four scalar ones; with them on, the same kernels took the same time (forward 251 / 251 us,
 // fused backward 584 / 584 us at batch 1024, both builds in turn).  Pairs of results are converted with one
-// v_cvt_pk_f16_f32 / v_cvt_pk_bf16_f32.  Only exp2 and the dropout hash stay per element.  (The attention files are built
-// without the SLP vectoriser, see build_ext.py: it would also pair up the adds of the DPP row reductions, which then cost a
-// v_mov_b32_dpp each instead of folding into v_add_f32_dpp.)
+// v_cvt_pk_f16_f32 / v_cvt_pk_bf16_f32.
 typedef float float2v __attribute__((ext_vector_type(2)));
 template <typename T> struct Pk2;
 template <> struct Pk2<_Float16> { typedef _Float16 type __attribute__((ext_vector_type(2))); };
@@ -43,16 +41,6 @@ __device__ __forceinline__ int cvt_pk(float lo, float hi) {  // two fp32 -> one 
   return __builtin_bit_cast(int, __builtin_convertvector(float2v{lo, hi}, typename Pk2<T>::type));
 }
 __device__ __forceinline__ float4v splat4(float v) { return float4v{v, v, v, v}; }
-// A 4-vector whose elements are consumed one by one (exp2 of each) would be taken apart by the optimiser BEFORE the
-// operation that produced it ("extract of a vector op = scalar op of the extracts"), i.e. four v_sub_f32 instead of two
-// v_pk_add_f32.  Passing the two halves through an empty asm statement as 64-bit operands keeps the producing operation
-// packed; it emits nothing.
-__device__ __forceinline__ float4v packed4(float4v v) {
-  float2v lo = {v[0], v[1]}, hi = {v[2], v[3]};
-  asm("" : "+v"(lo));
-  asm("" : "+v"(hi));
-  return float4v{lo[0], lo[1], hi[0], hi[1]};
-}
 template <typename T>
 __device__ __forceinline__ short8 pack_pair(const float4v& a, const float4v& b) {
   const int4v r = {cvt_pk<T>(a[0], a[1]), cvt_pk<T>(a[2], a[3]), cvt_pk<T>(b[0], b[1]), cvt_pk<T>(b[2], b[3])};
