@@ -20,14 +20,21 @@
 // the B operand of the next product; rows come through LDS in chunks of 64, double-buffered, filled by LDS-DMA.  A row
 // that no query may attend to is read as zeros: whatever its memory holds, NaN included, never meets a product.
 //
+// P and dS enter the products as 16-bit operands, the one place where something is rounded before the results are.  A second
+// operand with what that leaves would make 13 products of a training pass's 9; without it the results are off by 2.4e-3 of their
+// norm in bf16 and 2.9e-4 in fp16, where rounding the results alone leaves 1.7e-3 and 2.1e-4.
+//
 // Measured, forward / dQ / dK and dV (short: one backward kernel), us and the rate of the products that are wanted:
-//   1 x 17, 12 heads of 64          5.9                     a launch
-//   32 x 128, 16 heads              11.4                    a launch, then waves waiting for their rows
-//   256 x 128, 16 heads, fp16       53 / 133                memory and its latency: the four and eight arrays once are 104 together
-//   32 x 512, 12 heads, bf16        49 / 73 / 68            rounds of workgroups; masks and near tiles in every chunk
-//   2 x 4096, 16 heads, bf16        190 / 240 / 262         0.7, 0.85 and 1.0 PFLOP/s: LDS reads, exp2 and products share the issue
-//   1 x 8191, 12 heads, bf16        250 forward             0.82 PFLOP/s
-//   4 x 1001, 8 heads of 128, holes 40 / 56 / 46            less than two workgroups per CU
+//   1 x 17, 12 heads of 64          6.5                     a launch
+//   32 x 128, 16 heads              11.1                    a launch, then waves waiting for their rows
+//   256 x 128, 16 heads, fp16       53-63 / 135             memory and its latency: the four and eight arrays once are 104 together
+//   32 x 512, 12 heads, bf16        49 / 74 / 69            rounds of workgroups; masks and near tiles in every chunk
+//   2 x 4096, 16 heads, bf16        190 / 239 / 266         0.7, 0.85 and 1.0 PFLOP/s: LDS reads, exp2 and products share the issue, and
+//                                                           1024 workgroups make a round and a third of the 768 places of the first two
+//   1 x 8191, 12 heads, bf16        254 forward             0.82 PFLOP/s, one whole round
+//   4 x 1001, 8 heads of 128, holes 39 / 57 / 46            every chunk is masked: tiles read bias and mask from LDS also far out
+// With dropout 0.1: 256 x 128 without a mask, fp16 77 / 155 -> 82 / 203, bf16 72 / 142 -> 77 / 178; 32 x 512 51 / 78 / 70 -> 60 / 97 / 83;
+// 2 x 4096 188 / 239 / 267 -> 239 / 328 / 352 (a hash and a select per score, and registers that spill, see below).
 #include <mutex>
 #include <type_traits>
 #include <unordered_set>
@@ -43,8 +50,10 @@ constexpr int RA_MAX_FAR = 512;                 // largest max_distance
 constexpr int RA_MAX_STEPS = 32;                // logarithmic buckets per side
 constexpr float RA_SLACK = 8.0f, RA_SLACK_DROP = 4.0f;  // (with dropout p is divided by the share kept as well)
 // Waves per SIMD that the register allocation of a kernel with QB blocks of KS 32-column steps must allow.  At QB KS = 4:
-// forward and dQ 3 (166 registers; dQ with 2: 83 instead of 75 us at 32 x 512 tokens, 12 heads), dK / dV 2 (with 3 it spills: 86
-// instead of 73 us).
+// forward and dQ 3 (dQ with 2: 83 instead of 75 us at 32 x 512 tokens, 12 heads), dK / dV 2 (with 3 86 instead of 73 us).  Three
+// waves leave 168 registers, which hold the forward (154) but not all of dQ in its 128-row shape: 9 (fp16) and 10 (bf16) go to
+// scratch.  With dropout it spills 14 and 16, the 64-row shape 13 and 11, the forward 2; the 128-row short
+// backward, at 128 registers, 23 and 18.  The limits were chosen without dropout.
 #define RA_OCC_FWD __attribute__((amdgpu_waves_per_eu(KS * QB <= 4 ? 3 : 2, 8)))
 #define RA_OCC_DQ __attribute__((amdgpu_waves_per_eu(KS * QB <= 4 ? 3 : 2, 8)))
 #define RA_OCC_DKV __attribute__((amdgpu_waves_per_eu(KS * QB <= 2 ? 3 : 2, 8)))
@@ -1362,7 +1371,9 @@ static int ra_allow_lds(const void* kern, size_t bytes) {
 // with 32 rows each.  64 rows: two pairs of waves, a pair shares 32 rows and splits every chunk - up to half as slow again per
 // row in long sequences (2 x 4096 tokens, 16 heads: forward 231 against 189 us), but sequences of up to 64 rows keep all waves
 // busy, and small batches reach more CUs (12 heads, 1 x 300 tokens: backward 29.5 against 35.0 us, 1 x 2000: 100 against
-// 119 us).  Compared by rounds over the `slots` workgroups that run at a time.
+// 119 us).  Compared by rounds over the `slots` workgroups that run at a time: those of the default max_distance of 128.  The
+// arrays of dQ take 96 bytes more per unit of distance; at 512 one of its workgroups fills a CU (32 x 512 tokens, 12 heads: 183
+// instead of 78 us; forward and dK / dV stay), which this rule does not weigh.
 enum { RA_FWD, RA_DQ, RA_DKV, RA_SHORT };
 static int ra_rows(const PdtRelAttn& p, int which) {
   const int64_t len = p.cu ? (p.B ? p.T / p.B : 0) : p.S;  // (packed: the average)

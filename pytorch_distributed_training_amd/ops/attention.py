@@ -65,7 +65,8 @@ def relative_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, bias: 
     anything else is copied first).  With ``cu_seqlens`` (int32 ``[B + 1]`` on the GPU, ascending from 0) they are the packed rows
     ``[T, heads, dim]`` of sequences of different lengths instead, ``max_seqlen`` the longest of them; rows from
     ``cu_seqlens[-1]`` on belong to no sequence, their outputs and gradients are zero.  So are those of rows beyond
-    ``max_seqlen`` in a sequence that is longer after all: the sequence is cut there.
+    ``max_seqlen`` in a sequence that is longer after all: the sequence is cut there.  Memory for row statistics and the number of
+    workgroups grow with the number of sequences times ``max_seqlen``.
 
     ``bias``: ``[buckets, heads]``, fp32 or of q's dtype; ``None`` leaves it out.  ``max_distance`` (at most 512): where the
     last bucket of each side begins at the latest, see :func:`bucket_steps`.
