@@ -137,3 +137,72 @@ def test_layer_gradients_do_not_carry_the_rounding_of_the_output(S, packed, node
         if n.endswith(("self.query.weight", "self.query.bias", "relative_attention_bias.weight")):
             err = ((named[n].grad.float() - p.grad).norm() / p.grad.norm()).item()
             assert err < 0.25, (n, err)
+
+
+@pytest.mark.parametrize("S,positions", [(64, 512), (200, 512), (600, 1024)])
+def test_graphed_steps_of_position_models_match_eager(S, positions):
+    """Captured training steps, replayed, against eager ones (the tolerance of the same test without position options); with
+    dropout every replay draws new masks."""
+    from pytorch_distributed_training_amd.data.synthetic import fixed_batch
+    from pytorch_distributed_training_amd.engine import Engine
+    from pytorch_distributed_training_amd.models.bert import build_model
+    from pytorch_distributed_training_amd.optim import AdamW
+    from pytorch_distributed_training_amd.utils.graph import GraphedStep
+
+    def run(graphed, name, lr, steps):
+        torch.manual_seed(3)
+        eng = Engine(fp16=True, seed=11, init_scale=1024.0)
+        model = build_model(name, max_position_embeddings=positions, **OPTIONS["all"])
+        opt = AdamW(params=model.parameters(), lr=lr)
+        model, opt = eng.prepare(model, opt)
+        model.train()
+        batches = [fixed_batch(4, S, eng.unwrap_model(model).config.vocab_size, eng.device, seed=50 + i) for i in range(2)]
+        step = GraphedStep(eng, model, opt, warmup=2) if graphed else None
+        losses = []
+        for i in range(steps):
+            if graphed:
+                losses.append(float(step(batches[i % 2]).item()))
+                continue
+            out = model(**batches[i % 2])
+            eng.backward(out.loss)
+            opt.step()
+            opt.zero_grad()
+            losses.append(float(out.loss.item()))
+        return losses
+
+    eager, graphed = run(False, "bert-tiny-nodrop", 1e-3, 7), run(True, "bert-tiny-nodrop", 1e-3, 7)
+    assert max(abs(a - b) for a, b in zip(eager, graphed)) < 2e-3, (eager, graphed)
+    same = run(True, "bert-tiny", 0.0, 8)[3::2]  # replays of one batch at learning rate 0: only the masks change
+    assert len(set(same)) == len(same), same
+
+
+@pytest.mark.parametrize("S", [64, 200])
+def test_windows_on_several_streams_add_up_the_same_gradients(S, monkeypatch):
+    """Forward passes of the next micro-batch overlap the backward of the last one: the window's gradients are those of the
+    micro-batches one after the other, up to the order of two additions per element."""
+    from pytorch_distributed_training_amd.engine import Engine
+    from pytorch_distributed_training_amd.models.bert import build_model
+    from pytorch_distributed_training_amd.optim import AdamW
+
+    grads = []
+    for overlap in ("1", "0"):
+        monkeypatch.setenv("PDT_OVERLAP_MICRO", overlap)
+        torch.manual_seed(0)
+        eng = Engine(fp16=True, seed=1, init_scale=64.0)
+        model = build_model("bert-tiny", max_position_embeddings=512, **OPTIONS["all"])
+        model, opt = eng.prepare(model, AdamW(params=model.parameters(), lr=0.0))[:2]
+        inner = getattr(model, "module", model)
+        model.train()
+        batches = []
+        for i, lens in enumerate(([S, S - 7, 3, 40], [S // 2, S, 1, 9], [S, 5, 60, S - 1])):
+            b = _batch(inner.config, S=S, lens=lens)
+            b["sample_ids"] = torch.arange(4 * i, 4 * i + 4, device="cuda", dtype=torch.int32)
+            batches.append(_pack(b) if i == 1 else b)
+        for _ in range(3):
+            opt.zero_grad()
+            inner.arena.window = 5
+            eng.accumulate(model, batches)
+            torch.cuda.synchronize()
+        grads.append(inner.arena.grad.clone())
+    assert torch.isfinite(grads[0]).all() and grads[0].abs().max() > 0
+    torch.testing.assert_close(grads[0], grads[1], rtol=1e-5, atol=1e-5 * float(grads[1].abs().max()))
