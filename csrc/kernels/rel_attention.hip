@@ -152,7 +152,8 @@ __device__ __forceinline__ float ra_quad_sum(float v) {
 // the rows that share it to [1/2, 1), and the results are multiplied by 2^-lift: the factor rides on the exponent of P and on
 // final scales that are there anyway.  2^lift P over the share kept stays below 2^15; |ds| 2^lift stays below what output
 // gradients of size one give without a lift, half the sum of |v| over a row (p (1 - p) times the spread of dp) but for
-// dropout's factor.  bf16 has fp32's exponents: no lift.
+// dropout's factor.  bf16 has fp32's exponents: no lift.  Backward of 256 x 128 tokens, 16 heads: 150 -> 152 us, with dropout 184 ->
+// 197 (five more registers spill); of 2 x 4096 tokens no difference.
 template <typename T> constexpr bool RA_LIFTS = std::is_same<T, _Float16>::value;
 // the largest of the bits of |x| over eight 16-bit values (ordered like the values; infinities and NaN are larger than all numbers)
 __device__ __forceinline__ uint32_t ra_top(uint32_t top, const short8& x) {
